@@ -15,9 +15,11 @@
 #include <tuple>
 
 #include "kernels/attention.h"
+#include "kernels/controls.h"
 #include "kernels/decode_mega.h"
 #include "kernels/elementwise.h"
 #include "kernels/gemm.h"
+#include "kernels/kv4.h"
 #include "kernels/misc.h"
 #include "kernels/ep.h"
 #include "kernels/moe.h"
@@ -724,6 +726,178 @@ void paged_attention_(Tensor q, Tensor kc, Tensor vc, Tensor bt, Tensor seq_lens
   count(n_split > max_cluster && (int64_t)B * Hkv > kDecodeCtrs ? 2 : 1);
 }
 
+// ─── 4-bit KV cache ─────────────────────────────────────────────────────────
+// (Numbers enter the messages through std::to_string: streaming one into a TORCH_CHECK message crashes in this
+// toolchain's mix of C++ runtimes.)
+
+KV4View kv4_view(const Tensor& k, const Tensor& v, const Tensor& scale) {
+  CHECK_CUDA(k);
+  TORCH_CHECK(k.dim() == 4 && k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && k.sizes() == v.sizes(),
+              "kv4: k and v must be uint8 [pages, Hkv, page, hd / 2]");
+  const int64_t hd = 2 * k.size(3);
+  TORCH_CHECK(hd == 64 || hd == 128, "kv4: head_dim must be 64 or 128, got " + std::to_string(hd));
+  TORCH_CHECK(k.size(2) > 0 && k.size(2) % 16 == 0, "kv4: page size must be a multiple of 16, got " + std::to_string(k.size(2)));
+  TORCH_CHECK(scale.scalar_type() == at::kHalf && scale.dim() == 6 && scale.size(0) == k.size(0) &&
+                  scale.size(1) == k.size(1) && scale.size(2) == k.size(2) && scale.size(3) == 2 &&
+                  scale.size(4) == hd / 64 && scale.size(5) == 2,
+              "kv4: scale must be float16 [pages, Hkv, page, 2, hd / 64, 2]");
+  TORCH_CHECK(v.device() == k.device() && scale.device() == k.device(), "kv4: cache tensors on different devices");
+  CHECK_CONTIG(k);
+  CHECK_CONTIG(v);
+  CHECK_CONTIG(scale);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scale.data_ptr()) % 16 == 0,
+              "kv4: cache tensors must start on 16-byte boundaries");
+  return {ptr<uint8_t>(k), ptr<uint8_t>(v), ptr<__half2>(scale), k.size(0), (int)k.size(1), (int)k.size(2), (int)hd};
+}
+
+// [N, H, hd] bf16 rows that 16-byte loads can walk: unit inner stride, aligned rows; anything else is copied.
+Tensor kv4_rows(const Tensor& x, const char* what, const Tensor& cache, int64_t hd) {
+  TORCH_CHECK(x.device() == cache.device(), std::string(what) + " must be on the cache's device");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 3 && x.size(2) == hd, 
+              std::string(what) + " must be bfloat16 [rows, heads, " + std::to_string(hd) + "]");
+  const bool ok = x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+void kv4_write_(Tensor k, Tensor v, Tensor kc, Tensor vc, Tensor scale, Tensor slots) {
+  const KV4View c = kv4_view(kc, vc, scale);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  k = kv4_rows(k, "kv4_write: k", kc, c.hd);
+  v = kv4_rows(v, "kv4_write: v", kc, c.hd);
+  TORCH_CHECK(k.size(1) == c.Hkv && v.sizes() == k.sizes(), 
+              "kv4_write: k and v must be [rows, " + std::to_string(c.Hkv) + ", " + std::to_string(c.hd) + "]");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == k.size(0) &&
+                  slots.device() == kc.device(),
+              "kv4_write: slots must be int64 [rows] on the cache's device");
+  CHECK_CONTIG(slots);
+  kv4_write(ptr<bf16>(k), k.stride(0), k.stride(1), ptr<bf16>(v), v.stride(0), v.stride(1), ptr<int64_t>(slots),
+            (int)k.size(0), c, cur_stream());
+  if (k.size(0)) count();
+}
+
+void kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor slots, Tensor k, Tensor v) {
+  const KV4View c = kv4_view(kc, vc, scale);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.device() == kc.device(),
+              "kv4_read: slots must be int64 [rows] on the cache's device");
+  CHECK_CONTIG(slots);
+  for (const Tensor& t : {k, v}) {
+    CHECK_CONTIG(t);
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == slots.size(0) && t.size(1) == c.Hkv &&
+                    t.size(2) == c.hd && t.device() == kc.device(),
+                "kv4_read: outputs must be bfloat16 [rows, " + std::to_string(c.Hkv) + ", " + std::to_string(c.hd) +
+                    "] on the cache's device");
+  }
+  kv4_read(c, ptr<int64_t>(slots), (int)slots.size(0), ptr<bf16>(k), ptr<bf16>(v), cur_stream());
+  if (slots.size(0)) count();
+}
+
+Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
+  const KV4View c = kv4_view(kc, vc, scale_t);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  q = kv4_rows(q, "paged_attention_kv4: q", kc, c.hd);
+  const int64_t B = q.size(0), Hq = q.size(1);
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0, 
+              "paged_attention_kv4: " + std::to_string(Hq) + " query heads over " + std::to_string(c.Hkv) + " KV heads");
+  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == B && (bt.size(1) <= 1 || bt.stride(1) == 1) &&
+                  bt.device() == kc.device(),
+              "paged_attention_kv4: block_table must be int32 [rows, pages] on the cache's device");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.size(0) == B &&
+                  seq_lens.device() == kc.device(),
+              "paged_attention_kv4: seq_lens must be int32 [rows] on the cache's device");
+  CHECK_CONTIG(seq_lens);
+  Tensor out = torch::empty({B, Hq, c.hd}, q.options());
+  kv4_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
+                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), cur_stream());
+  if (B) count();
+  return out;
+}
+
+// ─── logit controls ─────────────────────────────────────────────────────────
+
+ControlsView controls_view(const std::vector<Tensor>& s) {
+  TORCH_CHECK(s.size() == 9, "logit controls: nine state tensors");
+  const Tensor &rep = s[0], &freq = s[1], &pres = s[2], &seen = s[3], &counts = s[4], &ids = s[5], &vals = s[6],
+               &mask = s[7], &mask_on = s[8];
+  CHECK_CUDA(counts);
+  const int64_t R = counts.size(0), V = counts.dim() == 2 ? counts.size(1) : 0, W = (V + 31) / 32;
+  TORCH_CHECK(counts.dim() == 2 && V > 0, "logit controls: counts must be [slots, vocabulary]");
+  for (const Tensor& t : s) {
+    TORCH_CHECK(t.is_contiguous() && t.device() == counts.device() && t.size(0) == R,
+                "logit controls: state tensors must be contiguous, on one device, with one row per slot");
+  }
+  for (const Tensor* t : {&rep, &freq, &pres}) TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 1, "logit controls: penalties must be float32 [slots]");
+  for (const Tensor* t : {&seen, &mask})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 2 && t->size(1) == W, 
+                "logit controls: seen and mask must be int32 [slots, " + std::to_string(W) + "]");
+  TORCH_CHECK(counts.scalar_type() == at::kInt && mask_on.scalar_type() == at::kInt && mask_on.dim() == 1,
+              "logit controls: counts and mask_on must be int32");
+  TORCH_CHECK(ids.scalar_type() == at::kInt && vals.scalar_type() == at::kFloat && ids.dim() == 2 && ids.sizes() == vals.sizes(),
+              "logit controls: bias_ids int32 and bias_vals float32 must be [slots, entries]");
+  return {ptr<float>(rep),    ptr<float>(freq),  ptr<float>(pres),    ptr<uint32_t>(seen), ptr<int>(counts), ptr<int>(ids),
+          ptr<float>(vals), ptr<uint32_t>(mask), ptr<int>(mask_on), R,                   (int)V,           (int)W,
+          (int)ids.size(1)};
+}
+
+SlotIds slot_ids(const Tensor& slots, const Tensor& state, const char* what) {
+  TORCH_CHECK((slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt) && slots.dim() == 1 &&
+                  slots.device() == state.device(),
+              std::string(what) + ": slots must be int32 or int64 [rows] on the state's device");
+  CHECK_CONTIG(slots);
+  return {slots.data_ptr(), slots.scalar_type() == at::kLong};
+}
+
+void load_tokens_(std::vector<Tensor> state, Tensor slots, Tensor tokens, Tensor cu, Tensor n_prompt) {
+  const ControlsView c = controls_view(state);
+  const Tensor& counts = state[4];
+  const c10::cuda::CUDAGuard guard(counts.device());
+  const SlotIds ids = slot_ids(slots, counts, "load_tokens");
+  const int64_t n = slots.size(0);
+  TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.dim() == 1 && tokens.device() == counts.device(),
+              "load_tokens: tokens must be int64 [total] on the state's device");
+  TORCH_CHECK(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) == n + 1 && n_prompt.scalar_type() == at::kInt &&
+                  n_prompt.dim() == 1 && n_prompt.size(0) == n && cu.device() == counts.device() &&
+                  n_prompt.device() == counts.device(),
+              "load_tokens: cu_tokens int32 [rows + 1] and n_prompt int32 [rows] on the state's device");
+  CHECK_CONTIG(tokens);
+  CHECK_CONTIG(cu);
+  CHECK_CONTIG(n_prompt);
+  load_tokens(c, ids, ptr<int64_t>(tokens), tokens.size(0), ptr<int>(cu), ptr<int>(n_prompt), (int)n, cur_stream());
+  if (n) count();
+}
+
+void apply_logit_controls_(Tensor logits, std::vector<Tensor> state, Tensor slots, c10::optional<Tensor> fresh,
+                           c10::optional<Tensor> done, Tensor out) {
+  const ControlsView c = controls_view(state);
+  const Tensor& counts = state[4];
+  const c10::cuda::CUDAGuard guard(counts.device());
+  const SlotIds ids = slot_ids(slots, counts, "apply_logit_controls");
+  const int64_t B = slots.size(0);
+  const bool half = logits.scalar_type() == at::kBFloat16;
+  TORCH_CHECK((half || logits.scalar_type() == at::kFloat) && logits.dim() == 2 && logits.size(0) == B && logits.size(1) == c.V &&
+                  logits.stride(1) == 1 && logits.device() == counts.device(),
+              "apply_logit_controls: logits must be float32 or bfloat16 [" + std::to_string(B) + ", " + std::to_string(c.V) +
+                  "] on the state's device");
+  TORCH_CHECK(out.scalar_type() == at::kFloat && out.dim() == 2 && out.size(0) == B && out.size(1) == c.V &&
+                  out.stride(1) == 1 && out.device() == counts.device(),
+              "apply_logit_controls: out must be float32 [" + std::to_string(B) + ", " + std::to_string(c.V) +
+                  "] on the state's device");
+  TORCH_CHECK(B <= 1 || out.stride(0) >= c.V, "apply_logit_controls: rows of out overlap");
+  if (out.data_ptr() == logits.data_ptr())
+    TORCH_CHECK(!half && (B <= 1 || out.stride(0) == logits.stride(0)), "apply_logit_controls: out must be logits or apart from it");
+  for (const auto* t : {&fresh, &done})
+    if (t->has_value() && (*t)->defined()) {
+      TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == B && (*t)->is_contiguous() && (*t)->device() == counts.device() &&
+                      (*t)->scalar_type() == (t == &fresh ? at::kLong : at::kInt),
+                  "apply_logit_controls: new_tokens int64 and done int32 must be [rows] on the state's device");
+    }
+  apply_logit_controls(logits.data_ptr(), half, logits.stride(0), c, ids, optr<int64_t>(fresh), optr<int>(done), (int)B,
+                       ptr<float>(out), out.stride(0), cur_stream());
+  if (B) count();
+}
+
 void decode_advance_(Tensor tok, Tensor lp, Tensor tok_in, Tensor pos, Tensor seq_lens, Tensor gen, Tensor max_new,
                      Tensor done, Tensor slot, Tensor bt, Tensor req, Tensor out_tok, Tensor out_lp, Tensor eos,
                      int64_t page) {
@@ -1336,6 +1510,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "paged decode attention; decode_step: the kernel before wrote only each sequence's newest K/V row");
   m.def("paged_decode_force_splits", [](int64_t n) { paged_decode_force_splits((int)n); },
         "decode attention split count override (0 = heuristic); for tests and benchmarks");
+  m.def("kv4_write", &kv4_write_, "quantise K / V rows into the 4-bit paged cache");
+  m.def("kv4_read", &kv4_read_, "the values the 4-bit paged cache holds at given slots");
+  m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache");
+  m.def("load_tokens", &load_tokens_, "token state (seen bits, generated counts) of admitted requests");
+  m.def("apply_logit_controls", &apply_logit_controls_, "penalties, biases and token masks on logits");
   m.def("decode_advance", &decode_advance_);
   m.def("cast_copy", &cast_copy);
   m.def("symm_alloc", &symm_alloc_, "cudaMalloc a symmetric-heap buffer (zeroed); returns the pointer");

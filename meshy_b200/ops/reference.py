@@ -166,6 +166,122 @@ def attention_decode_paged(
     return out.to(q.dtype)
 
 
+# ── 4-bit KV cache ───────────────────────────────────────────────────────────
+
+KV4_GROUP = 64
+_HALF_MAX = 65504.0
+
+
+def kv4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x [T, H, hd]`` to nibble bytes ``[T, H, hd / 2]`` uint8 and ``(a, z)`` pairs ``[T, H, hd / 64, 2]`` fp16
+    (:mod:`.kv4` describes the format)."""
+    T, H, hd = x.shape
+    G = hd // KV4_GROUP
+    xf = x.float().clamp(-_HALF_MAX, _HALF_MAX).reshape(T, H, G, KV4_GROUP)
+    lo, hi = xf.amin(-1, keepdim=True), xf.amax(-1, keepdim=True)
+    a, z = ((hi - lo) / 15.0).half(), lo.half()
+    af = a.float()
+    n = torch.where(af > 0, ((xf - z.float()) / torch.where(af > 0, af, 1.0)).round(), 0.0).clamp(0, 15)
+    n = n.to(torch.uint8).view(T, H, G, 8, 8).transpose(2, 3).reshape(T, H, hd)  # word u G + group, then nibble
+    return n[..., 0::2] | (n[..., 1::2] << 4), torch.cat([a, z], -1)
+
+
+def kv4_dequantize(b: torch.Tensor, pairs: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
+    """Values ``[T, H, hd]`` of :func:`kv4_quantize`'s output."""
+    T, H, half = b.shape
+    G = 2 * half // KV4_GROUP
+    n = torch.stack([b & 15, b >> 4], -1).reshape(T, H, 8, G, 8).transpose(2, 3).reshape(T, H, G, KV4_GROUP)
+    return (n.to(dtype) * pairs[..., :1].to(dtype) + pairs[..., 1:].to(dtype)).reshape(T, H, 2 * half)
+
+
+def _kv4_slots(cache, slots):
+    page = cache.k.shape[2]
+    ok = (slots >= 0) & (slots < cache.k.shape[0] * page)
+    s = slots.clamp(0, cache.k.shape[0] * page - 1).long()
+    return ok, s // page, s % page
+
+
+def kv4_write(k, v, cache, slots) -> None:
+    ok, pg, off = _kv4_slots(cache, slots)
+    for x, data, kv in ((k, cache.k, 0), (v, cache.v, 1)):
+        b, pairs = kv4_quantize(x[ok])
+        data[pg[ok], :, off[ok]] = b
+        cache.scale[pg[ok], :, off[ok], kv] = pairs
+
+
+def kv4_read(cache, slots, dtype=torch.float32):
+    ok, pg, off = _kv4_slots(cache, slots)
+    return tuple(torch.where(ok[:, None, None], kv4_dequantize(data[pg, :, off], cache.scale[pg, :, off, kv]), 0.0).to(dtype)
+                 for data, kv in ((cache.k, 0), (cache.v, 1)))
+
+
+def attention_decode_kv4(q, cache, block_table, seq_lens, scale: float | None = None) -> torch.Tensor:
+    """:func:`attention_decode_paged` over the values of a 4-bit cache; a row of length 0 gives zeros."""
+    B, Hq, hd = q.shape
+    Hkv, page = cache.k.shape[1], cache.k.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    out = torch.zeros(B, Hq, hd, dtype=torch.float32, device=q.device)
+    for b in range(B):
+        L = int(seq_lens[b])
+        if L <= 0:
+            continue
+        t = torch.arange(L, device=q.device)
+        k, v = kv4_read(cache, block_table[b, t // page].long() * page + t % page)
+        qb = q[b].float().view(Hkv, Hq // Hkv, hd)
+        p = torch.softmax(torch.einsum("grd,lgd->grl", qb, k) * scale, dim=-1)
+        out[b] = torch.einsum("grl,lgd->grd", p, v).reshape(Hq, hd)
+    return out.to(q.dtype)
+
+
+# ── logit controls ───────────────────────────────────────────────────────────
+
+def _unpack_bits(words: torch.Tensor, n: int) -> torch.Tensor:
+    sh = torch.arange(32, dtype=torch.int32, device=words.device)
+    return ((words.unsqueeze(-1) >> sh) & 1).bool().flatten(-2)[..., :n]
+
+
+def _set_bit(words: torch.Tensor, v: int) -> None:
+    bit = v % 32
+    words[v // 32] |= -(1 << 31) if bit == 31 else 1 << bit
+
+
+def load_tokens(ctl, slots, tokens, cu_tokens, n_prompt) -> None:
+    """Token state of admitted requests (see :mod:`.controls`)."""
+    cu = cu_tokens.tolist()
+    for i, slot in enumerate(slots.tolist()):
+        if not 0 <= slot < ctl.counts.shape[0]:
+            continue
+        ctl.seen[slot] = 0
+        ctl.counts[slot] = 0
+        for j, v in enumerate(tokens[cu[i]:cu[i + 1]].tolist()):
+            if 0 <= v < ctl.vocab:
+                _set_bit(ctl.seen[slot], v)
+                ctl.counts[slot, v] += j >= int(n_prompt[i])
+
+
+def apply_logit_controls(logits, ctl, slots, new_tokens=None, done=None, out=None) -> torch.Tensor:
+    """Penalties, biases and token masks on ``logits [B, V]`` (see :mod:`.controls`)."""
+    out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device) if out is None else out
+    for b, s in enumerate(slots.tolist()):
+        z = logits[b].float()
+        if 0 <= s < ctl.counts.shape[0]:
+            tok = int(new_tokens[b]) if new_tokens is not None and (done is None or int(done[b]) == 0) else -1
+            if 0 <= tok < ctl.vocab:
+                ctl.counts[s, tok] += 1
+                _set_bit(ctl.seen[s], tok)
+            c = ctl.counts[s].float()
+            r = ctl.repetition[s]
+            z = torch.where(_unpack_bits(ctl.seen[s], ctl.vocab), torch.where(z > 0, z / r, z * r), z)
+            z = z - ctl.frequency[s] * c - torch.where(c > 0, ctl.presence[s], 0.0)
+            ids = ctl.bias_ids[s].long()
+            use = (ids >= 0) & (ids < ctl.vocab)
+            z = z.index_add(0, ids[use], ctl.bias_vals[s][use])
+            if int(ctl.mask_on[s]):
+                z = z.masked_fill(~_unpack_bits(ctl.mask[s], ctl.vocab), float("-inf"))
+        out[b] = z
+    return out
+
+
 # ── LM head + log-softmax + entropy ──────────────────────────────────────────
 
 def lm_head_logprobs(

@@ -33,6 +33,9 @@ cuda_sources = [
     "csrc/kernels/topk.cu",
     "csrc/kernels/decode_noalloc.cu",
     "csrc/kernels/decode_mega.cu",
+    "csrc/kernels/kv4.cu",
+    "csrc/kernels/kv4_attn.cu",
+    "csrc/kernels/controls.cu",
 ]
 extra_cuda = [s for s in ("csrc/kernels/symm.cu", "csrc/kernels/fsdp.cu") if os.path.exists(os.path.join(ROOT, s))]
 
