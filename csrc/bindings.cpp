@@ -794,6 +794,26 @@ void kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor slots, Tensor k, Tenso
   if (slots.size(0)) count();
 }
 
+// Workspace of the attention kernel, one per (device, stream): partial sums and arrival counters (zeroed once, left
+// zero by every launch). A buffer that grew is kept: captured graphs may refer to it.
+struct KV4Workspace {
+  Tensor part, arrived;
+};
+KV4Workspace kv4_workspace(const Tensor& cache, int64_t segments) {
+  static std::map<std::pair<int, cudaStream_t>, std::vector<KV4Workspace>> all;
+  std::lock_guard<std::mutex> g(g_mu);
+  std::vector<KV4Workspace>& w = all[{cache.get_device(), cur_stream()}];
+  if (w.empty() || w.back().arrived.numel() < segments) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    MESHY_CUDA_CHECK(cudaStreamIsCapturing(cur_stream(), &cap));
+    TORCH_CHECK(cap == cudaStreamCaptureStatusNone,
+                "paged_attention_kv4: run this shape once on the capture stream before CUDA graph capture");
+    w.push_back({torch::empty({kv4_part_floats(128)}, cache.options().dtype(torch::kFloat)),
+                 torch::zeros({std::max<int64_t>(segments, 1 << 14)}, cache.options().dtype(torch::kInt32))});
+  }
+  return w.back();
+}
+
 Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
   const KV4View c = kv4_view(kc, vc, scale_t);
   const c10::cuda::CUDAGuard guard(kc.device());
@@ -809,9 +829,12 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
               "paged_attention_kv4: seq_lens must be int32 [rows] on the cache's device");
   CHECK_CONTIG(seq_lens);
   Tensor out = torch::empty({B, Hq, c.hd}, q.options());
+  if (B == 0) return out;
+  const KV4Workspace ws = kv4_workspace(kc, kv4_attention_segments((int)B, (int)Hq, c.Hkv));
   kv4_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
-                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), cur_stream());
-  if (B) count();
+                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ptr<float>(ws.part), ptr<unsigned>(ws.arrived),
+                cur_stream());
+  count();
   return out;
 }
 
