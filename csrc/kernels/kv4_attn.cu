@@ -9,9 +9,10 @@
 // One warp takes 16 tokens at a time (m16n8k16, fp16 in, fp32 sums):
 //   S^T [16 tokens, 8 heads] = K [16, hd] Q^T      A rows are tokens: a lane's 16 bytes of a K row are its A registers
 //   O^T [16 channels, 8 heads] += V^T [16, 16 tokens] P^T    A rows are channels: two byte permutes pair the tokens
-// Query heads that share a KV head fill the 8 columns, so every cached byte is read once for up to 8 heads, straight
-// from global memory to registers: nothing passes through shared memory, P changes from accumulator to operand by
-// movmatrix. tcgen05 would not help here: operands unpacked in registers would have to be stored to shared or tensor
+// Query heads that share a KV head fill the 8 columns, so every cached byte is read once for up to 8 heads. P changes
+// from accumulator to operand by movmatrix. Each warp keeps a ring of kStages tiles of its own in shared memory, filled
+// by 16-byte asynchronous copies, so three tiles are on their way while one is computed and no warp waits for
+// another; V's 16-byte chunks are swizzled on the way in (a lane reads 8 bytes of every second token). tcgen05 would not help here: operands unpacked in registers would have to be stored to shared or tensor
 // memory first, and at 8 query rows the matrix work is a fraction of the unpacking.
 //
 // P carries the scale of V (x = p a'), so it is kept in fp16's range by a reference (m, A) per warp: x = 64 p a' / A
@@ -25,6 +26,7 @@
 // CTA order, so results do not depend on timing.
 #include <cuda_runtime.h>
 
+#include "../include/sm100.cuh"
 #include "kv4.h"
 
 namespace meshy {
@@ -35,27 +37,44 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTok = 16;     // tokens of a tile
 constexpr int kHeads = 8;    // query heads of a segment
+constexpr int kStages = 4;   // tiles of a warp's ring
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBoost = 64.f, kLimit = 32768.f;
+constexpr float kBoost = 64.f;               // x of the largest p and a' right after the reference moved
+constexpr float kMaxP = 128.f, kMaxW = 256.f;  // x = p w stays below 2^15
 constexpr float kMinA = 5.9604645e-8f;  // 2^-24, the smallest fp16
 
 template <int HD>
-struct Tile {  // one lane's share of 16 tokens
-  uint32_t k[2][HD / 32];     // tokens g, g + 8: words (HD / 32) t ..
-  uint32_t v[4][HD / 64];     // tokens 2t, 2t + 1, 2t + 8, 2t + 9: words (HD / 64) g ..
-  uint32_t s[2][HD / 32];     // tokens g, g + 8: (a, z) pairs of K's groups, then V's
+struct Ring {  // one stage: 16 tokens of one head
+  static constexpr int ROW = HD / 2;             // nibble bytes of a token
+  static constexpr int K = 0, V = kTok * ROW, S = 2 * kTok * ROW;
+  static constexpr int BYTES = 2 * kTok * ROW + kTok * (HD / 8);  // the pairs take an eighth of the nibbles' bytes
+  static constexpr int WARP = kStages * BYTES;
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t* d, const void* p) {
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Byte of 16-byte chunk q of a tile's V rows: 128-byte lines, the chunk's place turned by the line, so that the lanes
+// of one read (chunks of tokens 0, 2, 4, 6 or 1, 3, 5, 7) fall on different banks.
+template <int HD>
+__device__ __forceinline__ int v_chunk(int q) {
+  return (q / 8) * 128 + ((q % 8) ^ (2 * ((q / 8) % (HD / 32)))) * 16;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* d, uint32_t p) {
   if constexpr (N == 4)
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                 : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(p));
   else if constexpr (N == 2)
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(p));
   else
-    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(d[0]) : "l"(p));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(d[0]) : "r"(p));
 }
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -104,6 +123,7 @@ struct Args {
   int max_pages;
   const int* seq_lens;
   int B, Hq, rep, blocks;  // blocks: groups of kHeads query heads per KV head
+  int page_shift;          // log2 of the tiles of a page, -1: not a power of two
   float scale;
   bf16* out;
   float* part;         // [2 CTAs][kHeads][hd + 2]
@@ -122,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   constexpr int G = HD / 64;
   constexpr int KW = HD / 32;       // K words a lane takes of a row
   constexpr int LD = HD + 4;        // row stride of the merge buffer: spreads the heads over the banks
-  __shared__ float so[kWarps][kHeads][LD];
+  extern __shared__ __align__(128) uint8_t smem[];  // the warps' rings; then the merge buffer
+  float(*so)[kHeads][LD] = reinterpret_cast<float(*)[kHeads][LD]>(smem);
   __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
   __shared__ long long scan[kWarps];
   __shared__ int s_row;
@@ -178,8 +199,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   int hseg = (int)((at - s_at) / U);
   long long seg0 = s_at + (long long)hseg * U;  // first tile of the segment
 
+  using R = Ring<HD>;
   const int ppt = a.c.page / kTok;  // tiles of a page
   const float sl2 = a.scale * kLog2e;
+  const uint32_t ring = smem_u32(smem) + warp * R::WARP;
+  const int64_t page_bytes = (int64_t)a.c.Hkv * a.c.page * R::ROW;
+  // this lane's places in a stage
+  const uint32_t k_at = R::K + g * R::ROW + t * (4 * KW), s_at4 = R::S + g * (8 * G);
+  uint32_t v_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at_byte = (2 * t + (i & 1) + 8 * (i >> 1)) * R::ROW + g * (4 * G);
+    v_at[i] = R::V + v_chunk<HD>(at_byte / 16) + at_byte % 16;
+  }
 
   while (at < end) {
     const int hk = hseg / a.blocks, h0 = (hseg % a.blocks) * kHeads;
@@ -248,43 +280,53 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     }
 
     const int* row_bt = a.bt + b * a.bt_stride;
+    auto page_at = [&](int tile) { return a.page_shift >= 0 ? tile >> a.page_shift : tile / ppt; };
     auto page_of = [&](int tile) -> int {
       if (tile >= last || tile * kTok >= n_tok) return -1;
-      const int p = row_bt[tile / ppt];
+      const int p = row_bt[page_at(tile)];
       return p < a.c.n_pages ? p : -1;
     };
-    auto load = [&](Tile<HD>& x, int tile, int page) {
-      if (page < 0) return;
-      const int64_t r = ((int64_t)page * a.c.Hkv + hk) * a.c.page + (tile % ppt) * kTok;
-      const uint8_t* kp = a.c.k + r * (HD / 2);
-      const uint8_t* vp = a.c.v + r * (HD / 2);
-      const __half2* sp = a.c.scale + r * (2 * G);
+    const uint8_t* kp = a.c.k + (int64_t)hk * a.c.page * R::ROW + lane * 16;
+    const uint8_t* vp = a.c.v + (int64_t)hk * a.c.page * R::ROW + lane * 16;
+    const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + (int64_t)hk * a.c.page * (8 * G) + lane * 16;
+    auto fetch = [&](uint32_t stage, int tile, int page) {
+      if (page >= 0) {
+        const int64_t off = page * page_bytes + (tile - page_at(tile) * ppt) * (kTok * R::ROW);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load_words<KW>(x.k[i], kp + (g + 8 * i) * (HD / 2) + t * (4 * KW));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) load_words<2 * G>(x.s[i], sp + (g + 8 * i) * (2 * G));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_words<G>(x.v[i], vp + (2 * t + (i & 1) + 8 * (i >> 1)) * (HD / 2) + g * (4 * G));
+        for (int i = 0; i < R::V / 512; ++i) {
+          copy16(stage + R::K + (lane + 32 * i) * 16, kp + off + 512 * i);
+          copy16(stage + R::V + v_chunk<HD>(lane + 32 * i), vp + off + 512 * i);
+        }
+        if (lane < R::BYTES / 16 - R::S / 16) copy16(stage + R::S + lane * 16, sp + (off >> 2));
+      }
+      copies_commit();
     };
-    auto compute = [&](Tile<HD>& x, int tile, int page) {
-      if (page < 0) return;
+    auto compute = [&](uint32_t stage, int tile) {
+      uint32_t kw[2][KW], vw[4][G], sw[2][2 * G];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) load_words<KW>(kw[i], stage + k_at + i * 8 * R::ROW);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], stage + s_at4 + i * 8 * (8 * G));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_words<G>(vw[i], stage + v_at[i]);
       float acc[G][4];
 #pragma unroll
       for (int i = 0; i < G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
-        uint32_t w0 = x.k[0][j], w1 = x.k[1][j];
+        uint32_t w0 = kw[0][j], w1 = kw[1][j];
         mma_f16(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
         w0 >>= 8;
         w1 >>= 8;
         mma_f16(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2], qf[j][3]);
       }
-      if (tile * kTok + kTok > n_tok) {  // the row ends inside this tile: what lies behind may be anything
+      const bool cut = tile * kTok + kTok > n_tok;  // the row ends inside this tile: what lies behind may be anything
+      if (cut) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (tile * kTok + g + 8 * i >= n_tok) {
 #pragma unroll
-            for (int j = 0; j < 2 * G; ++j) x.s[i][j] = 0u;
+            for (int j = 0; j < 2 * G; ++j) sw[i][j] = 0u;
           }
       }
       // scores: [token g + 8 i][head 2 t + r], base 2, relative to the reference
@@ -294,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
         float e[2] = {0.f, 0.f}, d[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-          const float2 k2 = unpack_half2(x.s[i][j]), v2 = unpack_half2(x.s[i][G + j]);
+          const float2 k2 = unpack_half2(sw[i][j]), v2 = unpack_half2(sw[i][G + j]);
           va[i][j] = v2.x;
           vz[i][j] = v2.y;
 #pragma unroll
@@ -303,26 +345,29 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
             e[r] = fmaf(k2.y, qs[r][j], e[r]);
           }
         }
-        const bool in = tile * kTok + g + 8 * i < n_tok;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) s[i][r] = in ? fmaf(cs[r], d[r], e[r]) : -INFINITY;
+        for (int r = 0; r < 2; ++r) s[i][r] = fmaf(cs[r], d[r], e[r]);
       }
-      float p[2][2], y[2][2][G], top = 0.f;
-      bool bad = fresh;
+      if (cut) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
+          if (tile * kTok + g + 8 * i >= n_tok) s[i][0] = s[i][1] = -INFINITY;
+      }
+      float p[2][2], w[2][G], top_p = 0.f, top_w = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           p[i][r] = ex2(s[i][r] - m[r]);
-          top = fmaxf(top, p[i][r]);  // of its own: a' may be 0
-#pragma unroll
-          for (int j = 0; j < G; ++j) {
-            y[i][r][j] = p[i][r] * (va[i][j] * inv[j]);
-            top = fmaxf(top, y[i][r][j]);
-          }
+          top_p = fmaxf(top_p, p[i][r]);
         }
-      bad |= !(top <= kLimit);
-      if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          w[i][j] = va[i][j] * inv[j];
+          top_w = fmaxf(top_w, w[i][j]);
+        }
+      }
+      if (__any_sync(0xffffffffu, fresh || top_p > kMaxP || top_w > kMaxW)) {
         // move the reference to the true maxima
         fresh = false;
         float keep[2];
@@ -347,13 +392,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
           z[j][1] *= keep[1];
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            p[i][r] = m[r] == -INFINITY && s[i][r] == -INFINITY ? 0.f : ex2(s[i][r] - m[r]);
+          for (int r = 0; r < 2; ++r) p[i][r] = m[r] == -INFINITY && s[i][r] == -INFINITY ? 0.f : ex2(s[i][r] - m[r]);
 #pragma unroll
-            for (int j = 0; j < G; ++j) y[i][r][j] = p[i][r] * (va[i][j] * inv[j]);
-          }
+          for (int j = 0; j < G; ++j) w[i][j] = va[i][j] * inv[j];
+        }
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -363,12 +407,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       }
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        const uint32_t b0 = transpose8x8(pack_half2(y[0][0][j], y[0][1][j]));
-        const uint32_t b1 = transpose8x8(pack_half2(y[1][0][j], y[1][1][j]));
+        const uint32_t b0 = transpose8x8(pack_half2(p[0][0] * w[0][j], p[0][1] * w[0][j]));
+        const uint32_t b1 = transpose8x8(pack_half2(p[1][0] * w[1][j], p[1][1] * w[1][j]));
 #pragma unroll
         for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half ..
           const uint32_t sel = half ? 0x7632u : 0x5410u;
-          uint32_t x01 = __byte_perm(x.v[0][j], x.v[1][j], sel), x23 = __byte_perm(x.v[2][j], x.v[3][j], sel);
+          uint32_t x01 = __byte_perm(vw[0][j], vw[1][j], sel), x23 = __byte_perm(vw[2][j], vw[3][j], sel);
           mma_f16(o[j][2 * half], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
           x01 >>= 8;
           x23 >>= 8;
@@ -377,28 +421,35 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       }
     };
 
-    // a tile in flight while the one before it is computed, its page id one step ahead
+    // kStages - 1 tiles on their way; a tile's page id is read one step before its copies start
     {
       int tile = first + warp;
-      int page = page_of(tile), next = page_of(tile + kWarps);
-      Tile<HD> x0, x1;
-      load(x0, tile, page);
-      while (tile < last) {
-        int ahead = page_of(tile + 2 * kWarps);
-        load(x1, tile + kWarps, next);
-        compute(x0, tile, page);
-        tile += kWarps;
-        page = next;
-        next = ahead;
-        if (tile >= last) break;
-        ahead = page_of(tile + 2 * kWarps);
-        load(x0, tile + kWarps, next);
-        compute(x1, tile, page);
-        tile += kWarps;
-        page = next;
-        next = ahead;
+      uint32_t valid = 0;  // bit i: the tile i steps ahead has a page
+      int next = page_of(tile);
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) {
+        const int page = next;
+        next = page_of(tile + (i + 1) * kWarps);
+        valid |= (page >= 0 ? 1u : 0u) << i;
+        fetch(ring + i * R::BYTES, tile + i * kWarps, page);
       }
+      uint32_t stage = ring, ahead = ring + (kStages - 1) * R::BYTES;
+      for (; tile < last; tile += kWarps) {
+        __syncwarp();  // every lane has read the stage that is filled again
+        const int page = next;
+        next = page_of(tile + kStages * kWarps);
+        valid |= (page >= 0 ? 1u : 0u) << (kStages - 1);
+        fetch(ahead, tile + (kStages - 1) * kWarps, page);
+        copies_wait<kStages - 1>();
+        __syncwarp();
+        if (valid & 1u) compute(stage, tile);
+        valid >>= 1;
+        ahead = stage;
+        stage = stage + R::BYTES == ring + R::WARP ? ring : stage + R::BYTES;
+      }
+      copies_wait<0>();
     }
+    __syncthreads();  // the rings are drained: the merge buffer takes their place
 
     // the warp's state: o in units of V, relative to m
 #pragma unroll
@@ -500,6 +551,19 @@ int sm_count() {
   return n[dev];
 }
 
+template <int HD>
+void launch(const Args& a, cudaStream_t st) {
+  constexpr int smem = std::max<int>(kWarps * Ring<HD>::WARP, kWarps * kHeads * (HD + 4) * 4);
+  static bool set[64] = {};
+  int dev = 0;
+  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!set[dev]) {
+    MESHY_CUDA_CHECK(cudaFuncSetAttribute(kv4_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    set[dev] = true;
+  }
+  launch_pdl(kv4_attn_kernel<HD>, dim3(2 * sm_count()), dim3(kThreads), smem, st, a);
+}
+
 }  // namespace
 
 int kv4_attention_ctas() { return 2 * sm_count(); }
@@ -510,13 +574,16 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
                    cudaStream_t st) {
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
-  const Args a{q,  qs,    qh,  c,    bt,     bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads, scale,
+  const int ppt = c.page / kTok;
+  int shift = -1;
+  if ((ppt & (ppt - 1)) == 0)
+    for (shift = 0; (1 << shift) < ppt;) ++shift;
+  const Args a{q,   qs,   qh,     c, bt, bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads, shift, scale,
                out, part, arrived};
-  const int grid = kv4_attention_ctas();
   if (c.hd == 128)
-    launch_pdl(kv4_attn_kernel<128>, dim3(grid), dim3(kThreads), 0, st, a);
+    launch<128>(a, st);
   else
-    launch_pdl(kv4_attn_kernel<64>, dim3(grid), dim3(kThreads), 0, st, a);
+    launch<64>(a, st);
 }
 
 }  // namespace meshy
