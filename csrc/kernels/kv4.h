@@ -34,7 +34,7 @@ void kv4_read(KV4View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStre
 // that may run at the same time need workspaces of their own.
 int kv4_attention_ctas();
 int64_t kv4_attention_segments(int B, int Hq, int Hkv);
-inline int64_t kv4_part_floats(int hd) { return (int64_t)2 * kv4_attention_ctas() * 8 * (hd + 2); }
+inline int64_t kv4_part_floats(int hd) { return (int64_t)2 * kv4_attention_ctas() * 8 * (hd + 4); }
 void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* bt, int64_t bt_stride, int max_pages,
                    const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived,
                    cudaStream_t st);

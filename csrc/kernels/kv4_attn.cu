@@ -123,7 +123,8 @@ struct Args {
   int max_pages;
   const int* seq_lens;
   int B, Hq, rep, blocks;  // blocks: groups of kHeads query heads per KV head
-  int page_shift;          // log2 of the tiles of a page, -1: not a power of two
+  int ppt;                 // tiles of a page
+  int page_bytes;          // nibble bytes of a page, all heads
   float scale;
   bf16* out;
   float* part;         // [2 CTAs][kHeads][hd + 2]
@@ -137,13 +138,39 @@ __device__ __forceinline__ int tokens_of(const Args& a, int b) {
 }
 __device__ __forceinline__ int tiles_of(int n) { return max(1, (n + kTok - 1) / kTok); }  // an empty row writes its zeros
 
+// A CTA's walk over its share of the tiles: segment (b, h), of whose U tiles it has [first, last); ``left`` tiles of the
+// share remain from ``first`` on.
+struct Walk {
+  int b, h, n, U, first, last, left;
+  __device__ __forceinline__ void enter(const Args& a) {
+    n = tokens_of(a, b);
+    U = tiles_of(n);
+    last = min(U, first + left);
+  }
+  __device__ __forceinline__ bool next(const Args& a) {
+    left -= last - first;
+    if (left <= 0) return false;
+    first = 0;
+    if (++h == a.c.Hkv * a.blocks) {
+      h = 0;
+      ++b;
+      n = tokens_of(a, b);
+      U = tiles_of(n);
+    }
+    last = min(U, left);
+    return true;
+  }
+};
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   constexpr int G = HD / 64;
   constexpr int KW = HD / 32;       // K words a lane takes of a row
   constexpr int LD = HD + 4;        // row stride of the merge buffer: spreads the heads over the banks
-  extern __shared__ __align__(128) uint8_t smem[];  // the warps' rings; then the merge buffer
-  float(*so)[kHeads][LD] = reinterpret_cast<float(*)[kHeads][LD]>(smem);
+  using R = Ring<HD>;
+  extern __shared__ __align__(128) uint8_t smem[];  // the warps' rings, then the merge buffer
+  float* merge = reinterpret_cast<float*>(smem + kWarps * R::WARP);
+  float(*so)[kHeads][LD] = reinterpret_cast<float(*)[kHeads][LD]>(merge);
   __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
   __shared__ long long scan[kWarps];
   __shared__ int s_row;
@@ -168,8 +195,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   total *= per_row;
   const long long n_cta = min((long long)gridDim.x, (total + kWarps - 1) / kWarps);
   if (blockIdx.x >= n_cta) return;
-  long long at = blockIdx.x * total / n_cta;
-  const long long end = (blockIdx.x + 1) * total / n_cta;
+  const long long at = blockIdx.x * total / n_cta, end = (blockIdx.x + 1) * total / n_cta;
   // the row that holds tile ``at``
   long long base = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
@@ -194,16 +220,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     if (base > at) break;
   }
   __syncthreads();
-  int b = s_row;
-  int n_tok = tokens_of(a, b), U = tiles_of(n_tok);
-  int hseg = (int)((at - s_at) / U);
-  long long seg0 = s_at + (long long)hseg * U;  // first tile of the segment
+  Walk cur;
+  cur.b = s_row;
+  {
+    const int U = tiles_of(tokens_of(a, cur.b));
+    cur.h = (int)((at - s_at) / U);
+    cur.first = (int)(at - s_at - (long long)cur.h * U);
+  }
+  cur.left = (int)(end - at);
+  cur.enter(a);
+  long long seg0 = at - cur.first;  // the segment's first tile in the sum
 
-  using R = Ring<HD>;
-  const int ppt = a.c.page / kTok;  // tiles of a page
   const float sl2 = a.scale * kLog2e;
   const uint32_t ring = smem_u32(smem) + warp * R::WARP;
-  const int64_t page_bytes = (int64_t)a.c.Hkv * a.c.page * R::ROW;
   // this lane's places in a stage
   const uint32_t k_at = R::K + g * R::ROW + t * (4 * KW), s_at4 = R::S + g * (8 * G);
   uint32_t v_at[4];
@@ -213,11 +242,65 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     v_at[i] = R::V + v_chunk<HD>(at_byte / 16) + at_byte % 16;
   }
 
-  while (at < end) {
-    const int hk = hseg / a.blocks, h0 = (hseg % a.blocks) * kHeads;
+  // The copies run kStages - 1 tiles ahead of the arithmetic, across the segments; a tile's page id is read one step
+  // before its copies start.
+  Walk f = cur;
+  int f_tile = f.first + warp, f_end = f.n ? f.last : 0, f_pi = f_tile / a.ppt, f_off = f_tile % a.ppt, f_page = -1;
+  int f_head = f.h / a.blocks * a.ppt;
+  const int step_pi = kWarps / a.ppt, step_off = kWarps % a.ppt;
+  const uint8_t* kp = a.c.k + lane * 16;
+  const uint8_t* vp = a.c.v + lane * 16;
+  const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + lane * 16;
+  auto settle = [&]() {  // on this warp's next tile, if its share has one
+    while (f_tile >= f_end) {
+      if (!f.next(a)) {
+        f_page = -1;
+        f_end = 0x7fffffff;  // nothing more: the cursor stays on pages that are not there
+        f_tile = 0;
+        f.left = 0;
+        return;
+      }
+      f_tile = warp;
+      f_end = f.n ? f.last : 0;
+      f_pi = f_tile / a.ppt;
+      f_off = f_tile % a.ppt;
+      f_head = f.h / a.blocks * a.ppt;
+    }
+    if (f.left > 0) f_page = a.bt[f.b * a.bt_stride + f_pi];
+  };
+  uint32_t valid = 0;  // bit i: the tile i steps ahead has a page
+  auto fetch = [&](uint32_t stage, int steps) {
+    if ((uint32_t)f_page < (uint32_t)a.c.n_pages) {
+      valid |= 1u << steps;
+      const int64_t off = (int64_t)f_page * a.page_bytes + (f_head + f_off) * (kTok * R::ROW);
+#pragma unroll
+      for (int i = 0; i < R::V / 512; ++i) {
+        copy16(stage + R::K + (lane + 32 * i) * 16, kp + off + 512 * i);
+        copy16(stage + R::V + v_chunk<HD>(lane + 32 * i), vp + off + 512 * i);
+      }
+      if (lane < (R::BYTES - R::S) / 16) copy16(stage + R::S + lane * 16, sp + (off >> 2));
+    }
+    copies_commit();
+    f_tile += kWarps;
+    f_pi += step_pi;
+    f_off += step_off;
+    if (f_off >= a.ppt) {
+      f_off -= a.ppt;
+      ++f_pi;
+    }
+    settle();
+  };
+  settle();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(ring + i * R::BYTES, i);
+  uint32_t stage = ring, ahead = ring + (kStages - 1) * R::BYTES;
+
+  while (true) {
+    const int hk = cur.h / a.blocks, h0 = (cur.h % a.blocks) * kHeads;
     const int nh = min(kHeads, a.rep - h0);
-    const int first = (int)(at - seg0);
-    const int last = (int)min((long long)U, end - seg0);
+    const int b = cur.b;
+    const int t_end = cur.n ? cur.last : 0;
+    const int cut = cur.n % kTok ? cur.U - 1 : -1;  // the row ends inside this tile
 
     // Q fragments: head g, channels of the words this lane reads of a K row; scaled so that the largest is in [2^14, 2^15)
     uint32_t qf[KW][4];
@@ -269,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     }
 
     float o[G][4][4], z[G][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, A[G], inv[G];
-    bool fresh = true;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
 #pragma unroll
@@ -279,36 +361,24 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       inv[i] = kBoost / kMinA;
     }
 
-    const int* row_bt = a.bt + b * a.bt_stride;
-    auto page_at = [&](int tile) { return a.page_shift >= 0 ? tile >> a.page_shift : tile / ppt; };
-    auto page_of = [&](int tile) -> int {
-      if (tile >= last || tile * kTok >= n_tok) return -1;
-      const int p = row_bt[page_at(tile)];
-      return p < a.c.n_pages ? p : -1;
-    };
-    const uint8_t* kp = a.c.k + (int64_t)hk * a.c.page * R::ROW + lane * 16;
-    const uint8_t* vp = a.c.v + (int64_t)hk * a.c.page * R::ROW + lane * 16;
-    const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + (int64_t)hk * a.c.page * (8 * G) + lane * 16;
-    auto fetch = [&](uint32_t stage, int tile, int page) {
-      if (page >= 0) {
-        const int64_t off = page * page_bytes + (tile - page_at(tile) * ppt) * (kTok * R::ROW);
-#pragma unroll
-        for (int i = 0; i < R::V / 512; ++i) {
-          copy16(stage + R::K + (lane + 32 * i) * 16, kp + off + 512 * i);
-          copy16(stage + R::V + v_chunk<HD>(lane + 32 * i), vp + off + 512 * i);
-        }
-        if (lane < R::BYTES / 16 - R::S / 16) copy16(stage + R::S + lane * 16, sp + (off >> 2));
-      }
-      copies_commit();
-    };
-    auto compute = [&](uint32_t stage, int tile) {
+    for (int tile = cur.first + warp; tile < t_end; tile += kWarps) {
+      __syncwarp();  // every lane has read the stage that is filled again
+      fetch(ahead, kStages - 1);
+      copies_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t here = stage;
+      ahead = stage;
+      stage = stage + R::BYTES == ring + R::WARP ? ring : stage + R::BYTES;
+      const bool there = valid & 1u;
+      valid >>= 1;
+      if (!there) continue;
       uint32_t kw[2][KW], vw[4][G], sw[2][2 * G];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load_words<KW>(kw[i], stage + k_at + i * 8 * R::ROW);
+      for (int i = 0; i < 2; ++i) load_words<KW>(kw[i], here + k_at + i * 8 * R::ROW);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], stage + s_at4 + i * 8 * (8 * G));
+      for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], here + s_at4 + i * 8 * (8 * G));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_words<G>(vw[i], stage + v_at[i]);
+      for (int i = 0; i < 4; ++i) load_words<G>(vw[i], here + v_at[i]);
       float acc[G][4];
 #pragma unroll
       for (int i = 0; i < G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -320,11 +390,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
         w1 >>= 8;
         mma_f16(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2], qf[j][3]);
       }
-      const bool cut = tile * kTok + kTok > n_tok;  // the row ends inside this tile: what lies behind may be anything
-      if (cut) {
+      float e[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+      if (tile == cut) {  // what lies behind the row's end may be anything
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (tile * kTok + g + 8 * i >= n_tok) {
+          if (g + 8 * i >= cur.n % kTok) {
+            e[i][0] = e[i][1] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 2 * G; ++j) sw[i][j] = 0u;
           }
@@ -333,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       float s[2][2], va[2][G], vz[2][G];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float e[2] = {0.f, 0.f}, d[2] = {0.f, 0.f};
+        float d[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           const float2 k2 = unpack_half2(sw[i][j]), v2 = unpack_half2(sw[i][G + j]);
@@ -342,16 +413,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             d[r] = fmaf(k2.x, acc[j][2 * i + r], d[r]);
-            e[r] = fmaf(k2.y, qs[r][j], e[r]);
+            e[i][r] = fmaf(k2.y, qs[r][j], e[i][r]);
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) s[i][r] = fmaf(cs[r], d[r], e[r]);
-      }
-      if (cut) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (tile * kTok + g + 8 * i >= n_tok) s[i][0] = s[i][1] = -INFINITY;
+        for (int r = 0; r < 2; ++r) s[i][r] = fmaf(cs[r], d[r], e[i][r]);
       }
       float p[2][2], w[2][G], top_p = 0.f, top_w = 0.f;
 #pragma unroll
@@ -367,9 +433,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
           top_w = fmaxf(top_w, w[i][j]);
         }
       }
-      if (__any_sync(0xffffffffu, fresh || top_p > kMaxP || top_w > kMaxW)) {
+      if (__any_sync(0xffffffffu, top_p > kMaxP || top_w > kMaxW)) {  // the first tile too: there p is infinite
         // move the reference to the true maxima
-        fresh = false;
         float keep[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -419,37 +484,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
           mma_f16(o[j][2 * half + 1], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
         }
       }
-    };
-
-    // kStages - 1 tiles on their way; a tile's page id is read one step before its copies start
-    {
-      int tile = first + warp;
-      uint32_t valid = 0;  // bit i: the tile i steps ahead has a page
-      int next = page_of(tile);
-#pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) {
-        const int page = next;
-        next = page_of(tile + (i + 1) * kWarps);
-        valid |= (page >= 0 ? 1u : 0u) << i;
-        fetch(ring + i * R::BYTES, tile + i * kWarps, page);
-      }
-      uint32_t stage = ring, ahead = ring + (kStages - 1) * R::BYTES;
-      for (; tile < last; tile += kWarps) {
-        __syncwarp();  // every lane has read the stage that is filled again
-        const int page = next;
-        next = page_of(tile + kStages * kWarps);
-        valid |= (page >= 0 ? 1u : 0u) << (kStages - 1);
-        fetch(ahead, tile + (kStages - 1) * kWarps, page);
-        copies_wait<kStages - 1>();
-        __syncwarp();
-        if (valid & 1u) compute(stage, tile);
-        valid >>= 1;
-        ahead = stage;
-        stage = stage + R::BYTES == ring + R::WARP ? ring : stage + R::BYTES;
-      }
-      copies_wait<0>();
     }
-    __syncthreads();  // the rings are drained: the merge buffer takes their place
 
     // the warp's state: o in units of V, relative to m
 #pragma unroll
@@ -476,8 +511,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     }
     __syncthreads();
     // join the warps; a whole segment is done, a piece of one goes to the workspace
-    const bool whole = first == 0 && last == U;
-    const int slot = 2 * blockIdx.x + (first == 0 ? 1 : 0);
+    const bool whole = cur.first == 0 && cur.last == cur.U;
+    const int slot = 2 * blockIdx.x + (cur.first == 0 ? 1 : 0);
     bf16* dst = a.out + ((int64_t)b * a.Hq + hk * a.rep + h0) * HD;
     for (int i = tid; i < nh * (HD / 2); i += kThreads) {
       const int h = i / (HD / 2), ch = 2 * (i % (HD / 2));
@@ -486,61 +521,76 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[w][h]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = sm[w][h] == -INFINITY ? 0.f : ex2(sm[w][h] - M);
-        L = fmaf(sl[w][h], f, L);
-        x = fmaf(so[w][h][ch], f, x);
-        y = fmaf(so[w][h][ch + 1], f, y);
+        const float c = sm[w][h] == -INFINITY ? 0.f : ex2(sm[w][h] - M);
+        L = fmaf(sl[w][h], c, L);
+        x = fmaf(so[w][h][ch], c, x);
+        y = fmaf(so[w][h][ch + 1], c, y);
       }
       if (whole) {
-        const float f = L == 0.f ? 0.f : 1.f / L;
-        *reinterpret_cast<uint32_t*>(dst + (int64_t)h * HD + ch) = pack_bf16x2(x * f, y * f);
+        const float c = L == 0.f ? 0.f : 1.f / L;
+        *reinterpret_cast<uint32_t*>(dst + (int64_t)h * HD + ch) = pack_bf16x2(x * c, y * c);
       } else {
-        float* pp = a.part + ((int64_t)slot * kHeads + h) * (HD + 2);
+        float* pp = a.part + ((int64_t)slot * kHeads + h) * (HD + 4);
         *reinterpret_cast<float2*>(pp + ch) = make_float2(x, y);
         if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(M, L);
       }
     }
     if (!whole) {
-      const long long c0 = ((seg0 + 1) * n_cta - 1) / total, c1 = ((seg0 + U) * n_cta - 1) / total;
-      unsigned* ctr = a.arrived + (int64_t)b * per_row + hseg;
+      const long long c0 = ((seg0 + 1) * n_cta - 1) / total;  // the CTAs that share the segment
+      const int np = (int)(((seg0 + cur.U) * n_cta - 1) / total - c0) + 1;
+      unsigned* ctr = a.arrived + (int64_t)b * per_row + cur.h;
       __threadfence();
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(ctr, 1u) == (unsigned)(c1 - c0);
+      if (tid == 0) s_last = atomicAdd(ctr, 1u) == (unsigned)(np - 1);
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int i = tid; i < nh * (HD / 2); i += kThreads) {
-          const int h = i / (HD / 2), ch = 2 * (i % (HD / 2));
-          float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-          for (long long c = c0; c <= c1; ++c) {
-            const float* pp = a.part + ((2 * c + (c == c0 ? 1 : 0)) * kHeads + h) * (HD + 2);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pp + HD));
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(pp + ch));
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;
-            const float Mn = fmaxf(M, ml.x), f = ex2(M - Mn), e = ex2(ml.x - Mn);
-            L = L * f + ml.y * e;
-            x = x * f + v.x * e;
-            y = y * f + v.y * e;
-            M = Mn;
+        static_assert(kWarps == kHeads, "one warp per head");
+        // every piece's weight, then the sum of the pieces, a few loads under way at a time
+        const float* p0 = a.part + c0 * 2 * kHeads * (HD + 4);
+        auto piece = [&](int c, int h) { return p0 + ((2 * c + (c == 0 ? 1 : 0)) * kHeads + h) * (HD + 4); };
+        float* wt = merge + warp * np;
+        if (warp < nh) {
+          float M = -INFINITY, L = 0.f;
+          for (int c = lane; c < np; c += 32) {
+            const float m1 = __ldcg(piece(c, warp) + HD);
+            wt[c] = m1;
+            M = fmaxf(M, m1);
           }
-          const float f = L == 0.f ? 0.f : 1.f / L;
-          *reinterpret_cast<uint32_t*>(dst + (int64_t)h * HD + ch) = pack_bf16x2(x * f, y * f);
+          M = warp_max(M);
+          for (int c = lane; c < np; c += 32) {
+            const float x = wt[c] == -INFINITY ? 0.f : ex2(wt[c] - M);
+            wt[c] = x;
+            L = fmaf(__ldcg(piece(c, warp) + HD + 1), x, L);
+          }
+          L = warp_sum(L);
+          if (lane == 0) sl[0][warp] = L;
+        }
+        __syncthreads();
+        for (int i = tid; i < nh * (HD / 4); i += kThreads) {
+          const int h = i / (HD / 4), ch = 4 * (i % (HD / 4));
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int c = 0; c < np; ++c) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(c, h) + ch));
+            const float e = merge[h * np + c];
+            x.x = fmaf(v.x, e, x.x);
+            x.y = fmaf(v.y, e, x.y);
+            x.z = fmaf(v.z, e, x.z);
+            x.w = fmaf(v.w, e, x.w);
+          }
+          const float L = sl[0][h], e = L == 0.f ? 0.f : 1.f / L;
+          *reinterpret_cast<uint2*>(dst + (int64_t)h * HD + ch) =
+              make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
         }
         if (tid == 0) *ctr = 0u;
       }
     }
+    seg0 += cur.U;
+    if (!cur.next(a)) break;
     __syncthreads();  // the merge buffer is free
-    at = seg0 + last;
-    if (at < end) {
-      seg0 += U;
-      if (++hseg == per_row) {
-        hseg = 0;
-        ++b;
-        n_tok = tokens_of(a, b);
-        U = tiles_of(n_tok);
-      }
-    }
   }
+  copies_wait<0>();
 }
 
 int sm_count() {
@@ -553,7 +603,7 @@ int sm_count() {
 
 template <int HD>
 void launch(const Args& a, cudaStream_t st) {
-  constexpr int smem = std::max<int>(kWarps * Ring<HD>::WARP, kWarps * kHeads * (HD + 4) * 4);
+  constexpr int smem = kWarps * Ring<HD>::WARP + kWarps * kHeads * (HD + 4) * 4;
   static bool set[64] = {};
   int dev = 0;
   MESHY_CUDA_CHECK(cudaGetDevice(&dev));
@@ -574,11 +624,9 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
                    cudaStream_t st) {
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
-  const int ppt = c.page / kTok;
-  int shift = -1;
-  if ((ppt & (ppt - 1)) == 0)
-    for (shift = 0; (1 << shift) < ppt;) ++shift;
-  const Args a{q,   qs,   qh,     c, bt, bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads, shift, scale,
+  const int64_t page_bytes = (int64_t)c.Hkv * c.page * (c.hd / 2);
+  MESHY_CHECK(page_bytes < (1LL << 31), "paged_attention_kv4: a page of all heads must be below 2 GB");
+  const Args a{q,   qs,   qh,     c, bt, bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads, c.page / kTok, (int)page_bytes, scale,
                out, part, arrived};
   if (c.hd == 128)
     launch<128>(a, st);
