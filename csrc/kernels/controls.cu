@@ -13,61 +13,141 @@ __device__ __forceinline__ int64_t slot_of(SlotIds s, int i) {
   return s.wide ? reinterpret_cast<const int64_t*>(s.p)[i] : (int64_t) reinterpret_cast<const int*>(s.p)[i];
 }
 
-// One CTA per request: clear the row, then one atomic per token (integers: the order does not matter).
-__global__ void __launch_bounds__(1024)
+// ─── token state ───────────────────────────────────────────────────────────
+// A row's counts are 4 V bytes that have to be written whatever its tokens are (608 KB at V = 151936), its tokens 8
+// bytes each. A CTA owns kSpan entries of the row: it counts the row's tokens that fall among them in shared memory
+// (16-bit halves would overflow, so 32-bit) and writes its span once, coalesced; nothing is cleared or added in
+// global memory. Every CTA reads the row's whole token list, from L2 after the first.
+constexpr int kSpan = 8192;
+constexpr int kLoadThreads = 512;
+
+__global__ void __launch_bounds__(kLoadThreads)
     load_tokens_kernel(ControlsView c, SlotIds slots, const int64_t* __restrict__ tokens, int64_t total,
                        const int* __restrict__ cu, const int* __restrict__ n_prompt) {
-  const int i = blockIdx.x;
+  __shared__ __align__(16) int cnt[kSpan];
+  __shared__ uint32_t seen[kSpan / 32];
+  const int i = blockIdx.y, v0 = blockIdx.x * kSpan, n_v = min(kSpan, c.V - v0);
+  pdl_wait();
+  pdl_trigger();
   const int64_t slot = slot_of(slots, i);
   if (slot < 0 || slot >= c.R) return;
-  uint32_t* seen = c.seen + slot * c.W;
-  int* counts = c.counts + slot * c.V;
-  for (int v = threadIdx.x; v < c.W; v += blockDim.x) seen[v] = 0u;
-  for (int v = threadIdx.x; v < c.V; v += blockDim.x) counts[v] = 0;
-  __syncthreads();
+  for (int v = threadIdx.x; v < kSpan / 4; v += kLoadThreads) reinterpret_cast<int4*>(cnt)[v] = make_int4(0, 0, 0, 0);
+  for (int v = threadIdx.x; v < kSpan / 32; v += kLoadThreads) seen[v] = 0u;
   const int64_t t0 = max(0, cu[i]);
   const int n = (int)(min((int64_t)cu[i + 1], total) - t0), np = n_prompt[i];
-  for (int j = threadIdx.x; j < n; j += blockDim.x) {
-    const int64_t tok = tokens[t0 + j];
-    if (tok < 0 || tok >= c.V) continue;
-    atomicOr(&seen[tok / 32], 1u << (tok % 32));
-    if (j >= np) atomicAdd(&counts[tok], 1);
+  __syncthreads();
+#pragma unroll 4
+  for (int j = threadIdx.x; j < n; j += kLoadThreads) {
+    const int64_t v = tokens[t0 + j] - v0;
+    if (v < 0 || v >= n_v) continue;
+    atomicOr(&seen[v / 32], 1u << (v % 32));
+    if (j >= np) atomicAdd(&cnt[v], 1);
+  }
+  __syncthreads();
+  int* dst = c.counts + slot * c.V + v0;
+  if (n_v % 4 == 0 && reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
+    for (int v = threadIdx.x; v < n_v / 4; v += kLoadThreads) reinterpret_cast<int4*>(dst)[v] = reinterpret_cast<int4*>(cnt)[v];
+  } else {
+    for (int v = threadIdx.x; v < n_v; v += kLoadThreads) dst[v] = cnt[v];
+  }
+  for (int v = threadIdx.x; v < (n_v + 31) / 32; v += kLoadThreads) c.seen[slot * c.W + v0 / 32 + v] = seen[v];
+}
+
+// ─── controls ──────────────────────────────────────────────────────────────
+// A CTA owns kChunk entries of one row (whole words of both bit rows). The bits say which entries change: the counts
+// and, in place, the logits are read only there, so a call costs V / 8 bytes a bit row and the entries it rewrites;
+// out of place it is one read and one write of the row.
+constexpr int kChunk = 4096;
+
+template <typename T, bool IN_PLACE, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+    controls_kernel(const T* logits, int64_t ls, ControlsView c, SlotIds slots,
+                    const int64_t* __restrict__ fresh, const int* __restrict__ done, float* out, int64_t os) {
+  const int b = blockIdx.y, v0 = blockIdx.x * kChunk, v1 = min(c.V, v0 + kChunk);
+  pdl_wait();
+  pdl_trigger();
+  const int64_t slot = slot_of(slots, b);
+  const bool on = slot >= 0 && slot < c.R;
+  if (IN_PLACE && !on) return;
+  const int64_t r = on ? slot : 0;
+  int* counts = c.counts + r * c.V;
+  uint32_t* seen = c.seen + r * c.W;
+  if (on && fresh) {
+    const int64_t tok = done && done[b] ? -1 : fresh[b];
+    const bool mine = tok >= v0 && tok < v1;
+    if (mine && threadIdx.x == 0) {
+      counts[tok] += 1;
+      seen[tok / 32] |= 1u << (tok % 32);
+    }
+    if (mine) __syncthreads();  // this CTA alone reads the token's count and word
+  }
+  const float rep = c.repetition[r], freq = c.frequency[r], pres = c.presence[r];
+  const bool penal = on && (rep != 1.f || freq != 0.f || pres != 0.f);
+  const bool masked = on && c.mask_on[r] != 0;
+  const T* z = logits + b * ls;
+  float* o = out + b * os;
+  auto control = [&](float x, int v, bool was_seen, bool allowed) {
+    if (was_seen) {
+      const float n = (float)counts[v];
+      x = x > 0.f ? x / rep : x * rep;
+      x = x - freq * n - (n > 0.f ? pres : 0.f);
+    }
+    return allowed ? x : -INFINITY;
+  };
+  constexpr int E = VEC ? 4 : 1;  // entries of a step
+#pragma unroll
+  for (int k = 0; k < kChunk / (E * kThreads); ++k) {
+    const int v = v0 + (k * kThreads + threadIdx.x) * E;
+    if (v >= v1) break;
+    const uint32_t field = (1u << E) - 1u;
+    const uint32_t s = penal ? (seen[v / 32] >> (v % 32)) & field : 0u;
+    const uint32_t a = masked ? (c.mask[r * c.W + v / 32] >> (v % 32)) & field : field;
+    if (IN_PLACE && s == 0u && a == field) continue;
+    float x[E];
+    if constexpr (VEC && sizeof(T) == 4) {
+      const float4 u = *reinterpret_cast<const float4*>(z + v);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+    } else if constexpr (VEC) {
+      const uint2 u = *reinterpret_cast<const uint2*>(z + v);
+      const float2 p = unpack_bf16x2(u.x), q = unpack_bf16x2(u.y);
+      x[0] = p.x, x[1] = p.y, x[2] = q.x, x[3] = q.y;
+    } else if constexpr (sizeof(T) == 4) {
+      x[0] = z[v];
+    } else {
+      x[0] = __bfloat162float(z[v]);
+    }
+    if (s != 0u || a != field) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = control(x[e], v + e, (s >> e) & 1u, (a >> e) & 1u);
+    }
+    if constexpr (VEC)
+      *reinterpret_cast<float4*>(o + v) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+      o[v] = x[0];
+  }
+  // biases, on what this CTA has written (ids of a row are distinct; a masked entry stays -inf)
+  if (!on || c.K == 0) return;
+  __syncthreads();
+  for (int j = threadIdx.x; j < c.K; j += kThreads) {
+    const int v = c.bias_ids[r * c.K + j];
+    if (v >= v0 && v < v1) o[v] += c.bias_vals[r * c.K + j];
   }
 }
 
-// One CTA per row.
-__global__ void __launch_bounds__(1024)
-    controls_kernel(const void* __restrict__ logits, bool is_bf16, int64_t ls, ControlsView c, SlotIds slots,
-                    const int64_t* __restrict__ fresh, const int* __restrict__ done, float* __restrict__ out,
-                    int64_t os) {
-  const int b = blockIdx.x;
-  const int64_t slot = slot_of(slots, b);
-  const bool on = slot >= 0 && slot < c.R;
-  const int64_t r = on ? slot : 0;
-  if (on && fresh && threadIdx.x == 0 && !(done && done[b])) {
-    const int64_t tok = fresh[b];
-    if (tok >= 0 && tok < c.V) {
-      c.counts[r * c.V + tok] += 1;
-      c.seen[r * c.W + tok / 32] |= 1u << (tok % 32);
-    }
-  }
-  __syncthreads();
-  for (int v = threadIdx.x; v < c.V; v += blockDim.x) {
-    float z = is_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(logits)[b * ls + v])
-                      : reinterpret_cast<const float*>(logits)[b * ls + v];
-    if (on) {
-      if ((c.seen[r * c.W + v / 32] >> (v % 32)) & 1u) {
-        const float rep = c.repetition[r];
-        const float n = (float)c.counts[r * c.V + v];
-        z = z > 0.f ? z / rep : z * rep;
-        z = z - c.frequency[r] * n - (n > 0.f ? c.presence[r] : 0.f);
-      }
-      for (int j = 0; j < c.K; ++j)
-        if (c.bias_ids[r * c.K + j] == v) z += c.bias_vals[r * c.K + j];
-      if (c.mask_on[r] && !((c.mask[r * c.W + v / 32] >> (v % 32)) & 1u)) z = -INFINITY;
-    }
-    out[b * os + v] = z;
-  }
+template <typename T>
+void launch_controls(const void* logits, int64_t ls, ControlsView c, SlotIds slots, const int64_t* fresh, const int* done,
+                     int B, float* out, int64_t os, cudaStream_t st) {
+  const T* z = reinterpret_cast<const T*>(logits);
+  const dim3 grid((c.V + kChunk - 1) / kChunk, B);
+  // four entries at a time where every row starts on a boundary of four and ends on one
+  const bool vec = c.V % 4 == 0 && (B == 1 || (ls % 4 == 0 && os % 4 == 0)) &&
+                   reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool in_place = logits == out;
+  auto go = [&](auto k) { launch_pdl(k, grid, dim3(kThreads), 0, st, z, ls, c, slots, fresh, done, out, os); };
+  if (in_place)
+    vec ? go(controls_kernel<T, true, true>) : go(controls_kernel<T, true, false>);
+  else
+    vec ? go(controls_kernel<T, false, true>) : go(controls_kernel<T, false, false>);
 }
 
 }  // namespace
@@ -75,15 +155,19 @@ __global__ void __launch_bounds__(1024)
 void load_tokens(ControlsView c, SlotIds slots, const int64_t* tokens, int64_t total, const int* cu, const int* n_prompt, int n,
                  cudaStream_t st) {
   if (n == 0) return;
-  load_tokens_kernel<<<n, 1024, 0, st>>>(c, slots, tokens, total, cu, n_prompt);
-  MESHY_CUDA_CHECK(cudaGetLastError());
+  MESHY_CHECK(n <= 65535, "load_tokens: at most 65535 rows");
+  launch_pdl(load_tokens_kernel, dim3((c.V + kSpan - 1) / kSpan, n), dim3(kLoadThreads), 0, st, c, slots, tokens, total, cu,
+             n_prompt);
 }
 
 void apply_logit_controls(const void* logits, bool is_bf16, int64_t ls, ControlsView c, SlotIds slots,
                           const int64_t* fresh, const int* done, int B, float* out, int64_t os, cudaStream_t st) {
   if (B == 0) return;
-  controls_kernel<<<B, 1024, 0, st>>>(logits, is_bf16, ls, c, slots, fresh, done, out, os);
-  MESHY_CUDA_CHECK(cudaGetLastError());
+  MESHY_CHECK(B <= 65535, "apply_logit_controls: at most 65535 rows");
+  if (is_bf16)
+    launch_controls<bf16>(logits, ls, c, slots, fresh, done, B, out, os, st);
+  else
+    launch_controls<float>(logits, ls, c, slots, fresh, done, B, out, os, st);
 }
 
 }  // namespace meshy

@@ -41,10 +41,11 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTok = 16;                       // tokens of a tile
 constexpr int kHeads = 8;                      // query heads of a segment
-constexpr int kStages = 3;
+constexpr int kStages = 2;
+constexpr uint32_t kWholeUnits = 40;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBoost = 64.f;                 // x of the largest p and a' right after the reference moved
-constexpr float kMaxP = 128.f, kMaxW = 256.f;  // x = p w stays below 2^15
+constexpr float kBoost = 2048.f;               // x of the largest p and a' right after the reference moved
+constexpr float kGrowP = 8.f, kGrowA = 2.f;    // how far either may pass it: x stays below 2^15
 constexpr float kMinA = 5.9604645e-8f;         // 2^-24, the smallest fp16
 
 template <int HD, int NT>  // NT tiles to a unit
@@ -59,7 +60,9 @@ struct Cfg {
   static constexpr int WARP = kStages * STAGE;
   static constexpr int Q = kWarps * WARP;
   static constexpr int QBYTES = kHeads * HD * 2;
-  static constexpr int SMEM = Q + 2 * QBYTES;
+  static constexpr int F = Q + 2 * QBYTES;               // two sets of query fragments: matrix B, sums (B too), factors
+  static constexpr int F_SUM = 32 * 16 * (HD / 32), F_FACTOR = F_SUM + 2 * 32 * 4, FBYTES = F_FACTOR + kHeads * 4;
+  static constexpr int SMEM = F + 2 * FBYTES;
   static constexpr int PART = HD + 4;                    // floats of a head in the workspace: sums, maximum, normaliser
 };
 
@@ -108,6 +111,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -172,14 +181,24 @@ struct Walk {
   }
 };
 
-// The share of CTA c of n: total / n units, the first total % n CTAs one more.
+// CTA c of n has units [begin(c), begin(c + 1)): total / n each, and the rest spread evenly (so that equal segments are
+// cut alike).
 struct Shares {
-  uint32_t per, more;
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + min(c, more); }
+  uint32_t total, n, per, more;
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + c * more / n; }
   __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
-    const uint32_t big = more * (per + 1);
-    return unit < big ? unit / (per + 1) : more + (unit - big) / per;
+    uint32_t c = min(n - 1, (uint32_t)((float)unit / (float)total * (float)n));
+    while (c + 1 < n && begin(c + 1) <= unit) ++c;
+    while (begin(c) > unit) --c;
+    return c;
   }
+};
+
+// A segment (b, h) that the CTA has a piece of: its first unit and its units; then the CTAs that share it.
+struct Piece {
+  int b, h;
+  uint32_t first, n;
+  bool last;  // this CTA arrived last
 };
 
 template <int HD, int NT>
@@ -191,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
   __shared__ uint32_t scan[kWarps], s_begin;
-  __shared__ int s_row, s_last;
+  __shared__ int s_row;
+  __shared__ Piece s_piece[2];
   __shared__ const float* so[kWarps];  // the warps' states
   __shared__ W s_cur, s_ahead[kWarps];  // touched once per segment: kept out of the registers
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -222,9 +242,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
   };
   for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
   const uint32_t all = total;
-  const uint32_t n_cta = min(gridDim.x, (all + kWarps - 1) / kWarps);
+  // a CTA per segment where that makes a few steps of every warp; else as many CTAs as give each warp a unit
+  const uint32_t segments = a.B * per_row;
+  const uint32_t n_cta = min(gridDim.x, all <= segments * kWholeUnits ? segments : (all + kWarps - 1) / kWarps);
   if (blockIdx.x >= n_cta) return;
-  const Shares shares{all / n_cta, all % n_cta};
+  const Shares shares{all, n_cta, all / n_cta, all % n_cta};
   const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
   if (a.B > kThreads) total = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
@@ -268,6 +290,43 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     if (i < min(kHeads, a.rep - h0))
       copy16(smem_u32(smem) + C::Q + buf * C::QBYTES + tid * 16,
              a.q + w.b * a.qs + (int64_t)(w.h / a.blocks * a.rep + h0 + i) * a.qh + (tid % (HD / 8)) * 8, true);
+  };
+  // A segment's query rows as matrix fragments, a warp per head: scaled so that the largest is in [2^14, 2^15), a
+  // word's channels 0 .. 7 as fp16 pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16; the sums over the groups' channels in
+  // units of 2^8 as three fp16 terms, against the bases; the factor that takes all that back, with the softmax scale.
+  auto prepare_q = [&](const W& w, int buf) {
+    static_assert(kWarps == kHeads, "a warp per head");
+    constexpr int CH = HD / 32;  // channels of a lane
+    uint8_t* f = smem + C::F + buf * C::FBYTES;
+    const bool real = (w.h % a.blocks) * kHeads + warp < a.rep;
+    float x[CH], mx = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      x[i] = real ? __bfloat162float(reinterpret_cast<const bf16*>(smem + C::Q + buf * C::QBYTES)[warp * HD + lane * CH + i]) : 0.f;
+      mx = fmaxf(mx, fabsf(x[i]));
+      sum += x[i];
+    }
+    mx = warp_max(mx);
+    const int ex = (mx > 0.f && mx < INFINITY) ? min(14 - ilogbf(mx), 126) : 0;
+    const float up = ldexpf(1.f, ex);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int ch = lane * CH + i, word = (ch % 64) / 8 * G + ch / 64, e = ch % 8;
+      reinterpret_cast<__half*>(f)[(((word % KW) * 32 + warp * 4 + word / KW) * 4 + e % 4) * 2 + e / 4] =
+          __float2half_rn(x[i] * (e % 2 ? up * 0.0625f : up));
+    }
+#pragma unroll
+    for (int o = 1; o < 64 / CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float y0 = __shfl_sync(0xffffffffu, sum, i * 16) * up * 0.00390625f;
+      const __half h0 = __float2half_rn(y0);
+      const float y1 = y0 - __half2float(h0);
+      const __half h1 = __float2half_rn(y1), h2 = __float2half_rn(y1 - __half2float(h1));
+      const __half h = lane == 0 ? h0 : lane == 1 ? h1 : lane == 2 ? h2 : __float2half_rn(0.f);
+      if (lane < 4) reinterpret_cast<uint32_t*>(f + C::F_SUM)[i * 32 + warp * 4 + lane] = (uint32_t)__half_as_ushort(h) << 16;
+    }
+    if (lane == 0) reinterpret_cast<float*>(f + C::F_FACTOR)[warp] = ldexpf(sl2, 24 - ex);
   };
   copy_q(s_cur, 0);
   copies_commit();
@@ -337,81 +396,42 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(ring + i * C::STAGE, i);
   uint32_t stage = ring, ahead = ring + (kStages - 1) * C::STAGE;
-  copies_wait<kStages - 1>();  // Q
+  copies_wait<kStages - 1>();  // the query rows
   __syncthreads();
-  int q_at = 0;
+  prepare_q(s_cur, 0);
+  __syncthreads();
+  int q_at = 0, pieces = 0;
 
+  W then = s_cur;
   while (true) {
-    const W cur = s_cur;
+    const W cur = then;
     const int hk = cur.h / a.blocks, h0 = (cur.h % a.blocks) * kHeads;
     const int nh = min(kHeads, a.rep - h0);
     const int b = cur.b;
     const int u_end = cur.n ? cur.last : 0;
 
-    // Q fragments: head g, channels of the words this lane reads of a K row; scaled so that the largest is in [2^14, 2^15)
-    uint32_t qf[KW][4];
-    float cs[2], qs[2][G];
-    {
-      float x[KW][8], mx = 0.f, sum[G];
+    const uint8_t* frags = smem + C::F + q_at * C::FBYTES;
+    uint32_t zf[2] = {0u, 0u};
+    float cs[2], ce[2];
 #pragma unroll
-      for (int i = 0; i < G; ++i) sum[i] = 0.f;
-      const bf16* src = reinterpret_cast<const bf16*>(smem + C::Q + q_at * C::QBYTES) + g * HD;
+    for (int i = 0; i < G; ++i) zf[i] = reinterpret_cast<const uint32_t*>(frags + C::F_SUM)[i * 32 + lane];
 #pragma unroll
-      for (int j = 0; j < KW; ++j) {
-        const int w = KW * t + j;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (g < nh) u = *reinterpret_cast<const uint4*>(src + 64 * (w % G) + 8 * (w / G));
-        const uint32_t us[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16x2(us[e]);
-          x[j][2 * e] = f.x;
-          x[j][2 * e + 1] = f.y;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          mx = fmaxf(mx, fabsf(x[j][e]));
-          sum[j % G] += x[j][e];
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-#pragma unroll
-        for (int i = 0; i < G; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-      }
-      const int ex = (mx > 0.f && mx < INFINITY) ? min(14 - ilogbf(mx), 126) : 0;
-      const float f = ldexpf(1.f, ex), c = ldexpf(sl2, 24 - ex);
-#pragma unroll
-      for (int j = 0; j < KW; ++j) {
-        qf[j][0] = pack_half2(x[j][0] * f, x[j][4] * f);
-        qf[j][1] = pack_half2(x[j][1] * f * 0.0625f, x[j][5] * f * 0.0625f);
-        qf[j][2] = pack_half2(x[j][2] * f, x[j][6] * f);
-        qf[j][3] = pack_half2(x[j][3] * f * 0.0625f, x[j][7] * f * 0.0625f);
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        cs[r] = __shfl_sync(0xffffffffu, c, (2 * t + r) * 4);
-#pragma unroll
-        for (int i = 0; i < G; ++i) qs[r][i] = __shfl_sync(0xffffffffu, sum[i], (2 * t + r) * 4) * sl2;
-      }
+    for (int r = 0; r < 2; ++r) {
+      cs[r] = reinterpret_cast<const float*>(frags + C::F_FACTOR)[2 * t + r];
+      ce[r] = cs[r] * 1.52587890625e-5f;  // the sums are in units of 2^8, the products in 2^24
     }
-
-    float o[G][4][4], z[G][2], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, inv[G];
-    float limit = -1.f;  // of p; below 0: no reference yet
+    const uint32_t f_at = smem_u32(frags) + lane * 16;
+    // o, z and l are relative to the reference m: p 2^-m; m < the true maximum, so that x fits fp16 well
+    float o[G][4][4], z[G][2], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+    float lim_p = -1.f, lim_a = kMinA * kGrowA;  // lim_p below 0: no reference yet
 #pragma unroll
     for (int i = 0; i < G; ++i) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
       z[i][0] = z[i][1] = 0.f;
-      inv[i] = kBoost / kMinA;
     }
-
-    if (cur.left > cur.last - cur.first) {  // the next segment's query rows
-      W w = cur;
-      w.next(a);
-      copy_q(w, q_at ^ 1);
-    }
+    const bool more = then.next(a);
+    if (more) copy_q(then, q_at ^ 1);
     int steps = 0;
     for (int unit = cur.first + warp; unit < u_end; unit += kWarps) {
       __syncwarp();  // every lane has read the stage that is filled again
@@ -425,110 +445,129 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
       const int count = valid & 1u ? cur.n - unit * C::UTOK : 0;
       valid >>= 1;
       ++steps;
+      // scores: tile n, row g + 8 i, head 2 t + r
+      float s[NT][2][2], va[NT][2][G], vz[NT][2][G];
+      {
+        uint32_t kw[NT][2][KW];
+        float acc[NT][G][4];
 #pragma unroll
-      for (int half = 0; half < NT; ++half) {
-        uint32_t kw[2][KW], vw[4][G], sw[2][2 * G];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) load_words<KW>(kw[i], here + k_at + (2 * half + i) * 8 * C::ROW);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], here + s_at + (2 * half + i) * 8 * C::PAIRS);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<G>(vw[i], here + v_at + (4 * half + i) * 4 * C::ROW);
-        float acc[G][4];
+          for (int i = 0; i < 2; ++i) load_words<KW>(kw[n][i], here + k_at + (2 * n + i) * 8 * C::ROW);
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
-          uint32_t w0 = kw[0][j], w1 = kw[1][j];
-          if (j < G)
-            mma_f16_first(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
-          else
-            mma_f16(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
-          w0 >>= 8;
-          w1 >>= 8;
-          mma_f16(acc[j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2], qf[j][3]);
-        }
-        // scores: [row g + 8 i][head 2 t + r], base 2, relative to the reference
-        float s[2][2], va[2][G], vz[2][G];
+          uint32_t qf[4];
+          load_words<4>(qf, f_at + j * 512);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float d[2] = {0.f, 0.f}, e[2] = {-m[0], -m[1]};
-#pragma unroll
-          for (int j = 0; j < G; ++j) {
-            const float2 k2 = unpack_half2(sw[i][j]), v2 = unpack_half2(sw[i][G + j]);
-            va[i][j] = v2.x;
-            vz[i][j] = v2.y;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              d[r] = fmaf(k2.x, acc[j][2 * i + r], d[r]);
-              e[r] = fmaf(k2.y, qs[r][j], e[r]);
-            }
+          for (int n = 0; n < NT; ++n) {
+            uint32_t w0 = kw[n][0][j], w1 = kw[n][1][j];
+            if (j < G)
+              mma_f16_first(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[0], qf[1]);
+            else
+              mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[0], qf[1]);
+            w0 >>= 8;
+            w1 >>= 8;
+            mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[2], qf[3]);
           }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) s[i][r] = fmaf(cs[r], d[r], e[r]);
         }
-        if (count < (half + 1) * kTok) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t sw[2][2 * G];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], here + s_at + (2 * n + i) * 8 * C::PAIRS);
+          float e[4];  // sum_g z_g sum(q_g): the pairs (a, z) against (0, sum)
+          mma_f16_first(e, sw[0][0], sw[1][0], G == 2 ? sw[0][G - 1] : 0u, G == 2 ? sw[1][G - 1] : 0u, zf[0], zf[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float d[2] = {0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+              const float ka = __low2float(*reinterpret_cast<const __half2*>(&sw[i][j]));
+              const float2 v2 = unpack_half2(sw[i][G + j]);
+              va[n][i][j] = v2.x;
+              vz[n][i][j] = v2.y;
+              d[0] = fmaf(ka, acc[n][j][2 * i], d[0]);
+              d[1] = fmaf(ka, acc[n][j][2 * i + 1], d[1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) s[n][i][r] = fmaf(cs[r], d[r], fmaf(ce[r], e[2 * i + r], -m[r]));
+          }
+        }
+      }
+      if (count < C::UTOK) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (half * kTok + tok_g + 8 * i >= count) {
-              s[i][0] = s[i][1] = -INFINITY;
+            if (n * kTok + tok_g + 8 * i >= count) {
+              s[n][i][0] = s[n][i][1] = -INFINITY;
 #pragma unroll
-              for (int j = 0; j < G; ++j) va[i][j] = vz[i][j] = 0.f;
+              for (int j = 0; j < G; ++j) va[n][i][j] = vz[n][i][j] = 0.f;
             }
-        }
-        float p[2][2], w[2][G], top_p = 0.f, top_w = 0.f;
+      }
+      float p[NT][2][2], top_p = 0.f, top_a = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            p[i][r] = ex2(s[i][r]);
-            top_p = fmaxf(top_p, p[i][r]);
+            p[n][i][r] = ex2(s[n][i][r]);
+            top_p = fmaxf(top_p, p[n][i][r]);
           }
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            w[i][j] = va[i][j] * inv[j];
-            top_w = fmaxf(top_w, w[i][j]);
-          }
+          for (int j = 0; j < G; ++j) top_a = fmaxf(top_a, va[n][i][j]);
         }
-        if (__any_sync(0xffffffffu, top_p > limit || top_w > kMaxW)) {
-          // move the reference to the true maxima
-          float keep[2];
-          bool found = false;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float mt = max_over_rows(fmaxf(s[0][r], s[1][r])) + m[r];
-            const float mn = limit < 0.f ? mt : fmaxf(m[r], mt);
-            keep[r] = limit < 0.f ? 0.f : ex2(m[r] - mn);
-            const float shift = mn == -INFINITY ? 0.f : m[r] - mn;
-            found |= mn != -INFINITY;
-            if (mn != -INFINITY) m[r] = mn;
-            l[r] *= keep[r];
-            p[0][r] = ex2(s[0][r] + shift);
-            p[1][r] = ex2(s[1][r] + shift);
-          }
-          if (__any_sync(0xffffffffu, found)) limit = kMaxP;
-#pragma unroll
-          for (int j = 0; j < G; ++j) {
-            const float to = fminf(inv[j], kBoost / fmaxf(max_over_rows(fmaxf(va[0][j], va[1][j])), kMinA)), f = to / inv[j];
-            inv[j] = to;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) o[j][q][x] *= f * keep[x & 1];
-            z[j][0] *= keep[0];
-            z[j][1] *= keep[1];
-            w[0][j] = va[0][j] * inv[j];
-            w[1][j] = va[1][j] * inv[j];
-          }
-        }
+      if (__any_sync(0xffffffffu, top_p > lim_p || top_a > lim_a)) {
+        // move the reference: to the true maxima, less what brings x to kBoost
+        const float A0 = lim_a / kGrowA, A = max_over_rows(fmaxf(A0, top_a)), lift = lg2(kBoost / A);
+        bool found = false;
+        float keep[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          l[r] += p[0][r] + p[1][r];
+          float top = s[0][0][r];
 #pragma unroll
-          for (int j = 0; j < G; ++j) z[j][r] = fmaf(p[0][r], vz[0][j], fmaf(p[1][r], vz[1][j], z[j][r]));
+          for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][0][r], s[n][1][r]));
+          top = max_over_rows(top) + m[r];
+          if (lim_p > 0.f) top = fmaxf(top, m[r] + lg2(kBoost / A0));
+          const bool real = top != -INFINITY;
+          const float to = real ? top - lift : m[r];
+          keep[r] = lim_p > 0.f ? ex2(m[r] - to) : 0.f;
+          found |= real;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) p[n][i][r] = ex2(s[n][i][r] + (m[r] - to));
+          m[r] = to;
+          l[r] *= keep[r];
+        }
+        if (__any_sync(0xffffffffu, found)) lim_p = kBoost / A * kGrowP;
+        lim_a = A * kGrowA;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[j][q][x] *= keep[x & 1];
+          z[j][0] *= keep[0];
+          z[j][1] *= keep[1];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t vw[4][G];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_words<G>(vw[i], here + v_at + (4 * n + i) * 4 * C::ROW);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          l[r] += p[n][0][r] + p[n][1][r];
+#pragma unroll
+          for (int j = 0; j < G; ++j) z[j][r] = fmaf(p[n][0][r], vz[n][0][j], fmaf(p[n][1][r], vz[n][1][j], z[j][r]));
         }
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-          const uint32_t b0 = transpose8x8(pack_half2(p[0][0] * w[0][j], p[0][1] * w[0][j]));
-          const uint32_t b1 = transpose8x8(pack_half2(p[1][0] * w[1][j], p[1][1] * w[1][j]));
+          const uint32_t b0 = transpose8x8(pack_half2(p[n][0][0] * va[n][0][j], p[n][0][1] * va[n][0][j]));
+          const uint32_t b1 = transpose8x8(pack_half2(p[n][1][0] * va[n][1][j], p[n][1][1] * va[n][1][j]));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half ..
             const uint32_t sel = half ? 0x7632u : 0x5410u;
@@ -550,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < G; ++j) {
         z[j][r] = sum_over_rows(z[j][r]);
-        const float f0 = 16777216.f / inv[j], f1 = 1048576.f / inv[j];
+        constexpr float f0 = 16777216.f, f1 = 1048576.f;
         float x[8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -562,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
         d[1] = make_float4(x[4], x[5], x[6], x[7]);
       }
       if (g == 0) {
-        sm[warp][2 * t + r] = limit < 0.f ? -INFINITY : m[r];
+        sm[warp][2 * t + r] = lim_p < 0.f ? -INFINITY : m[r];
         sl[warp][2 * t + r] = l[r];
       }
     }
@@ -597,69 +636,77 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
         if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(M, L);
       }
     }
-    if (!whole) {
-      const uint32_t c0 = shares.owner(seg0);  // the CTAs that share the segment
-      const int np = (int)(shares.owner(seg0 + cur.U - 1) - c0) + 1;
-      unsigned* ctr = a.arrived + (int64_t)b * per_row + cur.h;
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(ctr, 1u) == (unsigned)(np - 1);
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        // the pieces' maximum and normaliser, a warp per head; then their sum, a few loads under way at a time
-        const float* p0 = a.part + (int64_t)c0 * 2 * kHeads * C::PART;
-        auto piece = [&](int c, int h) { return p0 + ((2 * c + (c == 0 ? 1 : 0)) * kHeads + h) * C::PART; };
-        static_assert(kWarps == kHeads, "a warp per head");
-        if (warp < nh) {
-          float M = -INFINITY, L = 0.f;
-          for (int c = lane; c < np; c += 32) M = fmaxf(M, __ldcg(piece(c, warp) + HD));
-          M = warp_max(M);
-          for (int c = lane; c < np; c += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(c, warp) + HD));
-            L = fmaf(ml.y, ml.x == -INFINITY ? 0.f : ex2(ml.x - M), L);
-          }
-          L = warp_sum(L);
-          if (lane == 0) {
-            sm[0][warp] = M;
-            sl[0][warp] = L;
-          }
-        }
-        __syncthreads();
-        for (int i = tid; i < nh * (HD / 4); i += kThreads) {
-          const int h = i / (HD / 4), ch = 4 * (i % (HD / 4));
-          const float M = sm[0][h], L = sl[0][h];
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int c = 0; c < np; ++c) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(c, h) + ch));
-            const float m1 = __ldcg(piece(c, h) + HD), e = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-            x.x = fmaf(v.x, e, x.x);
-            x.y = fmaf(v.y, e, x.y);
-            x.z = fmaf(v.z, e, x.z);
-            x.w = fmaf(v.w, e, x.w);
-          }
-          const float e = L == 0.f ? 0.f : 1.f / L;
-          *reinterpret_cast<uint2*>(dst + (int64_t)h * HD + ch) =
-              make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
-        }
-        if (tid == 0) *ctr = 0u;
-      }
+    if (!whole) {  // at most the first and the last segment of the share
+      if (tid == 0) s_piece[pieces] = {b, cur.h, seg0, (uint32_t)cur.U, false};
+      ++pieces;
     }
+    if (!more) break;
     seg0 += cur.U;
-    if (cur.left <= cur.last - cur.first) break;
-    __syncthreads();  // the states have been read
-    if (tid == 0) {
-      W w = cur;
-      w.next(a);
-      s_cur = w;
-    }
     q_at ^= 1;
-    __syncthreads();
+    prepare_q(then, q_at);
+    __syncthreads();  // the states have been read, the fragments are there
   }
   copies_wait<0>();
+  if (pieces == 0) return;
+  // The last CTA to arrive at a segment joins its pieces; arrivals wait until the share is done, so that nothing else
+  // waits for their round trip.
+  __syncthreads();
+  if (tid < pieces) {
+    Piece& x = s_piece[tid];
+    const uint32_t c0 = shares.owner(x.first), np = shares.owner(x.first + x.n - 1) - c0 + 1;
+    x.first = c0;
+    x.n = np;
+    unsigned* ctr = a.arrived + (int64_t)x.b * per_row + x.h;
+    unsigned old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(ctr) : "memory");
+    x.last = old == np - 1;
+    if (x.last) *ctr = 0u;
+  }
+  __syncthreads();
+  for (int i = tid; i < pieces * kHeads * (HD / 4); i += kThreads) {
+    const Piece& x = s_piece[i / (kHeads * (HD / 4))];
+    const int h = i / (HD / 4) % kHeads, ch = 4 * (i % (HD / 4)), hk = x.h / a.blocks, h0 = (x.h % a.blocks) * kHeads;
+    if (!x.last || h0 + h >= a.rep) continue;
+    const float* p0 = a.part + ((int64_t)x.first * 2 * kHeads + h) * C::PART;
+    const int np = x.n;
+    float M = -INFINITY, L = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kBatch = 8;
+    for (int c0 = 0; c0 < np; c0 += kBatch) {
+      float4 v[kBatch];
+      float2 ml[kBatch];
+      float Mn = M;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int c = c0 + k;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < np) {
+          const float* pp = p0 + (2 * c + (c == 0 ? 1 : 0)) * kHeads * C::PART;
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(pp + HD));
+          v[k] = __ldcg(reinterpret_cast<const float4*>(pp + ch));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) Mn = fmaxf(Mn, ml[k].x);
+      const float keep = M == -INFINITY ? 0.f : ex2(M - Mn);
+      L *= keep;
+      y.x *= keep, y.y *= keep, y.z *= keep, y.w *= keep;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float e = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - Mn);
+        L = fmaf(ml[k].y, e, L);
+        y.x = fmaf(v[k].x, e, y.x);
+        y.y = fmaf(v[k].y, e, y.y);
+        y.z = fmaf(v[k].z, e, y.z);
+        y.w = fmaf(v[k].w, e, y.w);
+      }
+      M = Mn;
+    }
+    const float e = L == 0.f ? 0.f : 1.f / L;
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)x.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
+        make_uint2(pack_bf16x2(y.x * e, y.y * e), pack_bf16x2(y.z * e, y.w * e));
+  }
 }
 
 int sm_count() {
