@@ -59,6 +59,26 @@ __global__ void __launch_bounds__(kLoadThreads)
 // out of place it is one read and one write of the row.
 constexpr int kChunk = 4096;
 
+template <int E>
+__device__ __forceinline__ void load_entries(float* x, const float* p) {
+  if constexpr (E == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+  } else {
+    x[0] = *p;
+  }
+}
+template <int E>
+__device__ __forceinline__ void load_entries(float* x, const bf16* p) {
+  if constexpr (E == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+  } else {
+    x[0] = __bfloat162float(*p);
+  }
+}
+
 template <typename T, bool IN_PLACE, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     controls_kernel(const T* logits, int64_t ls, ControlsView c, SlotIds slots,
@@ -66,6 +86,19 @@ __global__ void __launch_bounds__(kThreads)
   const int b = blockIdx.y, v0 = blockIdx.x * kChunk, v1 = min(c.V, v0 + kChunk);
   pdl_wait();
   pdl_trigger();
+  const T* z = logits + b * ls;
+  float* o = out + b * os;
+  constexpr int E = VEC ? 4 : 1, STEPS = kChunk / (E * kThreads);  // entries of a step
+  constexpr int BATCH = 4;                                         // steps whose loads are under way together
+  constexpr uint32_t FIELD = (1u << E) - 1u;
+  float x[BATCH][E];
+  auto place = [&](int k) { return v0 + (k * kThreads + (int)threadIdx.x) * E; };
+  auto load_batch = [&](int k0) {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (place(k0 + k) < v1) load_entries<E>(x[k], z + place(k0 + k));
+  };
+  if (!IN_PLACE) load_batch(0);  // on their way while the slot is looked up
   const int64_t slot = slot_of(slots, b);
   const bool on = slot >= 0 && slot < c.R;
   if (IN_PLACE && !on) return;
@@ -84,46 +117,42 @@ __global__ void __launch_bounds__(kThreads)
   const float rep = c.repetition[r], freq = c.frequency[r], pres = c.presence[r];
   const bool penal = on && (rep != 1.f || freq != 0.f || pres != 0.f);
   const bool masked = on && c.mask_on[r] != 0;
-  const T* z = logits + b * ls;
-  float* o = out + b * os;
-  auto control = [&](float x, int v, bool was_seen, bool allowed) {
-    if (was_seen) {
-      const float n = (float)counts[v];
-      x = x > 0.f ? x / rep : x * rep;
-      x = x - freq * n - (n > 0.f ? pres : 0.f);
-    }
-    return allowed ? x : -INFINITY;
-  };
-  constexpr int E = VEC ? 4 : 1;  // entries of a step
+  for (int k0 = 0; k0 < STEPS; k0 += BATCH) {
+    uint32_t s[BATCH], m[BATCH];  // seen; allowed
+    int n[BATCH][E];
+    if (!IN_PLACE && k0 > 0) load_batch(k0);
 #pragma unroll
-  for (int k = 0; k < kChunk / (E * kThreads); ++k) {
-    const int v = v0 + (k * kThreads + threadIdx.x) * E;
-    if (v >= v1) break;
-    const uint32_t field = (1u << E) - 1u;
-    const uint32_t s = penal ? (seen[v / 32] >> (v % 32)) & field : 0u;
-    const uint32_t a = masked ? (c.mask[r * c.W + v / 32] >> (v % 32)) & field : field;
-    if (IN_PLACE && s == 0u && a == field) continue;
-    float x[E];
-    if constexpr (VEC && sizeof(T) == 4) {
-      const float4 u = *reinterpret_cast<const float4*>(z + v);
-      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-    } else if constexpr (VEC) {
-      const uint2 u = *reinterpret_cast<const uint2*>(z + v);
-      const float2 p = unpack_bf16x2(u.x), q = unpack_bf16x2(u.y);
-      x[0] = p.x, x[1] = p.y, x[2] = q.x, x[3] = q.y;
-    } else if constexpr (sizeof(T) == 4) {
-      x[0] = z[v];
-    } else {
-      x[0] = __bfloat162float(z[v]);
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = place(k0 + k);
+      s[k] = penal && v < v1 ? seen[v / 32] : 0u;
+      m[k] = masked && v < v1 ? c.mask[r * c.W + v / 32] : ~0u;
     }
-    if (s != 0u || a != field) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = control(x[e], v + e, (s >> e) & 1u, (a >> e) & 1u);
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = place(k0 + k);
+      s[k] = (s[k] >> (v % 32)) & FIELD;
+      m[k] = (m[k] >> (v % 32)) & FIELD;
+      if (IN_PLACE && (s[k] != 0u || m[k] != FIELD) && m[k] != 0u) load_entries<E>(x[k], z + v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) n[k][e] = (s[k] >> e) & 1u ? counts[v + e] : 0;
     }
-    if constexpr (VEC)
-      *reinterpret_cast<float4*>(o + v) = make_float4(x[0], x[1], x[2], x[3]);
-    else
-      o[v] = x[0];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = place(k0 + k);
+      if (v >= v1 || (IN_PLACE && s[k] == 0u && m[k] == FIELD)) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if ((s[k] >> e) & 1u) {
+          const float y = x[k][e] > 0.f ? x[k][e] / rep : x[k][e] * rep;
+          x[k][e] = y - freq * (float)n[k][e] - (n[k][e] > 0 ? pres : 0.f);
+        }
+        if (!((m[k] >> e) & 1u)) x[k][e] = -INFINITY;
+      }
+      if constexpr (VEC)
+        *reinterpret_cast<float4*>(o + v) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+      else
+        o[v] = x[k][0];
+    }
   }
   // biases, on what this CTA has written (ids of a row are distinct; a masked entry stays -inf)
   if (!on || c.K == 0) return;

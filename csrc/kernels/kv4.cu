@@ -83,84 +83,119 @@ __device__ __forceinline__ void quantise(const uint4& u, int lane, uint32_t* row
   uint32_t word = 0;
   if (af > 0.f) {
     const float rcp = __frcp_rn(af);
+    float n[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float n = fminf(fmaxf(quotient(x[q] - zf, af, rcp), 0.f), 15.f);
-      // adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits
-      word |= (__float_as_uint(n + 12582912.f) & 15u) << (4 * q);
+    for (int q = 0; q < 8; ++q) n[q] = quotient(x[q] - zf, af, rcp);
+    // the base is rounded: only where that moved it by a good part of a step does anything leave [0, 15]
+    if (quotient(lo - zf, af, rcp) < -0.5f || quotient(hi - zf, af, rcp) >= 15.5f) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) n[q] = fminf(fmaxf(n[q], 0.f), 15.f);
     }
+    // adding 1.5 2^23 rounds to whole numbers, halves to even; four of them fit a float's 24 bits side by side
+    constexpr float kRound = 12582912.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) n[q] = (n[q] + kRound) - kRound;
+    const float h0 = fmaf(fmaf(fmaf(n[3], 16.f, n[2]), 16.f, n[1]), 16.f, n[0]);
+    const float h1 = fmaf(fmaf(fmaf(n[7], 16.f, n[6]), 16.f, n[5]), 16.f, n[4]);
+    word = __byte_perm(__float_as_uint(h0 + kRound), __float_as_uint(h1 + kRound), 0x5410);
   }
   if (row == nullptr) return;
   row[lane % 8 * G + lane / 8] = word;
   if (lane % 8 == 0) pairs[lane / 8] = __halves2half2(a, z);
 }
 
-// HD / 8 lanes per (token, head); each takes its word of K and of V.
+// HD / 8 lanes per (token, head); each takes its word of K and of V, of kRows (token, head) pairs in one go so that
+// their loads are under way together.
+constexpr int kRows = 2;
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads)
     kv4_write_kernel(const bf16* __restrict__ k, int64_t ks, int64_t kh, const bf16* __restrict__ v, int64_t vs,
                      int64_t vh, const int64_t* __restrict__ slots, uint32_t rows, KV4View c, FastDiv heads, FastDiv page) {
-  constexpr int LANES = HD / 8, G = HD / 64;
-  const uint32_t i = blockIdx.x * kThreads + threadIdx.x, lane = i % LANES;
+  constexpr int LANES = HD / 8, G = HD / 64, BLOCK = kThreads / LANES;
+  const uint32_t lane = threadIdx.x % LANES, th0 = blockIdx.x * (kRows * BLOCK) + threadIdx.x / LANES;
   pdl_wait();
   pdl_trigger();
-  const bool act = i / LANES < rows;  // the lanes of a group stay together for the shuffles
-  const uint32_t th = act ? i / LANES : 0u, t = heads.div(th), h = th - t * heads.d;
-  const uint4 uk = *reinterpret_cast<const uint4*>(k + t * ks + h * kh + lane * 8);
-  const uint4 uv = *reinterpret_cast<const uint4*>(v + t * vs + h * vh + lane * 8);
-  const int64_t r = act ? row_of(c, page, slots[t], h) : -1;
-  uint32_t* kr = r < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.k + r * (HD / 2));
-  uint32_t* vr = r < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.v + r * (HD / 2));
-  __half2* pairs = c.scale + r * (2 * G);
-  quantise<HD>(uk, lane, kr, pairs);
-  quantise<HD>(uv, lane, vr, pairs + G);
-}
-
-// Eight channels of a word: a n + z, rounded once.
-__device__ __forceinline__ uint4 restore(uint32_t w, __half2 pair) {
-  const float2 az = __half22float2(pair);
-  uint32_t o[4];
-  float x[8];
+  uint4 uk[kRows], uv[kRows];
+  int64_t r[kRows];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {  // nibbles q and q + 4 as the low bits of the fp16 numbers 1024 + n
-    const uint32_t y = ((w >> (4 * q)) & 0x000F000Fu) | 0x64006400u;
-    const float2 n = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(1024.f)));
-    x[q] = fmaf(n.x, az.x, az.y);
-    x[q + 4] = fmaf(n.y, az.x, az.y);
+  for (int u = 0; u < kRows; ++u) {
+    const bool act = th0 + u * BLOCK < rows;  // the lanes of a group stay together for the shuffles
+    const uint32_t th = act ? th0 + u * BLOCK : 0u, t = heads.div(th), h = th - t * heads.d;
+    uk[u] = *reinterpret_cast<const uint4*>(k + t * ks + h * kh + lane * 8);
+    uv[u] = *reinterpret_cast<const uint4*>(v + t * vs + h * vh + lane * 8);
+    r[u] = act ? row_of(c, page, slots[t], h) : -1;
   }
 #pragma unroll
-  for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(x[2 * q], x[2 * q + 1]);
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  for (int u = 0; u < kRows; ++u) {
+    uint32_t* kr = r[u] < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.k + r[u] * (HD / 2));
+    uint32_t* vr = r[u] < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.v + r[u] * (HD / 2));
+    __half2* pairs = c.scale + r[u] * (2 * G);
+    quantise<HD>(uk[u], lane, kr, pairs);
+    quantise<HD>(uv[u], lane, vr, pairs + G);
+  }
+}
+
+// Eight channels of a word: a n + z, rounded once. A nibble masked in place is an fp16 subnormal, n 2^-24 or n 2^-20;
+// the scale takes the power back, exactly.
+__device__ __forceinline__ uint4 restore(uint32_t w, __half2 pair) {
+  const float2 az = __half22float2(pair);
+  const float a0 = az.x * 16777216.f, a1 = az.x * 1048576.f;
+  float x[8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q, w >>= 8) {
+    const uint32_t y0 = w & 0x000F000Fu, y1 = w & 0x00F000F0u;  // nibbles 2 q, 2 q + 4; 2 q + 1, 2 q + 5
+    const float2 n0 = __half22float2(*reinterpret_cast<const __half2*>(&y0));
+    const float2 n1 = __half22float2(*reinterpret_cast<const __half2*>(&y1));
+    x[2 * q] = fmaf(n0.x, a0, az.y);
+    x[2 * q + 4] = fmaf(n0.y, a0, az.y);
+    x[2 * q + 1] = fmaf(n1.x, a1, az.y);
+    x[2 * q + 5] = fmaf(n1.y, a1, az.y);
+  }
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads)
     kv4_read_kernel(KV4View c, const int64_t* __restrict__ slots, uint32_t rows, bf16* __restrict__ k, bf16* __restrict__ v,
                     FastDiv heads, FastDiv page) {
-  constexpr int LANES = HD / 8, G = HD / 64;
-  const uint32_t i = blockIdx.x * kThreads + threadIdx.x, lane = i % LANES, th = i / LANES;
+  constexpr int LANES = HD / 8, G = HD / 64, BLOCK = kThreads / LANES;
+  const uint32_t lane = threadIdx.x % LANES, th0 = blockIdx.x * (kRows * BLOCK) + threadIdx.x / LANES;
   pdl_wait();
   pdl_trigger();
-  if (th >= rows) return;
-  const uint32_t t = heads.div(th), h = th - t * heads.d;
-  const int64_t r = row_of(c, page, slots[t], h);
-  uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
-  if (r >= 0) {
-    const int at = lane % 8 * G + lane / 8;
-    const uint32_t wk = reinterpret_cast<const uint32_t*>(c.k + r * (HD / 2))[at];
-    const uint32_t wv = reinterpret_cast<const uint32_t*>(c.v + r * (HD / 2))[at];
-    const __half2* pairs = c.scale + r * (2 * G) + lane / 8;
-    ok = restore(wk, pairs[0]);
-    ov = restore(wv, pairs[G]);
+  int64_t r[kRows];
+  uint32_t wk[kRows], wv[kRows];
+  __half2 pk[kRows], pv[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t th = th0 + u * BLOCK, t = heads.div(th), h = th - t * heads.d;
+    r[u] = th < rows ? row_of(c, page, slots[t], h) : -1;
   }
-  const int64_t to = (int64_t)th * HD + lane * 8;
-  *reinterpret_cast<uint4*>(k + to) = ok;
-  *reinterpret_cast<uint4*>(v + to) = ov;
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    wk[u] = wv[u] = 0u;
+    pk[u] = pv[u] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+    if (r[u] < 0) continue;
+    const int at = lane % 8 * G + lane / 8;
+    const __half2* pairs = c.scale + r[u] * (2 * G) + lane / 8;
+    wk[u] = reinterpret_cast<const uint32_t*>(c.k + r[u] * (HD / 2))[at];
+    wv[u] = reinterpret_cast<const uint32_t*>(c.v + r[u] * (HD / 2))[at];
+    pk[u] = pairs[0];
+    pv[u] = pairs[G];
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t th = th0 + u * BLOCK;
+    if (th >= rows) continue;
+    const int64_t to = (int64_t)th * HD + lane * 8;
+    *reinterpret_cast<uint4*>(k + to) = restore(wk[u], pk[u]);
+    *reinterpret_cast<uint4*>(v + to) = restore(wv[u], pv[u]);
+  }
 }
 
 int blocks(int64_t threads) {
   MESHY_CHECK(threads < (1LL << 31), "kv4: too many rows for one call");
-  return (int)((threads + kThreads - 1) / kThreads);
+  return (int)((threads + kRows * kThreads - 1) / (kRows * kThreads));
 }
 
 }  // namespace
