@@ -18,14 +18,14 @@ __device__ __forceinline__ int64_t slot_of(SlotIds s, int i) {
 // bytes each. A CTA owns kSpan entries of the row: it counts the row's tokens that fall among them in shared memory
 // (16-bit halves would overflow, so 32-bit) and writes its span once, coalesced; nothing is cleared or added in
 // global memory. Every CTA reads the row's whole token list, from L2 after the first.
-constexpr int kSpan = 8192;
 constexpr int kLoadThreads = 512;
 
+template <int kSpan>
 __global__ void __launch_bounds__(kLoadThreads)
     load_tokens_kernel(ControlsView c, SlotIds slots, const int64_t* __restrict__ tokens, int64_t total,
                        const int* __restrict__ cu, const int* __restrict__ n_prompt) {
-  __shared__ __align__(16) int cnt[kSpan];
-  __shared__ uint32_t seen[kSpan / 32];
+  extern __shared__ __align__(16) int cnt[];  // [kSpan], then the bits [kSpan / 32]
+  uint32_t* seen = reinterpret_cast<uint32_t*>(cnt + kSpan);
   const int i = blockIdx.y, v0 = blockIdx.x * kSpan, n_v = min(kSpan, c.V - v0);
   pdl_wait();
   pdl_trigger();
@@ -54,10 +54,12 @@ __global__ void __launch_bounds__(kLoadThreads)
 }
 
 // ─── controls ──────────────────────────────────────────────────────────────
-// A CTA owns kChunk entries of one row (whole words of both bit rows). The bits say which entries change: the counts
-// and, in place, the logits are read only there, so a call costs V / 8 bytes a bit row and the entries it rewrites;
-// out of place it is one read and one write of the row.
-constexpr int kChunk = 4096;
+// A CTA owns kChunk entries of one row (whole words of both bit rows). Few tokens of a vocabulary have occurred (some
+// thousands of 150 thousand), so the work is split: a dense pass copies the logits and writes -inf where the mask
+// forbids, with nothing but wide loads and stores; then each thread looks at 16 bits of the seen row and rewrites the
+// entries that are set, from their logits and counts. In place the dense pass touches masked entries only, so a call
+// costs V / 8 bytes a bit row and what it changes.
+constexpr int kChunk = 16 * kThreads;
 
 template <int E>
 __device__ __forceinline__ void load_entries(float* x, const float* p) {
@@ -81,22 +83,22 @@ __device__ __forceinline__ void load_entries(float* x, const bf16* p) {
 
 template <typename T, bool IN_PLACE, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-    controls_kernel(const T* logits, int64_t ls, ControlsView c, SlotIds slots,
-                    const int64_t* __restrict__ fresh, const int* __restrict__ done, float* out, int64_t os) {
-  const int b = blockIdx.y, v0 = blockIdx.x * kChunk, v1 = min(c.V, v0 + kChunk);
+    controls_kernel(const T* logits, int64_t ls, ControlsView c, SlotIds slots, const int64_t* __restrict__ fresh,
+                    const int* __restrict__ done, float* out, int64_t os) {
+  const int b = blockIdx.y, v0 = blockIdx.x * kChunk, v1 = min(c.V, v0 + kChunk), tid = threadIdx.x;
   pdl_wait();
   pdl_trigger();
   const T* z = logits + b * ls;
   float* o = out + b * os;
-  constexpr int E = VEC ? 4 : 1, STEPS = kChunk / (E * kThreads);  // entries of a step
-  constexpr int BATCH = 4;                                         // steps whose loads are under way together
+  constexpr int E = VEC ? 4 : 1, STEPS = kChunk / (E * kThreads), BATCH = 4;  // steps whose loads are under way together
   constexpr uint32_t FIELD = (1u << E) - 1u;
   float x[BATCH][E];
-  auto place = [&](int k) { return v0 + (k * kThreads + (int)threadIdx.x) * E; };
   auto load_batch = [&](int k0) {
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (place(k0 + k) < v1) load_entries<E>(x[k], z + place(k0 + k));
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = v0 + ((k0 + k) * kThreads + tid) * E;
+      if (v < v1) load_entries<E>(x[k], z + v);
+    }
   };
   if (!IN_PLACE) load_batch(0);  // on their way while the slot is looked up
   const int64_t slot = slot_of(slots, b);
@@ -105,62 +107,89 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t r = on ? slot : 0;
   int* counts = c.counts + r * c.V;
   uint32_t* seen = c.seen + r * c.W;
+  const uint32_t* mask = c.mask + r * c.W;
   if (on && fresh) {
     const int64_t tok = done && done[b] ? -1 : fresh[b];
     const bool mine = tok >= v0 && tok < v1;
-    if (mine && threadIdx.x == 0) {
+    if (mine && tid == 0) {
       counts[tok] += 1;
       seen[tok / 32] |= 1u << (tok % 32);
     }
     if (mine) __syncthreads();  // this CTA alone reads the token's count and word
   }
   const float rep = c.repetition[r], freq = c.frequency[r], pres = c.presence[r];
-  const bool penal = on && (rep != 1.f || freq != 0.f || pres != 0.f);
   const bool masked = on && c.mask_on[r] != 0;
-  for (int k0 = 0; k0 < STEPS; k0 += BATCH) {
-    uint32_t s[BATCH], m[BATCH];  // seen; allowed
-    int n[BATCH][E];
-    if (!IN_PLACE && k0 > 0) load_batch(k0);
+  // this thread's 16 entries of the sparse pass: seen, and allowed (the others stay -inf)
+  const int w0 = v0 + 16 * tid;
+  uint32_t bits = 0u;
+  if (on && (rep != 1.f || freq != 0.f || pres != 0.f) && w0 < v1) {
+    bits = (seen[w0 / 32] >> (w0 % 32)) & 0xFFFFu;
+    if (masked) bits &= mask[w0 / 32] >> (w0 % 32);
+  }
+  if (!IN_PLACE || masked) {
+    for (int k0 = 0; k0 < STEPS; k0 += BATCH) {
+      if (!IN_PLACE && k0 > 0) load_batch(k0);
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      const int v = place(k0 + k);
-      s[k] = penal && v < v1 ? seen[v / 32] : 0u;
-      m[k] = masked && v < v1 ? c.mask[r * c.W + v / 32] : ~0u;
-    }
+      for (int k = 0; k < BATCH; ++k) {
+        const int v = v0 + ((k0 + k) * kThreads + tid) * E;
+        if (v >= v1) break;
+        const uint32_t m = masked ? (mask[v / 32] >> (v % 32)) & FIELD : FIELD;
+        if (IN_PLACE && m == FIELD) continue;
+        if (IN_PLACE && m != 0u) load_entries<E>(x[k], z + v);
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      const int v = place(k0 + k);
-      s[k] = (s[k] >> (v % 32)) & FIELD;
-      m[k] = (m[k] >> (v % 32)) & FIELD;
-      if (IN_PLACE && (s[k] != 0u || m[k] != FIELD) && m[k] != 0u) load_entries<E>(x[k], z + v);
-#pragma unroll
-      for (int e = 0; e < E; ++e) n[k][e] = (s[k] >> e) & 1u ? counts[v + e] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      const int v = place(k0 + k);
-      if (v >= v1 || (IN_PLACE && s[k] == 0u && m[k] == FIELD)) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if ((s[k] >> e) & 1u) {
-          const float y = x[k][e] > 0.f ? x[k][e] / rep : x[k][e] * rep;
-          x[k][e] = y - freq * (float)n[k][e] - (n[k][e] > 0 ? pres : 0.f);
-        }
-        if (!((m[k] >> e) & 1u)) x[k][e] = -INFINITY;
+        for (int e = 0; e < E; ++e)
+          if (!((m >> e) & 1u)) x[k][e] = -INFINITY;
+        if constexpr (VEC)
+          *reinterpret_cast<float4*>(o + v) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+        else
+          o[v] = x[k][0];
       }
-      if constexpr (VEC)
-        *reinterpret_cast<float4*>(o + v) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
-      else
-        o[v] = x[k][0];
     }
   }
+  if (!on) return;
+  __syncthreads();  // the dense pass of this chunk is written
+  while (bits) {
+    constexpr int N = 4;  // entries whose loads are under way together
+    int v[N], n[N];
+    float y[N][1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = bits ? w0 + __ffs(bits) - 1 : -1;
+      bits &= bits - 1u;
+      if (v[i] >= 0) {
+        n[i] = counts[v[i]];
+        load_entries<1>(y[i], z + v[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v[i] >= 0) {
+        const float p = y[i][0] > 0.f ? y[i][0] / rep : y[i][0] * rep;
+        o[v[i]] = p - freq * (float)n[i] - (n[i] > 0 ? pres : 0.f);
+      }
+  }
+  if (c.K == 0) return;
   // biases, on what this CTA has written (ids of a row are distinct; a masked entry stays -inf)
-  if (!on || c.K == 0) return;
   __syncthreads();
-  for (int j = threadIdx.x; j < c.K; j += kThreads) {
+  for (int j = tid; j < c.K; j += kThreads) {
     const int v = c.bias_ids[r * c.K + j];
     if (v >= v0 && v < v1) o[v] += c.bias_vals[r * c.K + j];
   }
+}
+
+template <int kSpan>
+void launch_load(ControlsView c, SlotIds slots, const int64_t* tokens, int64_t total, const int* cu, const int* n_prompt, int n,
+                 cudaStream_t st) {
+  constexpr int smem = kSpan * 4 + kSpan / 8;
+  static bool set[64] = {};
+  int dev = 0;
+  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!set[dev]) {
+    MESHY_CUDA_CHECK(cudaFuncSetAttribute(load_tokens_kernel<kSpan>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    set[dev] = true;
+  }
+  launch_pdl(load_tokens_kernel<kSpan>, dim3((c.V + kSpan - 1) / kSpan, n), dim3(kLoadThreads), smem, st, c, slots, tokens, total,
+             cu, n_prompt);
 }
 
 template <typename T>
@@ -185,8 +214,8 @@ void load_tokens(ControlsView c, SlotIds slots, const int64_t* tokens, int64_t t
                  cudaStream_t st) {
   if (n == 0) return;
   MESHY_CHECK(n <= 65535, "load_tokens: at most 65535 rows");
-  launch_pdl(load_tokens_kernel, dim3((c.V + kSpan - 1) / kSpan, n), dim3(kLoadThreads), 0, st, c, slots, tokens, total, cu,
-             n_prompt);
+  n >= 32 ? launch_load<24576>(c, slots, tokens, total, cu, n_prompt, n, st)
+          : launch_load<8192>(c, slots, tokens, total, cu, n_prompt, n, st);
 }
 
 void apply_logit_controls(const void* logits, bool is_bf16, int64_t ls, ControlsView c, SlotIds slots,

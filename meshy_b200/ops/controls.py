@@ -25,6 +25,8 @@ from typing import Mapping, Sequence
 import torch
 
 from . import reference as ref
+from ._ext import ext
+from .checks import check_range
 
 
 def _words(vocab: int) -> int:
@@ -132,12 +134,8 @@ def load_tokens(ctl: LogitControls, slots: torch.Tensor, tokens: torch.Tensor, c
     """Rewrite the token state of ``slots [n]`` (int32 or int64, distinct; negative: skipped): row ``i``'s tokens are
     ``tokens[cu_tokens[i]:cu_tokens[i + 1]]``, the first ``n_prompt[i]`` of them its prompt. Token ids outside the
     vocabulary are ignored."""
-    from .checks import check_range
-
     check_range("logit-control slots", slots, 0, ctl.counts.shape[0], skip_negative=True)
     if ctl.counts.is_cuda:
-        from ._ext import ext
-
         ext().load_tokens(ctl.state, slots, tokens, cu_tokens, n_prompt)
         return
     ref.load_tokens(ctl, slots, tokens, cu_tokens, n_prompt)
@@ -150,15 +148,11 @@ def apply_logit_controls(logits: torch.Tensor, ctl: LogitControls, slots: torch.
     (int32 or int64; negative: none). ``new_tokens [B]`` int64: the token each row sampled last is first counted as
     generated (negative: none; ``done [B]`` int32 nonzero: not counted). Rows that count must have distinct slots.
     ``out``: fp32 result; by default fp32 logits are rewritten in place."""
-    from .checks import check_range
-
     check_range("logit-control slots", slots, 0, ctl.counts.shape[0], skip_negative=True)
     if out is None:
         out = logits if logits.dtype == torch.float32 else torch.empty(logits.shape, dtype=torch.float32,
                                                                        device=logits.device)
     if logits.is_cuda:
-        from ._ext import ext
-
         ext().apply_logit_controls(logits, ctl.state, slots, new_tokens, done, out)
         return out
     return ref.apply_logit_controls(logits, ctl, slots, new_tokens, done, out)

@@ -23,6 +23,8 @@ from typing import NamedTuple
 import torch
 
 from . import reference as ref
+from ._ext import ext
+from .checks import check_paged, check_range
 
 GROUP = ref.KV4_GROUP
 
@@ -73,12 +75,8 @@ def kv4_from_bytes(raw: torch.Tensor, n_pages: int, n_kv: int, page: int, hd: in
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, slot_mapping: torch.Tensor) -> None:
     """``k/v [T, Hkv, hd]`` (any strides) into ``cache`` at ``slot_mapping [T]`` int64; slots must be distinct."""
-    from .checks import check_range
-
     check_range("KV-cache slots", slot_mapping, 0, cache.k.shape[0] * cache.k.shape[2], skip_negative=True)
     if k.is_cuda:
-        from ._ext import ext
-
         ext().kv4_write(k, v, cache.k, cache.v, cache.scale, slot_mapping)
         return
     ref.kv4_write(k, v, cache, slot_mapping)
@@ -86,14 +84,10 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, slot_mapping: t
 
 def kv4_read(cache: KV4Cache, slot_mapping: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """``k, v [T, Hkv, hd]``: the values the cache stands for at ``slot_mapping`` (zeros for a slot outside it)."""
-    from .checks import check_range
-
     check_range("KV-cache slots", slot_mapping, 0, cache.k.shape[0] * cache.k.shape[2], skip_negative=True)
     if cache.k.is_cuda:
         if dtype != torch.bfloat16:
             raise ValueError(f"kv4_read: bfloat16 on CUDA, got {dtype}")
-        from ._ext import ext
-
         shape = (slot_mapping.shape[0], cache.k.shape[1], 2 * cache.k.shape[3])
         k = torch.empty(shape, dtype=dtype, device=cache.k.device)
         v = torch.empty(shape, dtype=dtype, device=cache.k.device)
@@ -106,13 +100,9 @@ def paged_attention_kv4(q: torch.Tensor, cache: KV4Cache, block_table: torch.Ten
                         scale: float | None = None) -> torch.Tensor:
     """Decode attention of ``q [B, Hq, hd]`` over each row's first ``seq_lens [B]`` cached tokens, on the pages
     ``block_table [B, max_pages]``; query heads share the KV heads evenly. A row of length 0 gives zeros."""
-    from .checks import check_paged
-
     check_paged("paged attention", block_table, seq_lens, cache.k.shape[0], cache.k.shape[2])
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if q.is_cuda:
-        from ._ext import ext
-
         return ext().kv4_attention(q, cache.k, cache.v, cache.scale, block_table, seq_lens, float(scale))
     return ref.attention_decode_kv4(q, cache, block_table, seq_lens, scale)
 
