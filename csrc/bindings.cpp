@@ -777,21 +777,16 @@ void kv4_write_(Tensor k, Tensor v, Tensor kc, Tensor vc, Tensor scale, Tensor s
   if (k.size(0)) count();
 }
 
-void kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor slots, Tensor k, Tensor v) {
+std::tuple<Tensor, Tensor> kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor slots) {
   const KV4View c = kv4_view(kc, vc, scale);
   const c10::cuda::CUDAGuard guard(kc.device());
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.device() == kc.device(),
               "kv4_read: slots must be int64 [rows] on the cache's device");
   CHECK_CONTIG(slots);
-  for (const Tensor& t : {k, v}) {
-    CHECK_CONTIG(t);
-    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == slots.size(0) && t.size(1) == c.Hkv &&
-                    t.size(2) == c.hd && t.device() == kc.device(),
-                "kv4_read: outputs must be bfloat16 [rows, " + std::to_string(c.Hkv) + ", " + std::to_string(c.hd) +
-                    "] on the cache's device");
-  }
+  Tensor k = torch::empty({slots.size(0), c.Hkv, c.hd}, kc.options().dtype(torch::kBFloat16)), v = torch::empty_like(k);
   kv4_read(c, ptr<int64_t>(slots), (int)slots.size(0), ptr<bf16>(k), ptr<bf16>(v), cur_stream());
   if (slots.size(0)) count();
+  return {k, v};
 }
 
 // Workspace of the attention kernel, one per (device, stream): partial sums and arrival counters (zeroed once, left

@@ -88,11 +88,7 @@ def kv4_read(cache: KV4Cache, slot_mapping: torch.Tensor, dtype: torch.dtype = t
     if cache.k.is_cuda:
         if dtype != torch.bfloat16:
             raise ValueError(f"kv4_read: bfloat16 on CUDA, got {dtype}")
-        shape = (slot_mapping.shape[0], cache.k.shape[1], 2 * cache.k.shape[3])
-        k = torch.empty(shape, dtype=dtype, device=cache.k.device)
-        v = torch.empty(shape, dtype=dtype, device=cache.k.device)
-        ext().kv4_read(cache.k, cache.v, cache.scale, slot_mapping, k, v)
-        return k, v
+        return ext().kv4_read(cache.k, cache.v, cache.scale, slot_mapping)
     return ref.kv4_read(cache, slot_mapping, dtype)
 
 
