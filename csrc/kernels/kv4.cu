@@ -37,6 +37,19 @@ __device__ __forceinline__ float quotient(float x, float y, float rcp) {
   return fmaf(fmaf(-q, y, x), rcp, q);
 }
 
+// 1 / y, correctly rounded for every positive fp16 number y: the hardware's approximation and one Newton step.
+__device__ __forceinline__ float reciprocal(float y) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return fmaf(fmaf(-y, r, 1.f), r, r);
+}
+
+__device__ __forceinline__ float min_nan(float x, float y) {  // NaN if x is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 b) { return *reinterpret_cast<uint32_t*>(&b); }
 
@@ -48,7 +61,7 @@ __device__ __forceinline__ int64_t row_of(const KV4View& c, FastDiv page, int64_
   return (p * c.Hkv + h) * c.page + (slot - p * c.page);
 }
 
-// Eight lanes hold a group, eight channels (one word of nibbles) each.
+// Eight lanes hold a group, eight channels (one word of nibbles) each; ``row`` null: nothing is written.
 template <int HD>
 __device__ __forceinline__ void quantise(const uint4& u, int lane, uint32_t* row, __half2* pairs) {
   constexpr int G = HD / 64;
@@ -64,75 +77,71 @@ __device__ __forceinline__ void quantise(const uint4& u, int lane, uint32_t* row
                                            __hneg(__hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2))));
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) both = __hmax2_nan(both, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(both), o)));
-  float hi = __low2float(both), lo = -__high2float(both);
-  float x[8];
+  const float top = __low2float(both), low = -__high2float(both), hi = min_nan(top, kHalfMax), lo = -min_nan(-low, kHalfMax);
+  const __half a = __float2half_rn(quotient(hi - lo, 15.f, 1.f / 15.f)), z = __float2half_rn(lo);
+  const float af = __half2float(a), zf = __half2float(z), rcp = af > 0.f ? reciprocal(af) : 0.f;
+  float n[8];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const float2 f = unpack_bf16x2(us[q]);
-    x[2 * q] = f.x;
-    x[2 * q + 1] = f.y;
+    n[2 * q] = quotient(f.x - zf, af, rcp);
+    n[2 * q + 1] = quotient(f.y - zf, af, rcp);
   }
-  if (hi > kHalfMax || lo < -kHalfMax) {
-    hi = fminf(fmaxf(hi, -kHalfMax), kHalfMax);
-    lo = fminf(fmaxf(lo, -kHalfMax), kHalfMax);
+  // Nothing leaves [0, 15] while rounding moved the base by less than 0.4 steps and the scale by less than 2^-11 of it.
+  if (!(fabsf(lo) * 0.00048828125f < 0.4f * af && af >= 6.1035156e-5f && top == hi && low == lo)) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = fminf(fmaxf(x[q], -kHalfMax), kHalfMax);
-  }
-  const __half a = __float2half_rn(quotient(hi - lo, 15.f, 1.f / 15.f)), z = __float2half_rn(lo);
-  const float af = __half2float(a), zf = __half2float(z);
-  uint32_t word = 0;
-  if (af > 0.f) {
-    const float rcp = __frcp_rn(af);
-    float n[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) n[q] = quotient(x[q] - zf, af, rcp);
-    // the base is rounded: only where that moved it by a good part of a step does anything leave [0, 15]
-    if (quotient(lo - zf, af, rcp) < -0.5f || quotient(hi - zf, af, rcp) >= 15.5f) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) n[q] = fminf(fmaxf(n[q], 0.f), 15.f);
+    for (int q = 0; q < 8; ++q) {
+      const float2 f = unpack_bf16x2(us[q / 2]);
+      const float x = fminf(fmaxf(q % 2 ? f.y : f.x, -kHalfMax), kHalfMax);
+      n[q] = fminf(fmaxf(quotient(x - zf, af, rcp), 0.f), 15.f);
     }
-    // adding 1.5 2^23 rounds to whole numbers, halves to even; four of them fit a float's 24 bits side by side
-    constexpr float kRound = 12582912.f;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) n[q] = (n[q] + kRound) - kRound;
-    const float h0 = fmaf(fmaf(fmaf(n[3], 16.f, n[2]), 16.f, n[1]), 16.f, n[0]);
-    const float h1 = fmaf(fmaf(fmaf(n[7], 16.f, n[6]), 16.f, n[5]), 16.f, n[4]);
-    word = __byte_perm(__float_as_uint(h0 + kRound), __float_as_uint(h1 + kRound), 0x5410);
   }
+  // Adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits; the constant's own
+  // bits leave the sum again.
+  constexpr uint32_t kRoundBits = 0x4B400000u;  // 1.5 2^23
+  uint32_t word = 0u - kRoundBits * 0x11111111u;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) word += __float_as_uint(n[q] + 12582912.f) * (1u << (4 * q));
   if (row == nullptr) return;
-  row[lane % 8 * G + lane / 8] = word;
+  row[lane % 8 * G + lane / 8] = af > 0.f ? word : 0u;
   if (lane % 8 == 0) pairs[lane / 8] = __halves2half2(a, z);
 }
 
-// HD / 8 lanes per (token, head); each takes its word of K and of V, of kRows (token, head) pairs in one go so that
-// their loads are under way together.
-constexpr int kRows = 2;
-
-template <int HD>
+// HD / 8 lanes per token and NH heads of it: a lane takes its word of K and of V of each head, two heads' loads under
+// way together; the slot is resolved once.
+template <int HD, int NH>
 __global__ void __launch_bounds__(kThreads)
     kv4_write_kernel(const bf16* __restrict__ k, int64_t ks, int64_t kh, const bf16* __restrict__ v, int64_t vs,
-                     int64_t vh, const int64_t* __restrict__ slots, uint32_t rows, KV4View c, FastDiv heads, FastDiv page) {
-  constexpr int LANES = HD / 8, G = HD / 64, BLOCK = kThreads / LANES;
-  const uint32_t lane = threadIdx.x % LANES, th0 = blockIdx.x * (kRows * BLOCK) + threadIdx.x / LANES;
+                     int64_t vh, const int64_t* __restrict__ slots, uint32_t items, KV4View c, FastDiv splits, FastDiv page) {
+  constexpr int LANES = HD / 8, G = HD / 64, U = NH < 2 ? 1 : 2;
+  const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
   pdl_trigger();
-  uint4 uk[kRows], uv[kRows];
-  int64_t r[kRows];
+  const bool act = i < items;  // the lanes of a group stay together for the shuffles
+  const uint32_t t = act ? splits.div(i) : 0u;
+  const int h0 = act ? (i - t * splits.d) * NH : 0;
+  const bf16* kp = k + t * ks + h0 * kh + lane * 8;
+  const bf16* vp = v + t * vs + h0 * vh + lane * 8;
+  const int64_t r = act ? row_of(c, page, slots[t], h0) : -1;
+  uint32_t* kr = reinterpret_cast<uint32_t*>(c.k) + r * (HD / 8);
+  uint32_t* vr = reinterpret_cast<uint32_t*>(c.v) + r * (HD / 8);
+  __half2* pairs = c.scale + r * (2 * G);
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const bool act = th0 + u * BLOCK < rows;  // the lanes of a group stay together for the shuffles
-    const uint32_t th = act ? th0 + u * BLOCK : 0u, t = heads.div(th), h = th - t * heads.d;
-    uk[u] = *reinterpret_cast<const uint4*>(k + t * ks + h * kh + lane * 8);
-    uv[u] = *reinterpret_cast<const uint4*>(v + t * vs + h * vh + lane * 8);
-    r[u] = act ? row_of(c, page, slots[t], h) : -1;
-  }
+  for (int j = 0; j < NH; j += U) {
+    uint4 uk[U], uv[U];
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    uint32_t* kr = r[u] < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.k + r[u] * (HD / 2));
-    uint32_t* vr = r[u] < 0 ? nullptr : reinterpret_cast<uint32_t*>(c.v + r[u] * (HD / 2));
-    __half2* pairs = c.scale + r[u] * (2 * G);
-    quantise<HD>(uk[u], lane, kr, pairs);
-    quantise<HD>(uv[u], lane, vr, pairs + G);
+    for (int u = 0; u < U; ++u) {
+      const bool in = h0 + j + u < c.Hkv;
+      uk[u] = in ? *reinterpret_cast<const uint4*>(kp + (j + u) * kh) : make_uint4(0, 0, 0, 0);
+      uv[u] = in ? *reinterpret_cast<const uint4*>(vp + (j + u) * vh) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = r >= 0 && h0 + j + u < c.Hkv;
+      const int64_t to = (int64_t)(j + u) * c.page;
+      quantise<HD>(uk[u], lane, in ? kr + to * (HD / 8) : nullptr, pairs + to * (2 * G));
+      quantise<HD>(uv[u], lane, in ? vr + to * (HD / 8) : nullptr, pairs + to * (2 * G) + G);
+    }
   }
 }
 
@@ -155,47 +164,55 @@ __device__ __forceinline__ uint4 restore(uint32_t w, __half2 pair) {
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-template <int HD>
+template <int HD, int NH>
 __global__ void __launch_bounds__(kThreads)
-    kv4_read_kernel(KV4View c, const int64_t* __restrict__ slots, uint32_t rows, bf16* __restrict__ k, bf16* __restrict__ v,
-                    FastDiv heads, FastDiv page) {
-  constexpr int LANES = HD / 8, G = HD / 64, BLOCK = kThreads / LANES;
-  const uint32_t lane = threadIdx.x % LANES, th0 = blockIdx.x * (kRows * BLOCK) + threadIdx.x / LANES;
+    kv4_read_kernel(KV4View c, const int64_t* __restrict__ slots, uint32_t items, bf16* __restrict__ k, bf16* __restrict__ v,
+                    FastDiv splits, FastDiv page) {
+  constexpr int LANES = HD / 8, G = HD / 64;
+  const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
   pdl_trigger();
-  int64_t r[kRows];
-  uint32_t wk[kRows], wv[kRows];
-  __half2 pk[kRows], pv[kRows];
+  if (i >= items) return;
+  const uint32_t t = splits.div(i);
+  const int h0 = (i - t * splits.d) * NH;
+  const int64_t r = row_of(c, page, slots[t], h0);
+  const int at = lane % 8 * G + lane / 8;
+  const uint32_t* kr = reinterpret_cast<const uint32_t*>(c.k) + r * (HD / 8) + at;
+  const uint32_t* vr = reinterpret_cast<const uint32_t*>(c.v) + r * (HD / 8) + at;
+  const __half2* pairs = c.scale + r * (2 * G) + lane / 8;
+  uint32_t wk[NH], wv[NH];
+  __half2 pk[NH], pv[NH];
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const uint32_t th = th0 + u * BLOCK, t = heads.div(th), h = th - t * heads.d;
-    r[u] = th < rows ? row_of(c, page, slots[t], h) : -1;
+  for (int j = 0; j < NH; ++j) {
+    wk[j] = wv[j] = 0u;
+    pk[j] = pv[j] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+    if (r < 0 || h0 + j >= c.Hkv) continue;
+    const int64_t to = (int64_t)j * c.page;
+    wk[j] = kr[to * (HD / 8)];
+    wv[j] = vr[to * (HD / 8)];
+    pk[j] = pairs[to * (2 * G)];
+    pv[j] = pairs[to * (2 * G) + G];
   }
+  const int64_t o = ((int64_t)t * c.Hkv + h0) * HD + lane * 8;
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    wk[u] = wv[u] = 0u;
-    pk[u] = pv[u] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-    if (r[u] < 0) continue;
-    const int at = lane % 8 * G + lane / 8;
-    const __half2* pairs = c.scale + r[u] * (2 * G) + lane / 8;
-    wk[u] = reinterpret_cast<const uint32_t*>(c.k + r[u] * (HD / 2))[at];
-    wv[u] = reinterpret_cast<const uint32_t*>(c.v + r[u] * (HD / 2))[at];
-    pk[u] = pairs[0];
-    pv[u] = pairs[G];
-  }
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const uint32_t th = th0 + u * BLOCK;
-    if (th >= rows) continue;
-    const int64_t to = (int64_t)th * HD + lane * 8;
-    *reinterpret_cast<uint4*>(k + to) = restore(wk[u], pk[u]);
-    *reinterpret_cast<uint4*>(v + to) = restore(wv[u], pv[u]);
+  for (int j = 0; j < NH; ++j) {
+    if (h0 + j >= c.Hkv) break;
+    *reinterpret_cast<uint4*>(k + o + j * HD) = restore(wk[j], pk[j]);
+    *reinterpret_cast<uint4*>(v + o + j * HD) = restore(wv[j], pv[j]);
   }
 }
 
-int blocks(int64_t threads) {
-  MESHY_CHECK(threads < (1LL << 31), "kv4: too many rows for one call");
-  return (int)((threads + kRows * kThreads - 1) / (kRows * kThreads));
+// Four heads to a thread once that still leaves every SM its threads; one in a decode step, where only latency counts.
+constexpr int kManyRows = 1 << 16;
+
+struct Split {
+  uint32_t items, heads;  // (token, group of heads) pairs; groups of a token
+  int blocks;
+};
+Split split(int T, const KV4View& c, int nh) {
+  const int64_t heads = (c.Hkv + nh - 1) / nh, items = T * heads, per = kThreads / (c.hd / 8);
+  MESHY_CHECK(items < (1LL << 31), "kv4: too many rows for one call");
+  return {(uint32_t)items, (uint32_t)heads, (int)((items + per - 1) / per)};
 }
 
 }  // namespace
@@ -203,16 +220,29 @@ int blocks(int64_t threads) {
 void kv4_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs, int64_t vh, const int64_t* slots,
                int T, KV4View c, cudaStream_t st) {
   if (T == 0) return;
-  const int64_t rows = (int64_t)T * c.Hkv;
-  launch_pdl(c.hd == 128 ? kv4_write_kernel<128> : kv4_write_kernel<64>, dim3(blocks(rows * (c.hd / 8))), dim3(kThreads), 0, st,
-             k, ks, kh, v, vs, vh, slots, (uint32_t)rows, c, FastDiv(c.Hkv), FastDiv(c.page));
+  auto go = [&](auto kernel, int nh) {
+    const Split x = split(T, c, nh);
+    launch_pdl(kernel, dim3(x.blocks), dim3(kThreads), 0, st, k, ks, kh, v, vs, vh, slots, x.items, c, FastDiv(x.heads),
+               FastDiv(c.page));
+  };
+  const bool many = (int64_t)T * c.Hkv >= kManyRows;
+  if (c.hd == 128)
+    many ? go(kv4_write_kernel<128, 4>, 4) : go(kv4_write_kernel<128, 1>, 1);
+  else
+    many ? go(kv4_write_kernel<64, 4>, 4) : go(kv4_write_kernel<64, 1>, 1);
 }
 
 void kv4_read(KV4View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st) {
   if (T == 0) return;
-  const int64_t rows = (int64_t)T * c.Hkv;
-  launch_pdl(c.hd == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, dim3(blocks(rows * (c.hd / 8))), dim3(kThreads), 0, st, c,
-             slots, (uint32_t)rows, k, v, FastDiv(c.Hkv), FastDiv(c.page));
+  auto go = [&](auto kernel, int nh) {
+    const Split x = split(T, c, nh);
+    launch_pdl(kernel, dim3(x.blocks), dim3(kThreads), 0, st, c, slots, x.items, k, v, FastDiv(x.heads), FastDiv(c.page));
+  };
+  const bool many = (int64_t)T * c.Hkv >= kManyRows;
+  if (c.hd == 128)
+    many ? go(kv4_read_kernel<128, 4>, 4) : go(kv4_read_kernel<128, 1>, 1);
+  else
+    many ? go(kv4_read_kernel<64, 4>, 4) : go(kv4_read_kernel<64, 1>, 1);
 }
 
 }  // namespace meshy

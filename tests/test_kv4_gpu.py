@@ -89,7 +89,7 @@ def _setup(lens, Hq, Hkv, hd, page, seed=0, kscale=1.0, vscale=1.0, koff=0.0, ex
 # ── write and read-back ──────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("T,Hkv,hd,page", [(1, 1, 64, 16), (7, 2, 128, 64), (64, 2, 128, 64), (333, 8, 128, 48),
-                                           (1000, 3, 64, 32)])
+                                           (1000, 3, 64, 32), (13200, 5, 128, 64), (33000, 2, 64, 16), (70000, 1, 64, 64)])
 @pytest.mark.parametrize("spread", [1e-6, 1.0, 1000.0])
 def test_write_is_bit_exact(T, Hkv, hd, page, spread):
     from meshy_b200.ops import reference as ref
