@@ -61,87 +61,90 @@ __device__ __forceinline__ int64_t row_of(const KV4View& c, FastDiv page, int64_
   return (p * c.Hkv + h) * c.page + (slot - p * c.page);
 }
 
-// Eight lanes hold a group, eight channels (one word of nibbles) each; ``row`` null: nothing is written.
+// Four lanes hold a group, sixteen channels (two words of nibbles) each; ``row`` null: nothing is written.
 template <int HD>
-__device__ __forceinline__ void quantise(const uint4& u, int lane, uint32_t* row, __half2* pairs) {
+__device__ __forceinline__ void quantise(const uint4& u0, const uint4& u1, int lane, uint32_t* row, __half2* pairs) {
   constexpr int G = HD / 64;
-  const uint32_t us[4] = {u.x, u.y, u.z, u.w};
+  const uint32_t us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
   // extremes in bf16, where they are exact; (hi, -lo) side by side through the lanes; a NaN stays one
   __nv_bfloat162 hi2 = as_bf162(us[0]), lo2 = hi2;
 #pragma unroll
-  for (int q = 1; q < 4; ++q) {
+  for (int q = 1; q < 8; ++q) {
     hi2 = __hmax2_nan(hi2, as_bf162(us[q]));
     lo2 = __hmin2_nan(lo2, as_bf162(us[q]));
   }
-  __nv_bfloat162 both = __halves2bfloat162(__hmax_nan(__low2bfloat16(hi2), __high2bfloat16(hi2)),
-                                           __hneg(__hmin_nan(__low2bfloat16(lo2), __high2bfloat16(lo2))));
+  lo2 = __hneg2(lo2);
+  const uint32_t h = as_u32(hi2), l = as_u32(lo2);
+  __nv_bfloat162 both = __hmax2_nan(as_bf162(__byte_perm(h, l, 0x5410)), as_bf162(__byte_perm(h, l, 0x7632)));
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) both = __hmax2_nan(both, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(both), o)));
-  const float top = __low2float(both), low = -__high2float(both), hi = min_nan(top, kHalfMax), lo = -min_nan(-low, kHalfMax);
+  for (int o = 2; o > 0; o >>= 1) both = __hmax2_nan(both, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(both), o)));
+  const float top = __low2float(both), bot = __high2float(both);  // bot: -lo
+  const float hi = min_nan(top, kHalfMax), lo = -min_nan(bot, kHalfMax);
   const __half a = __float2half_rn(quotient(hi - lo, 15.f, 1.f / 15.f)), z = __float2half_rn(lo);
   const float af = __half2float(a), zf = __half2float(z), rcp = af > 0.f ? reciprocal(af) : 0.f;
-  float n[8];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float2 f = unpack_bf16x2(us[q]);
-    n[2 * q] = quotient(f.x - zf, af, rcp);
-    n[2 * q + 1] = quotient(f.y - zf, af, rcp);
-  }
   // Nothing leaves [0, 15] while rounding moved the base by less than 0.4 steps and the scale by less than 2^-11 of it.
-  if (!(fabsf(lo) * 0.00048828125f < 0.4f * af && af >= 6.1035156e-5f && top == hi && low == lo)) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float2 f = unpack_bf16x2(us[q / 2]);
-      const float x = fminf(fmaxf(q % 2 ? f.y : f.x, -kHalfMax), kHalfMax);
-      n[q] = fminf(fmaxf(quotient(x - zf, af, rcp), 0.f), 15.f);
-    }
-  }
-  // Adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits; the constant's own
-  // bits leave the sum again.
-  constexpr uint32_t kRoundBits = 0x4B400000u;  // 1.5 2^23
-  uint32_t word = 0u - kRoundBits * 0x11111111u;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) word += __float_as_uint(n[q] + 12582912.f) * (1u << (4 * q));
+  const bool tight = fabsf(lo) * 0.00048828125f < 0.4f * af && af >= 6.1035156e-5f && fmaxf(top, bot) <= kHalfMax;
   if (row == nullptr) return;
-  row[lane % 8 * G + lane / 8] = af > 0.f ? word : 0u;
-  if (lane % 8 == 0) pairs[lane / 8] = __halves2half2(a, z);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float n[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 f = unpack_bf16x2(us[4 * w + q]);
+      n[2 * q] = quotient(f.x - zf, af, rcp);
+      n[2 * q + 1] = quotient(f.y - zf, af, rcp);
+    }
+    if (!tight) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float2 f = unpack_bf16x2(us[4 * w + q / 2]);
+        const float x = fminf(fmaxf(q % 2 ? f.y : f.x, -kHalfMax), kHalfMax);
+        n[q] = fminf(fmaxf(quotient(x - zf, af, rcp), 0.f), 15.f);
+      }
+    }
+    // Adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits; the constant's
+    // own bits leave the sum again.
+    constexpr uint32_t kRoundBits = 0x4B400000u;  // 1.5 2^23
+    uint32_t word = 0u - kRoundBits * 0x11111111u;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) word += __float_as_uint(n[q] + 12582912.f) * (1u << (4 * q));
+    row[(lane % 4 * 2 + w) * G + lane / 4] = af > 0.f ? word : 0u;
+  }
+  if (lane % 4 == 0) pairs[lane / 4] = __halves2half2(a, z);
 }
 
-// HD / 8 lanes per token and NH heads of it: a lane takes its word of K and of V of each head, two heads' loads under
-// way together; the slot is resolved once.
+// HD / 16 lanes per token and NH heads of it: a lane takes its words of K and of V of each head; the slot is resolved
+// once.
 template <int HD, int NH>
 __global__ void __launch_bounds__(kThreads)
     kv4_write_kernel(const bf16* __restrict__ k, int64_t ks, int64_t kh, const bf16* __restrict__ v, int64_t vs,
                      int64_t vh, const int64_t* __restrict__ slots, uint32_t items, KV4View c, FastDiv splits, FastDiv page) {
-  constexpr int LANES = HD / 8, G = HD / 64, U = NH < 2 ? 1 : 2;
+  constexpr int LANES = HD / 16, G = HD / 64;
   const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
   pdl_trigger();
   const bool act = i < items;  // the lanes of a group stay together for the shuffles
   const uint32_t t = act ? splits.div(i) : 0u;
   const int h0 = act ? (i - t * splits.d) * NH : 0;
-  const bf16* kp = k + t * ks + h0 * kh + lane * 8;
-  const bf16* vp = v + t * vs + h0 * vh + lane * 8;
+  const bf16* kp = k + t * ks + h0 * kh + lane * 16;
+  const bf16* vp = v + t * vs + h0 * vh + lane * 16;
   const int64_t r = act ? row_of(c, page, slots[t], h0) : -1;
   uint32_t* kr = reinterpret_cast<uint32_t*>(c.k) + r * (HD / 8);
   uint32_t* vr = reinterpret_cast<uint32_t*>(c.v) + r * (HD / 8);
   __half2* pairs = c.scale + r * (2 * G);
 #pragma unroll
-  for (int j = 0; j < NH; j += U) {
-    uint4 uk[U], uv[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = h0 + j + u < c.Hkv;
-      uk[u] = in ? *reinterpret_cast<const uint4*>(kp + (j + u) * kh) : make_uint4(0, 0, 0, 0);
-      uv[u] = in ? *reinterpret_cast<const uint4*>(vp + (j + u) * vh) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = r >= 0 && h0 + j + u < c.Hkv;
-      const int64_t to = (int64_t)(j + u) * c.page;
-      quantise<HD>(uk[u], lane, in ? kr + to * (HD / 8) : nullptr, pairs + to * (2 * G));
-      quantise<HD>(uv[u], lane, in ? vr + to * (HD / 8) : nullptr, pairs + to * (2 * G) + G);
-    }
+  for (int j = 0; j < NH; ++j) {
+    if (h0 + j >= c.Hkv) kp = k, vp = v, kh = vh = 0;  // any row that is there: nothing of it is written
+    const bool in = r >= 0 && h0 + j < c.Hkv;
+    const uint4 k0 = reinterpret_cast<const uint4*>(kp)[0], k1 = reinterpret_cast<const uint4*>(kp)[1];
+    const uint4 v0 = reinterpret_cast<const uint4*>(vp)[0], v1 = reinterpret_cast<const uint4*>(vp)[1];
+    quantise<HD>(k0, k1, lane, in ? kr : nullptr, pairs);
+    quantise<HD>(v0, v1, lane, in ? vr : nullptr, pairs + G);
+    kp += kh;
+    vp += vh;
+    kr += (int64_t)c.page * (HD / 8);
+    vr += (int64_t)c.page * (HD / 8);
+    pairs += (int64_t)c.page * (2 * G);
   }
 }
 
@@ -209,8 +212,8 @@ struct Split {
   uint32_t items, heads;  // (token, group of heads) pairs; groups of a token
   int blocks;
 };
-Split split(int T, const KV4View& c, int nh) {
-  const int64_t heads = (c.Hkv + nh - 1) / nh, items = T * heads, per = kThreads / (c.hd / 8);
+Split split(int T, const KV4View& c, int nh, int channels) {  // channels of a lane
+  const int64_t heads = (c.Hkv + nh - 1) / nh, items = T * heads, per = kThreads / (c.hd / channels);
   MESHY_CHECK(items < (1LL << 31), "kv4: too many rows for one call");
   return {(uint32_t)items, (uint32_t)heads, (int)((items + per - 1) / per)};
 }
@@ -221,7 +224,7 @@ void kv4_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
                int T, KV4View c, cudaStream_t st) {
   if (T == 0) return;
   auto go = [&](auto kernel, int nh) {
-    const Split x = split(T, c, nh);
+    const Split x = split(T, c, nh, 16);
     launch_pdl(kernel, dim3(x.blocks), dim3(kThreads), 0, st, k, ks, kh, v, vs, vh, slots, x.items, c, FastDiv(x.heads),
                FastDiv(c.page));
   };
@@ -235,7 +238,7 @@ void kv4_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
 void kv4_read(KV4View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st) {
   if (T == 0) return;
   auto go = [&](auto kernel, int nh) {
-    const Split x = split(T, c, nh);
+    const Split x = split(T, c, nh, 8);
     launch_pdl(kernel, dim3(x.blocks), dim3(kThreads), 0, st, c, slots, x.items, k, v, FastDiv(x.heads), FastDiv(c.page));
   };
   const bool many = (int64_t)T * c.Hkv >= kManyRows;
