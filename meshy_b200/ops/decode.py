@@ -168,12 +168,16 @@ def _library_paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale):
 
 
 def sample(h, w, temperature: float, *, top_k: int = -1, top_p: float = 1.0, seed: int = 0,
-           step: torch.Tensor | None = None, generator=None):
+           step: torch.Tensor | None = None, generator=None, controls: tuple | None = None):
     """Returns ``(tokens int64 [B], logprobs fp32 [B])`` for hidden ``h [B, D]``.
 
     ``step`` is a device int64 counter folded into the Philox offset so a
-    captured CUDA graph draws fresh noise every replay.
+    captured CUDA graph draws fresh noise every replay. ``controls``:
+    ``(ctl, slots[, new_tokens, done])`` of :func:`.controls.apply_logit_controls`,
+    applied to the logits first; the log-probs are those of the controlled distribution.
     """
+    if controls is not None:
+        return _sample_controlled(h, w, temperature, top_k, top_p, seed, step, generator, *controls)
     if native(h) and temperature > 0 and top_k <= 0 and top_p >= 1.0:
         from ._ext import ext
 
@@ -196,6 +200,26 @@ def sample(h, w, temperature: float, *, top_k: int = -1, top_p: float = 1.0, see
         return _library_sample(h, w, temperature)
     logits = h.float() @ w.float().t() if not h.is_cuda else torch.nn.functional.linear(h, w).float()
     return ref.sample_with_logprob(logits, temperature, generator=generator, top_k=top_k, top_p=top_p)
+
+
+def _sample_controlled(h, w, temperature, top_k, top_p, seed, step, generator, ctl, slots, new_tokens=None, done=None):
+    from .controls import apply_logit_controls
+
+    B, V = h.shape[0], w.shape[0]
+    if native(h):
+        from ._ext import ext
+
+        logits = torch.empty(B, V, dtype=torch.float32, device=h.device)
+        ext().gemm(h.contiguous(), w, logits, False, False, None, None, None, 0, False, 0)
+    else:
+        logits = torch.nn.functional.linear(h.float(), w.float())
+    logits = apply_logit_controls(logits, ctl, slots, new_tokens=new_tokens, done=done)
+    if not native(h):
+        return ref.sample_with_logprob(logits, temperature, generator=generator, top_k=top_k, top_p=top_p)
+    tok = torch.empty(B, dtype=torch.int64, device=h.device)
+    lp = torch.empty(B, dtype=torch.float32, device=h.device)
+    ext().filtered_sample(logits, float(temperature), int(top_k), float(top_p), int(seed), step, tok, lp)
+    return tok, lp
 
 
 def _library_sample(h, w, temperature: float):

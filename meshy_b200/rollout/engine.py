@@ -20,12 +20,18 @@ Execution model:
 
 * weights live in one flat bf16 buffer with the trainer's layout;
 * the KV cache is ``[layers, 2, pages, kv_heads, page, head_dim]``; a host
-  block manager (:mod:`.kv_cache`) hands out pages;
+  block manager (:mod:`.kv_cache`) hands out pages. With ``kv_dtype="int4"``
+  it is a 4-bit cache per layer (:mod:`..ops.kv4`) that holds 3.55 times the
+  tokens in the same memory; prefill then attends to the values the cache
+  stands for, as decode does;
 * prefill runs new prompts as one packed varlen forward and writes their KV;
 * a decode step (embedding → layers → fused LM-head sampler → row advance) is
   captured once per batch-size bucket in a CUDA graph and replayed; rows that
   finish are compacted away every ``sync_every`` steps, the only host↔device
-  synchronisation of the loop.
+  synchronisation of the loop;
+* requests may carry penalties for repeated tokens, logit biases and a set of
+  allowed tokens (:mod:`..ops.controls`). Their log-probs are those of the
+  controlled distribution, the one the tokens were drawn from.
 """
 
 from __future__ import annotations
@@ -44,7 +50,12 @@ from ..models.args import ModelArgs
 from ..models.transformer import DecoderLM
 from ..ops import decode as D
 from ..ops import functional as Fx
+from ..ops import kv4 as K4
+from ..ops.controls import LogitControls, check_controls, load_tokens
 from .kv_cache import BlockManager
+
+#: entries of a request's ``logit_bias``
+MAX_LOGIT_BIAS = 300
 
 _BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 128, 160, 192, 224, 256, 320, 384, 448, 512)
 
@@ -58,6 +69,10 @@ class Request:
     top_k: int = -1
     top_p: float = 1.0
     ignore_eos: bool = False
+    #: keyword arguments of ``LogitControls.set_slot`` that differ from their defaults
+    controls: dict = field(default_factory=dict)
+    #: how many tokens at the end of ``prompt`` were generated earlier (a continued request); they count as output
+    n_generated: int = 0
     # engine state
     out_slot: int = -1
     pages: list[int] = field(default_factory=list)
@@ -104,10 +119,14 @@ class RolloutEngine:
         mem_fraction: float = 0.5,
         tp_group=None,
         ep: bool = False,
+        kv_dtype: str = "auto",
     ):
         from ..backend.flat import Slot, _align, flatten_module
 
+        if kv_dtype not in ("auto", "int4"):
+            raise ValueError(f"kv_dtype must be 'auto' (the model's dtype) or 'int4', got {kv_dtype!r}")
         self.args = args
+        self.kv4 = kv_dtype == "int4"
         self.device = torch.device(device)
         self.cuda = self.device.type == "cuda"
         self.dtype = torch.bfloat16 if self.cuda else torch.float32
@@ -160,7 +179,7 @@ class RolloutEngine:
         if max_total_tokens is None:
             if self.cuda:
                 free, _ = torch.cuda.mem_get_info(self.device)
-                max_total_tokens = int(free * mem_fraction) // max(1, self.local_args.kv_bytes_per_token(2))
+                max_total_tokens = int(free * mem_fraction) // max(1, self._kv_bytes_per_token())
             else:
                 max_total_tokens = 64 * 1024
         n_pages = max(1, max_total_tokens // page_size)
@@ -186,7 +205,7 @@ class RolloutEngine:
         self._mega = None
         self._mega_rows = 0
         self.mega_reason = "not on CUDA"
-        if self.cuda and self.tp_group is None:
+        if self.cuda and self.tp_group is None and not self.kv4:
             from .mega import MAX_ROWS, MegaDecoder
 
             self.mega_reason = MegaDecoder.reason(self.model, self.page_size)
@@ -195,23 +214,37 @@ class RolloutEngine:
                 self._mega_rows = MAX_ROWS
 
     # ------------------------------------------------------------------ memory
-    def _alloc_kv(self):
-        a = self.local_args  # this rank's KV heads
-        shape = [a.n_layers, 2, self.n_pages, a.n_kv_heads, self.page_size, a.head_dim]
+    def _kv_bytes_per_token(self) -> int:
+        a = self.local_args
+        return a.n_layers * a.n_kv_heads * K4.row_bytes(a.head_dim) if self.kv4 else a.kv_bytes_per_token(2)
+
+    def _alloc_kv4(self):
+        """One region of bytes, the layers' caches one after the other in it."""
+        a = self.local_args
+        per_layer = self.n_pages * a.n_kv_heads * self.page_size * K4.row_bytes(a.head_dim)
+        raw = self._kv_region([a.n_layers * per_layer], torch.uint8)
+        self.kv = [K4.kv4_from_bytes(raw[i * per_layer:(i + 1) * per_layer], self.n_pages, a.n_kv_heads, self.page_size,
+                                     a.head_dim) for i in range(a.n_layers)]
+
+    def _kv_region(self, shape, dtype) -> torch.Tensor:
+        """Zeroed KV memory: a virtual-memory region on CUDA (the one there is, mapped again)."""
         if not self.cuda:
-            self.kv = torch.zeros(*shape, dtype=self.dtype, device=self.device)
-            return
+            return torch.zeros(*shape, dtype=dtype, device=self.device)
         from ..ops._ext import ext
 
-        nbytes = math.prod(shape) * torch.empty((), dtype=self.dtype).element_size()
         reg = self._vmm.get("kv_cache") if hasattr(self, "_vmm") else None
         if reg is None:
-            reg = ext().VmmRegion(nbytes, self.device.index or 0)
+            reg = ext().VmmRegion(math.prod(shape) * dtype.itemsize, self.device.index or 0)
             self._vmm["kv_cache"] = reg
         elif not reg.mapped:
             reg.map()
-        self.kv = reg.view(0, shape, self.dtype)
-        self.kv.zero_()
+        return reg.view(0, list(shape), dtype).zero_()
+
+    def _alloc_kv(self):
+        if self.kv4:
+            return self._alloc_kv4()
+        a = self.local_args  # this rank's KV heads
+        self.kv = self._kv_region([a.n_layers, 2, self.n_pages, a.n_kv_heads, self.page_size, a.head_dim], self.dtype)
 
     def _init_state(self):
         B, dev = self.max_running, self.device
@@ -235,6 +268,8 @@ class RolloutEngine:
             "noeos": torch.zeros(0, dtype=i64, device=dev),
             "step": torch.zeros(1, dtype=i64, device=dev),
         }
+        self.ctl: LogitControls | None = None  # state of the output slots, made when a request first needs it
+        self._ctl_used: set[int] = set()       # slots whose controls are not neutral
         self.free_out_slots = list(range(R))
         self._park_rows(0)
 
@@ -349,23 +384,37 @@ class RolloutEngine:
 
     # ------------------------------------------------------------------ requests
     def submit(self, prompt: Sequence[int], max_new_tokens: int, *, rid=None, temperature=1.0, top_k=-1,
-               top_p=1.0, ignore_eos=False) -> Any:
+               top_p=1.0, ignore_eos=False, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+               presence_penalty: float = 0.0, logit_bias: dict[int, float] | None = None,
+               allowed_tokens: Sequence[int] | None = None, n_generated: int = 0) -> Any:
+        """Queue a request. The penalties, ``logit_bias`` and ``allowed_tokens`` act on the logits before temperature
+        and filters (:mod:`..ops.controls`); ``n_generated``: so many tokens at the prompt's end are output of an
+        earlier, aborted call (the frequency and presence penalties count them)."""
+        controls = {k: v for k, v, off in (("repetition_penalty", float(repetition_penalty), 1.0),
+                                           ("frequency_penalty", float(frequency_penalty), 0.0),
+                                           ("presence_penalty", float(presence_penalty), 0.0),
+                                           ("logit_bias", logit_bias or None, None),
+                                           ("allowed_tokens", allowed_tokens, None)) if v != off}
+        check_controls(self.args.vocab_size, MAX_LOGIT_BIAS, **controls)
+        if not 0 <= n_generated <= len(prompt):
+            raise ValueError(f"n_generated must be between 0 and the prompt's length, got {n_generated}")
         rid = next(self._rid) if rid is None else rid
         if len(prompt) + max_new_tokens > self.max_seq_len:
             max_new_tokens = max(1, self.max_seq_len - len(prompt))
         req = Request(rid, list(map(int, prompt)), int(max_new_tokens), float(temperature), int(top_k),
-                      float(top_p), bool(ignore_eos), submitted=time.time())
+                      float(top_p), bool(ignore_eos), controls, int(n_generated), submitted=time.time())
         with self.lock:
             self.waiting.append(req)
         return rid
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int | Sequence[int], *,
                  temperature: float = 1.0, top_k: int = -1, top_p: float = 1.0,
-                 ignore_eos: bool = False) -> list[Generation]:
-        """Blocking batch generation (the lock-step rollout's call)."""
+                 ignore_eos: bool = False, **controls) -> list[Generation]:
+        """Blocking batch generation (the lock-step rollout's call); ``controls``: as in :meth:`submit`, for every
+        prompt."""
         if isinstance(max_new_tokens, int):
             max_new_tokens = [max_new_tokens] * len(prompts)
-        rids = [self.submit(p, m, temperature=temperature, top_k=top_k, top_p=top_p, ignore_eos=ignore_eos)
+        rids = [self.submit(p, m, temperature=temperature, top_k=top_k, top_p=top_p, ignore_eos=ignore_eos, **controls)
                 for p, m in zip(prompts, max_new_tokens)]
         self.run_until_idle()
         return [self.finished.pop(r) for r in rids]
@@ -479,15 +528,22 @@ class RolloutEngine:
         for li, layer in enumerate(m.layers):
             h = Fx.rmsnorm(x, layer.attn_norm, a.norm_eps)
             qkv = Fx.linear(h, layer.wqkv, layer.bqkv)
-            q, k, v = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
-                                          a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1], slots,
-                                          keep_kv=True)
+            if self.kv4:
+                q, k, v = Fx.qkv_rope(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads, a.head_dim,
+                                      a.rope_theta, a.norm_eps)
+                K4.kv4_write(k, v, self.kv[li], slots)
+                k, v = K4.kv4_read(self.kv[li], slots, self.dtype)
+            else:
+                q, k, v = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
+                                              a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1],
+                                              slots, keep_kv=True)
             o = Fx.flash_attn_varlen(q, k, v, cu, max(lens))
             x = self._row_parallel(o.reshape(T, la.q_dim), layer.wo, x)
             h = Fx.rmsnorm(x, layer.mlp_norm, a.norm_eps)
             x = self._mlp(layer, h, x)
         last = (cu[1:] - 1).long()
         hl = Fx.rmsnorm(x[last], m.norm, a.norm_eps)
+        self._set_controls(batch, toks, cu)
         tok, lp = self._sample_rows(hl, batch)
         self.stats["prefill_tokens"] += T
         # append rows
@@ -544,18 +600,44 @@ class RolloutEngine:
         dist.all_reduce(y, group=self.tp_group)
         return (residual.float() + y).to(residual.dtype)
 
+    @property
+    def _controlled(self) -> bool:
+        return self.ctl is not None and any(r.controls for r in self.running)
+
+    def _set_controls(self, batch: Sequence[Request], toks: torch.Tensor, cu: torch.Tensor) -> None:
+        """Controls and token state of newly admitted requests (``toks`` / ``cu``: their prompts, packed); a slot
+        that last served a request with controls is reset."""
+        if self.ctl is None:
+            if not any(r.controls for r in batch):
+                return
+            self.ctl = LogitControls.create(self.max_running, self.args.vocab_size, device=self.device,
+                                            max_bias=MAX_LOGIT_BIAS)
+        for r in batch:
+            if r.controls or r.out_slot in self._ctl_used:
+                self.ctl.set_slot(r.out_slot, **r.controls)
+                (self._ctl_used.add if r.controls else self._ctl_used.discard)(r.out_slot)
+        if any(r.controls for r in batch):
+            i32 = dict(dtype=torch.int32, device=self.device)
+            load_tokens(self.ctl, torch.tensor([r.out_slot if r.controls else -1 for r in batch], **i32), toks, cu,
+                        torch.tensor([len(r.prompt) - r.n_generated for r in batch], **i32))
+
     def _sample_rows(self, h, reqs: Sequence[Request]):
         r0 = reqs[0]
         uniform = all(r.temperature == r0.temperature and r.top_k == r0.top_k and r.top_p == r0.top_p
                       for r in reqs)
         w = self.model.output_weight
+        slots = None  # first tokens: nothing generated yet that is not in the token state
+        if any(r.controls for r in reqs):
+            slots = torch.tensor([r.out_slot for r in reqs], dtype=torch.int32, device=self.device)
         if uniform:
             return D.sample(h, w, r0.temperature, top_k=r0.top_k, top_p=r0.top_p, seed=self.seed,
-                            step=self.st["step"], generator=self._gen if not self.cuda else None)
+                            step=self.st["step"], generator=self._gen if not self.cuda else None,
+                            controls=None if slots is None else (self.ctl, slots))
         toks, lps = [], []
         for i, r in enumerate(reqs):
             t, l = D.sample(h[i:i + 1], w, r.temperature, top_k=r.top_k, top_p=r.top_p, seed=self.seed,
-                            step=self.st["step"], generator=self._gen if not self.cuda else None)
+                            step=self.st["step"], generator=self._gen if not self.cuda else None,
+                            controls=None if slots is None else (self.ctl, slots[i:i + 1]))
             toks.append(t)
             lps.append(l)
         return torch.cat(toks), torch.cat(lps)
@@ -602,7 +684,7 @@ class RolloutEngine:
         L = len(m.layers)
         for li, layer in enumerate(m.layers):
             q = None
-            if prep is not None and fuse_rope:
+            if prep is not None and fuse_rope and not self.kv4:
                 q = D.qkv_rope_fused(xg[:b], layer.wqkv, layer.bqkv, pos, layer.q_norm, layer.k_norm, a.n_heads,
                                      a.n_kv_heads, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1],
                                      st["slot"][:b], part=prep, d=a.dim)
@@ -612,11 +694,19 @@ class RolloutEngine:
                     qkv = D.linear_norm_scaled(xg[:b], layer.wqkv, layer.bqkv, prep, a.dim, a.norm_eps)
                 if qkv is None:
                     qkv = Fx.rmsnorm_linear(x, layer.attn_norm, a.norm_eps, layer.wqkv, layer.bqkv)
-                q, _, _ = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
-                                              a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1],
-                                              st["slot"][:b])
-            o = D.paged_attention(q, self.kv[li, 0], self.kv[li, 1], st["block_table"][:b], st["seq_lens"][:b],
-                                  decode_step=True)
+                if self.kv4:
+                    q, k, v = Fx.qkv_rope(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads, a.head_dim,
+                                          a.rope_theta, a.norm_eps)
+                    K4.kv4_write(k, v, self.kv[li], st["slot"][:b])
+                else:
+                    q, _, _ = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
+                                                  a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0],
+                                                  self.kv[li, 1], st["slot"][:b])
+            if self.kv4:
+                o = K4.paged_attention_kv4(q, self.kv[li], st["block_table"][:b], st["seq_lens"][:b])
+            else:
+                o = D.paged_attention(q, self.kv[li, 0], self.kv[li, 1], st["block_table"][:b], st["seq_lens"][:b],
+                                      decode_step=True)
             o = o.reshape(b, la.q_dim)
             prep = None
             if layer.moe is None and split:
@@ -654,8 +744,9 @@ class RolloutEngine:
         sub = {k: (v[:b] if k not in ("out_tok", "out_lp", "eos", "noeos", "step") else v) for k, v in st.items()}
         sub["eos"] = eos
         # temperature-only sampling of <= 64 rows: LM head + sampler, then merge + row advance (2 kernels)
+        controls = (self.ctl, st["req"][:b], st["tok_in"][:b], st["done"][:b]) if self._controlled else None
         fused = (self.cuda and b <= 64 and r0.temperature > 0 and r0.top_k <= 0 and r0.top_p >= 1.0
-                 and os.environ.get("MESHY_FUSED_SAMPLER", "1") != "0")
+                 and controls is None and os.environ.get("MESHY_FUSED_SAMPLER", "1") != "0")
         h = self._decode_hidden(b, final_split=fused)
         part = None
         if isinstance(h, tuple):
@@ -667,7 +758,7 @@ class RolloutEngine:
             rstd = torch.rsqrt(part.sum(0)[:b] / a.dim + a.norm_eps)
             h = (h.float() * rstd[:, None]).to(h.dtype)
         tok, lp = D.sample(h, m.output_weight, r0.temperature, top_k=r0.top_k, top_p=r0.top_p, seed=self.seed,
-                           step=st["step"], generator=self._gen if not self.cuda else None)
+                           step=st["step"], generator=self._gen if not self.cuda else None, controls=controls)
         D.decode_advance(sub, tok, lp, self.page_size)
         st["step"] += 1
 
@@ -690,7 +781,7 @@ class RolloutEngine:
 
     def _sampling_key(self):
         r = self.running[0]
-        return (r.temperature, r.top_k, r.top_p)
+        return (r.temperature, r.top_k, r.top_p, self._controlled)
 
     def _capture(self, b: int, eos: torch.Tensor):
         # rows beyond len(running) are padding: mark them done so advance skips them
@@ -699,6 +790,7 @@ class RolloutEngine:
         with torch.cuda.stream(s):
             for _ in range(2):  # warm-up (allocator, tensor maps)
                 saved = {k: v.clone() for k, v in self.st.items()}
+                self.st["done"].fill_(1)  # rows that are done count no tokens (the token state is not in ``st``)
                 self._decode_body(b, eos)
                 for k, v in saved.items():
                     self.st[k].copy_(v)

@@ -4,7 +4,10 @@ Routes (the subset of SGLang's API the reference drives, ``meshy/engine/sglang.p
 
 * ``POST /generate`` ``{input_ids, sampling_params, return_logprob}`` →
   ``{output_ids, meta_info: {finish_reason: {type}, output_token_logprobs:
-  [[lp, id, null], ...], weight_version}}``
+  [[lp, id, null], ...], weight_version}}``. ``sampling_params`` takes
+  ``temperature``, ``top_k``, ``top_p``, ``max_new_tokens``, ``ignore_eos``, the penalties
+  ``repetition_penalty``, ``frequency_penalty``, ``presence_penalty``, ``logit_bias`` and
+  ``allowed_token_ids``
 * ``GET /health``, ``GET /health_generate``, ``GET /v1/loads``,
   ``GET /get_model_info``
 * ``POST /pause_generation {mode: "abort"|"wait"}``, ``POST /continue_generation``
@@ -30,6 +33,20 @@ import time
 from typing import Any
 
 log = logging.getLogger(__name__)
+
+
+def _controls(params: dict) -> dict:
+    """The engine's logit-control arguments from sampling parameters (SGLang's names; ``allowed_token_ids`` and
+    ``n_generated`` are this engine's)."""
+    out = {k: float(params[k]) for k in ("repetition_penalty", "frequency_penalty", "presence_penalty")
+           if params.get(k) is not None}
+    if params.get("logit_bias"):
+        out["logit_bias"] = {int(t): float(x) for t, x in dict(params["logit_bias"]).items()}
+    if params.get("allowed_token_ids") is not None:
+        out["allowed_tokens"] = [int(t) for t in params["allowed_token_ids"]]
+    if params.get("n_generated"):
+        out["n_generated"] = int(params["n_generated"])
+    return out
 
 
 class EngineRunner:
@@ -96,7 +113,7 @@ class EngineRunner:
         return self.engine.submit(prompt, int(params.get("max_new_tokens", 16384)),
                                   temperature=float(params.get("temperature", 1.0)),
                                   top_k=int(params.get("top_k", -1)), top_p=float(params.get("top_p", 1.0)),
-                                  ignore_eos=bool(params.get("ignore_eos", False)))
+                                  ignore_eos=bool(params.get("ignore_eos", False)), **_controls(params))
 
     def pause(self, mode: str = "abort") -> None:
         self.engine.pause()
@@ -123,7 +140,10 @@ def build_app(runner: EngineRunner, model_name: str = ""):
     async def generate(req):
         body = await req.json()
         params = dict(body.get("sampling_params") or {})
-        gen = await runner.generate(list(body["input_ids"]), params)
+        try:
+            gen = await runner.generate(list(body["input_ids"]), params)
+        except ValueError as e:  # unusable sampling parameters
+            return web.json_response({"error": str(e)}, status=400)
         out = {"output_ids": gen.output_ids,
                "meta_info": {"finish_reason": {"type": gen.finish_reason},
                              "completion_tokens": len(gen.output_ids), "weight_version": gen.weight_version}}
@@ -230,6 +250,8 @@ def main(argv=None):
     p.add_argument("--max-total-tokens", type=int, default=None)
     p.add_argument("--max-seq-len", type=int, default=None)
     p.add_argument("--mem-fraction", type=float, default=0.5)
+    p.add_argument("--kv-cache-dtype", choices=["auto", "int4"], default="auto",
+                   help="KV cache in the model's dtype, or in 4 bits (3.55 times the tokens)")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--eos", type=int, nargs="*", default=[])
     p.add_argument("--tp-size", type=int, default=1, help="tensor-parallel degree of this replica")
@@ -263,7 +285,7 @@ def _build_engine(a, device=None, tp_group=None):
     return RolloutEngine(get_model_args(name, flavor), device=device or a.device, max_running=a.max_running,
                          max_total_tokens=a.max_total_tokens, max_seq_len=a.max_seq_len,
                          mem_fraction=a.mem_fraction, seed=a.seed, eos_token_ids=a.eos, tp_group=tp_group,
-                         ep=a.ep_size > 1)
+                         ep=a.ep_size > 1, kv_dtype=a.kv_cache_dtype)
 
 
 def _rendezvous(a) -> tuple[str, int]:

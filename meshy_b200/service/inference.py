@@ -42,6 +42,7 @@ _ARG_MAP = {
     "max_seq_len": "--max-seq-len",
     "mem_fraction_static": "--mem-fraction",
     "mem_fraction": "--mem-fraction",
+    "kv_cache_dtype": "--kv-cache-dtype",
     "random_seed": "--seed",
     "tp_size": "--tp-size",
     "ep_size": "--ep-size",
