@@ -794,10 +794,10 @@ std::tuple<Tensor, Tensor> kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor 
 struct KV4Workspace {
   Tensor part, arrived;
 };
+std::map<std::pair<int, cudaStream_t>, std::vector<KV4Workspace>> g_kv4_ws;
 KV4Workspace kv4_workspace(const Tensor& cache, int64_t segments) {
-  static std::map<std::pair<int, cudaStream_t>, std::vector<KV4Workspace>> all;
   std::lock_guard<std::mutex> g(g_mu);
-  std::vector<KV4Workspace>& w = all[{cache.get_device(), cur_stream()}];
+  std::vector<KV4Workspace>& w = g_kv4_ws[{cache.get_device(), cur_stream()}];
   if (w.empty() || w.back().arrived.numel() < segments) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     MESHY_CUDA_CHECK(cudaStreamIsCapturing(cur_stream(), &cap));
@@ -807,6 +807,13 @@ KV4Workspace kv4_workspace(const Tensor& cache, int64_t segments) {
                  torch::zeros({std::max<int64_t>(segments, 1 << 14)}, cache.options().dtype(torch::kInt32))});
   }
   return w.back();
+}
+
+// After a device error (a wait that gave up) the counters may be left nonzero.
+void kv4_reset() {
+  std::lock_guard<std::mutex> g(g_mu);
+  for (auto& e : g_kv4_ws)
+    for (KV4Workspace& w : e.second) w.arrived.zero_();
 }
 
 Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
@@ -825,10 +832,11 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
   CHECK_CONTIG(seq_lens);
   Tensor out = torch::empty({B, Hq, c.hd}, q.options());
   if (B == 0) return out;
+  if (c.n_pages == 0 || bt.size(1) == 0) return out.zero_();
   const KV4Workspace ws = kv4_workspace(kc, kv4_attention_segments((int)B, (int)Hq, c.Hkv));
   kv4_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
                 ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ptr<float>(ws.part), ptr<unsigned>(ws.arrived),
-                cur_stream());
+                ptr<int>(scratch(0, 0).err), cur_stream());
   count();
   return out;
 }
@@ -1531,6 +1539,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv4_write", &kv4_write_, "quantise K / V rows into the 4-bit paged cache");
   m.def("kv4_read", &kv4_read_, "the values the 4-bit paged cache holds at given slots");
   m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache");
+  m.def("kv4_reset", &kv4_reset, "zero the attention's arrival counters after a device error");
   m.def("load_tokens", &load_tokens_, "token state (seen bits, generated counts) of admitted requests");
   m.def("apply_logit_controls", &apply_logit_controls_, "penalties, biases and token masks on logits");
   m.def("decode_advance", &decode_advance_);

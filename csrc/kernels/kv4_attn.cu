@@ -15,19 +15,25 @@
 // have to be stored to shared or tensor memory first, and at 8 query rows the matrix work is a fraction of the
 // unpacking.
 //
-// P carries the scale of V (x = p a'), so it is kept in fp16's range by a reference (m, A) per warp: x = 64 p a' / A
-// with p relative to m. The reference moves only when p passes 2^7 or 64 a' / A passes 2^8 (then to the true maxima),
-// so most tiles take neither the maximum's shuffles nor a rescaling; what falls below fp16's smallest number is less
-// than 2^-30 of the largest term.
+// P carries the scale of V (x = p a'), so a reference m per warp and head keeps it in fp16's range: p is taken relative
+// to m, which is set so that the largest x seen is 2^11, and moves again only when p or a' have outgrown what it was set
+// for by 8 or 2 (x stays below 2^15). So most units take neither the maximum's shuffles nor a rescaling, and what falls
+// below fp16's smallest number is less than 2^-35 of the largest term. P is rounded to fp16's 11 bits there; sums, the
+// normaliser and the bases' part stay in 32 bits.
 //
-// Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 16 tokens and every
-// CTA takes an equal share of the sum, whatever the lengths: the lengths are read on the device, a captured graph
-// follows them. A segment that spans CTAs leaves partial sums in a workspace; the last CTA to arrive joins them in
-// CTA order, so results do not depend on timing.
+// Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (16 where a
+// page is not a multiple of 32, 64 at head width 64 where it is one of 64) and every CTA, one per SM, takes an equal share of the sum, whatever the lengths: the
+// lengths are read on the device, a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment
+// that spans CTAs leaves partial sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one
+// order, and results do not depend on timing.
 //
-// Each warp keeps a ring of kStages units (32 tokens; 16 where a page is not a multiple of 32) of its own in shared
-// memory, filled by 16-byte asynchronous copies two units ahead, across the segments, so no warp waits for another
-// between joins. The query rows of the next segment come the same way.
+// Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory, filled by
+// 16-byte asynchronous copies two units ahead, across the segments, and at a segment's end leaves its state in one of
+// kSlots slots and goes on. Four helper warps prepare the query fragments of the coming segments and join the eight
+// states of the finished ones behind the others' backs. (With the joins in the computing warps' way, 256 rows of about
+// 1200 tokens took 105 us instead of 96; two CTAs of eight such warps and 128 registers each ran no faster on long rows
+// than one CTA with 168, as one of the two is always favoured and the other finishes alone.) Every wait is bounded; one
+// that gives up records an error code.
 #include <cuda_runtime.h>
 
 #include "../include/sm100.cuh"
@@ -37,12 +43,13 @@ namespace meshy {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kWarps = 8;                      // that compute
+constexpr int kHelpers = 4;
+constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = 16;                       // tokens of a tile
 constexpr int kHeads = 8;                      // query heads of a segment
-constexpr int kStages = 2;
-constexpr uint32_t kWholeUnits = 40;
+constexpr int kSlots = 3;                      // segments whose fragments or states are held
+constexpr uint32_t kWholeUnits = 40;           // units of a segment that a CTA takes whole
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 2048.f;               // x of the largest p and a' right after the reference moved
 constexpr float kGrowP = 8.f, kGrowA = 2.f;    // how far either may pass it: x stays below 2^15
@@ -53,16 +60,15 @@ struct Cfg {
   static constexpr int ROW = HD / 2;                     // nibble bytes of a token
   static constexpr int PAIRS = HD / 8;                   // bytes of a token's pairs (K and V)
   static constexpr int UTOK = NT * kTok;
-  static constexpr int K = 0, V = UTOK * ROW, S = 2 * UTOK * ROW;
-  static constexpr int LD = HD + 4;                      // row stride of a warp's state: spreads the heads over the banks
-  static constexpr int STAGE = 2 * (2 * kTok * ROW + kTok * PAIRS);  // room for a unit, and for a warp's state
-  static_assert(kHeads * LD * 4 <= STAGE && UTOK * (2 * ROW + PAIRS) <= STAGE, "a stage holds either");
-  static constexpr int WARP = kStages * STAGE;
-  static constexpr int Q = kWarps * WARP;
-  static constexpr int QBYTES = kHeads * HD * 2;
-  static constexpr int F = Q + 2 * QBYTES;               // two sets of query fragments: matrix B, sums (B too), factors
+  static constexpr int K = 0, V = UTOK * ROW, S = 2 * UTOK * ROW, STAGE = UTOK * (2 * ROW + PAIRS);
+  static constexpr int STAGES = 13824 / STAGE;           // 3 units of 32 tokens at head width 128
+  static constexpr int WARP = STAGES * STAGE;
+  static constexpr int LD = HD + 4;                      // row stride of a state: spreads the heads over the banks
+  static constexpr int STATES = kWarps * WARP;           // kSlots sets of the warps' states
+  static constexpr int STATE = kHeads * LD * 4;
+  static constexpr int F = STATES + kSlots * kWarps * STATE;  // kSlots sets of query fragments: matrix B, sums (B too), factors
   static constexpr int F_SUM = 32 * 16 * (HD / 32), F_FACTOR = F_SUM + 2 * 32 * 4, FBYTES = F_FACTOR + kHeads * 4;
-  static constexpr int SMEM = F + 2 * FBYTES;
+  static constexpr int SMEM = F + kSlots * FBYTES;
   static constexpr int PART = HD + 4;                    // floats of a head in the workspace: sums, maximum, normaliser
 };
 
@@ -126,6 +132,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 
+__device__ __forceinline__ void helper_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kHelpers) : "memory"); }
+
 __device__ __forceinline__ float max_over_rows(float v) {  // over the lanes that share lane % 4
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -151,6 +159,7 @@ struct Args {
   bf16* out;
   float* part;         // [2 CTAs][kHeads][PART]
   unsigned* arrived;   // [segments], zero between launches
+  int* err;
 };
 
 __device__ __forceinline__ int tokens_of(const Args& a, int b) {
@@ -161,15 +170,17 @@ __device__ __forceinline__ int tokens_of(const Args& a, int b) {
 template <int UTOK>
 __device__ __forceinline__ uint32_t units_of(int n) { return max(1, (n + UTOK - 1) / UTOK); }  // an empty row writes its zeros
 
-// A CTA's walk over its share of the units: segment (b, h), of whose U units it has [first, last); ``left`` units of the
-// share remain from ``first`` on.
+// A CTA's walk over its share of the units: segment (b, h), which starts at unit ``begin`` of the sum and of whose U units
+// the share has [first, last); ``left`` units of the share remain from ``first`` on.
 template <int UTOK>
 struct Walk {
   int b, h, n, U, first, last, left;
+  uint32_t begin;
   __device__ __forceinline__ bool next(const Args& a) {
     left -= last - first;
     if (left <= 0) return false;
     first = 0;
+    begin += U;
     if (++h == a.c.Hkv * a.blocks) {
       h = 0;
       ++b;
@@ -179,6 +190,9 @@ struct Walk {
     last = min(U, left);
     return true;
   }
+  __device__ __forceinline__ bool more() const { return left > last - first; }
+  __device__ __forceinline__ int end() const { return n ? last : 0; }  // of the units that hold tokens
+  __device__ __forceinline__ int first_of(int warp) const { return first + ((warp - (int)begin - first) & (kWarps - 1)); }
 };
 
 // CTA c of n has units [begin(c), begin(c + 1)): total / n each, and the rest spread evenly (so that equal segments are
@@ -202,21 +216,32 @@ struct Piece {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   using C = Cfg<HD, NT>;
   using W = Walk<C::UTOK>;
   constexpr int G = HD / 64;
   constexpr int KW = HD / 32;  // K words a lane takes of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
-  __shared__ uint32_t scan[kWarps], s_begin;
-  __shared__ int s_row;
+  __shared__ float sm[kSlots][kWarps][kHeads], sl[kSlots][kWarps][kHeads];
+  __shared__ W s_seg[kSlots], s_ahead[kWarps];
+  __shared__ uint64_t ready[kSlots], done[kSlots];  // fragments are there and the states free; the states are there
+  __shared__ float weight[kHeads][kWarps], total_max[kHeads], total_sum[kHeads];
   __shared__ Piece s_piece[2];
-  __shared__ const float* so[kWarps];  // the warps' states
-  __shared__ W s_cur, s_ahead[kWarps];  // touched once per segment: kept out of the registers
+  __shared__ uint32_t scan[kWarps + kHelpers], s_begin;
+  __shared__ int s_row, s_pieces, s_abort, s_ok;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t per_row = a.c.Hkv * a.blocks;  // segments of a row
+  volatile int* abort_flag = &s_abort;
 
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&ready[i], 1);
+      mbar_init(&done[i], kWarps);
+    }
+    s_abort = 0;
+    s_pieces = 0;
+    fence_mbar_init();
+  }
   pdl_wait();
   pdl_trigger();
 
@@ -235,16 +260,22 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     __syncthreads();
     before = total + incl - mine;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarps + kHelpers; ++w) {
       if (w < warp) before += scan[w];
       total += scan[w];
     }
   };
   for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
   const uint32_t all = total;
-  // a CTA per segment where that makes a few steps of every warp; else as many CTAs as give each warp a unit
+  // A CTA per segment where that makes a few steps of every warp. Else more of them: the steps shrink with their number,
+  // the join grows with it, so the best number goes with the root of the work; a whole number to a segment, if that
+  // is near (equal segments are then cut alike).
   const uint32_t segments = a.B * per_row;
-  const uint32_t n_cta = min(gridDim.x, all <= segments * kWholeUnits ? segments : (all + kWarps - 1) / kWarps);
+  uint32_t n_cta = segments;
+  if (all > segments * kWholeUnits)
+    n_cta = max(segments, min((all + kWarps - 1) / kWarps, (uint32_t)sqrtf(4.f * (float)all * (float)segments)));
+  n_cta = min(gridDim.x, n_cta);
+  if (n_cta > segments && n_cta % segments * 20 <= n_cta) n_cta -= n_cta % segments;
   if (blockIdx.x >= n_cta) return;
   const Shares shares{all, n_cta, all / n_cta, all % n_cta};
   const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
@@ -258,399 +289,451 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     if (total > at) break;
   }
   __syncthreads();
-  uint32_t seg0 = s_begin;  // the segment's first unit in the sum
-  int f_unit;
-  {
-    W w;
-    w.b = s_row;
-    w.n = tokens_of(a, w.b);
-    w.U = units_of<C::UTOK>(w.n);
-    w.h = (at - seg0) / w.U;
-    seg0 += w.h * w.U;
-    w.first = at - seg0;
-    w.left = end - at;
-    w.last = min(w.U, w.first + w.left);
-    f_unit = w.first + warp;
-    if (lane == 0) s_ahead[warp] = w;
-    if (tid == 0) s_cur = w;
-  }
-  __syncthreads();
-
-  const int g = lane / 4, t = lane % 4;
-  const int tok_g = g / 2 + 4 * (g % 2);  // token of matrix rows g and (8 further on) g + 8; V's are t, t + 4, t + 8, t + 12
+  W w0;
+  w0.b = s_row;
+  w0.n = tokens_of(a, w0.b);
+  w0.U = units_of<C::UTOK>(w0.n);
+  w0.h = (at - s_begin) / w0.U;
+  w0.begin = s_begin + w0.h * w0.U;
+  w0.first = at - w0.begin;
+  w0.left = end - at;
+  w0.last = min(w0.U, w0.first + w0.left);
   const float sl2 = a.scale * kLog2e;
-  const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-  // this lane's places in a stage
-  const uint32_t k_at = C::K + tok_g * C::ROW + t * (4 * KW), s_at = C::S + tok_g * C::PAIRS;
-  const uint32_t v_at = C::V + t * C::ROW + g * (4 * G);
 
-  // Query rows of a segment, a 16-byte chunk per thread (completed with the thread's next group of copies).
-  auto copy_q = [&](const W& w, int buf) {
-    const int h0 = (w.h % a.blocks) * kHeads, i = tid / (HD / 8);
-    if (i < min(kHeads, a.rep - h0))
-      copy16(smem_u32(smem) + C::Q + buf * C::QBYTES + tid * 16,
-             a.q + w.b * a.qs + (int64_t)(w.h / a.blocks * a.rep + h0 + i) * a.qh + (tid % (HD / 8)) * 8, true);
-  };
-  // A segment's query rows as matrix fragments, a warp per head: scaled so that the largest is in [2^14, 2^15), a
-  // word's channels 0 .. 7 as fp16 pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16; the sums over the groups' channels in
-  // units of 2^8 as three fp16 terms, against the bases; the factor that takes all that back, with the softmax scale.
-  auto prepare_q = [&](const W& w, int buf) {
-    static_assert(kWarps == kHeads, "a warp per head");
+  if (warp >= kWarps) {
+    // ───────────────────────────── helpers ─────────────────────────────
+    const int hw = warp - kWarps, ht = tid - 32 * kWarps;
+    // A segment's query rows as matrix fragments, a warp per head: scaled so that the largest is in [2^14, 2^15), a
+    // word's channels 0 .. 7 as fp16 pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16; the sums over the groups' channels
+    // in units of 2^8 as three fp16 terms, against the bases; the factor that takes all that back, with the softmax
+    // scale.
     constexpr int CH = HD / 32;  // channels of a lane
-    uint8_t* f = smem + C::F + buf * C::FBYTES;
-    const bool real = (w.h % a.blocks) * kHeads + warp < a.rep;
-    float x[CH], mx = 0.f, sum = 0.f;
+    uint32_t raw[kHeads / kHelpers][CH / 2];
+    auto load_q = [&](const W& w) {
+      const int h0 = (w.h % a.blocks) * kHeads;
+      const bf16* src = a.q + w.b * a.qs + (int64_t)(w.h / a.blocks * a.rep + h0) * a.qh + lane * CH;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      x[i] = real ? __bfloat162float(reinterpret_cast<const bf16*>(smem + C::Q + buf * C::QBYTES)[warp * HD + lane * CH + i]) : 0.f;
-      mx = fmaxf(mx, fabsf(x[i]));
-      sum += x[i];
-    }
-    mx = warp_max(mx);
-    const int ex = (mx > 0.f && mx < INFINITY) ? min(14 - ilogbf(mx), 126) : 0;
-    const float up = ldexpf(1.f, ex);
+      for (int k = 0; k < kHeads / kHelpers; ++k) {
+        const int h = hw + k * kHelpers;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int ch = lane * CH + i, word = (ch % 64) / 8 * G + ch / 64, e = ch % 8;
-      reinterpret_cast<__half*>(f)[(((word % KW) * 32 + warp * 4 + word / KW) * 4 + e % 4) * 2 + e / 4] =
-          __float2half_rn(x[i] * (e % 2 ? up * 0.0625f : up));
-    }
+        for (int i = 0; i < CH / 2; ++i)
+          raw[k][i] = h0 + h < a.rep ? *reinterpret_cast<const uint32_t*>(src + h * a.qh + 2 * i) : 0u;
+      }
+    };
+    auto prepare = [&](const W& w, int slot) {
+      uint8_t* f = smem + C::F + slot * C::FBYTES;
 #pragma unroll
-    for (int o = 1; o < 64 / CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int k = 0; k < kHeads / kHelpers; ++k) {
+        const int h = hw + k * kHelpers;
+        float x1[CH];
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float y0 = __shfl_sync(0xffffffffu, sum, i * 16) * up * 0.00390625f;
-      const __half h0 = __float2half_rn(y0);
-      const float y1 = y0 - __half2float(h0);
-      const __half h1 = __float2half_rn(y1), h2 = __float2half_rn(y1 - __half2float(h1));
-      const __half h = lane == 0 ? h0 : lane == 1 ? h1 : lane == 2 ? h2 : __float2half_rn(0.f);
-      if (lane < 4) reinterpret_cast<uint32_t*>(f + C::F_SUM)[i * 32 + warp * 4 + lane] = (uint32_t)__half_as_ushort(h) << 16;
-    }
-    if (lane == 0) reinterpret_cast<float*>(f + C::F_FACTOR)[warp] = ldexpf(sl2, 24 - ex);
-  };
-  copy_q(s_cur, 0);
-  copies_commit();
-
-  // The copies run kStages - 1 units ahead of the arithmetic, across the segments; a unit's page id is read one step
-  // before its copies start.
-  constexpr int kDone = -(1 << 30);  // the share holds no more units for this warp
-  int f_end, f_pi, f_off, f_head, f_page;
-  const int* f_bt;
-  const int step_pi = kWarps / a.upp, step_off = kWarps % a.upp;
-  const uint8_t* kp = a.c.k + lane * 16;
-  const uint8_t* vp = a.c.v + lane * 16;
-  const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + lane * 16;
-  auto aim = [&](const W& w) {
-    f_end = w.n ? w.last : 0;
-    f_pi = f_unit / a.upp;
-    f_off = f_unit % a.upp;
-    f_head = w.h / a.blocks * a.upp;
-    f_bt = a.bt + w.b * a.bt_stride;
-  };
-  auto settle = [&]() {  // on this warp's next unit, if its share has one
-    if (f_unit >= f_end) {
-      W w = s_ahead[warp];
-      do {
-        if (!w.next(a)) {
-          f_unit = kDone;
-          f_end = 0;
-          break;
+        for (int i = 0; i < CH / 2; ++i) {
+          const float2 y = unpack_bf16x2(raw[k][i]);
+          x1[2 * i] = y.x;
+          x1[2 * i + 1] = y.y;
         }
-        f_unit = warp;
-        aim(w);
-      } while (f_unit >= f_end);
-      __syncwarp();
-      if (lane == 0) s_ahead[warp] = w;
-      __syncwarp();
-    }
-    f_page = -1;
-    if (f_unit >= 0) f_page = f_bt[f_pi];
-  };
-  uint32_t valid = 0;  // bit i: the unit i steps ahead has a page
-  auto fetch = [&](uint32_t stage, int steps) {
-    const bool there = (uint32_t)f_page < (uint32_t)a.c.n_pages;
-    valid |= (there ? 1u : 0u) << steps;
-    const uint32_t n = there ? (uint32_t)f_page * (uint32_t)a.page_units + (uint32_t)(f_head + f_off) : 0u;  // unit of the cache
-    const uint8_t* ks = kp + (uint64_t)n * (C::UTOK * C::ROW);
-    const uint8_t* vs = vp + (uint64_t)n * (C::UTOK * C::ROW);
-    const uint8_t* ss = sp + (uint64_t)n * (C::UTOK * C::PAIRS);
-    const uint32_t dst = stage + lane * 16;
+        float mx = 0.f, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < C::UTOK * C::ROW / 512; ++i) {
-      copy16(dst + C::K + 512 * i, ks + 512 * i, there);
-      copy16(dst + C::V + 512 * i, vs + 512 * i, there);
+        for (int i = 0; i < CH; ++i) {
+          mx = fmaxf(mx, fabsf(x1[i]));
+          sum += x1[i];
+        }
+        mx = warp_max(mx);
+        const int ex = (mx > 0.f && mx < INFINITY) ? min(14 - ilogbf(mx), 126) : 0;
+        const float up = ldexpf(1.f, ex);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int ch = lane * CH + i, word = (ch % 64) / 8 * G + ch / 64, e = ch % 8;
+          reinterpret_cast<__half*>(f)[(((word % KW) * 32 + h * 4 + word / KW) * 4 + e % 4) * 2 + e / 4] =
+              __float2half_rn(x1[i] * (e % 2 ? up * 0.0625f : up));
+        }
+#pragma unroll
+        for (int o = 1; o < 64 / CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const float y0 = __shfl_sync(0xffffffffu, sum, i * 16) * up * 0.00390625f;
+          const __half t0 = __float2half_rn(y0);
+          const float y1 = y0 - __half2float(t0);
+          const __half t1 = __float2half_rn(y1), t2 = __float2half_rn(y1 - __half2float(t1));
+          const __half t = lane == 0 ? t0 : lane == 1 ? t1 : lane == 2 ? t2 : __float2half_rn(0.f);
+          if (lane < 4) reinterpret_cast<uint32_t*>(f + C::F_SUM)[i * 32 + h * 4 + lane] = (uint32_t)__half_as_ushort(t) << 16;
+        }
+        if (lane == 0) reinterpret_cast<float*>(f + C::F_FACTOR)[h] = ldexpf(sl2, 24 - ex);
+      }
+      if (ht == 0) s_seg[slot] = w;
+      helper_sync();
+      if (ht == 0) mbar_arrive(&ready[slot]);
+    };
+    W coming = w0;
+    bool more = true;
+    load_q(coming);
+    for (int i = 0; i < kSlots && more; ++i) {
+      prepare(coming, i);
+      more = coming.next(a);
+      if (more) load_q(coming);  // on its way until a slot is free
     }
-    if (C::UTOK * C::PAIRS == 512 || lane < C::UTOK * C::PAIRS / 16) copy16(dst + C::S, ss, there);
-    copies_commit();
-    f_unit += kWarps;
-    f_pi += step_pi;
-    f_off += step_off;
-    if (f_off >= a.upp) {
-      f_off -= a.upp;
-      ++f_pi;
+    int slot = 0, pieces = 0;
+    uint32_t phase = 0;
+    while (true) {
+      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue);
+      helper_sync();
+      if (!s_ok) break;
+      const W w = s_seg[slot];
+      const int hk = w.h / a.blocks, h0 = (w.h % a.blocks) * kHeads, nh = min(kHeads, a.rep - h0);
+      // the warps' weights: eight neighbouring threads have a head's eight states
+      if (ht < kHeads * kWarps) {
+        const int h = ht / kWarps, k = ht % kWarps;
+        const float m1 = sm[slot][k][h];
+        float M = m1;
+#pragma unroll
+        for (int o = 1; o < kWarps; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float e = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+        float L = sl[slot][k][h] * e;
+#pragma unroll
+        for (int o = 1; o < kWarps; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        weight[h][k] = e;
+        if (k == 0) {
+          total_max[h] = M;
+          total_sum[h] = L;
+        }
+      }
+      helper_sync();
+      // a whole segment is done, a piece of one goes to the workspace
+      const bool whole = w.first == 0 && w.last == w.U;
+      const int part = 2 * blockIdx.x + (w.first == 0 ? 1 : 0);
+      const float* states = reinterpret_cast<const float*>(smem + C::STATES + slot * kWarps * C::STATE);
+      for (int i = ht; i < nh * (HD / 4); i += 32 * kHelpers) {
+        const int h = i / (HD / 4), ch = 4 * (i % (HD / 4));
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          const float4 v = *reinterpret_cast<const float4*>(states + k * (C::STATE / 4) + h * C::LD + ch);
+          const float e = weight[h][k];
+          x.x = fmaf(v.x, e, x.x);
+          x.y = fmaf(v.y, e, x.y);
+          x.z = fmaf(v.z, e, x.z);
+          x.w = fmaf(v.w, e, x.w);
+        }
+        const float L = total_sum[h];
+        if (whole) {
+          const float e = L == 0.f ? 0.f : 1.f / L;
+          *reinterpret_cast<uint2*>(a.out + ((int64_t)w.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
+              make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
+        } else {
+          float* pp = a.part + ((int64_t)part * kHeads + h) * C::PART;
+          *reinterpret_cast<float4*>(pp + ch) = x;
+          if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(total_max[h], L);
+        }
+      }
+      if (!whole) {  // at most the first and the last segment of the share
+        if (ht == 0) s_piece[pieces] = {w.b, w.h, w.begin, (uint32_t)w.U, false};
+        ++pieces;
+      }
+      if (!w.more()) break;
+      helper_sync();  // the states and weights have been read
+      if (more) {
+        prepare(coming, slot);
+        more = coming.next(a);
+        if (more) load_q(coming);
+      }
+      if (++slot == kSlots) {
+        slot = 0;
+        phase ^= 1;
+      }
     }
+    if (ht == 0) s_pieces = pieces;
+  } else {
+    // ───────────────────────────── compute ─────────────────────────────
+    const int g = lane / 4, t = lane % 4;
+    const int tok_g = g / 2 + 4 * (g % 2);  // token of matrix rows g and (8 further on) g + 8; V's are t, t + 4, t + 8, t + 12
+    const uint32_t ring = smem_u32(smem) + warp * C::WARP;
+    // this lane's places in a stage
+    const uint32_t k_at = C::K + tok_g * C::ROW + t * (4 * KW), s_at = C::S + tok_g * C::PAIRS;
+    const uint32_t v_at = C::V + t * C::ROW + g * (4 * G);
+    if (lane == 0) s_ahead[warp] = w0;
+    __syncwarp();
+
+    // The copies run STAGES - 1 units ahead of the arithmetic, across the segments; a unit's page id is read one step
+    // before its copies start.
+    constexpr int kDone = -(1 << 30);  // the share holds no more units for this warp
+    int f_end, f_at, f_wrap, f_page;  // f_at: unit within the page of all heads, f_wrap: where this head's part of it ends
+    const int* f_bt;
+    const int step_pi = kWarps / a.upp, step_off = kWarps % a.upp;
+    const uint8_t* kp = a.c.k + lane * 16;
+    const uint8_t* vp = a.c.v + lane * 16;
+    const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + lane * 16;
+    int f_unit = w0.first_of(warp);
+    auto aim = [&](const W& w) {
+      f_end = w.end();
+      f_at = w.h / a.blocks * a.upp;
+      f_wrap = f_at + a.upp;
+      f_at += f_unit % a.upp;
+      f_bt = a.bt + w.b * a.bt_stride + f_unit / a.upp;
+    };
+    auto settle = [&]() {  // on this warp's next unit, if its share has one
+      if (f_unit >= f_end) {
+        W w = s_ahead[warp];
+        do {
+          if (!w.next(a)) {
+            f_unit = kDone;
+            f_end = 0;
+            break;
+          }
+          f_unit = w.first_of(warp);
+          aim(w);
+        } while (f_unit >= f_end);
+        __syncwarp();
+        if (lane == 0) s_ahead[warp] = w;
+        __syncwarp();
+      }
+      f_page = -1;
+      if (f_unit >= 0) f_page = *f_bt;
+    };
+    uint32_t valid = 0;  // bit i: the unit i steps ahead has a page
+    auto fetch = [&](uint32_t stage, int steps) {
+      const bool there = (uint32_t)f_page < (uint32_t)a.c.n_pages;
+      valid |= (there ? 1u : 0u) << steps;
+      const uint32_t n = there ? (uint32_t)f_page * (uint32_t)a.page_units + (uint32_t)f_at : 0u;  // unit of the cache
+      const uint8_t* ks = kp + (uint64_t)n * (C::UTOK * C::ROW);
+      const uint8_t* vs = vp + (uint64_t)n * (C::UTOK * C::ROW);
+      const uint8_t* ss = sp + (uint64_t)n * (C::UTOK * C::PAIRS);
+      const uint32_t dst = stage + lane * 16;
+#pragma unroll
+      for (int i = 0; i < C::UTOK * C::ROW / 512; ++i) {
+        copy16(dst + C::K + 512 * i, ks + 512 * i, there);
+        copy16(dst + C::V + 512 * i, vs + 512 * i, there);
+      }
+      if (C::UTOK * C::PAIRS == 512 || lane < C::UTOK * C::PAIRS / 16) copy16(dst + C::S, ss, there);
+      copies_commit();
+      f_unit += kWarps;
+      f_bt += step_pi;
+      f_at += step_off;
+      if (f_at >= f_wrap) {
+        f_at -= a.upp;
+        ++f_bt;
+      }
+      settle();
+    };
+    aim(w0);
     settle();
-  };
-  aim(s_ahead[warp]);
-  settle();
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(ring + i * C::STAGE, i);
-  uint32_t stage = ring, ahead = ring + (kStages - 1) * C::STAGE;
-  copies_wait<kStages - 1>();  // the query rows
-  __syncthreads();
-  prepare_q(s_cur, 0);
-  __syncthreads();
-  int q_at = 0, pieces = 0;
+    for (int i = 0; i < C::STAGES - 1; ++i) fetch(ring + i * C::STAGE, i);
+    uint32_t stage = ring, ahead = ring + (C::STAGES - 1) * C::STAGE;
+    int slot = 0;
+    uint32_t phase = 0;
 
-  W then = s_cur;
-  while (true) {
-    const W cur = then;
-    const int hk = cur.h / a.blocks, h0 = (cur.h % a.blocks) * kHeads;
-    const int nh = min(kHeads, a.rep - h0);
-    const int b = cur.b;
-    const int u_end = cur.n ? cur.last : 0;
-
-    const uint8_t* frags = smem + C::F + q_at * C::FBYTES;
-    uint32_t zf[2] = {0u, 0u};
-    float cs[2], ce[2];
+    while (true) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&ready[slot], phase, abort_flag, a.err, kErrTimeoutMma))) break;
+      const W* seg = &s_seg[slot];
+      const int n_tok = seg->n, u_end = seg->end();
+      int unit = seg->first_of(warp);
+      const bool more = seg->more();
+      const uint8_t* frags = smem + C::F + slot * C::FBYTES;
+      uint32_t zf[2] = {0u, 0u};
+      float cs[2];
 #pragma unroll
-    for (int i = 0; i < G; ++i) zf[i] = reinterpret_cast<const uint32_t*>(frags + C::F_SUM)[i * 32 + lane];
+      for (int i = 0; i < G; ++i) zf[i] = reinterpret_cast<const uint32_t*>(frags + C::F_SUM)[i * 32 + lane];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      cs[r] = reinterpret_cast<const float*>(frags + C::F_FACTOR)[2 * t + r];
-      ce[r] = cs[r] * 1.52587890625e-5f;  // the sums are in units of 2^8, the products in 2^24
-    }
-    const uint32_t f_at = smem_u32(frags) + lane * 16;
-    // o, z and l are relative to the reference m: p 2^-m; m < the true maximum, so that x fits fp16 well
-    float o[G][4][4], z[G][2], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
-    float lim_p = -1.f, lim_a = kMinA * kGrowA;  // lim_p below 0: no reference yet
+      for (int r = 0; r < 2; ++r) cs[r] = reinterpret_cast<const float*>(frags + C::F_FACTOR)[2 * t + r];
+      const uint32_t frag_at = smem_u32(frags) + lane * 16;
+      // o, z and l are relative to the reference m: p 2^-m; m < the true maximum, so that x fits fp16 well
+      float o[G][4][4], z[G][2], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+      float lim_p = -1.f, lim_a = kMinA * kGrowA;  // lim_p below 0: no reference yet
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
+      for (int i = 0; i < G; ++i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-      z[i][0] = z[i][1] = 0.f;
-    }
-    const bool more = then.next(a);
-    if (more) copy_q(then, q_at ^ 1);
-    int steps = 0;
-    for (int unit = cur.first + warp; unit < u_end; unit += kWarps) {
-      __syncwarp();  // every lane has read the stage that is filled again
-      fetch(ahead, kStages - 1);
-      copies_wait<kStages - 1>();
-      __syncwarp();
-      const uint32_t here = stage;
-      ahead = stage;
-      stage = stage + C::STAGE == ring + C::WARP ? ring : stage + C::STAGE;
-      // tokens of the unit to be counted; the rest may be anything
-      const int count = valid & 1u ? cur.n - unit * C::UTOK : 0;
-      valid >>= 1;
-      ++steps;
-      // scores: tile n, row g + 8 i, head 2 t + r
-      float s[NT][2][2], va[NT][2][G], vz[NT][2][G];
-      {
-        uint32_t kw[NT][2][KW];
-        float acc[NT][G][4];
+        for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+        z[i][0] = z[i][1] = 0.f;
+      }
+      for (; unit < u_end; unit += kWarps) {
+        copies_wait<C::STAGES - 2>();
+        __syncwarp();  // and every lane has read the stage that is filled again below
+        const uint32_t here = stage;
+        // tokens of the unit to be counted; the rest may be anything
+        const int count = valid & 1u ? n_tok - unit * C::UTOK : 0;
+        valid >>= 1;
+        // everything the unit needs from shared memory is asked for at once
+        uint32_t kw[NT][2][KW], qf[KW][4], sw[NT][2][2 * G], vw[NT][4][G];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) load_words<KW>(kw[n][i], here + k_at + (2 * n + i) * 8 * C::ROW);
 #pragma unroll
-        for (int j = 0; j < KW; ++j) {
-          uint32_t qf[4];
-          load_words<4>(qf, f_at + j * 512);
+        for (int j = 0; j < KW; ++j) load_words<4>(qf[j], frag_at + j * 512);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[n][i], here + s_at + (2 * n + i) * 8 * C::PAIRS);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) load_words<G>(vw[n][i], here + v_at + (4 * n + i) * 4 * C::ROW);
+        // scores: tile n, row g + 8 i, head 2 t + r
+        float s[NT][2][2], va[NT][2][G], vz[NT][2][G];
+        {
+          float acc[NT][G][4], e[NT][4];
+#pragma unroll
+          for (int j = 0; j < KW; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              uint32_t w0 = kw[n][0][j], w1 = kw[n][1][j];
+              if (j < G)
+                mma_f16_first(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
+              else
+                mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
+              w0 >>= 8;
+              w1 >>= 8;
+              mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2], qf[j][3]);
+            }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)  // sum_g z_g sum(q_g): the pairs (a, z) against (0, sum)
+            mma_f16_first(e[n], sw[n][0][0], sw[n][1][0], G == 2 ? sw[n][0][G - 1] : 0u, G == 2 ? sw[n][1][G - 1] : 0u, zf[0], zf[1]);
+          fetch(ahead, C::STAGES - 2);  // the next copies, while the products come in
+          ahead = stage;
+          stage = stage + C::STAGE == ring + C::WARP ? ring : stage + C::STAGE;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            uint32_t w0 = kw[n][0][j], w1 = kw[n][1][j];
-            if (j < G)
-              mma_f16_first(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[0], qf[1]);
-            else
-              mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[0], qf[1]);
-            w0 >>= 8;
-            w1 >>= 8;
-            mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[2], qf[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float d[2] = {0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < G; ++j) {
+                const float ka = __low2float(*reinterpret_cast<const __half2*>(&sw[n][i][j]));
+                const float2 v2 = unpack_half2(sw[n][i][G + j]);
+                va[n][i][j] = v2.x;
+                vz[n][i][j] = v2.y;
+                d[0] = fmaf(ka, acc[n][j][2 * i], d[0]);
+                d[1] = fmaf(ka, acc[n][j][2 * i + 1], d[1]);
+              }
+#pragma unroll
+              for (int r = 0; r < 2; ++r)  // the sums are in units of 2^8, the products in 2^24
+                s[n][i][r] = fmaf(cs[r], fmaf(e[n][2 * i + r], 1.52587890625e-5f, d[r]), -m[r]);
+            }
+          }
+        }
+        if (count < C::UTOK) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (n * kTok + tok_g + 8 * i >= count) {
+                s[n][i][0] = s[n][i][1] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < G; ++j) va[n][i][j] = vz[n][i][j] = 0.f;
+              }
+        }
+        float p[NT][2][2], top_p = 0.f, top_a = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              p[n][i][r] = ex2(s[n][i][r]);
+              top_p = fmaxf(top_p, p[n][i][r]);
+            }
+#pragma unroll
+            for (int j = 0; j < G; ++j) top_a = fmaxf(top_a, va[n][i][j]);
+          }
+        if (__any_sync(0xffffffffu, top_p > lim_p || top_a > lim_a)) {
+          // move the reference: to the true maxima, less what brings x to kBoost
+          const float A0 = lim_a / kGrowA, A = max_over_rows(fmaxf(A0, top_a)), lift = lg2(kBoost / A);
+          bool found = false;
+          float keep[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float top = s[0][0][r];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][0][r], s[n][1][r]));
+            top = max_over_rows(top) + m[r];
+            if (lim_p > 0.f) top = fmaxf(top, m[r] + lg2(kBoost / A0));
+            const bool real = top != -INFINITY;
+            const float to = real ? top - lift : m[r];
+            keep[r] = lim_p > 0.f ? ex2(m[r] - to) : 0.f;
+            found |= real;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) p[n][i][r] = ex2(s[n][i][r] + (m[r] - to));
+            m[r] = to;
+            l[r] *= keep[r];
+          }
+          if (__any_sync(0xffffffffu, found)) lim_p = kBoost / A * kGrowP;
+          lim_a = A * kGrowA;
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[j][q][x] *= keep[x & 1];
+            z[j][0] *= keep[0];
+            z[j][1] *= keep[1];
           }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint32_t sw[2][2 * G];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) load_words<2 * G>(sw[i], here + s_at + (2 * n + i) * 8 * C::PAIRS);
-          float e[4];  // sum_g z_g sum(q_g): the pairs (a, z) against (0, sum)
-          mma_f16_first(e, sw[0][0], sw[1][0], G == 2 ? sw[0][G - 1] : 0u, G == 2 ? sw[1][G - 1] : 0u, zf[0], zf[1]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float d[2] = {0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-              const float ka = __low2float(*reinterpret_cast<const __half2*>(&sw[i][j]));
-              const float2 v2 = unpack_half2(sw[i][G + j]);
-              va[n][i][j] = v2.x;
-              vz[n][i][j] = v2.y;
-              d[0] = fmaf(ka, acc[n][j][2 * i], d[0]);
-              d[1] = fmaf(ka, acc[n][j][2 * i + 1], d[1]);
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) s[n][i][r] = fmaf(cs[r], d[r], fmaf(ce[r], e[2 * i + r], -m[r]));
-          }
-        }
-      }
-      if (count < C::UTOK) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (n * kTok + tok_g + 8 * i >= count) {
-              s[n][i][0] = s[n][i][1] = -INFINITY;
-#pragma unroll
-              for (int j = 0; j < G; ++j) va[n][i][j] = vz[n][i][j] = 0.f;
-            }
-      }
-      float p[NT][2][2], top_p = 0.f, top_a = 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            p[n][i][r] = ex2(s[n][i][r]);
-            top_p = fmaxf(top_p, p[n][i][r]);
+            l[r] += p[n][0][r] + p[n][1][r];
+#pragma unroll
+            for (int j = 0; j < G; ++j) z[j][r] = fmaf(p[n][0][r], vz[n][0][j], fmaf(p[n][1][r], vz[n][1][j], z[j][r]));
           }
 #pragma unroll
-          for (int j = 0; j < G; ++j) top_a = fmaxf(top_a, va[n][i][j]);
-        }
-      if (__any_sync(0xffffffffu, top_p > lim_p || top_a > lim_a)) {
-        // move the reference: to the true maxima, less what brings x to kBoost
-        const float A0 = lim_a / kGrowA, A = max_over_rows(fmaxf(A0, top_a)), lift = lg2(kBoost / A);
-        bool found = false;
-        float keep[2];
+          for (int j = 0; j < G; ++j) {
+            const uint32_t b0 = transpose8x8(pack_half2(p[n][0][0] * va[n][0][j], p[n][0][1] * va[n][0][j]));
+            const uint32_t b1 = transpose8x8(pack_half2(p[n][1][0] * va[n][1][j], p[n][1][1] * va[n][1][j]));
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float top = s[0][0][r];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][0][r], s[n][1][r]));
-          top = max_over_rows(top) + m[r];
-          if (lim_p > 0.f) top = fmaxf(top, m[r] + lg2(kBoost / A0));
-          const bool real = top != -INFINITY;
-          const float to = real ? top - lift : m[r];
-          keep[r] = lim_p > 0.f ? ex2(m[r] - to) : 0.f;
-          found |= real;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) p[n][i][r] = ex2(s[n][i][r] + (m[r] - to));
-          m[r] = to;
-          l[r] *= keep[r];
-        }
-        if (__any_sync(0xffffffffu, found)) lim_p = kBoost / A * kGrowP;
-        lim_a = A * kGrowA;
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[j][q][x] *= keep[x & 1];
-          z[j][0] *= keep[0];
-          z[j][1] *= keep[1];
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        uint32_t vw[4][G];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<G>(vw[i], here + v_at + (4 * n + i) * 4 * C::ROW);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          l[r] += p[n][0][r] + p[n][1][r];
-#pragma unroll
-          for (int j = 0; j < G; ++j) z[j][r] = fmaf(p[n][0][r], vz[n][0][j], fmaf(p[n][1][r], vz[n][1][j], z[j][r]));
-        }
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const uint32_t b0 = transpose8x8(pack_half2(p[n][0][0] * va[n][0][j], p[n][0][1] * va[n][0][j]));
-          const uint32_t b1 = transpose8x8(pack_half2(p[n][1][0] * va[n][1][j], p[n][1][1] * va[n][1][j]));
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half ..
-            const uint32_t sel = half ? 0x7632u : 0x5410u;
-            uint32_t x01 = __byte_perm(vw[0][j], vw[1][j], sel), x23 = __byte_perm(vw[2][j], vw[3][j], sel);
-            mma_f16(o[j][2 * half], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
-            x01 >>= 8;
-            x23 >>= 8;
-            mma_f16(o[j][2 * half + 1], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
+            for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half ..
+              const uint32_t sel = half ? 0x7632u : 0x5410u;
+              uint32_t x01 = __byte_perm(vw[n][0][j], vw[n][1][j], sel), x23 = __byte_perm(vw[n][2][j], vw[n][3][j], sel);
+              mma_f16(o[j][2 * half], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
+              x01 >>= 8;
+              x23 >>= 8;
+              mma_f16(o[j][2 * half + 1], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
+            }
           }
         }
       }
-    }
 
-    // the warp's state, in the stage that is free: o in units of V, relative to m
-    float* state = reinterpret_cast<float*>(smem + (ahead - smem_u32(smem)));
+      // the warp's state: o in units of V, relative to m
+      float* state = reinterpret_cast<float*>(smem + C::STATES + (slot * kWarps + warp) * C::STATE);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] = sum_over_rows(l[r]);
+      for (int r = 0; r < 2; ++r) {
+        l[r] = sum_over_rows(l[r]);
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        z[j][r] = sum_over_rows(z[j][r]);
-        constexpr float f0 = 16777216.f, f1 = 1048576.f;
-        float x[8];
+        for (int j = 0; j < G; ++j) {
+          z[j][r] = sum_over_rows(z[j][r]);
+          constexpr float f0 = 16777216.f, f1 = 1048576.f;
+          float x[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          x[2 * q] = fmaf(o[j][q][r], f0, z[j][r]);
-          x[2 * q + 1] = fmaf(o[j][q][2 + r], f1, z[j][r]);
+          for (int q = 0; q < 4; ++q) {
+            x[2 * q] = fmaf(o[j][q][r], f0, z[j][r]);
+            x[2 * q + 1] = fmaf(o[j][q][2 + r], f1, z[j][r]);
+          }
+          float4* d = reinterpret_cast<float4*>(state + (2 * t + r) * C::LD + 64 * j + 8 * g);
+          d[0] = make_float4(x[0], x[1], x[2], x[3]);
+          d[1] = make_float4(x[4], x[5], x[6], x[7]);
         }
-        float4* d = reinterpret_cast<float4*>(state + (2 * t + r) * C::LD + 64 * j + 8 * g);
-        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        if (g == 0) {
+          sm[slot][warp][2 * t + r] = lim_p < 0.f ? -INFINITY : m[r];
+          sl[slot][warp][2 * t + r] = l[r];
+        }
       }
-      if (g == 0) {
-        sm[warp][2 * t + r] = lim_p < 0.f ? -INFINITY : m[r];
-        sl[warp][2 * t + r] = l[r];
-      }
-    }
-    if (lane == 0) so[warp] = state;
-    if (steps < kStages) {  // after kStages steps the next query rows have arrived anyway
-      copies_commit();
-      copies_wait<0>();
-    }
-    __syncthreads();
-    // join the warps; a whole segment is done, a piece of one goes to the workspace
-    const bool whole = cur.first == 0 && cur.last == cur.U;
-    const int slot = 2 * blockIdx.x + (cur.first == 0 ? 1 : 0);
-    bf16* dst = a.out + ((int64_t)b * a.Hq + hk * a.rep + h0) * HD;
-    for (int i = tid; i < nh * (HD / 2); i += kThreads) {
-      const int h = i / (HD / 2), ch = 2 * (i % (HD / 2));
-      float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[w][h]);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float c = sm[w][h] == -INFINITY ? 0.f : ex2(sm[w][h] - M);
-        L = fmaf(sl[w][h], c, L);
-        x = fmaf(so[w][h * C::LD + ch], c, x);
-        y = fmaf(so[w][h * C::LD + ch + 1], c, y);
-      }
-      if (whole) {
-        const float c = L == 0.f ? 0.f : 1.f / L;
-        *reinterpret_cast<uint32_t*>(dst + (int64_t)h * HD + ch) = pack_bf16x2(x * c, y * c);
-      } else {
-        float* pp = a.part + ((int64_t)slot * kHeads + h) * C::PART;
-        *reinterpret_cast<float2*>(pp + ch) = make_float2(x, y);
-        if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(M, L);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&done[slot]);
+      if (!more) break;
+      if (++slot == kSlots) {
+        slot = 0;
+        phase ^= 1;
       }
     }
-    if (!whole) {  // at most the first and the last segment of the share
-      if (tid == 0) s_piece[pieces] = {b, cur.h, seg0, (uint32_t)cur.U, false};
-      ++pieces;
-    }
-    if (!more) break;
-    seg0 += cur.U;
-    q_at ^= 1;
-    prepare_q(then, q_at);
-    __syncthreads();  // the states have been read, the fragments are there
+    copies_wait<0>();
   }
-  copies_wait<0>();
-  if (pieces == 0) return;
+
   // The last CTA to arrive at a segment joins its pieces; arrivals wait until the share is done, so that nothing else
   // waits for their round trip.
   __syncthreads();
+  const int pieces = s_pieces;
+  if (pieces == 0) return;
   if (tid < pieces) {
     Piece& x = s_piece[tid];
     const uint32_t c0 = shares.owner(x.first), np = shares.owner(x.first + x.n - 1) - c0 + 1;
@@ -671,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(const Args a) {
     const int np = x.n;
     float M = -INFINITY, L = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 16;
     for (int c0 = 0; c0 < np; c0 += kBatch) {
       float4 v[kBatch];
       float2 ml[kBatch];
@@ -733,26 +816,26 @@ void launch(Args a, cudaStream_t st) {
     MESHY_CUDA_CHECK(cudaFuncSetAttribute(kv4_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     set[dev] = true;
   }
-  launch_pdl(kv4_attn_kernel<HD, NT>, dim3(2 * sm_count()), dim3(kThreads), C::SMEM, st, a);
+  launch_pdl(kv4_attn_kernel<HD, NT>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
 }
 
 }  // namespace
 
-int kv4_attention_ctas() { return 2 * sm_count(); }
+int kv4_attention_ctas() { return sm_count(); }
 int64_t kv4_attention_segments(int B, int Hq, int Hkv) { return (int64_t)B * Hkv * ((Hq / Hkv + kHeads - 1) / kHeads); }
 
 void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* bt, int64_t bt_stride, int max_pages,
-                   const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived,
+                   const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived, int* err,
                    cudaStream_t st) {
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
   const Args a{q, qs, qh,  c,   bt,    bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads,
-               0, 0,  scale, out, part, arrived};
+               0, 0,  scale, out, part, arrived, err};
   const bool pairs = c.page % 32 == 0;
   if (c.hd == 128)
     pairs ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
   else
-    pairs ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
+    c.page % 64 == 0 ? launch<64, 4>(a, st) : pairs ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
 }
 
 }  // namespace meshy

@@ -812,15 +812,18 @@ class RolloutEngine:
         n = len(self.running)
         if n == 0:
             return
-        if self._mega is not None:
-            # the whole-step kernel reports a timed-out wait through the device error word (this is a
-            # host sync, like the finish-flag read below)
+        if self._mega is not None or (self.kv4 and self.cuda):
+            # kernels with waits of their own report one that timed out through the device error word (this is
+            # a host sync, like the finish-flag read below)
             from ..ops._ext import ext
 
             err = int(ext().device_error())
             if err:
                 ext().clear_device_error()
-                self._mega.reset()
+                if self._mega is not None:
+                    self._mega.reset()
+                if self.kv4:
+                    ext().kv4_reset()
                 raise RuntimeError(f"decode kernel reported device error {err} (a bounded wait timed out)")
         done = self.st["done"][:n].tolist()
         rows = [i for i, d in enumerate(done) if d]
