@@ -551,6 +551,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
         // tokens of the unit to be counted; the rest may be anything
         const int count = valid & 1u ? n_tok - unit * C::UTOK : 0;
         valid >>= 1;
+        // the next copies first: after the products of K, 8 rows of 131072 tokens took 66.2 us instead of 64.8
+        fetch(ahead, C::STAGES - 2);
+        ahead = stage;
+        stage = stage + C::STAGE == ring + C::WARP ? ring : stage + C::STAGE;
         // everything the unit needs from shared memory is asked for at once
         uint32_t kw[NT][2][KW], qf[KW][4], sw[NT][2][2 * G], vw[NT][4][G];
 #pragma unroll
@@ -587,9 +591,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)  // sum_g z_g sum(q_g): the pairs (a, z) against (0, sum)
             mma_f16_first(e[n], sw[n][0][0], sw[n][1][0], G == 2 ? sw[n][0][G - 1] : 0u, G == 2 ? sw[n][1][G - 1] : 0u, zf[0], zf[1]);
-          fetch(ahead, C::STAGES - 2);  // the next copies, while the products come in
-          ahead = stage;
-          stage = stage + C::STAGE == ring + C::WARP ? ring : stage + C::STAGE;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
