@@ -8,7 +8,7 @@ namespace meshy {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 __device__ __forceinline__ int64_t slot_of(SlotIds s, int i) {
   return s.wide ? reinterpret_cast<const int64_t*>(s.p)[i] : (int64_t) reinterpret_cast<const int*>(s.p)[i];
