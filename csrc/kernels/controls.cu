@@ -21,7 +21,7 @@ __device__ __forceinline__ int64_t slot_of(SlotIds s, int i) {
 // row in shared memory instead made every CTA read all tokens: 22 us where this takes 16 (64 rows of up to 16384
 // tokens).
 constexpr int kCluster = 8;
-constexpr int kLoadThreads = 512;
+constexpr int kLoadThreads = 256;
 
 __global__ void __launch_bounds__(kLoadThreads) __cluster_dims__(kCluster, 1, 1)
     load_tokens_kernel(ControlsView c, SlotIds slots, const int64_t* __restrict__ tokens, int64_t total,
