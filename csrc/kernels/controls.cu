@@ -8,7 +8,7 @@ namespace meshy {
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 64;
 
 __device__ __forceinline__ int64_t slot_of(SlotIds s, int i) {
   return s.wide ? reinterpret_cast<const int64_t*>(s.p)[i] : (int64_t) reinterpret_cast<const int*>(s.p)[i];
@@ -54,30 +54,50 @@ __global__ void __launch_bounds__(kLoadThreads) __cluster_dims__(kCluster, 1, 1)
 // ─── controls ──────────────────────────────────────────────────────────────
 // A CTA owns kChunk entries of one row (whole words of both bit rows). Few tokens of a vocabulary have occurred (some
 // thousands of 150 thousand), so the work is split: a dense pass copies the logits and writes -inf where the mask
-// forbids, with nothing but wide loads and stores; then each thread looks at 16 bits of the seen row and rewrites the
-// entries that are set, from their logits and counts. In place the dense pass touches masked entries only, so a call
-// costs V / 8 bytes a bit row and what it changes.
+// forbids, with nothing but 16-byte loads and stores; then each thread looks at 16 bits of the seen row and rewrites
+// the entries that are set, from their logits and counts. In place the dense pass touches masked entries only, so a
+// call costs V / 8 bytes a bit row and what it changes.
+// A CTA is a chain of four dependent reads (slot, the row's settings and bits, counts, the entry a bias lands on), so
+// the call is bound by how many CTAs are under way: small ones (64 threads: 41.8 us on 256 rows of 128256 bf16 logits,
+// 128: 43.3, 256: 48), two seen entries at a time (four: 44.4, for its registers), logits kept as they are stored
+// until they are written, biases read at the start. 41.8 us is 4.9 TB/s of the 204 MB that have to move; 64 rows of
+// 151936 fp32 logits take 17.8 us (4.5 TB/s).
 constexpr int kChunk = 16 * kThreads;
 
+__device__ __forceinline__ float entry(const float* p) { return *p; }
+__device__ __forceinline__ float entry(const bf16* p) { return __bfloat162float(*p); }
+
+// E neighbouring logits as they are stored; widened when they are used
+template <typename T, int E>
+struct Entries;
 template <int E>
-__device__ __forceinline__ void load_entries(float* x, const float* p) {
-  if constexpr (E == 4) {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-  } else {
-    x[0] = *p;
+struct Entries<float, E> {
+  float x[E];
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (E == 4)
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+    else
+      x[0] = *p;
   }
-}
+  __device__ __forceinline__ void widen(float* y) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = x[e];
+  }
+};
 template <int E>
-__device__ __forceinline__ void load_entries(float* x, const bf16* p) {
-  if constexpr (E == 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-  } else {
-    x[0] = __bfloat162float(*p);
+struct Entries<bf16, E> {
+  uint32_t x[(E + 1) / 2];
+  __device__ __forceinline__ void load(const bf16* p) {
+    if constexpr (E == 8)
+      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(p);
+    else
+      x[0] = *reinterpret_cast<const uint16_t*>(p);
   }
-}
+  __device__ __forceinline__ void widen(float* y) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = __uint_as_float(e % 2 ? x[e / 2] & 0xFFFF0000u : x[e / 2] << 16);
+  }
+};
 
 template <typename T, bool IN_PLACE, bool VEC>
 __global__ void __launch_bounds__(kThreads)
@@ -88,14 +108,22 @@ __global__ void __launch_bounds__(kThreads)
   pdl_trigger();
   const T* z = logits + b * ls;
   float* o = out + b * os;
-  constexpr int E = VEC ? 4 : 1, STEPS = kChunk / (E * kThreads), BATCH = 4;  // steps whose loads are under way together
+  constexpr int E = VEC ? (sizeof(T) == 4 ? 4 : 8) : 1, STEPS = kChunk / (E * kThreads), BATCH = STEPS < 4 ? STEPS : 4;
   constexpr uint32_t FIELD = (1u << E) - 1u;
-  float x[BATCH][E];
+  Entries<T, E> x[BATCH];
   auto load_batch = [&](int k0) {
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
       const int v = v0 + ((k0 + k) * kThreads + tid) * E;
-      if (v < v1) load_entries<E>(x[k], z + v);
+      if (v < v1) x[k].load(z + v);
+    }
+  };
+  auto store = [&](int v, const float* y) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(o + v + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+    } else {
+      o[v] = y[0];
     }
   };
   if (!IN_PLACE) load_batch(0);  // on their way while the slot is looked up
@@ -117,6 +145,13 @@ __global__ void __launch_bounds__(kThreads)
   }
   const float rep = c.repetition[r], freq = c.frequency[r], pres = c.presence[r];
   const bool masked = on && c.mask_on[r] != 0;
+  // this thread's bias, looked up early
+  int bias_at = -1;
+  float bias = 0.f;
+  if (on && tid < c.K) {
+    bias_at = c.bias_ids[r * c.K + tid];
+    bias = c.bias_vals[r * c.K + tid];
+  }
   // this thread's 16 entries of the sparse pass: seen, and allowed (the others stay -inf)
   const int w0 = v0 + 16 * tid;
   uint32_t bits = 0u;
@@ -124,52 +159,64 @@ __global__ void __launch_bounds__(kThreads)
     bits = (seen[w0 / 32] >> (w0 % 32)) & 0xFFFFu;
     if (masked) bits &= mask[w0 / 32] >> (w0 % 32);
   }
-  if (!IN_PLACE || masked) {
+  if (masked) {
     for (int k0 = 0; k0 < STEPS; k0 += BATCH) {
       if (!IN_PLACE && k0 > 0) load_batch(k0);
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
         const int v = v0 + ((k0 + k) * kThreads + tid) * E;
         if (v >= v1) break;
-        const uint32_t m = masked ? (mask[v / 32] >> (v % 32)) & FIELD : FIELD;
+        const uint32_t m = (mask[v / 32] >> (v % 32)) & FIELD;
         if (IN_PLACE && m == FIELD) continue;
-        if (IN_PLACE && m != 0u) load_entries<E>(x[k], z + v);
+        if (IN_PLACE && m != 0u) x[k].load(z + v);
+        float y[E];
+        x[k].widen(y);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (!((m >> e) & 1u)) x[k][e] = -INFINITY;
-        if constexpr (VEC)
-          *reinterpret_cast<float4*>(o + v) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
-        else
-          o[v] = x[k][0];
+          if (!((m >> e) & 1u)) y[e] = -INFINITY;
+        store(v, y);
+      }
+    }
+  } else if (!IN_PLACE) {
+    for (int k0 = 0; k0 < STEPS; k0 += BATCH) {
+      if (k0 > 0) load_batch(k0);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int v = v0 + ((k0 + k) * kThreads + tid) * E;
+        if (v >= v1) break;
+        float y[E];
+        x[k].widen(y);
+        store(v, y);
       }
     }
   }
   if (!on) return;
   __syncthreads();  // the dense pass of this chunk is written
   while (bits) {
-    constexpr int N = 4;  // entries whose loads are under way together
+    constexpr int N = 2;  // entries whose loads are under way together
     int v[N], n[N];
-    float y[N][1];
+    float y[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = bits ? w0 + __ffs(bits) - 1 : -1;
       bits &= bits - 1u;
       if (v[i] >= 0) {
         n[i] = counts[v[i]];
-        load_entries<1>(y[i], z + v[i]);
+        y[i] = entry(z + v[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (v[i] >= 0) {
-        const float p = y[i][0] > 0.f ? y[i][0] / rep : y[i][0] * rep;
+        const float p = y[i] > 0.f ? y[i] / rep : y[i] * rep;
         o[v[i]] = p - freq * (float)n[i] - (n[i] > 0 ? pres : 0.f);
       }
   }
   if (c.K == 0) return;
   // biases, on what this CTA has written (ids of a row are distinct; a masked entry stays -inf)
   __syncthreads();
-  for (int j = tid; j < c.K; j += kThreads) {
+  if (bias_at >= v0 && bias_at < v1) o[bias_at] += bias;
+  for (int j = tid + kThreads; j < c.K; j += kThreads) {
     const int v = c.bias_ids[r * c.K + j];
     if (v >= v0 && v < v1) o[v] += c.bias_vals[r * c.K + j];
   }
@@ -180,9 +227,11 @@ void launch_controls(const void* logits, int64_t ls, ControlsView c, SlotIds slo
                      int B, float* out, int64_t os, cudaStream_t st) {
   const T* z = reinterpret_cast<const T*>(logits);
   const dim3 grid((c.V + kChunk - 1) / kChunk, B);
-  // four entries at a time where every row starts on a boundary of four and ends on one
-  const bool vec = c.V % 4 == 0 && (B == 1 || (ls % 4 == 0 && os % 4 == 0)) &&
-                   reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  // 16 bytes at a time where every row starts on such a boundary and ends on one: 41.8 us on 256 rows of 128256 bf16
+  // logits where one at a time takes 56 (64 rows of 151936 fp32: 17.8, 20.2)
+  const int e = 16 / sizeof(T);
+  const bool vec = c.V % e == 0 && (B == 1 || (ls % e == 0 && os % 4 == 0)) &&
+                   reinterpret_cast<uintptr_t>(logits) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   const bool in_place = logits == out;
   auto go = [&](auto k) { launch_pdl(k, grid, dim3(kThreads), 0, st, z, ls, c, slots, fresh, done, out, os); };
   if (in_place)
