@@ -6,9 +6,11 @@
 // lose a step wherever a channel offset is some ten times the spread). Every step is an exactly rounded operation,
 // so the bytes are the same wherever the format is computed.
 //
-// Both kernels move 16 bytes of bf16 against 4 of nibbles per thread and are meant to run at the memory's rate; the
-// quotients are what stands in the way (nine channels a clock and SM at that rate), so each is one product and two
-// fused multiply-adds with the group's reciprocal instead of a division.
+// Both kernels should run at the memory's rate; in the write the quotients stand in the way (nine channels a clock and
+// SM at that rate), so each is a product and two fused multiply-adds with the group's reciprocal instead of a division,
+// on pairs of channels in one instruction. 32768 tokens of 8 heads of 128, at slots of shuffled pages: the write takes
+// 35.7 us for 172 MB (4.8 TB/s; instruction issue, 68 % of the slots before the quotients went in pairs at 38.2 us),
+// the read-back 28 us for as much (6.2 TB/s, the memory's rate). Decode-size calls take 5 us, launch and latency.
 #include <cuda_runtime.h>
 
 #include "kv4.h"
@@ -17,7 +19,7 @@ namespace meshy {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr float kHalfMax = 65504.f;
 
 // n / d for n < 2^31, as (n m) >> s with m = ceil(2^s / d), s = 31 + ceil(log2 d) (Granlund and Montgomery, 1994).
@@ -35,6 +37,28 @@ struct FastDiv {
 __device__ __forceinline__ float quotient(float x, float y, float rcp) {
   const float q = x * rcp;
   return fmaf(fmaf(-q, y, x), rcp, q);
+}
+
+// Two fp32 numbers and their sums and products, one instruction to a pair.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // 1 / y, correctly rounded for every positive fp16 number y: the hardware's approximation and one Newton step.
@@ -85,29 +109,33 @@ __device__ __forceinline__ void quantise(const uint4& u0, const uint4& u1, int l
   // Nothing leaves [0, 15] while rounding moved the base by less than 0.4 steps and the scale by less than 2^-11 of it.
   const bool tight = fabsf(lo) * 0.00048828125f < 0.4f * af && af >= 6.1035156e-5f && fmaxf(top, bot) <= kHalfMax;
   if (row == nullptr) return;
+  // Adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits; the constant's own
+  // bits leave the word again.
+  const uint64_t nz = pair(-zf, -zf), na = pair(-af, -af), rr = pair(rcp, rcp), round2 = pair(12582912.f, 12582912.f);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float n[8];
+    uint64_t n2[4];  // rounded quotients, two to a register pair
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float2 f = unpack_bf16x2(us[4 * w + q]);
-      n[2 * q] = quotient(f.x - zf, af, rcp);
-      n[2 * q + 1] = quotient(f.y - zf, af, rcp);
+      const uint64_t x = add2(pair(f.x, f.y), nz), y = mul2(x, rr);
+      n2[q] = add2(fma2(fma2(y, na, x), rr, y), round2);
     }
     if (!tight) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float2 f = unpack_bf16x2(us[4 * w + q / 2]);
-        const float x = fminf(fmaxf(q % 2 ? f.y : f.x, -kHalfMax), kHalfMax);
-        n[q] = fminf(fmaxf(quotient(x - zf, af, rcp), 0.f), 15.f);
+      for (int q = 0; q < 4; ++q) {
+        const float2 f = unpack_bf16x2(us[4 * w + q]);
+        const float x0 = fminf(fmaxf(f.x, -kHalfMax), kHalfMax), x1 = fminf(fmaxf(f.y, -kHalfMax), kHalfMax);
+        const float n0 = fminf(fmaxf(quotient(x0 - zf, af, rcp), 0.f), 15.f);
+        const float n1 = fminf(fmaxf(quotient(x1 - zf, af, rcp), 0.f), 15.f);
+        n2[q] = add2(pair(n0, n1), round2);
       }
     }
-    // Adding 1.5 2^23 rounds to whole numbers, halves to even, and leaves the number in the low bits; the constant's
-    // own bits leave the sum again.
     constexpr uint32_t kRoundBits = 0x4B400000u;  // 1.5 2^23
     uint32_t word = 0u - kRoundBits * 0x11111111u;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) word += __float_as_uint(n[q] + 12582912.f) * (1u << (4 * q));
+    for (int q = 0; q < 4; ++q)
+      word += (uint32_t)n2[q] * (1u << (8 * q)) + (uint32_t)(n2[q] >> 32) * (1u << (8 * q + 4));
     row[(lane % 4 * 2 + w) * G + lane / 4] = af > 0.f ? word : 0u;
   }
   if (lane % 4 == 0) pairs[lane / 4] = __halves2half2(a, z);
@@ -205,7 +233,8 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Four heads to a thread once that still leaves every SM its threads; one in a decode step, where only latency counts.
+// Four heads to a thread once that still leaves every SM its threads (32768 tokens of 8 heads: 35.7 us, with two 38.3,
+// with eight 38.7); one in a decode step, where a thread's heads come after one another and only latency counts.
 constexpr int kManyRows = 1 << 16;
 
 struct Split {
