@@ -29,8 +29,8 @@ struct SlotIds {
 
 // State of n requests from their ``total`` tokens so far: row i's are tokens[cu[i] .. cu[i + 1]), of which the first
 // n_prompt[i] belong to the prompt. The rows of slots[i] are rewritten; other rows keep their state.
-void load_tokens(ControlsView c, SlotIds slots, const int64_t* tokens, int64_t total, const int* cu, const int* n_prompt, int n,
-                 cudaStream_t st);
+void load_tokens(ControlsView c, SlotIds slots, const int64_t* tokens, int64_t total, const int* cu,
+                 const int* n_prompt, int n, cudaStream_t st);
 // out[b, v] = penalised, biased and masked logits[b, v]. ``logits`` are fp32 or bf16 with row stride ls; ``out`` is
 // fp32 with row stride os and may be ``logits`` itself. With ``fresh`` [B] the token fresh[b] is first counted as
 // generated in slot slots[b] (unless it is negative, or done[b] is nonzero). A slot outside [0, R) has no controls.

@@ -29,10 +29,10 @@ void kv4_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
 // The bf16 values the cache stands for at ``slots``: k, v [T, Hkv, hd] contiguous (zero for a slot outside it).
 void kv4_read(KV4View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st);
 // Decode attention of q [B, Hq, hd] (strides qs between rows, qh between heads) over each row's first
-// seq_lens[b] tokens, whose pages are bt[b, :]; a row of length 0 gives zeros. A bounded wait inside the kernel that gives
-// up records its code in ``err``. ``part`` holds
-// kv4_part_floats(hd) floats, ``arrived`` kv4_attention_segments() counters that are zero between launches; launches
-// that may run at the same time need workspaces of their own.
+// seq_lens[b] tokens, whose pages are bt[b, :]; a row of length 0 gives zeros. A bounded wait inside the kernel that
+// gives up records its code in ``err``. ``part`` holds kv4_part_floats(hd) floats, ``arrived``
+// kv4_attention_segments() counters that are zero between launches; launches that may run at the same time need
+// workspaces of their own.
 int kv4_attention_ctas();
 int64_t kv4_attention_segments(int B, int Hq, int Hkv);
 inline int64_t kv4_part_floats(int hd) { return (int64_t)2 * kv4_attention_ctas() * 8 * (hd + 4); }

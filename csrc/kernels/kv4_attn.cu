@@ -22,18 +22,26 @@
 // normaliser and the bases' part stay in 32 bits.
 //
 // Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (16 where a
-// page is not a multiple of 32, 64 at head width 64 where it is one of 64) and every CTA, one per SM, takes an equal share of the sum, whatever the lengths: the
-// lengths are read on the device, a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment
-// that spans CTAs leaves partial sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one
-// order, and results do not depend on timing.
+// page is not a multiple of 32; 64 at head width 64 where it is one of 64, as bytes of a unit are what hides latency)
+// and every CTA, one per SM, takes an equal share of the sum, whatever the lengths: they are read on the device, so a
+// captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs leaves partial
+// sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and results do not
+// depend on timing.
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory, filled by
 // 16-byte asynchronous copies two units ahead, across the segments, and at a segment's end leaves its state in one of
 // kSlots slots and goes on. Four helper warps prepare the query fragments of the coming segments and join the eight
 // states of the finished ones behind the others' backs. (With the joins in the computing warps' way, 256 rows of about
 // 1200 tokens took 105 us instead of 96; two CTAs of eight such warps and 128 registers each ran no faster on long rows
-// than one CTA with 168, as one of the two is always favoured and the other finishes alone.) Every wait is bounded; one
-// that gives up records an error code.
+// than one CTA with 168, as one of the two is always favoured and the other finishes alone; copies issued by warps of
+// their own left fewer registers and one more wait to a unit: 72 us instead of 66 on 8 rows of 131072 tokens.) Every
+// wait is bounded; one that gives up records an error code.
+//
+// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 302 MB) 65-68 us, 4.5 TB/s; 256 rows of up to 1500 (32 / 8
+// heads, 360 MB) 93 us, 3.9 TB/s; 64 rows of up to 8192 (12 / 2) 35 us; one row of 700 tokens 8.7 us. Bound by the
+// instructions' latency, not by memory: two computing warps on a scheduler keep 51-55 % of its issue slots busy, about
+// 2000 cycles to a unit (products of K 520, P V and the wait for the copies 770, scores 260, the next copies 285). With
+// few tokens it is the chain lengths, page id, copies, join (about 8 us).
 #include <cuda_runtime.h>
 
 #include "../include/sm100.cuh"
@@ -50,6 +58,7 @@ constexpr int kTok = 16;                       // tokens of a tile
 constexpr int kHeads = 8;                      // query heads of a segment
 constexpr int kSlots = 3;                      // segments whose fragments or states are held
 constexpr uint32_t kWholeUnits = 40;           // units of a segment that a CTA takes whole
+constexpr int kJoinSteps = 3;                  // steps of a warp that a join is worth
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 2048.f;               // x of the largest p and a' right after the reference moved
 constexpr float kGrowP = 8.f, kGrowA = 2.f;    // how far either may pass it: x stays below 2^15
@@ -66,8 +75,10 @@ struct Cfg {
   static constexpr int LD = HD + 4;                      // row stride of a state: spreads the heads over the banks
   static constexpr int STATES = kWarps * WARP;           // kSlots sets of the warps' states
   static constexpr int STATE = kHeads * LD * 4;
-  static constexpr int F = STATES + kSlots * kWarps * STATE;  // kSlots sets of query fragments: matrix B, sums (B too), factors
-  static constexpr int F_SUM = 32 * 16 * (HD / 32), F_FACTOR = F_SUM + 2 * 32 * 4, FBYTES = F_FACTOR + kHeads * 4;
+  // kSlots sets of query fragments: matrix B, sums (B too), factors
+  static constexpr int F = STATES + kSlots * kWarps * STATE;
+  static constexpr int F_SUM = 32 * 16 * (HD / 32), F_FACTOR = F_SUM + 2 * 32 * 4;
+  static constexpr int FBYTES = F_FACTOR + kHeads * 4;
   static constexpr int SMEM = F + kSlots * FBYTES;
   static constexpr int PART = HD + 4;                    // floats of a head in the workspace: sums, maximum, normaliser
 };
@@ -168,10 +179,12 @@ __device__ __forceinline__ int tokens_of(const Args& a, int b) {
   return n <= 0 ? 0 : (int)min((int64_t)n, cap);
 }
 template <int UTOK>
-__device__ __forceinline__ uint32_t units_of(int n) { return max(1, (n + UTOK - 1) / UTOK); }  // an empty row writes its zeros
+__device__ __forceinline__ uint32_t units_of(int n) {  // an empty row has one too, which writes its zeros
+  return max(1, (n + UTOK - 1) / UTOK);
+}
 
-// A CTA's walk over its share of the units: segment (b, h), which starts at unit ``begin`` of the sum and of whose U units
-// the share has [first, last); ``left`` units of the share remain from ``first`` on.
+// A CTA's walk over its share of the units: segment (b, h), which starts at unit ``begin`` of the sum and of whose U
+// units the share has [first, last); ``left`` units of the share remain from ``first`` on.
 template <int UTOK>
 struct Walk {
   int b, h, n, U, first, last, left;
@@ -227,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   __shared__ uint64_t ready[kSlots], done[kSlots];  // fragments are there and the states free; the states are there
   __shared__ float weight[kHeads][kWarps], total_max[kHeads], total_sum[kHeads];
   __shared__ Piece s_piece[2];
-  __shared__ uint32_t scan[kWarps + kHelpers], s_begin;
+  __shared__ uint32_t scan[kWarps + kHelpers], s_begin, s_row0;
   __shared__ int s_row, s_pieces, s_abort, s_ok;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t per_row = a.c.Hkv * a.blocks;  // segments of a row
@@ -257,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     }
     __syncthreads();
     if (lane == 31) scan[warp] = incl;
+    if (b0 == 0 && tid == 0) s_row0 = mine;
     __syncthreads();
     before = total + incl - mine;
 #pragma unroll
@@ -267,15 +281,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   };
   for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
   const uint32_t all = total;
-  // A CTA per segment where that makes a few steps of every warp. Else more of them: the steps shrink with their number,
-  // the join grows with it, so the best number goes with the root of the work; a whole number to a segment, if that
-  // is near (equal segments are then cut alike).
+  // A CTA per segment where that makes a few steps of every warp (up to 40 units: 9 us on one row of 700 tokens instead
+  // of 9.6, while 160 took 13.9 us on 8 rows of 2048 where this takes 10.6). Else more of them: the steps shrink with
+  // their number, the join grows with it, so the best number goes with the root of the work (the root itself took 11.5
+  // and 15.3 us on one row of 8192 and 32768 tokens, twice as many 11.9 and 15.8, four times 16.4 on the latter). Equal
+  // segments get a whole number of CTAs each, and are then cut alike, if that costs fewer steps than a join (4 rows of
+  // 16384 tokens 14.9 us instead of 17.8, 64 of 4096 22.6 instead of 26.1).
   const uint32_t segments = a.B * per_row;
   uint32_t n_cta = segments;
   if (all > segments * kWholeUnits)
-    n_cta = max(segments, min((all + kWarps - 1) / kWarps, (uint32_t)sqrtf(4.f * (float)all * (float)segments)));
+    n_cta = max(segments, min((all + kWarps - 1) / kWarps, (uint32_t)sqrtf((float)all * (float)segments)));
   n_cta = min(gridDim.x, n_cta);
-  if (n_cta > segments && n_cta % segments * 20 <= n_cta) n_cta -= n_cta % segments;
+  if (n_cta > segments && all == s_row0 * a.B) {  // equal, or as good as that: the cut is right either way
+    const uint32_t even = n_cta - n_cta % segments;
+    if ((float)all / even - (float)all / n_cta <= (float)(kJoinSteps * kWarps)) n_cta = even;
+  }
   if (blockIdx.x >= n_cta) return;
   const Shares shares{all, n_cta, all / n_cta, all % n_cta};
   const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
@@ -356,7 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
           const float y1 = y0 - __half2float(t0);
           const __half t1 = __float2half_rn(y1), t2 = __float2half_rn(y1 - __half2float(t1));
           const __half t = lane == 0 ? t0 : lane == 1 ? t1 : lane == 2 ? t2 : __float2half_rn(0.f);
-          if (lane < 4) reinterpret_cast<uint32_t*>(f + C::F_SUM)[i * 32 + h * 4 + lane] = (uint32_t)__half_as_ushort(t) << 16;
+          if (lane < 4)
+            reinterpret_cast<uint32_t*>(f + C::F_SUM)[i * 32 + h * 4 + lane] = (uint32_t)__half_as_ushort(t) << 16;
         }
         if (lane == 0) reinterpret_cast<float*>(f + C::F_FACTOR)[h] = ldexpf(sl2, 24 - ex);
       }
@@ -445,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   } else {
     // ───────────────────────────── compute ─────────────────────────────
     const int g = lane / 4, t = lane % 4;
-    const int tok_g = g / 2 + 4 * (g % 2);  // token of matrix rows g and (8 further on) g + 8; V's are t, t + 4, t + 8, t + 12
+    const int tok_g = g / 2 + 4 * (g % 2);  // token of matrix rows g and (8 further on) g + 8; V's: t, t + 4, t + 8, t + 12
     const uint32_t ring = smem_u32(smem) + warp * C::WARP;
     // this lane's places in a stage
     const uint32_t k_at = C::K + tok_g * C::ROW + t * (4 * KW), s_at = C::S + tok_g * C::PAIRS;
@@ -581,16 +602,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
             for (int n = 0; n < NT; ++n) {
               uint32_t w0 = kw[n][0][j], w1 = kw[n][1][j];
               if (j < G)
-                mma_f16_first(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
+                mma_f16_first(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                              qf[j][0], qf[j][1]);
               else
-                mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0], qf[j][1]);
+                mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][0],
+                        qf[j][1]);
               w0 >>= 8;
               w1 >>= 8;
-              mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2], qf[j][3]);
+              mma_f16(acc[n][j % G], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[j][2],
+                      qf[j][3]);
             }
 #pragma unroll
           for (int n = 0; n < NT; ++n)  // sum_g z_g sum(q_g): the pairs (a, z) against (0, sum)
-            mma_f16_first(e[n], sw[n][0][0], sw[n][1][0], G == 2 ? sw[n][0][G - 1] : 0u, G == 2 ? sw[n][1][G - 1] : 0u, zf[0], zf[1]);
+            mma_f16_first(e[n], sw[n][0][0], sw[n][1][0], G == 2 ? sw[n][0][G - 1] : 0u, G == 2 ? sw[n][1][G - 1] : 0u,
+                          zf[0], zf[1]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -676,7 +701,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
           for (int r = 0; r < 2; ++r) {
             l[r] += p[n][0][r] + p[n][1][r];
 #pragma unroll
-            for (int j = 0; j < G; ++j) z[j][r] = fmaf(p[n][0][r], vz[n][0][j], fmaf(p[n][1][r], vz[n][1][j], z[j][r]));
+            for (int j = 0; j < G; ++j)
+              z[j][r] = fmaf(p[n][0][r], vz[n][0][j], fmaf(p[n][1][r], vz[n][1][j], z[j][r]));
           }
 #pragma unroll
           for (int j = 0; j < G; ++j) {
@@ -685,11 +711,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // channels 8 g + 4 half ..
               const uint32_t sel = half ? 0x7632u : 0x5410u;
-              uint32_t x01 = __byte_perm(vw[n][0][j], vw[n][1][j], sel), x23 = __byte_perm(vw[n][2][j], vw[n][3][j], sel);
-              mma_f16(o[j][2 * half], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
+              uint32_t x01 = __byte_perm(vw[n][0][j], vw[n][1][j], sel);
+              uint32_t x23 = __byte_perm(vw[n][2][j], vw[n][3][j], sel);
+              mma_f16(o[j][2 * half], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0,
+                      b1);
               x01 >>= 8;
               x23 >>= 8;
-              mma_f16(o[j][2 * half + 1], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u, b0, b1);
+              mma_f16(o[j][2 * half + 1], x01 & 0x000F000Fu, x01 & 0x00F000F0u, x23 & 0x000F000Fu, x23 & 0x00F000F0u,
+                      b0, b1);
             }
           }
         }
@@ -814,7 +843,8 @@ void launch(Args a, cudaStream_t st) {
   int dev = 0;
   MESHY_CUDA_CHECK(cudaGetDevice(&dev));
   if (!set[dev]) {
-    MESHY_CUDA_CHECK(cudaFuncSetAttribute(kv4_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    MESHY_CUDA_CHECK(
+        cudaFuncSetAttribute(kv4_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     set[dev] = true;
   }
   launch_pdl(kv4_attn_kernel<HD, NT>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
