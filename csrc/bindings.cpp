@@ -821,10 +821,10 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
   const c10::cuda::CUDAGuard guard(kc.device());
   q = kv4_rows(q, "paged_attention_kv4: q", kc, c.hd);
   const int64_t B = q.size(0), Hq = q.size(1);
-  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0, 
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0,
               "paged_attention_kv4: " + std::to_string(Hq) + " query heads over " + std::to_string(c.Hkv) + " KV heads");
-  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == B && (bt.size(1) <= 1 || bt.stride(1) == 1) &&
-                  bt.device() == kc.device(),
+  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == B &&
+                  (bt.size(1) <= 1 || bt.stride(1) == 1) && bt.device() == kc.device(),
               "paged_attention_kv4: block_table must be int32 [rows, pages] on the cache's device");
   TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.size(0) == B &&
                   seq_lens.device() == kc.device(),
@@ -835,8 +835,8 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
   if (c.n_pages == 0 || bt.size(1) == 0) return out.zero_();
   const KV4Workspace ws = kv4_workspace(kc, kv4_attention_segments((int)B, (int)Hq, c.Hkv));
   kv4_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
-                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ptr<float>(ws.part), ptr<unsigned>(ws.arrived),
-                ptr<int>(scratch(0, 0).err), cur_stream());
+                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ptr<float>(ws.part),
+                ptr<unsigned>(ws.arrived), ptr<int>(scratch(0, 0).err), cur_stream());
   count();
   return out;
 }
@@ -854,17 +854,19 @@ ControlsView controls_view(const std::vector<Tensor>& s) {
     TORCH_CHECK(t.is_contiguous() && t.device() == counts.device() && t.size(0) == R,
                 "logit controls: state tensors must be contiguous, on one device, with one row per slot");
   }
-  for (const Tensor* t : {&rep, &freq, &pres}) TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 1, "logit controls: penalties must be float32 [slots]");
+  for (const Tensor* t : {&rep, &freq, &pres})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 1, "logit controls: penalties must be float32 [slots]");
   for (const Tensor* t : {&seen, &mask})
-    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 2 && t->size(1) == W, 
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 2 && t->size(1) == W,
                 "logit controls: seen and mask must be int32 [slots, " + std::to_string(W) + "]");
   TORCH_CHECK(counts.scalar_type() == at::kInt && mask_on.scalar_type() == at::kInt && mask_on.dim() == 1,
               "logit controls: counts and mask_on must be int32");
-  TORCH_CHECK(ids.scalar_type() == at::kInt && vals.scalar_type() == at::kFloat && ids.dim() == 2 && ids.sizes() == vals.sizes(),
+  TORCH_CHECK(ids.scalar_type() == at::kInt && vals.scalar_type() == at::kFloat && ids.dim() == 2 &&
+                  ids.sizes() == vals.sizes(),
               "logit controls: bias_ids int32 and bias_vals float32 must be [slots, entries]");
-  return {ptr<float>(rep),    ptr<float>(freq),  ptr<float>(pres),    ptr<uint32_t>(seen), ptr<int>(counts), ptr<int>(ids),
-          ptr<float>(vals), ptr<uint32_t>(mask), ptr<int>(mask_on), R,                   (int)V,           (int)W,
-          (int)ids.size(1)};
+  return {ptr<float>(rep),  ptr<float>(freq), ptr<float>(pres),    ptr<uint32_t>(seen), ptr<int>(counts),
+          ptr<int>(ids),    ptr<float>(vals), ptr<uint32_t>(mask), ptr<int>(mask_on),   R,
+          (int)V,           (int)W,           (int)ids.size(1)};
 }
 
 SlotIds slot_ids(const Tensor& slots, const Tensor& state, const char* what) {
@@ -883,9 +885,9 @@ void load_tokens_(std::vector<Tensor> state, Tensor slots, Tensor tokens, Tensor
   const int64_t n = slots.size(0);
   TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.dim() == 1 && tokens.device() == counts.device(),
               "load_tokens: tokens must be int64 [total] on the state's device");
-  TORCH_CHECK(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) == n + 1 && n_prompt.scalar_type() == at::kInt &&
-                  n_prompt.dim() == 1 && n_prompt.size(0) == n && cu.device() == counts.device() &&
-                  n_prompt.device() == counts.device(),
+  TORCH_CHECK(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) == n + 1 &&
+                  n_prompt.scalar_type() == at::kInt && n_prompt.dim() == 1 && n_prompt.size(0) == n &&
+                  cu.device() == counts.device() && n_prompt.device() == counts.device(),
               "load_tokens: cu_tokens int32 [rows + 1] and n_prompt int32 [rows] on the state's device");
   CHECK_CONTIG(tokens);
   CHECK_CONTIG(cu);
@@ -902,8 +904,8 @@ void apply_logit_controls_(Tensor logits, std::vector<Tensor> state, Tensor slot
   const SlotIds ids = slot_ids(slots, counts, "apply_logit_controls");
   const int64_t B = slots.size(0);
   const bool half = logits.scalar_type() == at::kBFloat16;
-  TORCH_CHECK((half || logits.scalar_type() == at::kFloat) && logits.dim() == 2 && logits.size(0) == B && logits.size(1) == c.V &&
-                  logits.stride(1) == 1 && logits.device() == counts.device(),
+  TORCH_CHECK((half || logits.scalar_type() == at::kFloat) && logits.dim() == 2 && logits.size(0) == B &&
+                  logits.size(1) == c.V && logits.stride(1) == 1 && logits.device() == counts.device(),
               "apply_logit_controls: logits must be float32 or bfloat16 [" + std::to_string(B) + ", " + std::to_string(c.V) +
                   "] on the state's device");
   TORCH_CHECK(out.scalar_type() == at::kFloat && out.dim() == 2 && out.size(0) == B && out.size(1) == c.V &&
@@ -912,7 +914,8 @@ void apply_logit_controls_(Tensor logits, std::vector<Tensor> state, Tensor slot
                   "] on the state's device");
   TORCH_CHECK(B <= 1 || out.stride(0) >= c.V, "apply_logit_controls: rows of out overlap");
   if (out.data_ptr() == logits.data_ptr())
-    TORCH_CHECK(!half && (B <= 1 || out.stride(0) == logits.stride(0)), "apply_logit_controls: out must be logits or apart from it");
+    TORCH_CHECK(!half && (B <= 1 || out.stride(0) == logits.stride(0)),
+                "apply_logit_controls: out must be logits or apart from it");
   for (const auto* t : {&fresh, &done})
     if (t->has_value() && (*t)->defined()) {
       TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == B && (*t)->is_contiguous() && (*t)->device() == counts.device() &&

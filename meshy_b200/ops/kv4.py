@@ -95,7 +95,10 @@ def kv4_read(cache: KV4Cache, slot_mapping: torch.Tensor, dtype: torch.dtype = t
 def paged_attention_kv4(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                         scale: float | None = None) -> torch.Tensor:
     """Decode attention of ``q [B, Hq, hd]`` over each row's first ``seq_lens [B]`` cached tokens, on the pages
-    ``block_table [B, max_pages]``; query heads share the KV heads evenly. A row of length 0 gives zeros."""
+    ``block_table [B, max_pages]``; query heads share the KV heads evenly. A row of length 0 gives zeros.
+
+    Calls on one stream share a workspace, which the first call of a size on that stream allocates: make one before
+    a capture on the stream, and replay graphs that were captured on one stream one after another."""
     check_paged("paged attention", block_table, seq_lens, cache.k.shape[0], cache.k.shape[2])
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if q.is_cuda:
