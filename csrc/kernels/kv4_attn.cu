@@ -23,8 +23,8 @@
 //
 // Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (16 where a
 // page is not a multiple of 32; 64 at head width 64 where it is one of 64, as bytes of a unit are what hides latency)
-// and every CTA, one per SM, takes an equal share of the sum, whatever the lengths: they are read on the device, so a
-// captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs leaves partial
+// and every CTA, one per SM, takes an equal share of the sum, whatever the lengths, a change of segments counted as some
+// units: they are read on the device, so a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs leaves partial
 // sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and results do not
 // depend on timing.
 //
@@ -38,7 +38,7 @@
 // wait is bounded; one that gives up records an error code.
 //
 // Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 302 MB) 65-68 us, 4.5 TB/s; 256 rows of up to 1500 (32 / 8
-// heads, 360 MB) 93 us, 3.9 TB/s; 64 rows of up to 8192 (12 / 2) 35 us; one row of 700 tokens 8.7 us. Bound by the
+// heads, 360 MB) 90 us, 4.0 TB/s; 64 rows of up to 8192 (12 / 2) 29 us; one row of 700 tokens 8.7 us. Bound by the
 // instructions' latency, not by memory: two computing warps on a scheduler keep 51-55 % of its issue slots busy, about
 // 2000 cycles to a unit (products of K 520, P V and the wait for the copies 770, scores 260, the next copies 285). With
 // few tokens it is the chain lengths, page id, copies, join (about 8 us).
@@ -58,6 +58,7 @@ constexpr int kTok = 16;                       // tokens of a tile
 constexpr int kHeads = 8;                      // query heads of a segment
 constexpr int kSlots = 3;                      // segments whose fragments or states are held
 constexpr uint32_t kWholeUnits = 40;           // units of a segment that a CTA takes whole
+constexpr int kPad = 16;                        // units that a change of segments costs
 constexpr int kJoinSteps = 3;                  // steps of a warp that a join is worth
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 2048.f;               // x of the largest p and a' right after the reference moved
@@ -184,12 +185,13 @@ __device__ __forceinline__ uint32_t units_of(int n) {  // an empty row has one t
 }
 
 // A CTA's walk over its share of the units: segment (b, h), which starts at unit ``begin`` of the sum and of whose U
-// units the share has [first, last); ``left`` units of the share remain from ``first`` on.
+// units (the last ``pad`` of them empty) the share has [first, last); ``left`` units of the share remain from ``first``
+// on.
 template <int UTOK>
 struct Walk {
   int b, h, n, U, first, last, left;
   uint32_t begin;
-  __device__ __forceinline__ bool next(const Args& a) {
+  __device__ __forceinline__ bool next(const Args& a, int pad) {
     left -= last - first;
     if (left <= 0) return false;
     first = 0;
@@ -198,13 +200,14 @@ struct Walk {
       h = 0;
       ++b;
       n = tokens_of(a, b);
-      U = units_of<UTOK>(n);
+      U = units_of<UTOK>(n) + pad;
     }
     last = min(U, left);
     return true;
   }
   __device__ __forceinline__ bool more() const { return left > last - first; }
-  __device__ __forceinline__ int end() const { return n ? last : 0; }  // of the units that hold tokens
+  __device__ __forceinline__ int end() const { return min(last, (n + UTOK - 1) / UTOK); }  // of the units with tokens
+  __device__ __forceinline__ bool whole() const { return first == 0 && last >= (int)units_of<UTOK>(n); }
   __device__ __forceinline__ int first_of(int warp) const { return first + ((warp - (int)begin - first) & (kWarps - 1)); }
 };
 
@@ -280,7 +283,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     }
   };
   for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
-  const uint32_t all = total;
   // A CTA per segment where that makes a few steps of every warp (up to 40 units: 9 us on one row of 700 tokens instead
   // of 9.6, while 160 took 13.9 us on 8 rows of 2048 where this takes 10.6). Else more of them: the steps shrink with
   // their number, the join grows with it, so the best number goes with the root of the work (the root itself took 11.5
@@ -289,35 +291,42 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   // 16384 tokens 14.9 us instead of 17.8, 64 of 4096 22.6 instead of 26.1).
   const uint32_t segments = a.B * per_row;
   uint32_t n_cta = segments;
-  if (all > segments * kWholeUnits)
-    n_cta = max(segments, min((all + kWarps - 1) / kWarps, (uint32_t)sqrtf((float)all * (float)segments)));
+  if (total > segments * kWholeUnits)
+    n_cta = max(segments, min((total + kWarps - 1) / kWarps, (uint32_t)sqrtf((float)total * (float)segments)));
   n_cta = min(gridDim.x, n_cta);
-  if (n_cta > segments && all == s_row0 * a.B) {  // equal, or as good as that: the cut is right either way
+  if (n_cta > segments && total == s_row0 * a.B) {  // equal, or as good as that: the cut is right either way
     const uint32_t even = n_cta - n_cta % segments;
-    if ((float)all / even - (float)all / n_cta <= (float)(kJoinSteps * kWarps)) n_cta = even;
+    if ((float)total / even - (float)total / n_cta <= (float)(kJoinSteps * kWarps)) n_cta = even;
   }
   if (blockIdx.x >= n_cta) return;
+  // Where CTAs have several segments, the change from one to the next counts as kPad empty units at a segment's end: a
+  // CTA with more segments gets fewer tokens (64 rows of up to 8192 tokens 29.0 us, with 8 units 29.9, with none 35.2;
+  // 200 rows of about 800 at head width 64 44.4, 45.5, 48.9). Where several CTAs share a segment there is no change.
+  const int pad = n_cta < 2 * segments ? kPad : 0;
+  const uint32_t all = total + pad * segments;
   const Shares shares{all, n_cta, all / n_cta, all % n_cta};
   const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
   if (a.B > kThreads) total = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
     if (a.B > kThreads) sum_rows(b0);
-    if (at - before < mine) {
+    const uint32_t row = before + pad * per_row * (b0 + tid);
+    if (b0 + tid < a.B && at - row < mine + pad * per_row) {
       s_row = b0 + tid;
-      s_begin = before;
+      s_begin = row;
     }
-    if (total > at) break;
+    if (total + pad * per_row * min(b0 + kThreads, a.B) > at) break;
   }
   __syncthreads();
   W w0;
   w0.b = s_row;
   w0.n = tokens_of(a, w0.b);
-  w0.U = units_of<C::UTOK>(w0.n);
+  w0.U = units_of<C::UTOK>(w0.n) + pad;
   w0.h = (at - s_begin) / w0.U;
   w0.begin = s_begin + w0.h * w0.U;
   w0.first = at - w0.begin;
   w0.left = end - at;
   w0.last = min(w0.U, w0.first + w0.left);
+  if (w0.first >= w0.U - pad && !w0.next(a, pad)) return;  // nothing of that segment is left
   const float sl2 = a.scale * kLog2e;
 
   if (warp >= kWarps) {
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     load_q(coming);
     for (int i = 0; i < kSlots && more; ++i) {
       prepare(coming, i);
-      more = coming.next(a);
+      more = coming.next(a, pad);
       if (more) load_q(coming);  // on its way until a slot is free
     }
     int slot = 0, pieces = 0;
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
       }
       helper_sync();
       // a whole segment is done, a piece of one goes to the workspace
-      const bool whole = w.first == 0 && w.last == w.U;
+      const bool whole = w.whole();
       const int part = 2 * blockIdx.x + (w.first == 0 ? 1 : 0);
       const float* states = reinterpret_cast<const float*>(smem + C::STATES + slot * kWarps * C::STATE);
       for (int i = ht; i < nh * (HD / 4); i += 32 * kHelpers) {
@@ -447,14 +456,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
         }
       }
       if (!whole) {  // at most the first and the last segment of the share
-        if (ht == 0) s_piece[pieces] = {w.b, w.h, w.begin, (uint32_t)w.U, false};
+        if (ht == 0) s_piece[pieces] = {w.b, w.h, w.begin, (uint32_t)(w.U - pad), false};
         ++pieces;
       }
       if (!w.more()) break;
       helper_sync();  // the states and weights have been read
       if (more) {
         prepare(coming, slot);
-        more = coming.next(a);
+        more = coming.next(a, pad);
         if (more) load_q(coming);
       }
       if (++slot == kSlots) {
@@ -495,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
       if (f_unit >= f_end) {
         W w = s_ahead[warp];
         do {
-          if (!w.next(a)) {
+          if (!w.next(a, pad)) {
             f_unit = kDone;
             f_end = 0;
             break;
@@ -837,7 +846,7 @@ void launch(Args a, cudaStream_t st) {
   a.page_units = a.c.Hkv * a.upp;
   // units are counted in 32 bits, in the cache and over the rows
   MESHY_CHECK(a.c.n_pages * a.c.Hkv * a.upp < (1LL << 32), "paged_attention_kv4: cache too large");
-  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * std::max<int64_t>(1, (int64_t)a.max_pages * a.upp) < (1LL << 31),
+  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.upp) + kPad) < (1LL << 31),
               "paged_attention_kv4: rows * heads * table width too large");
   static bool set[64] = {};
   int dev = 0;
