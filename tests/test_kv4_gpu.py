@@ -191,6 +191,23 @@ def test_attention_lengths(lens, Hq, Hkv, hd):
     assert torch.equal(out, K.paged_attention_kv4(q, c, bt, n))  # the same sums in the same order
 
 
+@pytest.mark.parametrize("B,longest,page", [(2, 9000, 64), (5, 3000, 64), (37, 700, 16), (75, 2000, 64), (90, 400, 32),
+                                            (149, 50, 64), (390, 90, 64), (800, 40, 48)])
+@pytest.mark.parametrize("Hq,Hkv,hd", [(6, 1, 128), (16, 4, 64)])
+def test_attention_ragged_splits(B, longest, page, Hq, Hkv, hd):
+    """The work's cuts fall anywhere: between rows, inside them, behind a row's last token."""
+    g = torch.Generator().manual_seed(B + longest)
+    lens = (torch.rand(B, generator=g) ** 2 * (longest + 1)).long()
+    lens[torch.randint(B, (max(1, B // 8),), generator=g)] = 0
+    lens[int(torch.randint(B, (1,), generator=g))] = longest
+    lens = lens.tolist()
+    q, c, bt, n = _setup(lens, Hq, Hkv, hd, page, seed=B)
+    out = K.paged_attention_kv4(q, c, bt, n)
+    _check(out, *_expect(q, c, bt, lens))
+    for b in (0, B // 2, B - 1):  # a row by itself: other cuts, the same numbers to rounding
+        _check(K.paged_attention_kv4(q[b:b + 1], c, bt[b:b + 1], n[b:b + 1]), *_expect(q[b:b + 1], c, bt[b:b + 1], [lens[b]]))
+
+
 @pytest.mark.parametrize("kscale,vscale,koff", [(1.0, 1e-4, 0.0), (1.0, 2000.0, 0.0), (4.0, 1.0, 0.0), (0.3, 1.0, 8.0),
                                                 (1e-4, 1.0, 0.0), (0.0, 1.0, 0.0), (1.0, 0.0, 0.0)])
 def test_attention_scales(kscale, vscale, koff):
