@@ -21,12 +21,16 @@
 // below fp16's smallest number is less than 2^-35 of the largest term. P is rounded to fp16's 11 bits there; sums, the
 // normaliser and the bases' part stay in 32 bits.
 //
-// Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (16 where a
-// page is not a multiple of 32; 64 at head width 64 where it is one of 64, as bytes of a unit are what hides latency)
-// and every CTA, one per SM, takes an equal share of the sum, whatever the lengths, a change of segments counted as some
-// units: they are read on the device, so a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs leaves partial
-// sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and results do not
-// depend on timing.
+// Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (64 at head
+// width 64: the same bytes, and enough of them under way to hide the memory's latency) and every CTA, one per SM, takes
+// an equal share of the sum, whatever the lengths, a change of segments counted as some units: they are read on the
+// device, so a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs
+// leaves partial sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and
+// results do not depend on timing.
+//
+// A unit lies in one page, or, where the page is not a multiple of it, in pieces of 16 or 32 tokens whose page ids
+// neighbouring lanes look up (8 rows of 131072 tokens: 67 us with pages of 16, 65 with pages of 64; units of 16 tokens
+// took 82 with the former. At head width 64, 128 rows of 16384: 71, 69 and 131).
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory, filled by
 // 16-byte asynchronous copies two units ahead, across the segments, and at a segment's end leaves its state in one of
@@ -65,11 +69,11 @@ constexpr float kBoost = 2048.f;               // x of the largest p and a' righ
 constexpr float kGrowP = 8.f, kGrowA = 2.f;    // how far either may pass it: x stays below 2^15
 constexpr float kMinA = 5.9604645e-8f;         // 2^-24, the smallest fp16
 
-template <int HD, int NT>  // NT tiles to a unit
+template <int HD, int NT, int NP>  // NT tiles to a unit, which lie in NP pieces (pages, or parts of one)
 struct Cfg {
   static constexpr int ROW = HD / 2;                     // nibble bytes of a token
   static constexpr int PAIRS = HD / 8;                   // bytes of a token's pairs (K and V)
-  static constexpr int UTOK = NT * kTok;
+  static constexpr int UTOK = NT * kTok, PTOK = UTOK / NP;  // tokens of a unit, of a piece
   static constexpr int K = 0, V = UTOK * ROW, S = 2 * UTOK * ROW, STAGE = UTOK * (2 * ROW + PAIRS);
   static constexpr int STAGES = 13824 / STAGE;           // 3 units of 32 tokens at head width 128
   static constexpr int WARP = STAGES * STAGE;
@@ -166,7 +170,7 @@ struct Args {
   int max_pages;
   const int* seq_lens;
   int B, Hq, rep, blocks;  // blocks: groups of kHeads query heads per KV head
-  int upp, page_units;     // units of a page, of a page of all heads
+  int ppp, page_pieces;    // pieces of a page, of a page of all heads
   float scale;
   bf16* out;
   float* part;         // [2 CTAs][kHeads][PART]
@@ -231,9 +235,9 @@ struct Piece {
   bool last;  // this CTA arrived last
 };
 
-template <int HD, int NT>
+template <int HD, int NT, int NP>
 __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
-  using C = Cfg<HD, NT>;
+  using C = Cfg<HD, NT, NP>;
   using W = Walk<C::UTOK>;
   constexpr int G = HD / 64;
   constexpr int KW = HD / 32;  // K words a lane takes of a row
@@ -475,7 +479,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   } else {
     // ───────────────────────────── compute ─────────────────────────────
     const int g = lane / 4, t = lane % 4;
-    const int tok_g = g / 2 + 4 * (g % 2);  // token of matrix rows g and (8 further on) g + 8; V's: t, t + 4, t + 8, t + 12
+    // token of matrix rows g and (8 further on) g + 8; V's are t, t + 4, t + 8, t + 12
+    const int tok_g = g / 2 + 4 * (g % 2);
     const uint32_t ring = smem_u32(smem) + warp * C::WARP;
     // this lane's places in a stage
     const uint32_t k_at = C::K + tok_g * C::ROW + t * (4 * KW), s_at = C::S + tok_g * C::PAIRS;
@@ -483,22 +488,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     if (lane == 0) s_ahead[warp] = w0;
     __syncwarp();
 
-    // The copies run STAGES - 1 units ahead of the arithmetic, across the segments; a unit's page id is read one step
-    // before its copies start.
+    // The copies run STAGES - 1 units ahead of the arithmetic, across the segments; a unit's page ids are read one step
+    // before its copies start, a piece's by every NP-th lane.
     constexpr int kDone = -(1 << 30);  // the share holds no more units for this warp
-    int f_end, f_at, f_wrap, f_page;  // f_at: unit within the page of all heads, f_wrap: where this head's part of it ends
+    const int sub = lane % NP;
+    int f_end, f_at, f_wrap, f_page;  // f_at: piece within the page of all heads, f_wrap: where this head's part ends
+    int f_piece, f_pieces;            // of the row: this lane's, all of them
     const int* f_bt;
-    const int step_pi = kWarps / a.upp, step_off = kWarps % a.upp;
+    const int step_pi = NP * kWarps / a.ppp, step_off = NP * kWarps % a.ppp;
     const uint8_t* kp = a.c.k + lane * 16;
     const uint8_t* vp = a.c.v + lane * 16;
     const uint8_t* sp = reinterpret_cast<const uint8_t*>(a.c.scale) + lane * 16;
     int f_unit = w0.first_of(warp);
     auto aim = [&](const W& w) {
       f_end = w.end();
-      f_at = w.h / a.blocks * a.upp;
-      f_wrap = f_at + a.upp;
-      f_at += f_unit % a.upp;
-      f_bt = a.bt + w.b * a.bt_stride + f_unit / a.upp;
+      f_piece = f_unit * NP + sub;
+      f_pieces = (w.n + C::PTOK - 1) / C::PTOK;
+      f_at = w.h / a.blocks * a.ppp;
+      f_wrap = f_at + a.ppp;
+      f_at += f_piece % a.ppp;
+      f_bt = a.bt + w.b * a.bt_stride + f_piece / a.ppp;
     };
     auto settle = [&]() {  // on this warp's next unit, if its share has one
       if (f_unit >= f_end) {
@@ -517,29 +526,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
         __syncwarp();
       }
       f_page = -1;
-      if (f_unit >= 0) f_page = *f_bt;
+      if (f_unit >= 0 && (NP == 1 || f_piece < f_pieces)) f_page = *f_bt;
     };
-    uint32_t valid = 0;  // bit i: the unit i steps ahead has a page
+    uint32_t valid = 0;  // bits i NP ..: the pieces of the unit i steps ahead have a page
     auto fetch = [&](uint32_t stage, int steps) {
       const bool there = (uint32_t)f_page < (uint32_t)a.c.n_pages;
-      valid |= (there ? 1u : 0u) << steps;
-      const uint32_t n = there ? (uint32_t)f_page * (uint32_t)a.page_units + (uint32_t)f_at : 0u;  // unit of the cache
-      const uint8_t* ks = kp + (uint64_t)n * (C::UTOK * C::ROW);
-      const uint8_t* vs = vp + (uint64_t)n * (C::UTOK * C::ROW);
-      const uint8_t* ss = sp + (uint64_t)n * (C::UTOK * C::PAIRS);
+      const uint32_t n = there ? (uint32_t)f_page * (uint32_t)a.page_pieces + (uint32_t)f_at : 0u;  // piece of the cache
       const uint32_t dst = stage + lane * 16;
+      static_assert(C::UTOK * C::PAIRS == 512, "a lane copies 16 bytes of pairs");
+      if constexpr (NP == 1) {
+        valid |= (there ? 1u : 0u) << steps;
+        const uint8_t* ks = kp + (uint64_t)n * (C::UTOK * C::ROW);
+        const uint8_t* vs = vp + (uint64_t)n * (C::UTOK * C::ROW);
+        const uint8_t* ss = sp + (uint64_t)n * (C::UTOK * C::PAIRS);
 #pragma unroll
-      for (int i = 0; i < C::UTOK * C::ROW / 512; ++i) {
-        copy16(dst + C::K + 512 * i, ks + 512 * i, there);
-        copy16(dst + C::V + 512 * i, vs + 512 * i, there);
+        for (int i = 0; i < C::UTOK * C::ROW / 512; ++i) {
+          copy16(dst + C::K + 512 * i, ks + 512 * i, there);
+          copy16(dst + C::V + 512 * i, vs + 512 * i, there);
+        }
+        copy16(dst + C::S, ss, there);
+      } else {
+        const uint32_t bits = __ballot_sync(0xffffffffu, there) & ((1u << NP) - 1u);
+        valid |= bits << (NP * steps);
+#pragma unroll
+        for (int i = 0; i < C::UTOK * C::ROW / 512; ++i) {
+          constexpr int N = C::PTOK * C::ROW;
+          const int piece = 512 * i / N;
+          const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, n, piece) * N + 512 * i % N;
+          copy16(dst + C::K + 512 * i, kp + at, bits >> piece & 1u);
+          copy16(dst + C::V + 512 * i, vp + at, bits >> piece & 1u);
+        }
+        constexpr int N = C::PTOK * C::PAIRS;
+        const int piece = lane * 16 / N;
+        const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, n, piece) * N - piece * N;  // sp has lane * 16 already
+        copy16(dst + C::S, sp + at, bits >> piece & 1u);
       }
-      if (C::UTOK * C::PAIRS == 512 || lane < C::UTOK * C::PAIRS / 16) copy16(dst + C::S, ss, there);
       copies_commit();
       f_unit += kWarps;
+      f_piece += NP * kWarps;
       f_bt += step_pi;
       f_at += step_off;
       if (f_at >= f_wrap) {
-        f_at -= a.upp;
+        f_at -= a.ppp;
         ++f_bt;
       }
       settle();
@@ -579,8 +607,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
         __syncwarp();  // and every lane has read the stage that is filled again below
         const uint32_t here = stage;
         // tokens of the unit to be counted; the rest may be anything
-        const int count = valid & 1u ? n_tok - unit * C::UTOK : 0;
-        valid >>= 1;
+        const int count = n_tok - unit * C::UTOK;
+        const uint32_t pieces = valid & ((1u << NP) - 1u);
+        valid >>= NP;
         // the next copies first: after the products of K, 8 rows of 131072 tokens took 66.2 us instead of 64.8
         fetch(ahead, C::STAGES - 2);
         ahead = stage;
@@ -645,12 +674,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
             }
           }
         }
-        if (count < C::UTOK) {
+        if (count < C::UTOK || pieces != (1u << NP) - 1u) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (n * kTok + tok_g + 8 * i >= count) {
+              if (n * kTok + tok_g + 8 * i >= count || !(pieces >> (n * kTok / C::PTOK) & 1u)) {
                 s[n][i][0] = s[n][i][1] = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < G; ++j) va[n][i][j] = vz[n][i][j] = 0.f;
@@ -839,24 +868,24 @@ int sm_count() {
   return n[dev];
 }
 
-template <int HD, int NT>
+template <int HD, int NT, int NP>
 void launch(Args a, cudaStream_t st) {
-  using C = Cfg<HD, NT>;
-  a.upp = a.c.page / C::UTOK;
-  a.page_units = a.c.Hkv * a.upp;
-  // units are counted in 32 bits, in the cache and over the rows
-  MESHY_CHECK(a.c.n_pages * a.c.Hkv * a.upp < (1LL << 32), "paged_attention_kv4: cache too large");
-  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.upp) + kPad) < (1LL << 31),
+  using C = Cfg<HD, NT, NP>;
+  a.ppp = a.c.page / C::PTOK;
+  a.page_pieces = a.c.Hkv * a.ppp;
+  // pieces are counted in 32 bits, in the cache and over the rows
+  MESHY_CHECK(a.c.n_pages * a.page_pieces < (1LL << 32) - 1, "paged_attention_kv4: cache too large");
+  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.ppp) + kPad) < (1LL << 31),
               "paged_attention_kv4: rows * heads * table width too large");
   static bool set[64] = {};
   int dev = 0;
   MESHY_CUDA_CHECK(cudaGetDevice(&dev));
   if (!set[dev]) {
     MESHY_CUDA_CHECK(
-        cudaFuncSetAttribute(kv4_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        cudaFuncSetAttribute(kv4_attn_kernel<HD, NT, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     set[dev] = true;
   }
-  launch_pdl(kv4_attn_kernel<HD, NT>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
+  launch_pdl(kv4_attn_kernel<HD, NT, NP>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
 }
 
 }  // namespace
@@ -871,11 +900,10 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
   const int rep = Hq / c.Hkv;
   const Args a{q, qs, qh,  c,   bt,    bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads,
                0, 0,  scale, out, part, arrived, err};
-  const bool pairs = c.page % 32 == 0;
   if (c.hd == 128)
-    pairs ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
+    c.page % 32 == 0 ? launch<128, 2, 1>(a, st) : launch<128, 2, 2>(a, st);
   else
-    c.page % 64 == 0 ? launch<64, 4>(a, st) : pairs ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
+    c.page % 64 == 0 ? launch<64, 4, 1>(a, st) : c.page % 32 == 0 ? launch<64, 4, 2>(a, st) : launch<64, 4, 4>(a, st);
 }
 
 }  // namespace meshy
