@@ -61,7 +61,7 @@ constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = 16;                       // tokens of a tile
 constexpr int kHeads = 8;                      // query heads of a segment
 constexpr int kSlots = 3;                      // segments whose fragments or states are held
-constexpr uint32_t kWholeUnits = 40;           // units of a segment that a CTA takes whole
+constexpr uint32_t kWholeUnits = 24;           // units of equal segments that a CTA takes whole
 constexpr int kPad = 16;                        // units that a change of segments costs
 constexpr int kJoinSteps = 3;                  // steps of a warp that a join is worth
 constexpr float kLog2e = 1.4426950408889634f;
@@ -287,26 +287,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     }
   };
   for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
-  // A CTA per segment where that makes a few steps of every warp (up to 40 units: 9 us on one row of 700 tokens instead
-  // of 9.6, while 160 took 13.9 us on 8 rows of 2048 where this takes 10.6). Else more of them: the steps shrink with
-  // their number, the join grows with it, so the best number goes with the root of the work (the root itself took 11.5
-  // and 15.3 us on one row of 8192 and 32768 tokens, twice as many 11.9 and 15.8, four times 16.4 on the latter). Equal
-  // segments get a whole number of CTAs each, and are then cut alike, if that costs fewer steps than a join (4 rows of
-  // 16384 tokens 14.9 us instead of 17.8, 64 of 4096 22.6 instead of 26.1).
+  // A CTA per segment where that makes a few steps of every warp: for equal segments up to 24 units (one row of 700
+  // tokens 9.0 us; more CTAs, with a join, 9.9), one step for others, whose shares are cut and joined anyway (16 rows
+  // of up to 1400 tokens 11.2 us, with up to 24 units 14.9). Else more of them: the steps shrink with their number,
+  // the join grows with it, so the best number goes with the root of the work (the root itself took 11.5 and 15.3 us on
+  // one row of 8192 and 32768 tokens, twice as many 11.9 and 15.8, four times 16.4 on the latter). Equal segments get a
+  // whole number of CTAs each, and are then cut alike, if that costs fewer steps than a join (4 rows of 16384 tokens
+  // 14.9 us instead of 17.8, 64 of 4096 22.6 instead of 26.1).
   const uint32_t segments = a.B * per_row;
+  const bool equal = total == s_row0 * a.B;  // or as good as that: the cut is right either way
   uint32_t n_cta = segments;
-  if (total > segments * kWholeUnits)
+  if (total > segments * (equal ? kWholeUnits : kWarps))
     n_cta = max(segments, min((total + kWarps - 1) / kWarps, (uint32_t)sqrtf((float)total * (float)segments)));
   n_cta = min(gridDim.x, n_cta);
-  if (n_cta > segments && total == s_row0 * a.B) {  // equal, or as good as that: the cut is right either way
+  if (equal && n_cta > segments) {
     const uint32_t even = n_cta - n_cta % segments;
     if ((float)total / even - (float)total / n_cta <= (float)(kJoinSteps * kWarps)) n_cta = even;
   }
   if (blockIdx.x >= n_cta) return;
   // Where CTAs have several segments, the change from one to the next counts as kPad empty units at a segment's end: a
   // CTA with more segments gets fewer tokens (64 rows of up to 8192 tokens 29.0 us, with 8 units 29.9, with none 35.2;
-  // 200 rows of about 800 at head width 64 44.4, 45.5, 48.9). Where several CTAs share a segment there is no change.
-  const int pad = n_cta < 2 * segments ? kPad : 0;
+  // 200 rows of about 800 at head width 64 44.4, 45.5, 48.9; 33 rows of up to 4000 15.5, 16.2, 21.5). Where several
+  // CTAs share each of equal segments there is no change.
+  const int pad = equal && n_cta >= 2 * segments ? 0 : kPad;
   const uint32_t all = total + pad * segments;
   const Shares shares{all, n_cta, all / n_cta, all % n_cta};
   const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
