@@ -146,7 +146,8 @@ __device__ __forceinline__ void quantise(const uint4& u0, const uint4& u1, int l
 template <int HD, int NH>
 __global__ void __launch_bounds__(kThreads)
     kv4_write_kernel(const bf16* __restrict__ k, int64_t ks, int64_t kh, const bf16* __restrict__ v, int64_t vs,
-                     int64_t vh, const int64_t* __restrict__ slots, uint32_t items, KV4View c, FastDiv splits, FastDiv page) {
+                     int64_t vh, const int64_t* __restrict__ slots, uint32_t items, KV4View c, FastDiv splits,
+                     FastDiv page) {
   constexpr int LANES = HD / 16, G = HD / 64;
   const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
@@ -197,8 +198,8 @@ __device__ __forceinline__ uint4 restore(uint32_t w, __half2 pair) {
 
 template <int HD, int NH>
 __global__ void __launch_bounds__(kThreads)
-    kv4_read_kernel(KV4View c, const int64_t* __restrict__ slots, uint32_t items, bf16* __restrict__ k, bf16* __restrict__ v,
-                    FastDiv splits, FastDiv page) {
+    kv4_read_kernel(KV4View c, const int64_t* __restrict__ slots, uint32_t items, bf16* __restrict__ k,
+                    bf16* __restrict__ v, FastDiv splits, FastDiv page) {
   constexpr int LANES = HD / 8, G = HD / 64;
   const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
