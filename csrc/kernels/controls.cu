@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kThreads)
   uint32_t bits = 0u;
   if (on && (rep != 1.f || freq != 0.f || pres != 0.f) && w0 < v1) {
     bits = (seen[w0 / 32] >> (w0 % 32)) & 0xFFFFu;
+    if (v1 - w0 < 16) bits &= (1u << (v1 - w0)) - 1u;  // the last word's bits behind the vocabulary are no tokens
     if (masked) bits &= mask[w0 / 32] >> (w0 % 32);
   }
   if (masked) {

@@ -52,8 +52,8 @@ class LogitControls:
     repetition: torch.Tensor  # [R] fp32, 1: off
     frequency: torch.Tensor   # [R] fp32, 0: off
     presence: torch.Tensor    # [R] fp32, 0: off
-    seen: torch.Tensor        # [R, W] int32 bits: token in the prompt or the output
-    counts: torch.Tensor      # [R, V] int32: times the token was generated
+    seen: torch.Tensor        # [R, W] int32 bits: token in the prompt or the output (bits past V are ignored)
+    counts: torch.Tensor      # [R, V] int32: times the token was generated; a token with a count is a seen one
     bias_ids: torch.Tensor    # [R, K] int32, -1: unused; distinct within a row
     bias_vals: torch.Tensor   # [R, K] fp32
     mask: torch.Tensor        # [R, W] int32 bits: token allowed

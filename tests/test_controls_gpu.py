@@ -130,6 +130,32 @@ def test_infinite_and_nan_logits():
     _check(out, want.float().double(), size)
 
 
+@pytest.mark.parametrize("V", [1, 15, 17, 33, 100, 1009, 4097])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bits_behind_the_vocabulary_are_no_tokens(V, dtype):
+    """Every bit of the seen rows set, those of the last word past V too: nothing outside a row is touched."""
+    B = 3
+    ctl = _state(B, V, 2 if V > 1 else 0, seed=V)
+    ctl.seen.fill_(-1)
+    ctl.repetition.fill_(1.3)
+    ids = torch.tensor([2, 0, 1], device=DEV)
+    z = (torch.randn(B, V, generator=_gen(V), device=DEV) * 4).to(dtype)
+    want, size = _expect(z, ctl, ids)
+    counts = ctl.counts.clone()
+    for pad in (0, 64):  # rows right behind one another, and apart
+        room = torch.full((64 + B * (V + pad) + 64,), 7.0, device=DEV)
+        out = room[64:64 + B * (V + pad)].view(B, V + pad)[:, :V]
+        if dtype == torch.float32:
+            out.copy_(z)
+            C.apply_logit_controls(out, ctl, ids)
+            _check(out, want, size)
+            out.fill_(7.0)
+        C.apply_logit_controls(z, ctl, ids, out=out)
+        _check(out, want, size)
+        out.fill_(7.0)
+        assert bool((room == 7).all()) and torch.equal(ctl.counts, counts)
+
+
 def test_mask_that_leaves_nothing():
     ctl = C.LogitControls.create(1, 100, device=DEV, max_bias=0)
     ctl.set_mask(0, torch.zeros(4, dtype=torch.int32))
