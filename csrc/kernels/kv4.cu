@@ -74,6 +74,12 @@ __device__ __forceinline__ float min_nan(float x, float y) {  // NaN if x is
   return r;
 }
 
+__device__ __forceinline__ float to_half_range(float x) {  // NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(min_nan(x, kHalfMax)), "f"(-kHalfMax));
+  return r;
+}
+
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 b) { return *reinterpret_cast<uint32_t*>(&b); }
 
@@ -103,7 +109,7 @@ __device__ __forceinline__ void quantise(const uint4& u0, const uint4& u1, int l
 #pragma unroll
   for (int o = 2; o > 0; o >>= 1) both = __hmax2_nan(both, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(both), o)));
   const float top = __low2float(both), bot = __high2float(both);  // bot: -lo
-  const float hi = min_nan(top, kHalfMax), lo = -min_nan(bot, kHalfMax);
+  const float hi = to_half_range(top), lo = -to_half_range(bot);  // both ends: a group may lie beyond the range whole
   const __half a = __float2half_rn(quotient(hi - lo, 15.f, 1.f / 15.f)), z = __float2half_rn(lo);
   const float af = __half2float(a), zf = __half2float(z), rcp = af > 0.f ? reciprocal(af) : 0.f;
   // Nothing leaves [0, 15] while rounding moved the base by less than 0.4 steps and the scale by less than 2^-11 of it.

@@ -62,6 +62,16 @@ def test_constant_extreme_and_nan_groups():
     assert bool(k[3, 0, 64:].isnan().all()) and bool((k[3, 0, :64] == 0).all())
 
 
+@pytest.mark.parametrize("side", [70000.0, -70000.0, 3e38, -3e38, math.inf, -math.inf])
+def test_groups_beyond_the_range_are_clamped(side):
+    x = torch.zeros(1, 1, 128)
+    x[..., :64] = side * (1 + torch.arange(64) % 3 / 16.0)
+    c = K.kv4_empty(1, 1, 16, 128, "cpu")
+    K.kv4_write(x, -x, c, torch.tensor([2]))
+    k, v = K.kv4_read(c, torch.tensor([2]), torch.float32)
+    assert torch.equal(k, x.clamp(-65504, 65504)) and torch.equal(v, -k)
+
+
 def test_slots_outside_the_cache_are_skipped():
     c = K.kv4_empty(2, 1, 16, 64, "cpu")
     x = torch.ones(3, 1, 64)

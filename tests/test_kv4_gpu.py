@@ -135,6 +135,28 @@ def test_write_special_values_and_ties():
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
 
 
+def test_write_groups_beyond_the_range():
+    """All channels of a group on one side of fp16's range: both extremes are clamped."""
+    from meshy_b200.ops import reference as ref
+
+    inf = float("inf")
+    sides = [70000.0, -70000.0, 1e6, -1e6, 3e38, -3e38, inf, -inf, 65504.0, -65504.0]
+    x = torch.zeros(2 * len(sides), 1, 128, device=DEV)
+    for i, s in enumerate(sides):
+        x[2 * i, 0, :64] = s                                            # constant
+        x[2 * i + 1, 0, 64:] = s * (1 + torch.arange(64, device=DEV) % 3 / 16.0)  # spread, on the same side
+    x = x.bfloat16()
+    c = K.kv4_empty(2, 1, 16, 128, DEV)
+    slots = torch.arange(len(x), device=DEV)
+    K.kv4_write(x, -x, c, slots)
+    for y, data, kv in ((x, c.k, 0), (-x, c.v, 1)):
+        b, pairs = ref.kv4_quantize(y.cpu())
+        assert torch.equal(data.transpose(1, 2).reshape(32, 1, 64)[slots].cpu(), b)
+        assert torch.equal(c.scale.transpose(1, 2).reshape(32, 1, 2, 2, 2)[slots][:, :, kv].cpu(), pairs)
+    k, v = K.kv4_read(c, slots)
+    assert bool(k.isfinite().all()) and torch.equal(k, x.clamp(-65504, 65504)) and torch.equal(v, -k)
+
+
 def test_slots_outside_are_skipped_and_empty_calls():
     c = K.kv4_empty(2, 2, 16, 128, DEV)
     x = torch.ones(4, 2, 128, device=DEV).bfloat16()
