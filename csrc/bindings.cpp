@@ -877,6 +877,19 @@ SlotIds slot_ids(const Tensor& slots, const Tensor& state, const char* what) {
   return {slots.data_ptr(), slots.scalar_type() == at::kLong};
 }
 
+// Whether rows of a and b [B, V] (unit inner stride, rows apart) share memory. Rows of two tensors may take turns within
+// one block of memory; other arrangements count as shared where the whole spans meet.
+bool rows_meet(const Tensor& a, const Tensor& b) {
+  const int64_t B = a.size(0), wa = a.size(1) * a.element_size(), wb = b.size(1) * b.element_size();
+  if (B == 0) return false;
+  const int64_t sa = B > 1 ? a.stride(0) * a.element_size() : wa, sb = B > 1 ? b.stride(0) * b.element_size() : wb;
+  const int64_t pa = reinterpret_cast<int64_t>(a.data_ptr()), pb = reinterpret_cast<int64_t>(b.data_ptr());
+  if (pa + (B - 1) * sa + wa <= pb || pb + (B - 1) * sb + wb <= pa) return false;
+  if (B == 1 || sa != sb) return true;
+  const int64_t d = ((pb - pa) % sa + sa) % sa;  // from the start of a row of a to the next of b
+  return d < wa || d + wb > sa;
+}
+
 void load_tokens_(std::vector<Tensor> state, Tensor slots, Tensor tokens, Tensor cu, Tensor n_prompt) {
   const ControlsView c = controls_view(state);
   const Tensor& counts = state[4];
@@ -913,9 +926,9 @@ void apply_logit_controls_(Tensor logits, std::vector<Tensor> state, Tensor slot
               "apply_logit_controls: out must be float32 [" + std::to_string(B) + ", " + std::to_string(c.V) +
                   "] on the state's device");
   TORCH_CHECK(B <= 1 || out.stride(0) >= c.V, "apply_logit_controls: rows of out overlap");
-  if (out.data_ptr() == logits.data_ptr())
-    TORCH_CHECK(!half && (B <= 1 || out.stride(0) == logits.stride(0)),
-                "apply_logit_controls: out must be logits or apart from it");
+  const bool in_place =
+      out.data_ptr() == logits.data_ptr() && !half && (B <= 1 || out.stride(0) == logits.stride(0));
+  TORCH_CHECK(in_place || !rows_meet(logits, out), "apply_logit_controls: out must be logits or apart from it");
   for (const auto* t : {&fresh, &done})
     if (t->has_value() && (*t)->defined()) {
       TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == B && (*t)->is_contiguous() && (*t)->device() == counts.device() &&

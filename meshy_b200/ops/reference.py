@@ -262,6 +262,7 @@ def load_tokens(ctl, slots, tokens, cu_tokens, n_prompt) -> None:
 def apply_logit_controls(logits, ctl, slots, new_tokens=None, done=None, out=None) -> torch.Tensor:
     """Penalties, biases and token masks on ``logits [B, V]`` (see :mod:`.controls`)."""
     out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device) if out is None else out
+    rows = []
     for b, s in enumerate(slots.tolist()):
         z = logits[b].float()
         if 0 <= s < ctl.counts.shape[0]:
@@ -278,6 +279,8 @@ def apply_logit_controls(logits, ctl, slots, new_tokens=None, done=None, out=Non
             z = z.index_add(0, ids[use], ctl.bias_vals[s][use])
             if int(ctl.mask_on[s]):
                 z = z.masked_fill(~_unpack_bits(ctl.mask[s], ctl.vocab), float("-inf"))
+        rows.append(z)
+    for b, z in enumerate(rows):  # after every read: the two may share memory
         out[b] = z
     return out
 

@@ -40,6 +40,16 @@ def test_formula():
         assert float(out[0, v]) == pytest.approx(x, abs=1e-5)
 
 
+def test_out_that_shares_memory_with_the_logits():
+    ctl = C.LogitControls.create(2, 8, device="cpu", max_bias=1)
+    ctl.set_slot(0, logit_bias={3: 2.0})
+    room = torch.arange(24.0)
+    z = room[:16].view(2, 8).clone()
+    out = C.apply_logit_controls(room[:16].view(2, 8), ctl, torch.tensor([0, 1]), out=room[8:].view(2, 8))
+    z[0, 3] += 2.0
+    assert torch.equal(out, z)
+
+
 def test_done_rows_and_unused_slots():
     ctl = C.LogitControls.create(2, 40, device="cpu", max_bias=0)
     C.load_tokens(ctl, torch.tensor([0, -1]), torch.tensor([1, 2, 99, -4]), _ints(0, 4, 4), _ints(1, 0))

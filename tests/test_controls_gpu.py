@@ -235,6 +235,28 @@ def test_graph_replay_counts():
     assert out[0, 100:103].tolist() == [-1.0] * 3 and float(out[0].sum()) == -3.0
 
 
+def test_out_apart_from_the_logits_or_the_logits():
+    """An output that shares memory with the logits other than entry by entry is refused; rows that take turns are not."""
+    V, B = 64, 3
+    ctl = _state(B, V, 2, seed=1)
+    ids = torch.arange(B, device=DEV)
+    room = torch.randn(2 * (B + 1) * V, generator=_gen(2), device=DEV)
+    whole = room.clone()
+    rows = lambda at, stride, n=B: room.as_strided((n, V), (stride, 1), at)
+    for z, out in ((rows(0, V), rows(4, V)), (rows(4, V), rows(0, V)), (rows(0, V), rows(V, V)), (rows(0, V), rows(0, 2 * V)),
+                   (rows(0, 2 * V), rows(V - 1, 2 * V)), (rows(0, 2 * V), rows(V + 1, 2 * V)), (rows(V + 4, 2 * V), rows(0, 2 * V + 4)),
+                   (room.view(torch.bfloat16)[:B * V].view(B, V), rows(0, V)), (rows(0, V, 1), rows(V - 1, V, 1))):
+        with pytest.raises(RuntimeError, match="apart"):
+            C.apply_logit_controls(z, ctl, ids[:len(z)], out=out)
+    assert torch.equal(room, whole)
+    for z, out in ((rows(0, 2 * V), rows(V, 2 * V)), (rows(V, 2 * V), rows(0, 2 * V)), (rows(0, V), rows(B * V, V)),
+                   (rows(0, V, 1), rows(V, V, 1))):
+        want, size = _expect(z, ctl, ids[:len(z)])
+        C.apply_logit_controls(z, ctl, ids[:len(z)], out=out)
+        _check(out, want, size)
+        room.copy_(whole)
+
+
 def test_refusals():
     V = 50
     ctl = C.LogitControls.create(2, V, device=DEV, max_bias=0)
