@@ -735,6 +735,7 @@ KV4View kv4_view(const Tensor& k, const Tensor& v, const Tensor& scale) {
   TORCH_CHECK(k.dim() == 4 && k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && k.sizes() == v.sizes(),
               "kv4: k and v must be uint8 [pages, Hkv, page, hd / 2]");
   const int64_t hd = 2 * k.size(3);
+  TORCH_CHECK(k.size(1) > 0, "kv4: a cache needs at least one KV head");
   TORCH_CHECK(hd == 64 || hd == 128, "kv4: head_dim must be 64 or 128, got " + std::to_string(hd));
   TORCH_CHECK(k.size(2) > 0 && k.size(2) % 16 == 0, "kv4: page size must be a multiple of 16, got " + std::to_string(k.size(2)));
   TORCH_CHECK(scale.scalar_type() == at::kHalf && scale.dim() == 6 && scale.size(0) == k.size(0) &&

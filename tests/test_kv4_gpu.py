@@ -384,3 +384,17 @@ def test_refusals():
             f()
             pytest.fail(f"call {i} was accepted")
     assert K.paged_attention_kv4(q[:0], c, bt[:0], n[:0]).shape == (0, 12, 128)
+
+
+def test_a_cache_without_heads_is_refused():
+    none = K.KV4Cache(torch.empty(2, 0, 16, 64, dtype=torch.uint8, device=DEV),
+                      torch.empty(2, 0, 16, 64, dtype=torch.uint8, device=DEV),
+                      torch.empty(2, 0, 16, 2, 2, 2, dtype=torch.float16, device=DEV))
+    x = torch.zeros(3, 0, 128, device=DEV).bfloat16()
+    slots = torch.arange(3, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    for f in (lambda: K.kv4_write(x, x, none, slots), lambda: K.kv4_read(none, slots),
+              lambda: K.paged_attention_kv4(torch.zeros(1, 4, 128, device=DEV).bfloat16(), none, torch.zeros(1, 1, **i32),
+                                            torch.ones(1, **i32))):
+        with pytest.raises(RuntimeError, match="KV head"):
+            f()
