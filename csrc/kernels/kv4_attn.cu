@@ -46,6 +46,8 @@
 // instructions' latency, not by memory: two computing warps on a scheduler keep 51-55 % of its issue slots busy, about
 // 2000 cycles to a unit (products of K 520, P V and the wait for the copies 770, scores 260, the next copies 285). With
 // few tokens it is the chain lengths, page id, copies, join (about 8 us).
+#include <climits>
+
 #include <cuda_runtime.h>
 
 #include "../include/sm100.cuh"
@@ -901,6 +903,7 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
                    cudaStream_t st) {
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
+  max_pages = std::min(max_pages, (INT_MAX - 63) / c.page);  // lengths are rounded up to units in 32 bits
   const Args a{q, qs, qh,  c,   bt,    bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads,
                0, 0,  scale, out, part, arrived, err};
   if (c.hd == 128)

@@ -308,6 +308,15 @@ def test_pages_and_lengths_outside_are_masked():
     assert bool((K.paged_attention_kv4(q, c, bt, torch.tensor([-3], dtype=torch.int32, device=DEV)) == 0).all())
 
 
+def test_length_at_the_end_of_32_bits():
+    """A table that spans 2^31 tokens and a length of 2^31 - 1: rounding it up to whole units must not wrap."""
+    q, c, bt, n = _setup([200], 2, 1, 128, 64)
+    wide = torch.full((1, (1 << 25) + 1), -1, dtype=torch.int32, device=DEV)
+    wide[:, :2] = bt[:, :2]
+    n.fill_(2 ** 31 - 1)
+    _check(K.paged_attention_kv4(q, c, wide, n), *_expect(q, c, bt, [128]))
+
+
 def test_offsets_beyond_32_bits():
     page, Hkv, hd = 64, 2, 128
     P = (1 << 31) // (Hkv * page * hd // 2) + 64  # more than 2^31 bytes of K
