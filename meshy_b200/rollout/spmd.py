@@ -23,6 +23,9 @@ LOCKSTEP = frozenset({
     "submit", "step", "run_until_idle", "generate", "abort_all", "pause", "resume", "release_memory",
     "resume_memory", "update_weights_from_state_dict", "update_weights_from_disk", "update_weights_from_ipc",
 })
+# of these, the calls that refuse unusable requests before anything else happens on any rank
+REFUSING = frozenset({"submit", "generate"})
+_REFUSED = "__refused__"
 
 
 def _to_host(obj):
@@ -59,7 +62,12 @@ class EngineLeader:
         def call(*args, **kwargs):
             with self._order:
                 self._broadcast((name, args, kwargs))
-                return attr(*args, **kwargs)
+                try:
+                    return attr(*args, **kwargs)
+                except (TypeError, ValueError):
+                    if name in REFUSING:  # the followers refused the call too: they go on
+                        self._broadcast((_REFUSED, (), {}))
+                    raise
 
         return call
 
@@ -69,14 +77,29 @@ class EngineLeader:
 
 
 def follow(engine, ctrl_group) -> None:
-    """A follower rank's loop: run every broadcast call on the local engine until rank 0 stops."""
+    """A follower rank's loop: run every broadcast call on the local engine until rank 0 stops. A request that this
+    rank refuses is one that rank 0 refuses too, and says so; every other exception ends the loop, so that the
+    replica's collectives fail instead of waiting for this rank."""
+    refused = None
     while True:
         box = [None]
         dist.broadcast_object_list(box, src=0, group=ctrl_group)
         name, args, kwargs = box[0]
+        if name == _REFUSED:
+            if refused is None:
+                raise RuntimeError("rank 0 refused a request that this rank accepted")
+            refused = None
+            continue
+        if refused is not None:
+            raise RuntimeError("this rank refused a request that rank 0 accepted") from refused
         if name == "__stop__":
             return
-        getattr(engine, name)(*args, **kwargs)
+        try:
+            getattr(engine, name)(*args, **kwargs)
+        except (TypeError, ValueError) as e:
+            if name not in REFUSING:
+                raise
+            refused = e
         engine.finished.clear()  # only rank 0 answers clients
 
 
