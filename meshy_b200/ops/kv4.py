@@ -52,12 +52,19 @@ def row_bytes(hd: int) -> int:
     return hd + 8 * (hd // GROUP)
 
 
-def kv4_empty(n_pages: int, n_kv: int, page: int, hd: int, device) -> KV4Cache:
-    """A zeroed cache."""
+def check_geometry(n_kv: int, page: int, hd: int) -> None:
+    """``ValueError`` for a cache that the kernels do not take."""
     if hd not in (64, 128):
         raise ValueError(f"4-bit KV cache: head_dim must be 64 or 128, got {hd}")
     if page <= 0 or page % 16:
         raise ValueError(f"4-bit KV cache: page size must be a multiple of 16, got {page}")
+    if n_kv <= 0:
+        raise ValueError(f"4-bit KV cache: at least one KV head is needed, got {n_kv}")
+
+
+def kv4_empty(n_pages: int, n_kv: int, page: int, hd: int, device) -> KV4Cache:
+    """A zeroed cache."""
+    check_geometry(n_kv, page, hd)
     return KV4Cache(torch.zeros(n_pages, n_kv, page, hd // 2, dtype=torch.uint8, device=device),
                     torch.zeros(n_pages, n_kv, page, hd // 2, dtype=torch.uint8, device=device),
                     torch.zeros(n_pages, n_kv, page, 2, hd // GROUP, 2, dtype=torch.float16, device=device))
@@ -65,6 +72,7 @@ def kv4_empty(n_pages: int, n_kv: int, page: int, hd: int, device) -> KV4Cache:
 
 def kv4_from_bytes(raw: torch.Tensor, n_pages: int, n_kv: int, page: int, hd: int) -> KV4Cache:
     """A cache laid over ``raw`` (uint8, at least ``n_pages * n_kv * page * row_bytes(hd)`` of them, 16-byte aligned)."""
+    check_geometry(n_kv, page, hd)
     n = n_pages * n_kv * page
     half = n * (hd // 2)
     if raw.dtype != torch.uint8 or raw.dim() != 1 or raw.numel() < n * row_bytes(hd):
@@ -106,4 +114,4 @@ def paged_attention_kv4(q: torch.Tensor, cache: KV4Cache, block_table: torch.Ten
     return ref.attention_decode_kv4(q, cache, block_table, seq_lens, scale)
 
 
-__all__ = ["KV4Cache", "kv4_empty", "kv4_from_bytes", "kv4_read", "kv4_write", "paged_attention_kv4", "row_bytes"]
+__all__ = ["KV4Cache", "check_geometry", "kv4_empty", "kv4_from_bytes", "kv4_read", "kv4_write", "paged_attention_kv4", "row_bytes"]

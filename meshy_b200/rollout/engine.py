@@ -127,6 +127,8 @@ class RolloutEngine:
             raise ValueError(f"kv_dtype must be 'auto' (the model's dtype) or 'int4', got {kv_dtype!r}")
         self.args = args
         self.kv4 = kv_dtype == "int4"
+        if self.kv4:
+            K4.check_geometry(args.n_kv_heads, page_size, args.head_dim)
         self.device = torch.device(device)
         self.cuda = self.device.type == "cuda"
         self.dtype = torch.bfloat16 if self.cuda else torch.float32

@@ -119,3 +119,11 @@ def test_cache_over_bytes():
 def test_unsupported_shapes_are_refused(page, hd):
     with pytest.raises(ValueError):
         K.kv4_empty(1, 1, page, hd, "cpu")
+
+
+@pytest.mark.parametrize("n_kv,page,hd", [(1, 16, 32), (1, 16, 192), (2, 24, 64), (1, 0, 128), (0, 16, 64)])
+def test_unsupported_shapes_are_refused_over_bytes_too(n_kv, page, hd):
+    with pytest.raises(ValueError, match="4-bit KV cache"):
+        K.kv4_from_bytes(torch.zeros(1 << 16, dtype=torch.uint8), 1, n_kv, page, hd)
+    with pytest.raises(ValueError, match="4-bit KV cache"):
+        K.kv4_empty(1, n_kv, page, hd, "cpu")

@@ -107,6 +107,15 @@ def test_unknown_kv_dtype_is_refused():
         _engine(kv_dtype="fp8")
 
 
+@pytest.mark.parametrize("head_dim,page", [(32, 16), (192, 16), (64, 24)])
+def test_unsupported_geometry_of_the_4bit_cache_is_refused(head_dim, page):
+    args = get_model_args("qwen3", "debugmodel", head_dim=head_dim)
+    model = build_model(args, seed=3)
+    with pytest.raises(ValueError, match="4-bit KV cache"):
+        RolloutEngine(args, model=model, max_running=4, max_total_tokens=768, max_seq_len=96, page_size=page, kv_dtype="int4")
+    RolloutEngine(args, model=model, max_running=4, max_total_tokens=768, max_seq_len=96, page_size=page)
+
+
 def test_server_takes_the_parameters_and_answers_400():
     pytest.importorskip("aiohttp")
     from aiohttp.test_utils import TestClient, TestServer
