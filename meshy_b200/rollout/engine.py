@@ -489,8 +489,19 @@ class RolloutEngine:
             req.pages = pages
             req.out_slot = self.free_out_slots.pop()
             batch.append(self.waiting.pop(0))
-        if batch:
+        if not batch:
+            return
+        try:
             self._prefill(batch)
+        except Exception:
+            # back to the head of the queue, where an abort finds the requests; rows that were begun are idle again
+            for req in batch:
+                self.blocks.free(req.pages)
+                self.free_out_slots.append(req.out_slot)
+                req.pages, req.out_slot = [], -1
+            self.waiting[:0] = batch
+            self._park_rows(len(self.running))
+            raise
 
     def _ensure_pages(self, rows: Sequence[int], lookahead: int) -> None:
         """Grow page lists so every row can decode ``lookahead`` more tokens."""

@@ -102,6 +102,33 @@ def test_unusable_values_are_refused(kw):
     assert not e.waiting
 
 
+@pytest.mark.parametrize("kv_dtype", ["auto", "int4"])
+def test_requests_of_a_prefill_that_raises_are_not_lost(kv_dtype, monkeypatch):
+    e = _engine(kv_dtype=kv_dtype)
+    want = _greedy(e, PROMPTS, 6, presence_penalty=0.5)
+    real = e._sample_rows
+
+    def fails(h, reqs):
+        raise RuntimeError("no logits")
+
+    monkeypatch.setattr(e, "_sample_rows", fails)
+    rids = [e.submit(p, 6, temperature=0.0, presence_penalty=0.5) for p in PROMPTS]
+    free, slots = e.blocks.num_free, len(e.free_out_slots)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no logits"):
+            e.step()
+    assert [r.rid for r in e.waiting] == rids and not e.running
+    assert e.blocks.num_free == free and len(e.free_out_slots) == slots and int(e.st["done"].min()) == 1
+    monkeypatch.setattr(e, "_sample_rows", real)
+    e.run_until_idle()  # served after all
+    assert [e.finished.pop(r).output_ids for r in rids] == want
+    monkeypatch.setattr(e, "_sample_rows", fails)
+    rids = [e.submit(p, 6) for p in PROMPTS]
+    with pytest.raises(RuntimeError, match="no logits"):
+        e.step()
+    assert [g.rid for g in e.abort_all()] == rids and not e.has_work()
+
+
 def test_unknown_kv_dtype_is_refused():
     with pytest.raises(ValueError, match="kv_dtype"):
         _engine(kv_dtype="fp8")
