@@ -108,11 +108,14 @@ class EngineClient(_Base):
     async def _generate_once(self, prompt, params):
         url = f"{self._next()}/generate"
         payload = {"input_ids": prompt, "sampling_params": params, "return_logprob": True}
-        last = None
+        last = refused = None
         for i in range(self.attempts):
             try:
                 s = await self._sess()
                 async with s.post(url, json=payload) as r:
+                    if r.status == 400:  # the request itself: another attempt would be refused too
+                        refused = await r.text()
+                        break
                     if r.status != 200:
                         raise RuntimeError(f"status {r.status}")
                     body = await r.json()
@@ -124,6 +127,8 @@ class EngineClient(_Base):
                 last = e
                 if i + 1 < self.attempts:
                     await asyncio.sleep(min(self.backoff * (i + 1), self.backoff_max))
+        if refused is not None:
+            raise ValueError(f"engine refused the request: {refused}")
         raise last
 
     # ------------------------------------------------------------------ management
