@@ -63,7 +63,8 @@ class _Base:
                     return res
                 p["max_new_tokens"] = remaining
             if res.output_ids and any(p.get(k) for k in ("frequency_penalty", "presence_penalty")):
-                p["n_generated"] = len(res.output_ids)  # resubmitted below as part of the prompt
+                # resubmitted below as part of the prompt, behind what the caller had generated before
+                p["n_generated"] = int(params.get("n_generated") or 0) + len(res.output_ids)
             toks, lps, reason, version = await self._generate_once(prompt + res.output_ids, p)
             if any(not math.isfinite(x) for x in lps):
                 raise ValueError("engine returned non-finite log-probs")

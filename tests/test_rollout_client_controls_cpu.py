@@ -4,7 +4,7 @@ import asyncio
 
 import pytest
 
-from meshy_b200.engine.rollout_client import EngineClient
+from meshy_b200.engine.rollout_client import EngineClient, _Base
 
 PROMPT = [5, 9, 77, 300, 12]
 
@@ -50,3 +50,25 @@ def test_a_refused_request_is_not_sent_again(params):
 
     posts, ids = _with_server(use)
     assert posts == 2 and len(ids) == 4
+
+
+class _Aborting(_Base):
+    """Answers with the given pieces of output, all but the last of them cut off by an abort."""
+
+    def __init__(self, *pieces):
+        self.pieces, self.seen = list(pieces), []
+
+    async def _generate_once(self, prompt, params):
+        self.seen.append((prompt, params))
+        out = self.pieces.pop(0)
+        return out, [0.0] * len(out), "abort" if self.pieces else "stop", 0
+
+
+@pytest.mark.parametrize("before,want", [({}, [None, 2, 3]), ({"n_generated": 4}, [4, 6, 7])])
+def test_a_continued_request_keeps_what_was_generated_before(before, want):
+    c = _Aborting([1, 2], [3], [4, 5])
+    params = dict(before, presence_penalty=0.5, max_new_tokens=9)
+    res = asyncio.run(c.generate(PROMPT, params))
+    assert res.output_ids == [1, 2, 3, 4, 5] and [p.get("n_generated") for _, p in c.seen] == want
+    assert [p for p, _ in c.seen] == [PROMPT, PROMPT + [1, 2], PROMPT + [1, 2, 3]]
+    assert params == dict(before, presence_penalty=0.5, max_new_tokens=9)
