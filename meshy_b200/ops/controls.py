@@ -87,6 +87,8 @@ class LogitControls:
                  presence_penalty: float = 0.0, logit_bias: Mapping[int, float] | None = None,
                  allowed_tokens: Sequence[int] | None = None) -> None:
         """The controls of one slot (defaults: off). Its token state is :func:`load_tokens`'s."""
+        if allowed_tokens is not None:
+            allowed_tokens = [int(t) for t in allowed_tokens]
         check_controls(self.vocab, self.max_bias, repetition_penalty, frequency_penalty, presence_penalty, logit_bias,
                        allowed_tokens)
         self.repetition[slot] = float(repetition_penalty)

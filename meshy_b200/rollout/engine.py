@@ -392,11 +392,14 @@ class RolloutEngine:
         """Queue a request. The penalties, ``logit_bias`` and ``allowed_tokens`` act on the logits before temperature
         and filters (:mod:`..ops.controls`); ``n_generated``: so many tokens at the prompt's end are output of an
         earlier, aborted call (the frequency and presence penalties count them)."""
-        controls = {k: v for k, v, off in (("repetition_penalty", float(repetition_penalty), 1.0),
-                                           ("frequency_penalty", float(frequency_penalty), 0.0),
-                                           ("presence_penalty", float(presence_penalty), 0.0),
-                                           ("logit_bias", logit_bias or None, None),
-                                           ("allowed_tokens", allowed_tokens, None)) if v != off}
+        # (copies: the request is looked at again when it is admitted)
+        controls = {k: float(v) for k, v, off in (("repetition_penalty", repetition_penalty, 1.0),
+                                                  ("frequency_penalty", frequency_penalty, 0.0),
+                                                  ("presence_penalty", presence_penalty, 0.0)) if float(v) != off}
+        if logit_bias:
+            controls["logit_bias"] = dict(logit_bias)
+        if allowed_tokens is not None:
+            controls["allowed_tokens"] = [int(t) for t in allowed_tokens]
         check_controls(self.args.vocab_size, MAX_LOGIT_BIAS, **controls)
         if not 0 <= n_generated <= len(prompt):
             raise ValueError(f"n_generated must be between 0 and the prompt's length, got {n_generated}")

@@ -69,6 +69,13 @@ def test_values_are_refused(kw):
         ctl.set_slot(0, **kw)
 
 
+def test_allowed_tokens_may_be_an_iterator():
+    ctl = C.LogitControls.create(1, 40, device="cpu", max_bias=0)
+    ctl.set_slot(0, allowed_tokens=iter([3, 33]))
+    out = C.apply_logit_controls(torch.zeros(1, 40), ctl, torch.tensor([0]))
+    assert out[0].isfinite().nonzero().flatten().tolist() == [3, 33]
+
+
 def test_sizes_are_refused():
     for slots, vocab, k in ((0, 4, 0), (1, 0, 0), (1, 4, -1)):
         with pytest.raises(ValueError):

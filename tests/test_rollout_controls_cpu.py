@@ -46,6 +46,27 @@ def test_allowed_tokens_and_bias():
     assert out == [[123] * 4] * 3
 
 
+@pytest.mark.parametrize("kind", ["array", "tensor", "range", "set", "iterator"])
+def test_allowed_tokens_of_any_kind(kind):
+    np = pytest.importorskip("numpy")
+    ids = [7, 8, 9]
+    allowed = {"array": np.array(ids), "tensor": torch.tensor(ids), "range": range(7, 10), "set": set(ids), "iterator": iter(ids)}[kind]
+    e = _engine()
+    rid = e.submit(PROMPTS[0], 6, temperature=0.0, allowed_tokens=allowed)
+    e.run_until_idle()
+    assert set(e.finished[rid].output_ids) <= set(ids)
+
+
+def test_controls_changed_after_submit_do_not_reach_the_request():
+    e = _engine()
+    allowed, bias = [7, 8], {7: 1e4}
+    rid = e.submit(PROMPTS[0], 3, temperature=0.0, allowed_tokens=allowed, logit_bias=bias)
+    allowed[:] = [10 ** 6]
+    bias[-1] = 0.0
+    e.run_until_idle()
+    assert e.finished[rid].output_ids == [7] * 3
+
+
 def test_presence_penalty_never_repeats_and_continues():
     e = _engine()
     out = _greedy(e, PROMPTS, 20, presence_penalty=1e4)
