@@ -18,7 +18,6 @@ On CUDA each function is one native kernel on the current stream and can be capt
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 from typing import Mapping, Sequence
 
@@ -27,6 +26,9 @@ import torch
 from . import reference as ref
 from ._ext import ext
 from .checks import check_range
+
+
+_FP32 = torch.finfo(torch.float32)
 
 
 def _words(vocab: int) -> int:
@@ -111,11 +113,12 @@ class LogitControls:
 def check_controls(vocab: int, max_bias: int, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
                    presence_penalty: float = 0.0, logit_bias: Mapping[int, float] | None = None,
                    allowed_tokens: Sequence[int] | None = None) -> None:
-    """``ValueError`` unless the values of one request are usable."""
-    if not (repetition_penalty > 0 and math.isfinite(repetition_penalty)):
+    """``ValueError`` unless the values of one request are usable (they are held in fp32, where 1e39 is no number and
+    1e-50 is zero)."""
+    if not (_FP32.tiny <= repetition_penalty <= _FP32.max):
         raise ValueError(f"repetition_penalty must be positive, got {repetition_penalty}")
     for name, x in (("frequency_penalty", frequency_penalty), ("presence_penalty", presence_penalty)):
-        if not math.isfinite(x):
+        if not abs(x) <= _FP32.max:
             raise ValueError(f"{name} must be finite, got {x}")
     if logit_bias:
         if len(logit_bias) > max_bias:
@@ -123,7 +126,7 @@ def check_controls(vocab: int, max_bias: int, repetition_penalty: float = 1.0, f
         ids = [int(v) for v in logit_bias]
         if len(set(ids)) < len(ids) or min(ids) < 0 or max(ids) >= vocab:
             raise ValueError(f"logit_bias token ids must be distinct and in [0, {vocab})")
-        if not all(math.isfinite(float(x)) for x in logit_bias.values()):
+        if not all(abs(float(x)) <= _FP32.max for x in logit_bias.values()):
             raise ValueError("logit_bias values must be finite (allowed_tokens forbids tokens)")
     if allowed_tokens is not None:
         ids = [int(v) for v in allowed_tokens]

@@ -69,6 +69,14 @@ def test_values_are_refused(kw):
         ctl.set_slot(0, **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=1e39), dict(repetition_penalty=1e-50), dict(repetition_penalty=math.nan),
+                                dict(frequency_penalty=1e39), dict(presence_penalty=-1e39), dict(logit_bias={1: -1e39})])
+def test_values_outside_fp32_are_refused(kw):
+    ctl = C.LogitControls.create(1, 40, device="cpu", max_bias=2)
+    with pytest.raises(ValueError):
+        ctl.set_slot(0, **kw)
+
+
 def test_allowed_tokens_may_be_an_iterator():
     ctl = C.LogitControls.create(1, 40, device="cpu", max_bias=0)
     ctl.set_slot(0, allowed_tokens=iter([3, 33]))
