@@ -89,6 +89,7 @@ class LogitControls:
                  presence_penalty: float = 0.0, logit_bias: Mapping[int, float] | None = None,
                  allowed_tokens: Sequence[int] | None = None) -> None:
         """The controls of one slot (defaults: off). Its token state is :func:`load_tokens`'s."""
+        self._check_slot(slot)
         if allowed_tokens is not None:
             allowed_tokens = [int(t) for t in allowed_tokens]
         check_controls(self.vocab, self.max_bias, repetition_penalty, frequency_penalty, presence_penalty, logit_bias,
@@ -103,9 +104,16 @@ class LogitControls:
             self.bias_vals[slot, :n] = torch.tensor([float(x) for x in logit_bias.values()])
         self.set_mask(slot, None if allowed_tokens is None else token_bits(allowed_tokens, self.vocab))
 
+    def _check_slot(self, slot: int) -> None:
+        if not 0 <= slot < self.counts.shape[0]:
+            raise ValueError(f"logit controls: slot {slot} outside [0, {self.counts.shape[0]})")
+
     def set_mask(self, slot: int, bits: torch.Tensor | None) -> None:
         """Token mask of one slot as a bitmask ``[W]`` int32 (see :func:`token_bits`); ``None``: every token allowed."""
+        self._check_slot(slot)
         if bits is not None:
+            if bits.dtype != torch.int32 or bits.shape != self.mask.shape[1:]:
+                raise ValueError(f"token mask must be int32 [{self.mask.shape[1]}], got {bits.dtype} {list(bits.shape)}")
             self.mask[slot].copy_(bits)
         self.mask_on[slot] = 0 if bits is None else 1
 

@@ -77,6 +77,20 @@ def test_values_outside_fp32_are_refused(kw):
         ctl.set_slot(0, **kw)
 
 
+def test_slots_and_masks_are_checked():
+    ctl = C.LogitControls.create(2, 70, device="cpu", max_bias=0)
+    ok = C.token_bits([5], 70)
+    for slot, bits in ((0, ok[:1]), (0, ok[None]), (0, ok.long()), (0, ok.bool()), (-1, ok), (2, ok), (-1, None)):
+        with pytest.raises(ValueError):
+            ctl.set_mask(slot, bits)
+    for slot in (-1, 2):
+        with pytest.raises(ValueError):
+            ctl.set_slot(slot, presence_penalty=1.0)
+    assert ctl.mask_on.tolist() == [0, 0] and ctl.presence.tolist() == [0.0, 0.0] and bool((ctl.mask == -1).all())
+    ctl.set_mask(1, ok)
+    assert ctl.mask[1].tolist() == ok.tolist() and ctl.mask_on.tolist() == [0, 1]
+
+
 def test_allowed_tokens_may_be_an_iterator():
     ctl = C.LogitControls.create(1, 40, device="cpu", max_bias=0)
     ctl.set_slot(0, allowed_tokens=iter([3, 33]))
