@@ -52,6 +52,17 @@ def test_a_refused_request_is_not_sent_again(params):
     assert posts == 2 and len(ids) == 4
 
 
+@pytest.mark.parametrize("params", [dict(logit_bias=[3, 4]), dict(allowed_token_ids=5), dict(presence_penalty=[1]),
+                                    dict(allowed_token_ids=[None]), dict(logit_bias={"a": 1})])
+def test_parameters_of_another_type_are_refused(params):
+    async def use(c, counts):
+        with pytest.raises(ValueError, match="refused"):
+            await c.generate(PROMPT, dict(params, max_new_tokens=4))
+        return counts["posts"]
+
+    assert _with_server(use) == 1
+
+
 class _Aborting(_Base):
     """Answers with the given pieces of output, all but the last of them cut off by an abort."""
 
