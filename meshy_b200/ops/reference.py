@@ -216,17 +216,19 @@ def kv4_read(cache, slots, dtype=torch.float32):
 
 
 def attention_decode_kv4(q, cache, block_table, seq_lens, scale: float | None = None) -> torch.Tensor:
-    """:func:`attention_decode_paged` over the values of a 4-bit cache; a row of length 0 gives zeros."""
+    """:func:`attention_decode_paged` over the values of a 4-bit cache. Tokens of pages outside the cache or past the
+    block table do not count; a row without tokens gives zeros."""
     B, Hq, hd = q.shape
-    Hkv, page = cache.k.shape[1], cache.k.shape[2]
+    pages, Hkv, page = cache.k.shape[:3]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     out = torch.zeros(B, Hq, hd, dtype=torch.float32, device=q.device)
     for b in range(B):
-        L = int(seq_lens[b])
-        if L <= 0:
+        t = torch.arange(max(0, min(int(seq_lens[b]), block_table.shape[1] * page)), device=q.device)
+        pg = block_table[b, t // page].long()
+        there = (pg >= 0) & (pg < pages)
+        if not bool(there.any()):
             continue
-        t = torch.arange(L, device=q.device)
-        k, v = kv4_read(cache, block_table[b, t // page].long() * page + t % page)
+        k, v = kv4_read(cache, (pg * page + t % page)[there])
         qb = q[b].float().view(Hkv, Hq // Hkv, hd)
         p = torch.softmax(torch.einsum("grd,lgd->grl", qb, k) * scale, dim=-1)
         out[b] = torch.einsum("grl,lgd->grd", p, v).reshape(Hq, hd)

@@ -105,6 +105,18 @@ def test_attention_matches_softmax_over_stored_values():
                 assert torch.allclose(out[i, h].double(), p @ v[rows, h // 3], rtol=1e-5, atol=1e-5)
 
 
+def test_pages_and_lengths_outside_are_masked():
+    g = torch.Generator().manual_seed(5)
+    c = K.kv4_empty(4, 2, 16, 64, "cpu")
+    K.kv4_write(torch.randn(64, 2, 64, generator=g), torch.randn(64, 2, 64, generator=g), c, torch.arange(64))
+    q = torch.randn(1, 4, 64, generator=g)
+    run = lambda pages, n: K.paged_attention_kv4(q, c, torch.tensor([pages], dtype=torch.int32), torch.tensor([n], dtype=torch.int32))
+    want = run([2, 0], 32)
+    assert torch.allclose(run([2, 0, 4, -1], 60), want) and torch.allclose(run([2, -7, 0], 48), want)
+    assert torch.equal(run([2, 0], 1 << 30), want)
+    assert bool((run([-1, 9], 20) == 0).all()) and bool((run([2, 0], -3) == 0).all())
+
+
 def test_cache_over_bytes():
     assert K.row_bytes(128) == 144 and K.row_bytes(64) == 72
     raw = torch.zeros(3 * 2 * 16 * 144, dtype=torch.uint8)
