@@ -16,9 +16,11 @@
 // unpacking.
 //
 // P carries the scale of V (x = p a'), so a reference m per warp and head keeps it in fp16's range: p is taken relative
-// to m, which is set so that the largest x seen is 2^11, and moves again only when p or a' have outgrown what it was set
-// for by 8 or 2 (x stays below 2^15). So most units take neither the maximum's shuffles nor a rescaling, and what falls
-// below fp16's smallest number is less than 2^-35 of the largest term. P is rounded to fp16's 11 bits there; sums, the
+// to m, which is set so that the largest p a' seen, a' being the larger scale of a token's groups, is 2^11, and moves
+// again only when a later one passes 2^15. So most units take neither the maximum's shuffles nor a rescaling. x is
+// rounded to fp16's 11 bits, or by 2^-25 where it is below 2^-14: less than 2^-35 of the largest p a'. (A reference for
+// the largest p and the largest a' apart lost the values of a long tail where tokens of no weight had values that spread
+// 2^16 times as far.) Scales below 2^-24, the smallest there is, count as that, so that p stays below 2^39; sums, the
 // normaliser and the bases' part stay in 32 bits.
 //
 // Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (64 at head
@@ -67,8 +69,8 @@ constexpr uint32_t kWholeUnits = 24;           // units of equal segments that a
 constexpr int kPad = 16;                        // units that a change of segments costs
 constexpr int kJoinSteps = 3;                  // steps of a warp that a join is worth
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBoost = 2048.f;               // x of the largest p and a' right after the reference moved
-constexpr float kGrowP = 8.f, kGrowA = 2.f;    // how far either may pass it: x stays below 2^15
+constexpr float kBoost = 11.f;                 // log2 of the largest p a' right after the reference moved
+constexpr float kLimit = 32768.f;              // how far later ones may go
 constexpr float kMinA = 5.9604645e-8f;         // 2^-24, the smallest fp16
 
 template <int HD, int NT, int NP>  // NT tiles to a unit, which lie in NP pieces (pages, or parts of one)
@@ -598,9 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) cs[r] = reinterpret_cast<const float*>(frags + C::F_FACTOR)[2 * t + r];
       const uint32_t frag_at = smem_u32(frags) + lane * 16;
-      // o, z and l are relative to the reference m: p 2^-m; m < the true maximum, so that x fits fp16 well
+      // o, z and l are relative to the reference m: p 2^-m, so that x fits fp16 well
       float o[G][4][4], z[G][2], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
-      float lim_p = -1.f, lim_a = kMinA * kGrowA;  // lim_p below 0: no reference yet
+      float limit = -1.f;  // below 0: no reference yet
 #pragma unroll
       for (int i = 0; i < G; ++i) {
 #pragma unroll
@@ -690,34 +692,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
                 for (int j = 0; j < G; ++j) va[n][i][j] = vz[n][i][j] = 0.f;
               }
         }
-        float p[NT][2][2], top_p = 0.f, top_a = 0.f;
+        float p[NT][2][2], top_x = 0.f;
+        auto largest_a = [&](int n, int i) { return fmaxf(kMinA, G == 2 ? fmaxf(va[n][i][0], va[n][i][G - 1]) : va[n][i][0]); };
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
+            const float a1 = largest_a(n, i);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               p[n][i][r] = ex2(s[n][i][r]);
-              top_p = fmaxf(top_p, p[n][i][r]);
+              top_x = fmaxf(top_x, p[n][i][r] * a1);
             }
-#pragma unroll
-            for (int j = 0; j < G; ++j) top_a = fmaxf(top_a, va[n][i][j]);
           }
-        if (__any_sync(0xffffffffu, top_p > lim_p || top_a > lim_a)) {
-          // move the reference: to the true maxima, less what brings x to kBoost
-          const float A0 = lim_a / kGrowA, A = max_over_rows(fmaxf(A0, top_a)), lift = lg2(kBoost / A);
+        if (__any_sync(0xffffffffu, top_x > limit)) {
+          // move the reference: to the largest p a', less what brings that to 2^kBoost
           bool found = false;
           float keep[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float top = s[0][0][r];
+            float top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][0][r], s[n][1][r]));
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) top = fmaxf(top, s[n][i][r] + lg2(largest_a(n, i)));
             top = max_over_rows(top) + m[r];
-            if (lim_p > 0.f) top = fmaxf(top, m[r] + lg2(kBoost / A0));
+            if (limit > 0.f) top = fmaxf(top, m[r] + kBoost);
             const bool real = top != -INFINITY;
-            const float to = real ? top - lift : m[r];
-            keep[r] = lim_p > 0.f ? ex2(m[r] - to) : 0.f;
+            const float to = real ? top - kBoost : m[r];
+            keep[r] = limit > 0.f ? ex2(m[r] - to) : 0.f;
             found |= real;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -726,8 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
             m[r] = to;
             l[r] *= keep[r];
           }
-          if (__any_sync(0xffffffffu, found)) lim_p = kBoost / A * kGrowP;
-          lim_a = A * kGrowA;
+          if (__any_sync(0xffffffffu, found)) limit = kLimit;
 #pragma unroll
           for (int j = 0; j < G; ++j) {
 #pragma unroll
@@ -787,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
           d[1] = make_float4(x[4], x[5], x[6], x[7]);
         }
         if (g == 0) {
-          sm[slot][warp][2 * t + r] = lim_p < 0.f ? -INFINITY : m[r];
+          sm[slot][warp][2 * t + r] = limit < 0.f ? -INFINITY : m[r];
           sl[slot][warp][2 * t + r] = l[r];
         }
       }

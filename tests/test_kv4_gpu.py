@@ -267,6 +267,36 @@ def test_attention_long_tail_keeps_its_mass(peak):
     assert bool(((out.double() - want).abs() <= 2 ** -7 * want.abs()).all())
 
 
+@pytest.mark.parametrize("L", [700, 20000])
+@pytest.mark.parametrize("every", [0, 100000, 256, 32])
+def test_small_values_beside_tokens_of_large_ones(L, every):
+    """Values that carry the result keep their precision beside tokens of next to no weight whose values spread a hundred
+    thousand times as far, and below peaks that have no spread at all. Weights and their products with the scales are
+    held in 11 bits, scores to 2^-12, the result in bf16: 2^-9 |o| + 2^-9 sum p |v|."""
+    hd = 128
+    g = _gen(12)
+    t = torch.arange(L, device=DEV)
+    k = torch.zeros(L, 1, hd, device=DEV)
+    v = 10 + 4 * torch.rand(L, 1, hd, generator=g, device=DEV)
+    k[t % 256 == 5, 0, 0] = 16.0         # a factor 2^22 ahead of the others
+    v[t % 256 == 5] = 0
+    if every:
+        k[t % every == 0, 0, 0] = -64.0  # 2^-88 of the others
+        v[t % every == 0] = 65504.0 * (torch.arange(hd, device=DEV) % 2 * 2 - 1)
+    q = torch.zeros(1, 2, hd, device=DEV).bfloat16()
+    q[..., 0] = 1.0
+    scale = 22 * math.log(2) / 16
+    bt = torch.arange(-(-L // 64), dtype=torch.int32, device=DEV)[None]
+    c = K.kv4_empty(bt.shape[1], 1, 64, hd, DEV)
+    K.kv4_write(k.bfloat16(), v.bfloat16(), c, t)
+    out = K.paged_attention_kv4(q, c, bt, torch.tensor([L], dtype=torch.int32, device=DEV), scale)
+    kk, vv = _value64(c, t, 0)[:, 0], _value64(c, t, 1)[:, 0]
+    p = torch.softmax(kk @ q[0, 0].double() * scale, 0)
+    want, size = p @ vv, (p * vv.abs().amax(1)).sum()
+    err = (out[0].double() - want).abs()
+    assert bool((err <= 2 ** -9 * want.abs() + 2 ** -9 * size).all()), float((err / size).max())
+
+
 def test_attention_rising_scores():
     """Every tile's maximum above the last: the running maximum moves at every step, late keys carry the weight."""
     L, hd = 5000, 128
