@@ -206,7 +206,7 @@ class RolloutEngine:
         self._init_state()
         self._mega = None
         self._mega_rows = 0
-        self.mega_reason = "not on CUDA"
+        self.mega_reason = ("not on CUDA" if not self.cuda else "4-bit KV cache" if self.kv4 else "tensor parallelism")
         if self.cuda and self.tp_group is None and not self.kv4:
             from .mega import MAX_ROWS, MegaDecoder
 

@@ -77,3 +77,8 @@ def test_head_width_128_and_bias_model():
         out.append(e.generate([[3, 1, 4] * 100, [2, 7] * 9], 40, temperature=0.0))
     # a random model's next token is a near tie, so only the shapes and the first steps' agreement say something
     assert all(len(g.output_ids) == 40 for o in out for g in o)
+
+
+def test_whole_step_kernel_is_off_for_the_4bit_cache_and_says_why():
+    assert _engine(kv_dtype="int4").mega_reason == "4-bit KV cache"
+    assert _engine().mega_reason is None or "4-bit" not in _engine().mega_reason
