@@ -157,6 +157,32 @@ def test_write_groups_beyond_the_range():
     assert bool(k.isfinite().all()) and torch.equal(k, x.clamp(-65504, 65504)) and torch.equal(v, -k)
 
 
+def test_every_scale_is_written_as_divided():
+    """Each fp16 scale that a group can have, with channels at and around the halves: the quotients by multiplication
+    have the bits of a division."""
+    from meshy_b200.ops import reference as ref
+
+    a = torch.arange(1, 0x7C00, dtype=torch.int16).view(torch.float16).float()
+    a = a[15 * a <= 2 * 65504]
+    span = (15 * a).to(DEV)
+    hi = (span.view(torch.int32) & -65536).view(torch.float32)  # the upper 8 bits; the rest is a bf16 number too
+    hi = torch.minimum(hi, torch.full_like(hi, 65280.0))
+    lo = -(span - hi)
+    g = _gen(11)
+    x = lo[:, None] + span[:, None] * torch.rand(len(a), 64, generator=g, device=DEV)
+    x[:, 32:] = lo[:, None] + a.to(DEV)[:, None] * (torch.randint(30, (len(a), 32), generator=g, device=DEV) / 2.0)
+    x[:, 0], x[:, 63] = lo, hi
+    x = x.bfloat16().clamp(lo.bfloat16()[:, None], hi.bfloat16()[:, None])[:, None]
+    pages = -(-len(a) // 64)
+    c = K.kv4_empty(pages, 1, 64, 64, DEV)
+    slots = torch.arange(len(a), device=DEV)
+    K.kv4_write(x, x, c, slots)
+    b, pairs = ref.kv4_quantize(x.cpu())
+    assert torch.equal(c.k.view(-1, 1, 32)[slots].cpu(), b)
+    assert torch.equal(c.scale.view(-1, 1, 2, 1, 2)[slots][:, :, 0].cpu(), pairs)
+    assert len(pairs[..., 0].unique()) > 0.9 * len(a)
+
+
 def test_slots_outside_are_skipped_and_empty_calls():
     c = K.kv4_empty(2, 2, 16, 128, DEV)
     x = torch.ones(4, 2, 128, device=DEV).bfloat16()
@@ -228,6 +254,58 @@ def test_attention_ragged_splits(B, longest, page, Hq, Hkv, hd):
     _check(out, *_expect(q, c, bt, lens))
     for b in (0, B // 2, B - 1):  # a row by itself: other cuts, the same numbers to rounding
         _check(K.paged_attention_kv4(q[b:b + 1], c, bt[b:b + 1], n[b:b + 1]), *_expect(q[b:b + 1], c, bt[b:b + 1], [lens[b]]))
+
+
+def _count_setup(lens, Hq, Hkv, hd, page, seed, channel):
+    """Keys of zero, so that every token has the same weight, and values that are one in channel ``channel(t, head)``
+    (where that is one) and zero elsewhere: out[ch] is the number of a row's tokens with that channel, over its length."""
+    g = _gen(seed)
+    need = [-(-n // page) for n in lens]
+    P = sum(need) + 1
+    c = K.kv4_empty(P, Hkv, page, hd, DEV)
+    c.scale.fill_(float("nan"))
+    bt = torch.full((len(lens), max(need + [1])), -7, dtype=torch.int32, device=DEV)
+    order = torch.randperm(P, generator=g, device=DEV)
+    want = torch.zeros(len(lens), Hkv, hd, dtype=torch.float64, device=DEV)
+    one = 15 * float(torch.tensor(1 / 15).half())  # what the cache holds for 1
+    at = 0
+    for i, n in enumerate(lens):
+        pg = order[at:at + need[i]]
+        at += need[i]
+        bt[i, :need[i]] = pg.int()
+        if n:
+            t = torch.arange(n, device=DEV)
+            ch = channel(t[:, None], torch.arange(Hkv, device=DEV)[None])
+            v = ((ch[..., None] == torch.arange(hd, device=DEV))).bfloat16()
+            K.kv4_write(torch.zeros_like(v), v, c, pg[t // page] * page + t % page)
+            want[i] = v.double().sum(0) * one / n
+    q = torch.randn(len(lens), Hq, hd, generator=g, device=DEV).bfloat16()
+    return q, c, bt, torch.tensor(lens, dtype=torch.int32, device=DEV), want.repeat_interleave(Hq // Hkv, 1)
+
+
+def _check_counts(lens, Hq, Hkv, hd, page, seed, channel):
+    # a weight and its product with the scale are rounded to 2^-11 at most, the result to 2^-9; a channel whose count is
+    # below 128 shows one token more or less
+    q, c, bt, n, want = _count_setup(lens, Hq, Hkv, hd, page, seed, channel)
+    err = (K.paged_attention_kv4(q, c, bt, n).double() - want).abs()
+    assert bool((err <= 2 ** -8 * want).all()), float((err / want.clamp(min=1e-9)).max())
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(12, 2, 128), (14, 2, 64), (17, 1, 128)])
+@pytest.mark.parametrize("lens,page", [([1], 64), ([31, 32, 33, 63, 64, 65], 32), ([700], 64), ([3001, 0, 129, 1, 4097], 16),
+                                       ([9000, 5, 8999], 48), ([20011], 64), ([70001], 32), ([257] * 150 + [3000], 64),
+                                       ([100, 0, 7] * 100, 16), ([4096] * 8, 64), ([16384, 16383], 64)])
+def test_no_block_of_tokens_is_lost_or_doubled(lens, page, Hq, Hkv, hd):
+    for block in (1, 16, 32, 100):
+        _check_counts(lens, Hq, Hkv, hd, page, len(lens) + block, lambda t, h: (t // block + h) % hd)
+
+
+@pytest.mark.parametrize("lens,page,Hq,Hkv,hd", [([20011], 64, 8, 8, 128), ([9000], 48, 16, 4, 64), ([2500, 0, 5001, 77], 16, 8, 8, 64),
+                                                 ([1500] * 20 + [33], 64, 16, 8, 128), ([70001], 64, 16, 16, 128)])
+def test_every_token_counts_once(lens, page, Hq, Hkv, hd):
+    """A window of hd tokens to a head, a token to a channel: wherever the work is cut, out[ch] is 1 / length."""
+    for first in range(0, max(lens), hd * Hkv):
+        _check_counts(lens, Hq, Hkv, hd, page, first, lambda t, h: t - first - h * hd)
 
 
 @pytest.mark.parametrize("kscale,vscale,koff", [(1.0, 1e-4, 0.0), (1.0, 2000.0, 0.0), (4.0, 1.0, 0.0), (0.3, 1.0, 8.0),
@@ -403,6 +481,25 @@ def test_two_streams_at_once():
         outs.append((oa, ob))
     torch.cuda.synchronize()
     assert all(torch.equal(oa, wa) and torch.equal(ob, wb) for oa, ob in outs)
+
+
+def test_workspace_grows_with_the_segments():
+    """More segments than the first counters hold (16384), on a stream that has used the smaller ones."""
+    B, Hkv, hd, page = 2100, 8, 64, 16
+    s = torch.cuda.Stream()
+    small = _setup([40, 3000], 8, Hkv, hd, page, seed=3)
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 40, (B,), generator=g).tolist()
+    many = _setup(lens, 8, Hkv, hd, page, seed=4)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        a = K.paged_attention_kv4(*small)
+        b = [K.paged_attention_kv4(*many) for _ in range(2)]
+        a2 = K.paged_attention_kv4(*small)
+    s.synchronize()
+    _check(a, *_expect(*small[:3], [40, 3000]))
+    _check(b[0], *_expect(*many[:3], lens))
+    assert torch.equal(a, a2) and torch.equal(*b)
 
 
 def test_refusals():

@@ -82,3 +82,29 @@ def test_head_width_128_and_bias_model():
 def test_whole_step_kernel_is_off_for_the_4bit_cache_and_says_why():
     assert _engine(kv_dtype="int4").mega_reason == "4-bit KV cache"
     assert _engine().mega_reason is None or "4-bit" not in _engine().mega_reason
+
+
+@pytest.mark.parametrize("flavor,kw", [(("qwen2_5_math", "R1-Distill-1.5B"), dict(n_layers=2, vocab_size=4096)),
+                                       (("qwen3", "debugmodel"), {})])
+def test_int4_prefill_and_decode_see_the_same_cache(flavor, kw):
+    """A prompt that ends before a generated token gives that token the log-probability that it had when it was drawn:
+    decode attends to the cache, prefill reads it back. (Log-probs differ by the order of bf16 sums and by keys that land
+    on the other side of a nibble's step: 0.05 at logits of unit spread.)"""
+    from meshy_b200.models import build_model, get_model_args
+    from meshy_b200.rollout.engine import RolloutEngine
+
+    args = get_model_args(*flavor, **kw)
+    model = build_model(args, seed=1, device="cuda", dtype=torch.bfloat16)
+    e = RolloutEngine(args, device="cuda", model=model, max_running=8, max_total_tokens=16384, max_seq_len=1024,
+                      kv_dtype="int4", sync_every=4)
+    g = e.generate([[3, 1, 4, 15] * 40], 24, temperature=1.0, ignore_eos=True)[0]
+    seen, sample = [], e._sample_rows
+
+    def spy(h, reqs):
+        seen.append(torch.log_softmax(h.float() @ e.model.output_weight.float().t(), -1))
+        return sample(h, reqs)
+
+    e._sample_rows = spy
+    for i, (tok, lp) in enumerate(zip(g.output_ids, g.output_logprobs)):
+        e.generate([g.prompt_ids + g.output_ids[:i]], 1, temperature=1.0)
+        assert float(seen[-1][0, tok]) == pytest.approx(lp, abs=5e-2), i
