@@ -284,11 +284,11 @@ def _count_setup(lens, Hq, Hkv, hd, page, seed, channel):
 
 
 def _check_counts(lens, Hq, Hkv, hd, page, seed, channel):
-    # a weight and its product with the scale are rounded to 2^-11 at most, the result to 2^-9; a channel whose count is
-    # below 128 shows one token more or less
+    # products of weights and scales are rounded to 11 bits (2^-11), the result to 8 (2^-8); a channel whose count is below
+    # 200 shows one token more or less
     q, c, bt, n, want = _count_setup(lens, Hq, Hkv, hd, page, seed, channel)
     err = (K.paged_attention_kv4(q, c, bt, n).double() - want).abs()
-    assert bool((err <= 2 ** -8 * want).all()), float((err / want.clamp(min=1e-9)).max())
+    assert bool((err <= (2 ** -8 + 2 ** -10) * want).all()), float((err / want.clamp(min=1e-9)).max())
 
 
 @pytest.mark.parametrize("Hq,Hkv,hd", [(12, 2, 128), (14, 2, 64), (17, 1, 128)])
@@ -350,7 +350,7 @@ def test_attention_long_tail_keeps_its_mass(peak):
 def test_small_values_beside_tokens_of_large_ones(L, every):
     """Values that carry the result keep their precision beside tokens of next to no weight whose values spread a hundred
     thousand times as far, and below peaks that have no spread at all. Weights and their products with the scales are
-    held in 11 bits, scores to 2^-12, the result in bf16: 2^-9 |o| + 2^-9 sum p |v|."""
+    held in 11 bits, scores to 2^-12, the result in bf16: 2^-8 |o| + 2^-9 sum p |v|."""
     hd = 128
     g = _gen(12)
     t = torch.arange(L, device=DEV)
@@ -372,7 +372,7 @@ def test_small_values_beside_tokens_of_large_ones(L, every):
     p = torch.softmax(kk @ q[0, 0].double() * scale, 0)
     want, size = p @ vv, (p * vv.abs().amax(1)).sum()
     err = (out[0].double() - want).abs()
-    assert bool((err <= 2 ** -9 * want.abs() + 2 ** -9 * size).all()), float((err / size).max())
+    assert bool((err <= 2 ** -8 * want.abs() + 2 ** -9 * size).all()), float((err / size).max())
 
 
 def test_attention_rising_scores():
