@@ -9,8 +9,8 @@
 // Both kernels should run at the memory's rate; in the write the quotients stand in the way (nine channels a clock and
 // SM at that rate), so each is a product and two fused multiply-adds with the group's reciprocal instead of a division,
 // on pairs of channels in one instruction. 32768 tokens of 8 heads of 128, at slots of shuffled pages: the write takes
-// 35.7 us for 172 MB (4.8 TB/s; instruction issue, 68 % of the slots before the quotients went in pairs at 38.2 us),
-// the read-back 28 us for as much (6.2 TB/s, the memory's rate). Decode-size calls take 5 us, launch and latency.
+// 36-37 us for 172 MB (4.7 TB/s; instruction issue, 65 % of the slots), the read-back 28-30 us for as much (5.9 TB/s, the
+// memory's rate). Decode-size calls take 4 us for both in a stream, launch and latency.
 #include <cuda_runtime.h>
 
 #include "kv4.h"

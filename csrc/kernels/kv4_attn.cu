@@ -31,8 +31,8 @@
 // results do not depend on timing.
 //
 // A unit lies in one page, or, where the page is not a multiple of it, in pieces of 16 or 32 tokens whose page ids
-// neighbouring lanes look up (8 rows of 131072 tokens: 67 us with pages of 16, 65 with pages of 64; units of 16 tokens
-// took 82 with the former. At head width 64, 128 rows of 16384: 71, 69 and 131).
+// neighbouring lanes look up (8 rows of 131072 tokens: 68 us with pages of 16, 65 with pages of 64; units of 16 tokens
+// took 82 with the former. At head width 64, 128 rows of 16384: 72, 71 and 131).
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory, filled by
 // 16-byte asynchronous copies two units ahead, across the segments, and at a segment's end leaves its state in one of
@@ -43,9 +43,10 @@
 // their own left fewer registers and one more wait to a unit: 72 us instead of 66 on 8 rows of 131072 tokens.) Every
 // wait is bounded; one that gives up records an error code.
 //
-// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 302 MB) 65-68 us, 4.5 TB/s; 256 rows of up to 1500 (32 / 8
-// heads, 360 MB) 90 us, 4.0 TB/s; 64 rows of up to 8192 (12 / 2) 29 us; one row of 700 tokens 8.7 us. Bound by the
-// instructions' latency, not by memory: two computing warps on a scheduler keep 51-55 % of its issue slots busy, about
+// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 302 MB) 65-69 us, 4.5 TB/s; 256 rows of up to 1500 (32 / 8
+// heads, 360 MB) 88-92 us, 4.0 TB/s; 64 rows of up to 8192 (12 / 2) 29 us; 128 rows of 16384 at head width 64 (14 / 2, 302
+// MB) 71 us; one row of 700 tokens 8.8 us. In this schedule the instructions' latency decides, not memory: two computing
+// warps on a scheduler keep 51-56 % of its issue slots busy (44 % on the ragged rows), with DRAM at half its rate; about
 // 2000 cycles to a unit (products of K 520, P V and the wait for the copies 770, scores 260, the next copies 285). With
 // few tokens it is the chain lengths, page id, copies, join (about 8 us).
 #include <climits>

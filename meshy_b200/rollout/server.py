@@ -7,7 +7,7 @@ Routes (the subset of SGLang's API the reference drives, ``meshy/engine/sglang.p
   [[lp, id, null], ...], weight_version}}``. ``sampling_params`` takes
   ``temperature``, ``top_k``, ``top_p``, ``max_new_tokens``, ``ignore_eos``, the penalties
   ``repetition_penalty``, ``frequency_penalty``, ``presence_penalty``, ``logit_bias`` and
-  ``allowed_token_ids``
+  ``allowed_token_ids``; unusable values are answered with 400 and ``{error}``
 * ``GET /health``, ``GET /health_generate``, ``GET /v1/loads``,
   ``GET /get_model_info``
 * ``POST /pause_generation {mode: "abort"|"wait"}``, ``POST /continue_generation``
