@@ -142,7 +142,7 @@ def build_app(runner: EngineRunner, model_name: str = ""):
         params = dict(body.get("sampling_params") or {})
         try:
             gen = await runner.generate(list(body["input_ids"]), params)
-        except (TypeError, ValueError) as e:  # unusable sampling parameters
+        except (TypeError, ValueError, OverflowError) as e:  # unusable sampling parameters
             return web.json_response({"error": str(e)}, status=400)
         out = {"output_ids": gen.output_ids,
                "meta_info": {"finish_reason": {"type": gen.finish_reason},

@@ -23,8 +23,8 @@ LOCKSTEP = frozenset({
     "submit", "step", "run_until_idle", "generate", "abort_all", "pause", "resume", "release_memory",
     "resume_memory", "update_weights_from_state_dict", "update_weights_from_disk", "update_weights_from_ipc",
 })
-# of these, the calls that refuse unusable requests before anything else happens on any rank
-REFUSING = frozenset({"submit", "generate"})
+# of these, the calls that refuse unusable requests before any rank has begun to work on them, and how
+REFUSING = {"submit": Exception, "generate": (TypeError, ValueError, OverflowError)}
 _REFUSED = "__refused__"
 
 
@@ -64,9 +64,8 @@ class EngineLeader:
                 self._broadcast((name, args, kwargs))
                 try:
                     return attr(*args, **kwargs)
-                except (TypeError, ValueError):
-                    if name in REFUSING:  # the followers refused the call too: they go on
-                        self._broadcast((_REFUSED, (), {}))
+                except REFUSING.get(name, ()):  # the followers refused the call too: they go on
+                    self._broadcast((_REFUSED, (), {}))
                     raise
 
         return call
@@ -96,9 +95,7 @@ def follow(engine, ctrl_group) -> None:
             return
         try:
             getattr(engine, name)(*args, **kwargs)
-        except (TypeError, ValueError) as e:
-            if name not in REFUSING:
-                raise
+        except REFUSING.get(name, ()) as e:
             refused = e
         engine.finished.clear()  # only rank 0 answers clients
 

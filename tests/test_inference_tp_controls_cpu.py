@@ -12,7 +12,7 @@ PROMPTS = [[3, 14, 15, 92, 65, 35], [8, 97, 93, 23, 84, 62, 64, 33, 83, 27], [2,
 CONTROLS = dict(repetition_penalty=1.3, frequency_penalty=0.2, presence_penalty=0.3, logit_bias={11: 2.0},
                 allowed_tokens=list(range(5, 1500)))
 UNUSABLE = [dict(repetition_penalty=-1.0), dict(allowed_tokens=[]), dict(logit_bias={5000: 1.0}), dict(n_generated=99),
-            dict(temperature="warm"), dict(frequency_penalty=None)]
+            dict(temperature="warm"), dict(frequency_penalty=None), dict(logit_bias={float("inf"): 1.0})]
 
 
 def _engine(group=None, **kw):
@@ -48,7 +48,7 @@ def _worker(rank, port, q, what):
                         try:
                             call()
                             out["accepted"] = bad
-                        except (TypeError, ValueError):
+                        except (TypeError, ValueError, OverflowError):
                             pass
                 out["again"] = _run(lead)
             else:

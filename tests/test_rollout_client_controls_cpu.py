@@ -53,7 +53,8 @@ def test_a_refused_request_is_not_sent_again(params):
 
 
 @pytest.mark.parametrize("params", [dict(logit_bias=[3, 4]), dict(allowed_token_ids=5), dict(presence_penalty=[1]),
-                                    dict(allowed_token_ids=[None]), dict(logit_bias={"a": 1})])
+                                    dict(allowed_token_ids=[None]), dict(logit_bias={"a": 1}),
+                                    dict(allowed_token_ids=[float("inf")])])
 def test_parameters_of_another_type_are_refused(params):
     async def use(c, counts):
         with pytest.raises(ValueError, match="refused"):
