@@ -20,9 +20,12 @@
 #include "kernels/elementwise.h"
 #include "kernels/gemm.h"
 #include "kernels/kv4.h"
+#include "kernels/kv8.h"
 #include "kernels/misc.h"
 #include "kernels/ep.h"
 #include "kernels/moe.h"
+#include "kernels/paging.h"
+#include "kernels/rotary.h"
 #include "kernels/symm.h"
 
 using torch::Tensor;
@@ -753,7 +756,7 @@ KV4View kv4_view(const Tensor& k, const Tensor& v, const Tensor& scale) {
 }
 
 // [N, H, hd] bf16 rows that 16-byte loads can walk: unit inner stride, aligned rows; anything else is copied.
-Tensor kv4_rows(const Tensor& x, const char* what, const Tensor& cache, int64_t hd) {
+Tensor cache_rows(const Tensor& x, const char* what, const Tensor& cache, int64_t hd) {
   TORCH_CHECK(x.device() == cache.device(), std::string(what) + " must be on the cache's device");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 3 && x.size(2) == hd, 
               std::string(what) + " must be bfloat16 [rows, heads, " + std::to_string(hd) + "]");
@@ -765,8 +768,8 @@ Tensor kv4_rows(const Tensor& x, const char* what, const Tensor& cache, int64_t 
 void kv4_write_(Tensor k, Tensor v, Tensor kc, Tensor vc, Tensor scale, Tensor slots) {
   const KV4View c = kv4_view(kc, vc, scale);
   const c10::cuda::CUDAGuard guard(kc.device());
-  k = kv4_rows(k, "kv4_write: k", kc, c.hd);
-  v = kv4_rows(v, "kv4_write: v", kc, c.hd);
+  k = cache_rows(k, "kv4_write: k", kc, c.hd);
+  v = cache_rows(v, "kv4_write: v", kc, c.hd);
   TORCH_CHECK(k.size(1) == c.Hkv && v.sizes() == k.sizes(), 
               "kv4_write: k and v must be [rows, " + std::to_string(c.Hkv) + ", " + std::to_string(c.hd) + "]");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == k.size(0) &&
@@ -820,7 +823,7 @@ void kv4_reset() {
 Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
   const KV4View c = kv4_view(kc, vc, scale_t);
   const c10::cuda::CUDAGuard guard(kc.device());
-  q = kv4_rows(q, "paged_attention_kv4: q", kc, c.hd);
+  q = cache_rows(q, "paged_attention_kv4: q", kc, c.hd);
   const int64_t B = q.size(0), Hq = q.size(1);
   TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0,
               "paged_attention_kv4: " + std::to_string(Hq) + " query heads over " + std::to_string(c.Hkv) + " KV heads");
@@ -840,6 +843,231 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
                 ptr<unsigned>(ws.arrived), ptr<int>(scratch(0, 0).err), cur_stream());
   count();
   return out;
+}
+
+// ─── 8-bit KV cache ─────────────────────────────────────────────────────────
+
+KV8View kv8_view(const Tensor& k, const Tensor& v, const Tensor& scale) {
+  CHECK_CUDA(k);
+  TORCH_CHECK(k.dim() == 4 && k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && k.sizes() == v.sizes(),
+              "kv8: k and v must be uint8 [pages, Hkv, page, hd]");
+  const int64_t hd = k.size(3);
+  TORCH_CHECK(k.size(1) > 0, "kv8: a cache needs at least one KV head");
+  TORCH_CHECK(hd == 64 || hd == 128, "kv8: head_dim must be 64 or 128, got " + std::to_string(hd));
+  TORCH_CHECK(k.size(2) > 0 && k.size(2) % kKV8Block == 0,
+              "kv8: page size must be a multiple of 16, got " + std::to_string(k.size(2)));
+  TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 4 && scale.size(0) == k.size(0) &&
+                  scale.size(1) == k.size(1) && scale.size(2) == k.size(2) / kKV8Block && scale.size(3) == 2,
+              "kv8: scale must be float32 [pages, Hkv, page / 16, 2]");
+  TORCH_CHECK(v.device() == k.device() && scale.device() == k.device(), "kv8: cache tensors on different devices");
+  CHECK_CONTIG(k);
+  CHECK_CONTIG(v);
+  CHECK_CONTIG(scale);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scale.data_ptr()) % 16 == 0,
+              "kv8: cache tensors must start on 16-byte boundaries");
+  TORCH_CHECK(k.size(1) <= (1 << 20) && k.size(2) <= (1 << 20), "kv8: too many heads or tokens in a page");
+  return {ptr<uint8_t>(k), ptr<uint8_t>(v), ptr<float>(scale), k.size(0), (int)k.size(1), (int)k.size(2), (int)hd};
+}
+
+void check_slots(const Tensor& slots, const Tensor& cache, int64_t rows, const char* what) {
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && (rows < 0 || slots.size(0) == rows) &&
+                  slots.device() == cache.device(),
+              std::string(what) + ": slots must be int64 [rows] on the cache's device");
+  TORCH_CHECK(slots.is_contiguous(), std::string(what) + ": slots must be contiguous");
+  TORCH_CHECK(slots.size(0) < (1LL << 31) - 64, std::string(what) + ": too many rows for one call");
+}
+
+c10::optional<std::tuple<Tensor, Tensor>> kv8_write_(Tensor k, Tensor v, Tensor kc, Tensor vc, Tensor scale, Tensor slots,
+                                                     bool keep) {
+  const KV8View c = kv8_view(kc, vc, scale);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  k = cache_rows(k, "kv8_write: k", kc, c.hd);
+  v = cache_rows(v, "kv8_write: v", kc, c.hd);
+  TORCH_CHECK(k.size(1) == c.Hkv && v.sizes() == k.sizes(),
+              "kv8_write: k and v must be [rows, " + std::to_string(c.Hkv) + ", " + std::to_string(c.hd) + "]");
+  check_slots(slots, kc, k.size(0), "kv8_write");
+  Tensor ko, vo;
+  if (keep) {
+    ko = torch::empty({k.size(0), c.Hkv, c.hd}, k.options());
+    vo = torch::empty_like(ko);
+  }
+  kv8_write(ptr<bf16>(k), k.stride(0), k.stride(1), ptr<bf16>(v), v.stride(0), v.stride(1), ptr<int64_t>(slots),
+            (int)k.size(0), c, keep ? ptr<bf16>(ko) : nullptr, keep ? ptr<bf16>(vo) : nullptr, cur_stream());
+  if (k.size(0)) count();
+  if (!keep) return c10::nullopt;
+  return std::make_tuple(ko, vo);
+}
+
+std::tuple<Tensor, Tensor> kv8_read_(Tensor kc, Tensor vc, Tensor scale, Tensor slots) {
+  const KV8View c = kv8_view(kc, vc, scale);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  check_slots(slots, kc, -1, "kv8_read");
+  Tensor k = torch::empty({slots.size(0), c.Hkv, c.hd}, kc.options().dtype(torch::kBFloat16)), v = torch::empty_like(k);
+  kv8_read(c, ptr<int64_t>(slots), (int)slots.size(0), ptr<bf16>(k), ptr<bf16>(v), cur_stream());
+  if (slots.size(0)) count();
+  return {k, v};
+}
+
+Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
+  const KV8View c = kv8_view(kc, vc, scale_t);
+  const c10::cuda::CUDAGuard guard(kc.device());
+  q = cache_rows(q, "paged_attention_kv8: q", kc, c.hd);
+  const int64_t B = q.size(0), Hq = q.size(1);
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0,
+              "paged_attention_kv8: " + std::to_string(Hq) + " query heads over " + std::to_string(c.Hkv) + " KV heads");
+  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == B &&
+                  (bt.size(1) <= 1 || bt.stride(1) == 1) && bt.device() == kc.device(),
+              "paged_attention_kv8: block_table must be int32 [rows, pages] on the cache's device");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.size(0) == B &&
+                  seq_lens.device() == kc.device(),
+              "paged_attention_kv8: seq_lens must be int32 [rows] on the cache's device");
+  CHECK_CONTIG(seq_lens);
+  Tensor out = torch::empty({B, Hq, c.hd}, q.options());
+  if (B == 0) return out;
+  if (c.n_pages == 0 || bt.size(1) == 0) return out.zero_();
+  kv8_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
+                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), cur_stream());
+  count();
+  return out;
+}
+
+// ─── paged tables ───────────────────────────────────────────────────────────
+
+void check_i32(const Tensor& t, const Tensor& table, int64_t n, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && (n < 0 || t.size(0) == n) && t.device() == table.device() &&
+                  t.is_contiguous() && t.size(0) < (1LL << 31) - 4096,
+              std::string(what) + " must be contiguous int32 of one dimension on the table's device" +
+                  (n < 0 ? "" : ", [" + std::to_string(n) + "]"));
+}
+
+void check_table(const Tensor& bt) {
+  CHECK_CUDA(bt);
+  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && (bt.size(1) <= 1 || bt.stride(1) == 1) &&
+                  bt.size(0) < (1LL << 31) && bt.size(1) < (1LL << 31),
+              "block_table must be int32 [rows, pages] with neighbouring columns");
+}
+
+void assign_pages_(Tensor bt, Tensor rows, Tensor have, Tensor need, Tensor pages) {
+  check_table(bt);
+  const c10::cuda::CUDAGuard guard(bt.device());
+  check_i32(rows, bt, -1, "assign_pages: rows");
+  check_i32(have, bt, rows.size(0), "assign_pages: have");
+  check_i32(need, bt, rows.size(0), "assign_pages: need");
+  check_i32(pages, bt, -1, "assign_pages: pages");
+  assign_pages(ptr<int>(bt), bt.stride(0), (int)bt.size(0), (int)bt.size(1), ptr<int>(rows), ptr<int>(have),
+               ptr<int>(need), (int)rows.size(0), ptr<int>(pages), (int)pages.size(0), cur_stream());
+  if (rows.size(0) && pages.size(0)) count();
+}
+
+std::tuple<Tensor, Tensor, Tensor> token_maps_(Tensor bt, Tensor rows, Tensor start, Tensor lens, int64_t total,
+                                               int64_t page) {
+  check_table(bt);
+  const c10::cuda::CUDAGuard guard(bt.device());
+  check_i32(rows, bt, -1, "token_maps: rows");
+  check_i32(start, bt, rows.size(0), "token_maps: start");
+  check_i32(lens, bt, rows.size(0), "token_maps: lens");
+  TORCH_CHECK(total >= 0 && total < (1LL << 31) - 4096, "token_maps: total out of range: " + std::to_string(total));
+  TORCH_CHECK(page > 0 && page < (1LL << 31), "token_maps: page must be positive, got " + std::to_string(page));
+  Tensor positions = torch::empty({total}, rows.options()), slots = torch::empty({total}, rows.options().dtype(at::kLong));
+  Tensor cu = torch::empty({rows.size(0) + 1}, rows.options());
+  token_maps(ptr<int>(bt), bt.stride(0), (int)bt.size(0), (int)bt.size(1), ptr<int>(rows), ptr<int>(start),
+             ptr<int>(lens), (int)rows.size(0), (int)page, ptr<int>(positions), ptr<int64_t>(slots), ptr<int>(cu),
+             (int)total, cur_stream());
+  count();
+  return {positions, slots, cu};
+}
+
+// ─── rotary positions ───────────────────────────────────────────────────────
+
+// [T, width] bf16 rows that 8-byte loads can walk; anything else is copied.
+Tensor rotary_rows(const Tensor& x) {
+  const bool ok = x.stride(1) == 1 && x.stride(0) % 4 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 8 == 0;
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+RotaryShape rotary_shape(const Tensor& qkv, const Tensor& pos, const c10::optional<Tensor>& qn,
+                         const c10::optional<Tensor>& kn, const Tensor& turns, int64_t Hq, int64_t Hkv, int64_t hd,
+                         bool interleaved) {
+  CHECK_CUDA(qkv);
+  TORCH_CHECK(Hq > 0 && Hkv > 0 && hd > 0, "rotary: heads and head_dim must be positive");
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * hd,
+              "rotary: qkv must be bfloat16 [rows, " + std::to_string((Hq + 2 * Hkv) * hd) + "]");
+  TORCH_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == qkv.size(0) && pos.is_contiguous() &&
+                  pos.device() == qkv.device(),
+              "rotary: positions must be int32 [rows] on qkv's device");
+  TORCH_CHECK(qn.has_value() == kn.has_value(), "rotary: both norm weights or none");
+  for (const c10::optional<Tensor>* w : {&qn, &kn})
+    if (w->has_value())
+      TORCH_CHECK((*w)->scalar_type() == at::kBFloat16 && (*w)->dim() == 1 && (*w)->size(0) == hd && (*w)->is_contiguous() &&
+                      (*w)->device() == qkv.device() && reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 8 == 0,
+                  "rotary: norm weights must be bfloat16 [" + std::to_string(hd) + "] on qkv's device, on 8-byte boundaries");
+  TORCH_CHECK(turns.scalar_type() == at::kLong && turns.dim() == 1 && turns.is_contiguous() && turns.device() == qkv.device(),
+              "rotary: the table must be int64 on qkv's device");
+  TORCH_CHECK(qkv.size(0) < (1LL << 31), "rotary: too many rows for one call");
+  return {(int)qkv.size(0), (int)Hq, (int)Hkv, (int)hd, (int)(2 * turns.size(0)), interleaved};
+}
+
+// q [T, Hq, hd], k and v [T, Hkv, hd]; with caches [pages, Hkv, page, hd], k and v go there too (and are returned if
+// ``keep``).
+std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> rotary_fwd_(
+    Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
+    c10::optional<Tensor> kn, int64_t Hq, int64_t Hkv, int64_t hd, double eps, c10::optional<Tensor> kc,
+    c10::optional<Tensor> vc, c10::optional<Tensor> slots, bool keep) {
+  const RotaryShape s = rotary_shape(qkv, pos, qn, kn, turns, Hq, Hkv, hd, interleaved);
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  qkv = rotary_rows(qkv);
+  RotaryCache cache{};
+  if (kc.has_value()) {
+    TORCH_CHECK(vc.has_value() && slots.has_value() && kc->dim() == 4 && kc->sizes() == vc->sizes() && kc->size(1) == Hkv &&
+                    kc->size(3) == hd && kc->scalar_type() == at::kBFloat16 && vc->scalar_type() == at::kBFloat16 &&
+                    kc->is_contiguous() && vc->is_contiguous() && kc->device() == qkv.device() && vc->device() == qkv.device(),
+                "rotary: caches must be contiguous bfloat16 [pages, Hkv, page, hd] on qkv's device");
+    check_slots(*slots, *kc, qkv.size(0), "rotary");
+    TORCH_CHECK(kc->size(2) > 0 && kc->size(2) < (1LL << 31), "rotary: empty pages");
+    cache = {ptr<bf16>(*kc), ptr<bf16>(*vc), ptr<int64_t>(*slots), kc->size(0), (int)kc->size(2)};
+  }
+  Tensor q = torch::empty({qkv.size(0), Hq, hd}, qkv.options());
+  c10::optional<Tensor> k, v;
+  if (keep) {
+    k = torch::empty({qkv.size(0), Hkv, hd}, qkv.options());
+    v = torch::empty_like(*k);
+  }
+  rotary_fwd(s, ptr<bf16>(qkv), qkv.stride(0), ptr<int>(pos), ptr<uint64_t>(turns), (float)factor, optr<bf16>(qn),
+             optr<bf16>(kn), (float)eps, ptr<bf16>(q), optr<bf16>(k), optr<bf16>(v), cache, cur_stream());
+  if (s.T) count();
+  return {q, k, v};
+}
+
+// gqkv; gqn / gkn (fp32) get the norms' gradients added.
+Tensor rotary_bwd_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
+                   c10::optional<Tensor> kn, Tensor gq, Tensor gk, Tensor gv, c10::optional<Tensor> gqn,
+                   c10::optional<Tensor> gkn, double eps) {
+  TORCH_CHECK(gq.dim() == 3 && gk.dim() == 3 && gv.sizes() == gk.sizes() && gq.size(2) == gk.size(2) &&
+                  gq.size(0) == qkv.size(0) && gk.size(0) == qkv.size(0),
+              "rotary: gradients must be [rows, heads, head_dim]");
+  const RotaryShape s = rotary_shape(qkv, pos, qn, kn, turns, gq.size(1), gk.size(1), gq.size(2), interleaved);
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  for (const Tensor* g : {&gq, &gk, &gv})
+    TORCH_CHECK(g->scalar_type() == at::kBFloat16 && g->is_contiguous() && g->device() == qkv.device() &&
+                    reinterpret_cast<uintptr_t>(g->data_ptr()) % 8 == 0,
+                "rotary: gradients must be contiguous bfloat16 on qkv's device");
+  Tensor part;
+  if (qn.has_value()) {
+    TORCH_CHECK(gqn.has_value() && gkn.has_value(), "rotary: the norms' gradients have no destination");
+    for (const c10::optional<Tensor>* g : {&gqn, &gkn})
+      TORCH_CHECK((*g)->scalar_type() == at::kFloat && (*g)->numel() == s.hd && (*g)->is_contiguous() &&
+                      (*g)->device() == qkv.device(),
+                  "rotary: the norms' gradients must be float32 [head_dim] on qkv's device");
+    part = torch::empty({rotary_part_floats(s)}, qkv.options().dtype(at::kFloat));
+  }
+  qkv = rotary_rows(qkv);
+  Tensor gqkv = torch::empty({qkv.size(0), qkv.size(1)}, qkv.options());
+  rotary_bwd(s, ptr<bf16>(qkv), qkv.stride(0), ptr<int>(pos), ptr<uint64_t>(turns), (float)factor, optr<bf16>(qn),
+             optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(gqkv), optr<float>(gqn),
+             optr<float>(gkn), part.defined() ? ptr<float>(part) : nullptr, cur_stream());
+  if (s.T) count(qn.has_value() ? 2 : 1);
+  return gqkv;
 }
 
 // ─── logit controls ─────────────────────────────────────────────────────────
@@ -1556,6 +1784,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv4_write", &kv4_write_, "quantise K / V rows into the 4-bit paged cache");
   m.def("kv4_read", &kv4_read_, "the values the 4-bit paged cache holds at given slots");
   m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache");
+  m.def("kv8_write", &kv8_write_, "quantise K / V rows into the 8-bit paged cache");
+  m.def("kv8_read", &kv8_read_, "the values the 8-bit paged cache holds at given slots");
+  m.def("kv8_attention", &kv8_attention_, "paged decode attention over the 8-bit cache");
+  m.def("assign_pages", &assign_pages_, "pages dealt to the rows of a block table");
+  m.def("token_maps", &token_maps_, "positions, slots and offsets of packed new tokens");
+  m.def("rotary_fwd", &rotary_fwd_, "rotary positions of a fused QKV projection");
+  m.def("rotary_bwd", &rotary_bwd_, "gradient of rotary_fwd");
   m.def("kv4_reset", &kv4_reset, "zero the attention's arrival counters after a device error");
   m.def("load_tokens", &load_tokens_, "token state (seen bits, generated counts) of admitted requests");
   m.def("apply_logit_controls", &apply_logit_controls_, "penalties, biases and token masks on logits");

@@ -13,6 +13,7 @@
 // memory's rate). Decode-size calls take 4 us for both in a stream, launch and latency.
 #include <cuda_runtime.h>
 
+#include "../include/fastdiv.cuh"
 #include "kv4.h"
 
 namespace meshy {
@@ -21,16 +22,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr float kHalfMax = 65504.f;
-
-// n / d for n < 2^31, as (n m) >> s with m = ceil(2^s / d), s = 31 + ceil(log2 d) (Granlund and Montgomery, 1994).
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t d_) : d(d_), s(31) {
-    while ((1ull << (s - 31)) < d) ++s;
-    m = (uint32_t)(((1ull << s) + d - 1) / d);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> s); }
-};
 
 // Correctly rounded x / y from y's correctly rounded reciprocal: one Newton step on the quotient with the exact
 // remainder (Markstein, 1990).

@@ -46,6 +46,37 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return out.to(x.dtype)
 
 
+def rotary_angles(positions: torch.Tensor, rope) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos/sin ``[T, rotary_dim / 2]`` (fp64) of a :class:`.rotary.Rope`, its factor included."""
+    f = torch.tensor(rope.frequencies(), dtype=torch.float64, device=positions.device)
+    w = positions.double().unsqueeze(-1) * f
+    return torch.cos(w) * rope.factor, torch.sin(w) * rope.factor
+
+
+def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rope) -> torch.Tensor:
+    """``x [T, H, hd]`` turned as ``rope`` says."""
+    rot = rope.rotary_dim
+    r, rest = x[..., :rot], x[..., rot:]
+    a, b = (r[..., 0::2], r[..., 1::2]) if rope.interleaved else r.chunk(2, -1)
+    c, s = cos.unsqueeze(1), sin.unsqueeze(1)
+    pair = (a * c - b * s, b * c + a * s)
+    return torch.cat([torch.stack(pair, -1).flatten(-2) if rope.interleaved else torch.cat(pair, -1), rest], -1)
+
+
+def qkv_rotary(qkv, positions, rope, n_heads, n_kv, q_norm=None, k_norm=None, eps: float = 1e-6):
+    """See :func:`.rotary.qkv_rotary`; in fp32 (fp64 for fp64 inputs), rounded once."""
+    q, k, v = qkv.view(qkv.shape[0], -1, rope.head_dim).split([n_heads, n_kv, n_kv], 1)
+    cos, sin = rotary_angles(positions, rope)
+
+    def turned(x, w):
+        y = x if x.dtype == torch.float64 else x.float()
+        if w is not None:
+            y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.to(y.dtype)
+        return apply_rotary(y, cos.to(y.dtype), sin.to(y.dtype), rope).to(x.dtype)
+
+    return turned(q, q_norm), turned(k, k_norm), v.contiguous()
+
+
 # ── SwiGLU with the block-interleaved fused gate/up weight ───────────────────
 
 def deinterleave_w13(h: torch.Tensor, block: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -218,6 +249,10 @@ def kv4_read(cache, slots, dtype=torch.float32):
 def attention_decode_kv4(q, cache, block_table, seq_lens, scale: float | None = None) -> torch.Tensor:
     """:func:`attention_decode_paged` over the values of a 4-bit cache. Tokens of pages outside the cache or past the
     block table do not count; a row without tokens gives zeros."""
+    return _attention_decode_read(kv4_read, q, cache, block_table, seq_lens, scale)
+
+
+def _attention_decode_read(read, q, cache, block_table, seq_lens, scale):
     B, Hq, hd = q.shape
     pages, Hkv, page = cache.k.shape[:3]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
@@ -228,11 +263,94 @@ def attention_decode_kv4(q, cache, block_table, seq_lens, scale: float | None = 
         there = (pg >= 0) & (pg < pages)
         if not bool(there.any()):
             continue
-        k, v = kv4_read(cache, (pg * page + t % page)[there])
+        k, v = read(cache, (pg * page + t % page)[there])
         qb = q[b].float().view(Hkv, Hq // Hkv, hd)
         p = torch.softmax(torch.einsum("grd,lgd->grl", qb, k) * scale, dim=-1)
         out[b] = torch.einsum("grl,lgd->grd", p, v).reshape(Hq, hd)
     return out.to(q.dtype)
+
+
+# ── 8-bit KV cache ───────────────────────────────────────────────────────────
+
+KV8_BLOCK = 16
+_KV8_LEAST, _KV8_MOST = 2.0 ** -100, 2.0 ** 126
+
+
+def kv8_steps(amax: torch.Tensor) -> torch.Tensor:
+    """Steps per unit ``r`` (fp32) of blocks with these largest magnitudes (:mod:`.kv8` describes the format)."""
+    q = 127.0 / amax.float().clamp(_KV8_LEAST, _KV8_MOST)
+    return torch.where(q.isnan(), q, (q.view(torch.int32) & -65536).view(torch.float32))
+
+
+def kv8_write(k, v, cache, slots) -> None:
+    pages, Hkv, page, hd = cache.k.shape
+    ok = (slots >= 0) & (slots < pages * page)
+    slots = slots[ok].long()
+    which, mine = torch.unique(slots // KV8_BLOCK, return_inverse=True)
+    per, place = page // KV8_BLOCK, slots % KV8_BLOCK
+    for i in range(which.numel()):
+        pg, bl = int(which[i]) // per, int(which[i]) % per
+        at = place[mine == i]
+        for x, data, kv in ((k, cache.k, 0), (v, cache.v, 1)):
+            x = x[ok][mine == i].float()  # [rows, Hkv, hd]
+            block = data[pg, :, bl * KV8_BLOCK:(bl + 1) * KV8_BLOCK]
+            r = kv8_steps(x.abs().amax((0, 2)))
+            if not bool((at == 0).any()):
+                old = cache.scale[pg, :, bl, kv]
+                r_old = torch.where(old == 0, torch.inf, 1.0 / old).bfloat16().float()
+                r = torch.minimum(r, r_old)
+                n = (block.float() - 128) * r[:, None, None] / r_old[:, None, None]
+                block.copy_(torch.where((r < r_old)[:, None, None], (n.round() + 128).nan_to_num(0).to(torch.uint8), block))
+            n = (x.clamp(-_KV8_MOST, _KV8_MOST) * r[:, None]).round().nan_to_num(0) + 128
+            block[:, at] = n.to(torch.uint8).transpose(0, 1)
+            cache.scale[pg, :, bl, kv] = 1.0 / r
+
+
+def kv8_read(cache, slots, dtype=torch.float32):
+    page = cache.k.shape[2]
+    ok, pg, off = _kv4_slots(cache, slots)
+    a = cache.scale[pg, :, off // KV8_BLOCK]
+    return tuple(torch.where(ok[:, None, None], (data[pg, :, off].float() - 128) * a[..., kv, None], 0.0).to(dtype)
+                 for data, kv in ((cache.k, 0), (cache.v, 1)))
+
+
+def attention_decode_kv8(q, cache, block_table, seq_lens, scale: float | None = None) -> torch.Tensor:
+    """:func:`attention_decode_paged` over the values of an 8-bit cache. Tokens of pages outside the cache or past the
+    block table do not count; a row without tokens gives zeros."""
+    return _attention_decode_read(kv8_read, q, cache, block_table, seq_lens, scale)
+
+
+# ── paged tables ─────────────────────────────────────────────────────────────
+
+def assign_pages(block_table, rows, have, need, pages) -> None:
+    """See :func:`.paging.assign_pages`."""
+    at, R, M = 0, *block_table.shape
+    for row, h, n in zip(rows.tolist(), have.tolist(), need.tolist()):
+        h = max(h, 0)
+        got = pages[at:at + max(0, n - h)]
+        at += max(0, n - h)
+        if 0 <= row < R and h < M:
+            got = got[:M - h]
+            block_table[row, h:h + got.numel()] = got
+
+
+def token_maps(block_table, rows, start, lens, total: int, page: int):
+    """See :func:`.paging.token_maps`."""
+    R, M = block_table.shape
+    dev = block_table.device
+    positions = torch.zeros(total, dtype=torch.int32, device=dev)
+    slots = torch.full((total,), -1, dtype=torch.int64, device=dev)
+    cu = [0]
+    for row, s, n in zip(rows.tolist(), start.tolist(), lens.tolist()):
+        n = max(n, 0)
+        at, p = cu[-1], torch.arange(s, s + max(0, min(n, total - cu[-1])), dtype=torch.int64, device=dev)
+        cu.append(at + n)
+        positions[at:at + p.numel()] = p.int()
+        if 0 <= row < R and M:
+            pg = block_table[row].long()[(p // page).clamp(0, M - 1)]
+            there = (p >= 0) & (p < M * page) & (p < 1 << 31) & (pg >= 0)
+            slots[at:at + p.numel()] = torch.where(there, pg * page + p % page, -1)
+    return positions, slots, torch.tensor(cu, dtype=torch.int64, device=dev).clamp(max=(1 << 31) - 1).int()
 
 
 # ── logit controls ───────────────────────────────────────────────────────────

@@ -36,6 +36,10 @@ cuda_sources = [
     "csrc/kernels/kv4.cu",
     "csrc/kernels/kv4_attn.cu",
     "csrc/kernels/controls.cu",
+    "csrc/kernels/kv8.cu",
+    "csrc/kernels/kv8_attn.cu",
+    "csrc/kernels/paging.cu",
+    "csrc/kernels/rotary.cu",
 ]
 extra_cuda = [s for s in ("csrc/kernels/symm.cu", "csrc/kernels/fsdp.cu") if os.path.exists(os.path.join(ROOT, s))]
 

@@ -1,0 +1,414 @@
+"""8-bit KV cache on the GPU: bytes against the definition, attention against 64 bits."""
+
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16 = 2.0 ** -8  # half a step of bf16, relative
+
+
+def _rows(T, H, hd, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, H, hd, generator=g) * spread * torch.exp(0.5 * torch.randn(H, hd, generator=g))).bfloat16()
+
+
+def _pair(pages, H, page, hd):
+    from meshy_b200.ops.kv8 import kv8_empty
+
+    return kv8_empty(pages, H, page, hd, "cpu"), kv8_empty(pages, H, page, hd, "cuda")
+
+
+def _same(cpu, gpu):
+    for a, b, name in zip(cpu, gpu, cpu._fields):
+        b = b.cpu()
+        if a.dtype.is_floating_point:
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)), name
+        else:
+            assert torch.equal(a, b), name
+
+
+def _write(cpu, gpu, k, v, slots, keep=True):
+    from meshy_b200.ops.kv8 import kv8_read, kv8_write
+
+    want = kv8_write(k, v, cpu, slots, keep=True)
+    got = kv8_write(k.cuda(), v.cuda(), gpu, slots.cuda(), keep=keep)
+    if keep:
+        for a, b in zip(want, got):
+            assert torch.equal(a.nan_to_num(7.0), b.cpu().nan_to_num(7.0))
+    for a, b in zip(kv8_read(cpu, slots, torch.bfloat16), kv8_read(gpu, slots.cuda())):
+        assert torch.equal(a.nan_to_num(7.0), b.cpu().nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T, H, page", [(1, 1, 16), (5, 2, 16), (16, 8, 64), (100, 3, 32), (700, 5, 48), (3001, 2, 128)])
+def test_prompt_bytes(T, H, page, hd):
+    pages = -(-T // page) + 2
+    cpu, gpu = _pair(pages, H, page, hd)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(1))
+    at = torch.arange(T)
+    slots = order[at // page] * page + at % page
+    k, v = _rows(T, H, hd), _rows(T, H, hd, 1, 30.0)
+    _write(cpu, gpu, k, v, slots)
+    _same(cpu, gpu)
+    # the next prompt in the same pages starts the blocks anew
+    _write(cpu, gpu, v, k, slots, keep=False)
+    _same(cpu, gpu)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_appended_tokens_requantise(hd):
+    H, page, rows = 3, 32, 40
+    cpu, gpu = _pair(rows + 1, H, page, hd)
+    rng = random.Random(2)
+    length = [0] * rows
+    for step in range(40):
+        who = sorted(rng.sample(range(rows), rng.randint(1, rows)))
+        slots = torch.tensor([(r + 1) * page + length[r] % page for r in who])
+        spread = 2.0 ** torch.tensor([float(rng.randint(-8, 8)) for _ in who])
+        k = (_rows(len(who), H, hd, step).float() * spread[:, None, None]).bfloat16()
+        v = (_rows(len(who), H, hd, 100 + step).float() / spread[:, None, None]).bfloat16()
+        _write(cpu, gpu, k, v, slots, keep=bool(step % 2))
+        _same(cpu, gpu)
+        for r in who:
+            length[r] += 1
+    # the same token again changes nothing
+    before = [x.clone() for x in gpu]
+    _write(cpu, gpu, k, v, slots)
+    assert all(torch.equal(a, b) for a, b in zip(before, gpu))
+
+
+def test_runs_in_any_order_and_slots_outside():
+    H, page, hd = 2, 16, 64
+    cpu, gpu = _pair(6, H, page, hd)
+    parts = []
+    rng = random.Random(4)
+    for b in (3, 1, 5, 2):  # blocks in any order, their rows too, some of them left out
+        at = rng.sample(range(16), rng.randint(1, 16))
+        parts += [b * 16 + p for p in at] + [-1, 6 * 16, 1 << 40]
+    slots = torch.tensor([-5] * 40 + parts + [-1] * 3)
+    k, v = _rows(len(slots), H, hd), _rows(len(slots), H, hd, 1)
+    _write(cpu, gpu, k, v, slots)
+    _same(cpu, gpu)
+    assert int(gpu.k[0].sum()) == 0 and int(gpu.k[4].sum()) == 0
+
+
+def test_values_far_and_not_finite():
+    H, page, hd = 2, 16, 128
+    cpu, gpu = _pair(12, H, page, hd)
+    k = torch.zeros(16 * 11, H, hd).bfloat16()
+    v = _rows(16 * 11, H, hd)
+    blocks = k.view(11, 16, H, hd)
+    blocks[1] = 2.0 ** -130                                    # below the smallest scale
+    blocks[2, 3, 0, 5] = 2.0 ** -100
+    blocks[3] = _rows(16, H, hd, 3, 1e30)
+    blocks[4, 0, 0, 0], blocks[4, 2, 0, 1] = math.inf, -math.inf
+    blocks[5, 7, 1, 9] = math.nan
+    blocks[6] = torch.finfo(torch.bfloat16).max
+    blocks[7, :, :, ::2], blocks[7, :, :, 1::2] = 1.0, 0.5     # halves of the step
+    blocks[8] = _rows(16, H, hd, 5) * 2.0 ** -126
+    blocks[9, 0] = -3.0
+    slots = torch.arange(16 * 11) + 16
+    _write(cpu, gpu, k, v, slots)
+    _same(cpu, gpu)
+    # a NaN that is appended, and one that a new first token clears
+    _write(cpu, gpu, blocks[5, 7:8].clone(), v[:1], torch.tensor([4 * 16 + 3]))
+    _same(cpu, gpu)
+    _write(cpu, gpu, v[:1], v[1:2], torch.tensor([6 * 16]))
+    _same(cpu, gpu)
+
+
+def test_repeated_slots_stay_inside():
+    """Idle rows all name one slot: it holds one of them, nothing else is touched."""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_read, kv8_write
+
+    c = kv8_empty(4, 2, 16, 64, "cuda")
+    k, v = _rows(200, 2, 64).cuda(), _rows(200, 2, 64, 1).cuda()
+    slots = torch.zeros(200, dtype=torch.int64, device="cuda")
+    slots[:3] = torch.tensor([20, 21, 22])
+    kv8_write(k, v, c, slots)
+    want = kv8_empty(4, 2, 16, 64, "cuda")
+    kv8_write(k[:3], v[:3], want, slots[:3])
+    for a, b in zip(c, want):
+        assert torch.equal(a[1:], b[1:])
+    assert int(c.k[0, :, 1:].sum()) == 0
+    assert bool(kv8_read(c, slots[3:4])[0].isfinite().all())
+
+
+def test_strided_rows_and_none():
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_read, kv8_write
+
+    wide = torch.randn(24, 7, 130, device="cuda").bfloat16()
+    slots = torch.arange(24, device="cuda")
+    for k in (wide[:, 2:4, :64], wide[:, 2:4, 1:65], wide.transpose(0, 1)[:2, :, :64].transpose(0, 1),
+              wide.float().transpose(1, 2)[:, :64, 3:5].transpose(1, 2).bfloat16()):
+        a, b = kv8_empty(2, 2, 16, 64, "cuda"), kv8_empty(2, 2, 16, 64, "cuda")
+        kv8_write(k, k, a, slots)
+        kv8_write(k.contiguous(), k.contiguous(), b, slots)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert kv8_write(k[:0], k[:0], a, slots[:0]) is None
+    assert kv8_write(k[:0], k[:0], a, slots[:0], keep=True)[0].shape == (0, 2, 64)
+    assert kv8_read(a, slots[:0])[0].shape == (0, 2, 64)
+
+
+# ── attention ────────────────────────────────────────────────────────────────
+
+def _filled(lens, Hkv, hd, page, seed=0, spread=1.0, extra=3):
+    """A cache with the rows' tokens on shuffled pages, NaN scales and any bytes elsewhere; (cache, block table)."""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_write
+
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + extra
+    c = kv8_empty(pages, Hkv, page, hd, "cuda")
+    g = torch.Generator().manual_seed(seed)
+    for x in (c.k, c.v):
+        x.copy_(torch.randint(0, 256, x.shape, generator=g, dtype=torch.uint8))
+    c.scale.fill_(math.nan)
+    order = torch.randperm(pages, generator=g).tolist()
+    bt = torch.full((len(lens), max(need + [1]) + 1), -1, dtype=torch.int32)
+    at = 0
+    for i, (n, p) in enumerate(zip(lens, need)):
+        bt[i, :p] = torch.tensor(order[at:at + p], dtype=torch.int32)
+        at += p
+        if n:
+            t = torch.arange(n)
+            slots = bt[i, t // page].long() * page + t % page
+            kv8_write(_rows(n, Hkv, hd, seed + 2 * i + 1, spread).cuda(), _rows(n, Hkv, hd, seed + 2 * i + 2).cuda(), c,
+                      slots.cuda())
+    return c, bt.cuda()
+
+
+def _exact(q, c, bt, lens, scale):
+    """The attention in 64 bits, the sum of p |v|, and how large the scores' terms are."""
+    B, Hq, hd = q.shape
+    Hkv, page = c.k.shape[1], c.k.shape[2]
+    out = torch.zeros(B, Hq, hd, dtype=torch.float64, device="cuda")
+    size, terms = torch.zeros_like(out), torch.zeros(B, Hq, 1, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        t = torch.arange(max(0, min(n, bt.shape[1] * page)), device="cuda")
+        pg = bt[b, t // page].long()
+        there = (pg >= 0) & (pg < c.k.shape[0])
+        pg, off = pg[there], (t % page)[there]
+        if not pg.numel():
+            continue
+        for h in range(Hq):
+            hk = h // (Hq // Hkv)
+            a = c.scale[pg, hk, off // 16].double()
+            k = (c.k[pg, hk, off].double() - 128) * a[:, :1]
+            v = (c.v[pg, hk, off].double() - 128) * a[:, 1:]
+            p = torch.softmax(k @ q[b, h].double() * scale, 0)
+            out[b, h], size[b, h] = p @ v, p @ v.abs()
+            terms[b, h] = 255 * a[:, 0].max() * q[b, h].double().abs().sum() * abs(scale)
+    return out, size, terms
+
+
+def _check(q, c, bt, lens, scale=None):
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = paged_attention_kv8(q, c, bt, sl, scale)
+    want, size, terms = _exact(q, c, bt, lens, scale if scale is not None else 1 / math.sqrt(q.shape[-1]))
+    # bf16 output; a weight times its value's scale has fp16's 11 bits (half a step 2^-11, relative); scores are fp32
+    # sums of 10 steps over terms of at most ``terms``, which moves a weight by twice that; exponentials 2^-20
+    weights = 2.0 ** -11 + 2 * (10 * 2.0 ** -23 * terms + 2.0 ** -20)
+    off, bound = (got.double() - want).abs(), BF16 * want.abs() + weights * size + 1e-30
+    assert bool((off <= bound).all()), f"off by {(off / bound).max().item():.3g} of the bound"
+    return got
+
+
+def _q(B, Hq, hd, seed=9):
+    return torch.randn(B, Hq, hd, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").bfloat16()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 128])
+@pytest.mark.parametrize("Hq, Hkv", [(1, 1), (12, 2), (14, 2), (8, 8), (24, 2)])
+def test_attention_over_lengths(hd, page, Hq, Hkv):
+    lens = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 300, 511, 1000, 0]
+    c, bt = _filled(lens, Hkv, hd, page)
+    _check(_q(len(lens), Hq, hd), c, bt, lens)
+
+
+@pytest.mark.parametrize("hd, page, Hq, Hkv, lens", [
+    (128, 64, 12, 2, [700]), (128, 64, 16, 2, [20011]), (64, 16, 14, 2, [5001, 0, 17, 3333]),
+    (128, 64, 32, 8, [900, 1500, 1, 1024]), (128, 16, 6, 1, [4096] * 5), (128, 128, 16, 2, [9000, 1] * 3),
+    (64, 64, 4, 2, [2048] * 40), (128, 64, 12, 2, list(range(1, 8000, 211))),
+    (64, 32, 8, 8, [(37 * i) % 900 for i in range(300)]),
+], ids=lambda x: str(x)[:24])
+def test_attention_over_shapes(hd, page, Hq, Hkv, lens):
+    c, bt = _filled(lens, Hkv, hd, page)
+    _check(_q(len(lens), Hq, hd), c, bt, lens)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_every_token_counts_once(hd):
+    """Equal scores: the output is the mean of V, which names each token."""
+    from meshy_b200.ops.kv8 import KV8Cache, paged_attention_kv8
+
+    page, Hkv = 16, 2
+    lens = [1, 5, 16, 100, 1023, 2500, 7001, 33, 64]
+    c, bt = _filled(lens, Hkv, hd, page)
+    q = torch.zeros(len(lens), 4, hd, device="cuda").bfloat16()
+    got = paged_attention_kv8(q, KV8Cache(*c), bt, torch.tensor(lens, dtype=torch.int32, device="cuda")).double()
+    want, size, _ = _exact(q, c, bt, lens, 1.0)
+    # weights are all 1: times a scale, rounded to 11 bits (one rounding for the 16 tokens of a block)
+    assert bool(((got - want).abs() <= BF16 * want.abs() + 2.0 ** -11 * size + 2.0 ** -22 * size).all())
+
+
+def test_pages_and_lengths_outside():
+    hd, page, Hkv = 128, 16, 2
+    lens = [100, 70, 33, 16, 20]
+    c, bt = _filled(lens, Hkv, hd, page)
+    bt[0, 2], bt[1, 0], bt[1, 4], bt[2, :] = -1, 1 << 30, c.k.shape[0], -9
+    _check(_q(5, 12, hd), c, bt, lens)
+    # lengths past the table end with it (row 4 has pages to its end), those below zero are empty
+    bt[3, :], bt[4, :] = bt[3, 0], bt[4, 0]
+    lens[3], lens[4] = (1 << 31) - 1, bt.shape[1] * page
+    got = _check(_q(5, 12, hd), c, bt[:, :1], [16, 70, 33, (1 << 31) - 1, -5])
+    assert float(got[4].abs().sum()) == 0.0 and float(got[2].abs().sum()) == 0.0
+
+
+def test_scores_far_apart():
+    """Weights from one to nothing, values of no weight that are far larger, values of many sizes."""
+    from meshy_b200.ops.kv8 import kv8_write
+
+    hd, page, Hkv = 128, 64, 2
+    lens = [2000, 555]
+    for spread in (1.0, 40.0, 1000.0):
+        c, bt = _filled(lens, Hkv, hd, page, seed=5, spread=spread)
+        _check(_q(2, 16, hd), c, bt, lens, scale=0.7)
+    c, bt = _filled(lens, Hkv, hd, page, seed=5)
+    for i, n in enumerate(lens):
+        t = torch.arange(n)
+        slots = bt[i].cpu()[t // page].long() * page + t % page
+        size = 10.0 ** (torch.arange(n) // 16 % 17 - 8).float()[:, None, None]
+        for s in (size, size.flip(0), 1e-30 * size.clamp(max=1.0), torch.where(size > 1, 0.0, size)):
+            kv8_write(_rows(n, Hkv, hd, 3, 4.0).cuda(), (_rows(n, Hkv, hd, 4).float() * s).bfloat16().cuda(), c, slots.cuda())
+            if float(s.max()) > 1e-20:
+                _check(_q(2, 16, hd), c, bt, lens, scale=0.7)
+
+
+def test_strided_queries_and_a_part_of_a_table():
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [40, 100, 7]
+    c, bt = _filled(lens, 2, 64, 16)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    wide = torch.randn(3, 20, 100, device="cuda").bfloat16()
+    wbt = torch.cat((bt, bt), 1)
+    for q in (wide[:, 3:7, :64], wide[:, 3:7, 3:67], wide[:, ::5, 8:72]):
+        want = paged_attention_kv8(q.contiguous(), c, bt, sl)
+        assert torch.equal(paged_attention_kv8(q, c, bt, sl), want)
+        assert torch.equal(paged_attention_kv8(q, c, wbt[:, :bt.shape[1]], sl), want)
+
+
+def test_captured_graphs_follow_lengths_and_share_nothing():
+    """Two graphs captured on one stream, replayed at the same time on others."""
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [9000, 1, 3000, 0]
+    c, bt = _filled(lens, 2, 128, 64)
+    qs = [_q(4, 12, 128, s) for s in (1, 2)]
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([paged_attention_kv8(q, c, bt, sl) for _ in range(3)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in qs]
+    for new in (lens, [17, 8000, 0, 2000], [0, 0, 0, 0], [9000, 1, 3000, 0]):
+        now = torch.tensor([min(a, b) for a, b in zip(new, lens)], dtype=torch.int32)
+        sl.copy_(now)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for q, o in zip(qs, outs):
+            want = _check(q, c, bt, now.tolist())
+            assert all(torch.equal(x, want) for x in o)
+
+
+def test_many_calls_on_streams_at_once():
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [5000, 300, 4000]
+    c, bt = _filled(lens, 2, 128, 64)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = [_q(3, 16, 128, s) for s in range(4)]
+    want = [paged_attention_kv8(q, c, bt, sl) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = []
+    for _ in range(10):
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(paged_attention_kv8(q, c, bt, sl))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 4]) for i, g in enumerate(got))
+
+
+def test_a_step_together():
+    """Rotary, maps, write and attention as a decode step chains them, against the functions of the CPU."""
+    from meshy_b200.ops import kv8, paging, rotary
+
+    Hq, Hkv, hd, page, B = 4, 2, 64, 16, 3
+    rope = rotary.Rope(hd, 1e4, 32, True, {"rope_type": "linear", "factor": 2.0})
+    lens = [20, 1, 47]
+    T = sum(lens)
+    g = torch.Generator().manual_seed(0)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * hd, generator=g).bfloat16()
+    step = torch.randn(4, B, (Hq + 2 * Hkv) * hd, generator=g).bfloat16()
+
+    def run(dev):
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        c = kv8.kv8_empty(16, Hkv, page, hd, dev)
+        bt, rows = torch.zeros(5, 4, dtype=torch.int32, device=dev), i32([4, 0, 2])
+        paging.assign_pages(bt, rows, i32([0] * B), i32([-(-(n + 4) // page) for n in lens]), i32(range(1, 12)))
+        m = paging.token_maps(bt, rows, i32([0] * B), i32(lens), T, page)
+        _, k, v = rotary.qkv_rotary(qkv.to(dev), m.positions, rope, Hq, Hkv)
+        outs = [*kv8.kv8_write(k, v, c, m.slots, keep=True)]
+        for s in range(4):
+            now = i32([n + s for n in lens])
+            m = paging.token_maps(bt, rows, now, i32([1] * B), B, page)
+            q, k, v = rotary.qkv_rotary(step[s].to(dev), m.positions, rope, Hq, Hkv)
+            kv8.kv8_write(k, v, c, m.slots)
+            outs.append(kv8.paged_attention_kv8(q, c, bt[rows.long()], now + 1))
+        return [x.cpu().double() for x in outs]
+
+    for a, b in zip(run("cpu"), run("cuda")):
+        # bf16 at every stage: a channel that falls on the other side of a rounding moves a value by a step of the cache
+        assert float((a - b).abs().max()) <= 0.06 and float((a - b).abs().mean()) <= 2.0 ** -8
+
+
+def test_refusals():
+    from meshy_b200.ops.kv8 import KV8Cache, kv8_empty, kv8_read, kv8_write, paged_attention_kv8
+
+    c = kv8_empty(4, 2, 16, 64, "cuda")
+    k = torch.zeros(3, 2, 64, device="cuda").bfloat16()
+    s = torch.arange(3, device="cuda")
+    bt, sl = torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for a in ((k.float(), k, c, s), (k, k[:, :1], c, s), (k[:2], k[:2], c, s), (k, k, c, s.int()), (k, k, c, s.cpu()),
+              (k[..., :32], k[..., :32], c, s), (k, k, KV8Cache(c.k, c.v[:2], c.scale), s),
+              (k, k, KV8Cache(c.k, c.v, c.scale[:2]), s), (k, k, KV8Cache(c.k, c.v, c.scale.half()), s),
+              (k, k, KV8Cache(c.k[:, :, :8], c.v[:, :, :8], c.scale), s),
+              (k, k, KV8Cache(c.k.transpose(2, 3).contiguous().transpose(2, 3), c.v, c.scale), s)):
+        with pytest.raises(RuntimeError):
+            kv8_write(*a)
+    with pytest.raises(RuntimeError):
+        kv8_read(c, s.int())
+    with pytest.raises(ValueError):
+        kv8_read(c, s, torch.float32)
+    q = torch.zeros(3, 4, 64, device="cuda").bfloat16()
+    for a in ((q[:, :3], c, bt, sl), (q.half(), c, bt, sl), (q, c, bt.long(), sl), (q, c, bt, sl.long()), (q, c, bt[:2], sl),
+              (q, c, bt, sl[:2]), (q, c, bt.t().contiguous().t(), sl), (q, c, bt.cpu(), sl)):
+        with pytest.raises(RuntimeError):
+            paged_attention_kv8(*a)
+    for hd, page, n in ((32, 16, 2), (64, 8, 2), (64, 16, 0), (64, 0, 2)):
+        with pytest.raises(ValueError):
+            kv8_empty(2, n, page, hd, "cuda")
