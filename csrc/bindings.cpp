@@ -10,6 +10,7 @@
 
 #include <atomic>
 #include <cstdlib>
+#include <list>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -909,6 +910,129 @@ std::tuple<Tensor, Tensor> kv8_read_(Tensor kc, Tensor vc, Tensor scale, Tensor 
   return {k, v};
 }
 
+// Workspaces of the attention kernel: partial sums and arrival counters (zeroed once, left zero by every launch). Launches
+// that may run at the same time must not share one, so each stream has its own, and so has each stream of each capture:
+// graphs replay beside one another, whatever stream they were captured on. A graph owns its workspaces (as a user object
+// of it); they return to the pool when the graph and what was instantiated from it are gone.
+struct KV8Workspace {
+  int dev;
+  int64_t segments;
+  float* part;
+  unsigned* arrived;
+};
+
+class KV8Workspaces {
+ public:
+  static KV8Workspaces& get() {
+    static KV8Workspaces* all = new KV8Workspaces;  // graphs may outlive static destruction
+    return *all;
+  }
+
+  KV8Workspace take(int dev, cudaStream_t st, int64_t segments) {
+    std::unique_lock<std::mutex> g(mu_);
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    cudaGraph_t graph = nullptr;
+    MESHY_CUDA_CHECK(cudaStreamGetCaptureInfo_v2(st, &status, &capture, &graph, nullptr, nullptr));
+    TORCH_CHECK(status != cudaStreamCaptureStatusInvalidated, "paged_attention_kv8: the stream's capture was invalidated");
+    const bool capturing = status == cudaStreamCaptureStatusActive;
+    const Key key{dev, st, capturing, capture};
+    auto it = held_.find(key);
+    if (it != held_.end() && it->second->segments >= segments) return *it->second;
+    KV8Workspace* w = pooled(dev, segments);
+    if (capturing) {
+      // (a smaller one of this capture stays with the graph, whose earlier launches use it)
+      Lease* lease = new Lease{key, w};
+      cudaUserObject_t object = nullptr;
+      cudaError_t e = cudaUserObjectCreate(&object, lease, &KV8Workspaces::give_back, 1, cudaUserObjectNoDestructorSync);
+      if (e == cudaSuccess) e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+      if (e != cudaSuccess) {
+        g.unlock();
+        if (object)
+          cudaUserObjectRelease(object, 1);  // gives it back
+        else
+          give_back(lease);
+        MESHY_CUDA_CHECK(e);
+      }
+    }
+    held_[key] = w;  // a stream's smaller one is kept unused: launches under way may be using it
+    return *w;
+  }
+
+  void reset() {
+    std::lock_guard<std::mutex> g(mu_);
+    for (KV8Workspace& w : all_) {
+      const c10::cuda::CUDAGuard guard((c10::DeviceIndex)w.dev);
+      MESHY_CUDA_CHECK(cudaMemsetAsync(w.arrived, 0, w.segments * sizeof(unsigned), cur_stream()));
+    }
+  }
+
+ private:
+  struct Key {
+    int dev;
+    cudaStream_t st;
+    bool capturing;
+    unsigned long long capture;
+    bool operator<(const Key& o) const {
+      return std::tie(dev, st, capturing, capture) < std::tie(o.dev, o.st, o.capturing, o.capture);
+    }
+  };
+  struct Lease {
+    Key key;
+    KV8Workspace* w;
+  };
+
+  static void CUDART_CB give_back(void* p) {  // calls no CUDA function, as its caller demands
+    Lease* lease = static_cast<Lease*>(p);
+    KV8Workspaces& s = get();
+    std::lock_guard<std::mutex> g(s.mu_);
+    auto it = s.held_.find(lease->key);
+    if (it != s.held_.end() && it->second == lease->w) s.held_.erase(it);
+    s.free_.push_back(lease->w);
+    delete lease;
+  }
+
+  KV8Workspace* pooled(int dev, int64_t segments) {
+    for (size_t i = 0; i < free_.size(); ++i)
+      if (free_[i]->dev == dev && free_[i]->segments >= segments) {
+        KV8Workspace* w = free_[i];
+        free_.erase(free_.begin() + i);
+        return w;
+      }
+    // memory that no capture sees: neither the allocation nor the clearing is part of the graph
+    struct Mode {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      Mode() { MESHY_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode)); }
+      ~Mode() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    } relaxed;
+    int64_t n = 1 << 14;
+    while (n < segments) n *= 2;
+    const size_t floats = kv8_part_floats() * sizeof(float);
+    void* mem = nullptr;
+    MESHY_CUDA_CHECK(cudaMalloc(&mem, floats + n * sizeof(unsigned)));
+    unsigned* arrived = reinterpret_cast<unsigned*>(static_cast<char*>(mem) + floats);
+    cudaStream_t st = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(arrived, 0, n * sizeof(unsigned), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (st) cudaStreamDestroy(st);
+    if (e != cudaSuccess) {
+      cudaFree(mem);
+      MESHY_CUDA_CHECK(e);
+    }
+    all_.push_back({dev, n, static_cast<float*>(mem), arrived});
+    return &all_.back();
+  }
+
+  std::mutex mu_;
+  std::list<KV8Workspace> all_;
+  std::vector<KV8Workspace*> free_;
+  std::map<Key, KV8Workspace*> held_;
+};
+
+// After a device error (a wait that gave up) the counters may be left nonzero.
+void kv8_reset() { KV8Workspaces::get().reset(); }
+
 Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
   const KV8View c = kv8_view(kc, vc, scale_t);
   const c10::cuda::CUDAGuard guard(kc.device());
@@ -926,8 +1050,11 @@ Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
   Tensor out = torch::empty({B, Hq, c.hd}, q.options());
   if (B == 0) return out;
   if (c.n_pages == 0 || bt.size(1) == 0) return out.zero_();
+  const KV8Workspace ws = KV8Workspaces::get().take(kc.get_device(), cur_stream(),
+                                                    kv8_attention_segments((int)B, (int)Hq, c.Hkv));
   kv8_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
-                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), cur_stream());
+                ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ws.part, ws.arrived,
+                ptr<int>(scratch(0, 0).err), cur_stream());
   count();
   return out;
 }
@@ -1787,6 +1914,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv8_write", &kv8_write_, "quantise K / V rows into the 8-bit paged cache");
   m.def("kv8_read", &kv8_read_, "the values the 8-bit paged cache holds at given slots");
   m.def("kv8_attention", &kv8_attention_, "paged decode attention over the 8-bit cache");
+  m.def("kv8_reset", &kv8_reset, "zero the attention's arrival counters after a device error");
   m.def("assign_pages", &assign_pages_, "pages dealt to the rows of a block table");
   m.def("token_maps", &token_maps_, "positions, slots and offsets of packed new tokens");
   m.def("rotary_fwd", &rotary_fwd_, "rotary positions of a fused QKV projection");

@@ -182,11 +182,12 @@ def _filled(lens, Hkv, hd, page, seed=0, spread=1.0, extra=3):
 
 
 def _exact(q, c, bt, lens, scale):
-    """The attention in 64 bits, the sum of p |v|, and how large the scores' terms are."""
+    """The attention in 64 bits, the sum of p |v|, how large the scores' terms are, and the sum of p a (a step of V)."""
     B, Hq, hd = q.shape
     Hkv, page = c.k.shape[1], c.k.shape[2]
     out = torch.zeros(B, Hq, hd, dtype=torch.float64, device="cuda")
     size, terms = torch.zeros_like(out), torch.zeros(B, Hq, 1, dtype=torch.float64, device="cuda")
+    step = torch.zeros_like(terms)
     for b, n in enumerate(lens):
         t = torch.arange(max(0, min(n, bt.shape[1] * page)), device="cuda")
         pg = bt[b, t // page].long()
@@ -202,7 +203,8 @@ def _exact(q, c, bt, lens, scale):
             p = torch.softmax(k @ q[b, h].double() * scale, 0)
             out[b, h], size[b, h] = p @ v, p @ v.abs()
             terms[b, h] = 255 * a[:, 0].max() * q[b, h].double().abs().sum() * abs(scale)
-    return out, size, terms
+            step[b, h] = p @ a[:, 1]
+    return out, size, terms, step
 
 
 def _check(q, c, bt, lens, scale=None):
@@ -210,11 +212,17 @@ def _check(q, c, bt, lens, scale=None):
 
     sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
     got = paged_attention_kv8(q, c, bt, sl, scale)
-    want, size, terms = _exact(q, c, bt, lens, scale if scale is not None else 1 / math.sqrt(q.shape[-1]))
+    want, size, terms, step = _exact(q, c, bt, lens, scale if scale is not None else 1 / math.sqrt(q.shape[-1]))
     # bf16 output; a weight times its value's scale has fp16's 11 bits (half a step 2^-11, relative); scores are fp32
     # sums of 10 steps over terms of at most ``terms``, which moves a weight by twice that; exponentials 2^-20
+    n = max(lens)
     weights = 2.0 ** -11 + 2 * (10 * 2.0 ** -23 * terms + 2.0 ** -20)
-    off, bound = (got.double() - want).abs(), BF16 * want.abs() + weights * size + 1e-30
+    # The output's fp32 sums: a block's two products add 2 x 17 numbers, each cut at 2^-24 of the largest, which is at
+    # most 128 x (x = p a, the bytes' offset of 128) or the sum so far; a warp sums n / 128 blocks. And an x far below
+    # the largest one, 2^11, is off by up to 2^-25, that is 2^-36 of it, times at most 127.
+    weights = weights + 34 * 2.0 ** -24 * (n / 128 + 1)
+    low = (34 * 128 * 2.0 ** -24 + n * 127 * 2.0 ** -36) * step
+    off, bound = (got.double() - want).abs(), BF16 * want.abs() + weights * size + low + 1e-30
     assert bool((off <= bound).all()), f"off by {(off / bound).max().item():.3g} of the bound"
     return got
 
@@ -253,9 +261,10 @@ def test_every_token_counts_once(hd):
     c, bt = _filled(lens, Hkv, hd, page)
     q = torch.zeros(len(lens), 4, hd, device="cuda").bfloat16()
     got = paged_attention_kv8(q, KV8Cache(*c), bt, torch.tensor(lens, dtype=torch.int32, device="cuda")).double()
-    want, size, _ = _exact(q, c, bt, lens, 1.0)
-    # weights are all 1: times a scale, rounded to 11 bits (one rounding for the 16 tokens of a block)
-    assert bool(((got - want).abs() <= BF16 * want.abs() + 2.0 ** -11 * size + 2.0 ** -22 * size).all())
+    want, size, _, step = _exact(q, c, bt, lens, 1.0)
+    # weights are all 1: times a scale, rounded to 11 bits (one rounding for the 16 tokens of a block); sums as above
+    sums = 34 * 2.0 ** -24 * (max(lens) / 128 + 1) * size + 34 * 128 * 2.0 ** -24 * step
+    assert bool(((got - want).abs() <= BF16 * want.abs() + 2.0 ** -11 * size + sums).all())
 
 
 def test_pages_and_lengths_outside():
