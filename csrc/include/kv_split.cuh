@@ -133,25 +133,50 @@ struct Walk {
   __device__ __forceinline__ int first_of(int warp) const { return first + ((warp - (int)begin - first) & (WARPS - 1)); }
 };
 
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x / d for quotients below 2^20, r ~ 1 / d
+__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d, float r) {
+  uint32_t q = (uint32_t)((float)x * r);
+  const int rest = (int)(x - q * d);
+  if (rest < 0) --q;
+  if (rest >= (int)d) ++q;
+  return q;
+}
+
 // CTA c of n has units [begin(c), begin(c + 1)): total / n each, and the rest spread evenly (so that equal segments are
 // cut alike).
 struct Shares {
   uint32_t total, n, per, more;
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + c * more / n; }
+  float r;  // ~ 1 / n
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + quotient(c * more, n, r); }
   __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
-    uint32_t c = min(n - 1, (uint32_t)((float)unit / (float)total * (float)n));
+    uint32_t c = min(n - 1, (uint32_t)((float)unit * rcp_approx((float)total) * (float)n));
     while (c + 1 < n && begin(c + 1) <= unit) ++c;
     while (begin(c) > unit) --c;
     return c;
   }
 };
 
-// A segment (b, h) that the CTA has a piece of: its first unit and its units; then the CTAs that share it.
+// A segment (b, h) that the CTA has a piece of, and the n CTAs from ``first`` on that share it.
 struct Piece {
   int b, h;
   uint32_t first, n;
   bool last;  // this CTA arrived last
 };
+template <class W>
+__device__ __forceinline__ Piece piece_of(const W& w, int pad, const Shares& shares) {
+  const uint32_t c0 = shares.owner(w.begin);
+  return {w.b, w.h, c0, shares.owner(w.begin + w.U - pad - 1) - c0 + 1, false};
+}
 
 // The split's constants, which each kernel measured for itself.
 struct Rules {
@@ -164,7 +189,7 @@ struct Rules {
 template <int THREADS>
 struct PlanShared {
   uint32_t scan[THREADS / 32], begin, row0;
-  int row;
+  int row, n;
 };
 
 template <class W>
@@ -182,8 +207,10 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
   p.work = false;
   // all units (row by row), this CTA's share of them and the row it starts in
   uint32_t total = 0, mine = 0, before = 0;
+  int tokens = 0;
   auto sum_rows = [&](int b0) {  // the units of rows b0 + tid, of the rows before it, and of all up to this block of rows
-    mine = b0 + tid < a.B ? units_of<UTOK>(tokens_of(a, b0 + tid)) * (uint32_t)a.per_row : 0;
+    tokens = b0 + tid < a.B ? tokens_of(a, b0 + tid) : 0;
+    mine = b0 + tid < a.B ? units_of<UTOK>(tokens) * (uint32_t)a.per_row : 0;
     uint32_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -210,18 +237,19 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
   const bool equal = total == s.row0 * a.B;  // or as good as that: the cut is right either way
   uint32_t n_cta = segments;
   if (total > segments * (equal ? rules.whole_units : WARPS))
-    n_cta = max(segments, min((total + WARPS - 1) / WARPS, (uint32_t)sqrtf((float)total * (float)segments)));
+    n_cta = max(segments, min((total + WARPS - 1) / WARPS, (uint32_t)sqrt_approx((float)total * (float)segments)));
   n_cta = min(gridDim.x, n_cta);
   if (equal && n_cta > segments) {
-    const uint32_t even = n_cta - n_cta % segments;
-    if ((float)total / even - (float)total / n_cta <= (float)(rules.join_steps * WARPS)) n_cta = even;
+    const uint32_t even = quotient(n_cta, segments, rcp_approx((float)segments)) * segments;
+    if ((float)total * (rcp_approx((float)even) - rcp_approx((float)n_cta)) <= (float)(rules.join_steps * WARPS)) n_cta = even;
   }
   if (blockIdx.x >= n_cta) return p;
   // Where CTAs have several segments, the change from one to the next counts as ``pad`` empty units at a segment's end: a
   // CTA with more segments gets fewer tokens. Where several CTAs share each of equal segments there is no change.
   p.pad = equal && n_cta >= 2 * segments ? 0 : rules.pad;
   const uint32_t all = total + p.pad * segments;
-  p.shares = Shares{all, n_cta, all / n_cta, all % n_cta};
+  const uint32_t per = all / n_cta;
+  p.shares = Shares{all, n_cta, per, all - per * n_cta, rcp_approx((float)n_cta)};
   const uint32_t at = p.shares.begin(blockIdx.x), end = p.shares.begin(blockIdx.x + 1);
   if (a.B > THREADS) total = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
@@ -229,15 +257,16 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
     const uint32_t row = before + p.pad * a.per_row * (b0 + tid);
     if (b0 + tid < a.B && at - row < mine + p.pad * a.per_row) {
       s.row = b0 + tid;
+      s.n = tokens;
       s.begin = row;
     }
     if (total + p.pad * a.per_row * min(b0 + THREADS, a.B) > at) break;
   }
   __syncthreads();
   p.w.b = s.row;
-  p.w.n = tokens_of(a, p.w.b);
+  p.w.n = s.n;
   p.w.U = units_of<UTOK>(p.w.n) + p.pad;
-  p.w.h = (at - s.begin) / p.w.U;
+  p.w.h = quotient(at - s.begin, p.w.U, rcp_approx((float)p.w.U));
   p.w.begin = s.begin + p.w.h * p.w.U;
   p.w.first = at - p.w.begin;
   p.w.left = end - at;
@@ -246,23 +275,20 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
   return p;
 }
 
-// The last CTA to arrive at a segment joins its pieces; arrivals wait until the share is done, so that nothing else
-// waits for their round trip. ``part``: [2 CTAs][kHeads][HD + 4] floats (sums, maximum, normaliser), of which CTA c's
-// segment that began before its share is at 2 c, another at 2 c + 1; ``arrived``: zero between launches.
+// The last CTA to arrive at a segment joins its pieces. ``part``: [2 CTAs][kHeads][HD + 4] floats (sums, maximum,
+// normaliser), of which CTA c's segment that began before its share is at 2 c, another at 2 c + 1; ``arrived``: zero
+// between launches. Every thread takes part, the CTA's own pieces having been written before a barrier.
 template <int HD, int THREADS>
-__device__ __forceinline__ void join_pieces(const Rows& a, const Shares& shares, Piece* piece, int pieces, const float* part,
-                                            unsigned* arrived, int blocks, int rep, int Hq, bf16* out) {
+__device__ __forceinline__ void join_pieces(const Rows& a, Piece* piece, int pieces, const float* part, unsigned* arrived,
+                                            int blocks, int rep, int Hq, bf16* out) {
   constexpr int PART = HD + 4;
   const int tid = threadIdx.x;
   if (tid < pieces) {
     Piece& x = piece[tid];
-    const uint32_t c0 = shares.owner(x.first), np = shares.owner(x.first + x.n - 1) - c0 + 1;
-    x.first = c0;
-    x.n = np;
     unsigned* ctr = arrived + (int64_t)x.b * a.per_row + x.h;
     unsigned old;
     asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(ctr) : "memory");
-    x.last = old == np - 1;
+    x.last = old == x.n - 1;
     if (x.last) *ctr = 0u;
   }
   __syncthreads();

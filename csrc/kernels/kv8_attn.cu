@@ -12,8 +12,9 @@
 //   S^T [16 tokens, 8 heads] = K [16, hd] Q^T      A rows are tokens: a word of a K row is two operands, masked and moved
 //   O^T [16 channels, 8 heads] += V^T [16, 16 tokens] P^T    A rows are channels: a byte permute pairs two tokens' words
 // Query heads that share a KV head fill the 8 columns, so every cached byte is read once for up to 8 heads. P changes
-// from accumulator to operand by movmatrix. Copies place a row's 16-byte chunks so that lanes that read together, of K
-// (rows i and i + 4) and of V (four neighbouring rows), meet in no bank. tcgen05 would not help: the operands would have
+// from accumulator to operand by movmatrix. The copies swizzle the 16-byte chunks of 128 bytes
+// by the line, and the tokens are dealt to the matrix rows so that lanes that read together, of K or of V, meet in no
+// bank. tcgen05 would not help: the operands would have
 // to be unpacked and stored once more before it could read them, and 8 query rows leave it nothing to win.
 //
 // P carries the scale of V (x = p a'), so a reference m per warp and head keeps it in fp16's range: p is taken relative
@@ -23,10 +24,11 @@
 // 2^79; sums and the normaliser stay in 32 bits.
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory (a unit is
-// a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies units ahead, across the
-// segments, and at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare the
-// query fragments of the coming segments and join the eight states of the finished ones. Every wait is bounded; one that
-// gives up records an error code. How the work is split over CTAs stands in kv_split.cuh.
+// a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead, across the segments, and
+// at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare the query fragments
+// of the coming segments and join the eight states of the finished ones; the states of a share's last segment are joined
+// by all twelve. Every wait is bounded; one that gives up records an error code. How the work is split over CTAs stands
+// in kv_split.cuh.
 #include <climits>
 
 #include <cuda_runtime.h>
@@ -44,11 +46,13 @@ constexpr int kWarps = 8;  // that compute
 constexpr int kHelpers = 4;
 constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = kKV8Block;
+constexpr int kStages = 3;
 constexpr int kSlots = 2;  // segments whose fragments or states are held
-constexpr Rules kRules{24, 16, 3};
+constexpr int kHold = 8;   // units whose offset is taken out together
+constexpr Rules kRules{24, 24, 6};
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBoost = 11.f;        // log2 of the largest p a' right after the reference moved
-constexpr float kLimit = 32768.f;     // how far later ones may go
+constexpr float kBoost = 11.f;           // log2 of the largest p a' right after the reference moved
+constexpr float kLimit = 32768.f;        // how far later ones may go
 constexpr float kMinA = 5.4210109e-20f;  // 2^-64
 
 template <int HD>
@@ -56,11 +60,10 @@ struct Cfg {
   static constexpr int NT = 128 / HD;                   // blocks of a unit
   static constexpr int UTOK = NT * kTok;
   static constexpr int BLOCK = kTok * HD;               // bytes of a block of K
-  static constexpr int K = 0, V = NT * BLOCK, S = 2 * NT * BLOCK, STAGE = 2 * NT * BLOCK + 16;
-  static constexpr int STAGES = 4;
-  static constexpr int WARP = STAGES * STAGE;
+  static constexpr int K = 0, V = NT * BLOCK, STAGE = 2 * NT * BLOCK;
+  static constexpr int SCALES = kWarps * kStages * STAGE;  // a pair (K, V) for each block of each stage
   static constexpr int LD = HD + 4;                     // row stride of a state: spreads the heads over the banks
-  static constexpr int STATES = kWarps * WARP;          // kSlots sets of the warps' states
+  static constexpr int STATES = SCALES + kWarps * kStages * NT * 8;  // kSlots sets of the warps' states
   static constexpr int STATE = kHeads * LD * 4;
   // kSlots sets of query fragments: matrix B, -128 sum(q), factors
   static constexpr int F = STATES + kSlots * kWarps * STATE;
@@ -69,13 +72,21 @@ struct Cfg {
   static constexpr int FBYTES = F_FACTOR + kHeads * 4;
   static constexpr int SMEM = F + kSlots * FBYTES;
   static constexpr int PART = HD + 4;                   // floats of a head in the workspace: sums, maximum, normaliser
+  static_assert(STAGE == 4096 && SMEM + 4096 <= 232448);
 };
 
-// Where chunk c (16 bytes) of a block's row j stands.
+// Token of a block that matrix row r (0 .. 7, or those less 8) stands for. Rows 2 i and 2 i + 1 lie in different halves of
+// their swizzled lines, and rows 0, 2, 4, 6 (or 1, 3, 5, 7) spread over all eight chunks.
+template <int HD>
+__device__ __forceinline__ int token_of(int r) {
+  if constexpr (HD == 128) return r ^ (r & 1) << 2;
+  return (r & 4) + (r & 1 ? 3 - (r & 3) / 2 : (r & 3) / 2);
+}
+// Where chunk c (16 bytes) of a block's token j stands: lines of 128 bytes, chunks swizzled by the line.
 template <int HD>
 __device__ __forceinline__ uint32_t chunk_at(int j, int c) {
-  if constexpr (HD == 128) return j * 128 + 16 * (c ^ 2 * (j & 3) ^ (j & 4));
-  return j / 2 * 128 + ((j ^ j >> 2) & 1) * 64 + 16 * (c ^ (j & 2));
+  if constexpr (HD == 128) return j * 128 + 16 * (c ^ (j & 7));
+  return j / 2 * 128 + 16 * ((j % 2 * 4 + c) ^ (j / 2 & 7));
 }
 
 __device__ __forceinline__ void helper_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kHelpers) : "memory"); }
@@ -95,16 +106,27 @@ struct Args : Rows {
   int* err;
 };
 
+// Takes the bytes' offset out of the sums.
+template <int N>
+__device__ __forceinline__ void settle_off(float (&o)[N][4], float (&off)[4]) {
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[q][x] += off[x & 1];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) off[x] = 0.f;
+}
+
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    kv8_attn_kernel(const Args a) {
   using C = Cfg<HD>;
   using W = Walk<C::UTOK, kWarps>;
   constexpr int NT = C::NT, KW = C::KW, VW = HD / 32;  // V words of a lane and row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sm[kSlots][kWarps][kHeads], sl[kSlots][kWarps][kHeads];
+  __shared__ __align__(16) float sm[kSlots][kHeads][kWarps], sl[kSlots][kHeads][kWarps];
   __shared__ W s_seg[kSlots], s_ahead[kWarps];
   __shared__ uint64_t ready[kSlots], done[kSlots];  // fragments are there and the states free; the states are there
-  __shared__ float weight[kHeads][kWarps], total_max[kHeads], total_sum[kHeads];
   __shared__ Piece s_piece[2];
   __shared__ PlanShared<kThreads> s_plan;
   __shared__ int s_pieces, s_abort, s_ok;
@@ -117,16 +139,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
       mbar_init(&done[i], kWarps);
     }
     s_abort = 0;
-    s_pieces = 0;
-    fence_mbar_init();
   }
+  fence_mbar_init();
   pdl_wait();
   pdl_trigger();
   const auto plan = make_plan<C::UTOK, kWarps, kThreads>(a, s_plan, kRules);
   if (!plan.work) return;
   const W w0 = plan.w;
   const int pad = plan.pad;
-  const float sl2 = a.scale * kLog2e;
+  int slot = 0;  // of the segment at hand; at the end, of the share's last
+
+  // The eight warps' states of a segment, joined by n threads of which this is the i-th: a whole segment is done, a piece
+  // of one goes to the workspace.
+  auto join_states = [&](const W& w, int slot, int i, int n) {
+    const int hk = w.h / a.blocks, h0 = (w.h % a.blocks) * kHeads, nh = min(kHeads, a.rep - h0);
+    const float* states = reinterpret_cast<const float*>(smem + C::STATES + slot * kWarps * C::STATE);
+    for (; i < nh * (HD / 4); i += n) {
+      const int h = i / (HD / 4), ch = 4 * (i % (HD / 4));
+      float m1[kWarps], l1[kWarps], M = -INFINITY, L = 0.f;
+      float4 v[kWarps], x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; k += 4) {
+        *reinterpret_cast<float4*>(m1 + k) = *reinterpret_cast<const float4*>(&sm[slot][h][k]);
+        *reinterpret_cast<float4*>(l1 + k) = *reinterpret_cast<const float4*>(&sl[slot][h][k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) v[k] = *reinterpret_cast<const float4*>(states + k * (C::STATE / 4) + h * C::LD + ch);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, m1[k]);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float e = m1[k] == -INFINITY ? 0.f : ex2(m1[k] - M);
+        L = fmaf(l1[k], e, L);
+        x.x = fmaf(v[k].x, e, x.x);
+        x.y = fmaf(v[k].y, e, x.y);
+        x.z = fmaf(v[k].z, e, x.z);
+        x.w = fmaf(v[k].w, e, x.w);
+      }
+      constexpr float f = 16777216.f;  // the bytes' 2^-24
+      if (w.whole()) {
+        const float e = L == 0.f ? 0.f : __fdividef(f, L);
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)w.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
+            make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
+      } else {
+        float* pp = a.part + ((int64_t)(2 * blockIdx.x + (w.first == 0 ? 1 : 0)) * kHeads + h) * C::PART;
+        *reinterpret_cast<float4*>(pp + ch) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+        if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(M, L);
+      }
+    }
+  };
 
   if (warp >= kWarps) {
     // ───────────────────────────── helpers ─────────────────────────────
@@ -135,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
     // times their sum, in units of 2^-24 as the products are; the factor that takes the powers back, with the softmax
     // scale (2^12 of it are left to the blocks' scales).
     constexpr int CH = HD / 32;  // channels of a lane
+    const float sl2 = a.scale * (kLog2e * 4096.f);
     uint32_t raw[kHeads / kHelpers][CH / 2];
     auto load_q = [&](const W& w) {
       const int h0 = (w.h % a.blocks) * kHeads;
@@ -149,35 +211,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
     };
     auto prepare = [&](const W& w, int slot) {
       uint8_t* f = smem + C::F + slot * C::FBYTES;
+      float x[kHeads / kHelpers][CH], mx[kHeads / kHelpers], sum[kHeads / kHelpers], down[kHeads / kHelpers];
 #pragma unroll
       for (int k = 0; k < kHeads / kHelpers; ++k) {
-        const int h = hw + k * kHelpers;
-        float x[CH];
 #pragma unroll
         for (int i = 0; i < CH / 2; ++i) {
           const float2 y = unpack_bf16x2(raw[k][i]);
-          x[2 * i] = y.x;
-          x[2 * i + 1] = y.y;
+          x[k][2 * i] = y.x;
+          x[k][2 * i + 1] = y.y;
         }
-        float mx = 0.f, sum = 0.f;
+        mx[k] = 0.f;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) mx = fmaxf(mx, fabsf(x[i]));
-        mx = warp_max(mx);
-        const int ex = (mx > 0.f && mx < INFINITY) ? min(14 - ilogbf(mx), 126) : 0;
-        const float up = ldexpf(1.f, ex);
+        for (int i = 0; i < CH; ++i) mx[k] = fmaxf(mx[k], fabsf(x[k][i]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < kHeads / kHelpers; ++k) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+#pragma unroll
+      for (int k = 0; k < kHeads / kHelpers; ++k) {
+        // 2^14 over the largest's power of two; magnitudes outside [2^-100, 2^126) as they are at its ends
+        const uint32_t power = min(max(__float_as_uint(mx[k]), 27u << 23), (252u << 23)) & 0x7F800000u;
+        const float up = __uint_as_float(((127u + 14u + 127u) << 23) - power);
+        down[k] = __uint_as_float(power - (14u << 23));
+        sum[k] = 0.f;
+        __half y[CH];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-          const int ch = lane * CH + i, t = ch / 16 % 4, w = ch % 16 / 4 + 4 * (ch / 64), e = ch % 4;
-          const __half y = __float2half_rn(x[i] * up);
-          sum += __half2float(y);
-          reinterpret_cast<__half*>(f)[(((w / 2 * 32 + h * 4 + t) * 4) + w % 2 * 2 + e % 2) * 2 + e / 2] = y;
+          y[i] = __float2half_rn(x[k][i] * up);
+          sum[k] += __half2float(y[i]);
         }
-        sum = warp_sum(sum);
-        if (lane == 0) {
-          reinterpret_cast<float*>(f + C::F_BIAS)[h] = sum * -7.62939453125e-6f;  // -128 2^-24
-          reinterpret_cast<float*>(f + C::F_FACTOR)[h] = ldexpf(sl2, 12 - ex);
+        // channel ch: chunk ch / 16 belongs to lane (ch / 16) % 4 of a matrix row, byte e = ch % 4 of its word w; bytes 0, 2
+        // are operand 0, bytes 1, 3 operand 1
+        const int h = hw + k * kHelpers, ch = lane * CH, t = ch / 16 % 4, w = ch % 16 / 4 + 4 * (ch / 64);
+        uint32_t* at = reinterpret_cast<uint32_t*>(f) + (w / 2 * 32 + h * 4 + t) * 4 + w % 2 * 2;
+        if constexpr (CH == 4) {
+          *reinterpret_cast<__half2*>(at) = __halves2half2(y[0], y[2]);
+          *reinterpret_cast<__half2*>(at + 1) = __halves2half2(y[1], y[3]);
+        } else {
+          reinterpret_cast<__half*>(at)[lane % 2] = y[0];
+          reinterpret_cast<__half*>(at + 1)[lane % 2] = y[1];
         }
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < kHeads / kHelpers; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+      if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < kHeads / kHelpers; ++k) {
+          reinterpret_cast<float*>(f + C::F_BIAS)[hw + k * kHelpers] = sum[k] * -7.62939453125e-6f;  // -128 2^-24
+          reinterpret_cast<float*>(f + C::F_FACTOR)[hw + k * kHelpers] = sl2 * down[k];
+        }
       if (ht == 0) s_seg[slot] = w;
       helper_sync();
       if (ht == 0) mbar_arrive(&ready[slot]);
@@ -190,65 +275,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
       more = coming.next(a, pad);
       if (more) load_q(coming);  // on its way until a slot is free
     }
-    int slot = 0, pieces = 0;
+    int pieces = 0;
     uint32_t phase = 0;
     while (true) {
-      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue);
-      helper_sync();
-      if (!s_ok) break;
       const W w = s_seg[slot];
-      const int hk = w.h / a.blocks, h0 = (w.h % a.blocks) * kHeads, nh = min(kHeads, a.rep - h0);
-      // the warps' weights: eight neighbouring threads have a head's eight states
-      if (ht < kHeads * kWarps) {
-        const int h = ht / kWarps, k = ht % kWarps;
-        const float m1 = sm[slot][k][h];
-        float M = m1;
-#pragma unroll
-        for (int o = 1; o < kWarps; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float e = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-        float L = sl[slot][k][h] * e;
-#pragma unroll
-        for (int o = 1; o < kWarps; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        weight[h][k] = e;
-        if (k == 0) {
-          total_max[h] = M;
-          total_sum[h] = L;
-        }
-      }
-      helper_sync();
-      // a whole segment is done, a piece of one goes to the workspace
-      const bool whole = w.whole();
-      const int part = 2 * blockIdx.x + (w.first == 0 ? 1 : 0);
-      const float* states = reinterpret_cast<const float*>(smem + C::STATES + slot * kWarps * C::STATE);
-      for (int i = ht; i < nh * (HD / 4); i += 32 * kHelpers) {
-        const int h = i / (HD / 4), ch = 4 * (i % (HD / 4));
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-          const float4 v = *reinterpret_cast<const float4*>(states + k * (C::STATE / 4) + h * C::LD + ch);
-          const float e = weight[h][k];
-          x.x = fmaf(v.x, e, x.x);
-          x.y = fmaf(v.y, e, x.y);
-          x.z = fmaf(v.z, e, x.z);
-          x.w = fmaf(v.w, e, x.w);
-        }
-        const float L = total_sum[h];
-        if (whole) {
-          const float e = L == 0.f ? 0.f : 1.f / L;
-          *reinterpret_cast<uint2*>(a.out + ((int64_t)w.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
-              make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
-        } else {
-          float* pp = a.part + ((int64_t)part * kHeads + h) * C::PART;
-          *reinterpret_cast<float4*>(pp + ch) = x;
-          if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(total_max[h], L);
-        }
-      }
-      if (!whole) {  // at most the first and the last segment of the share
-        if (ht == 0) s_piece[pieces] = {w.b, w.h, w.begin, (uint32_t)(w.U - pad), false};
+      if (!w.whole()) {  // at most the first and the last segment of the share
+        if (ht == 32) s_piece[pieces] = piece_of(w, pad, plan.shares);
         ++pieces;
       }
       if (!w.more()) break;
-      helper_sync();  // the states and weights have been read
+      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue);
+      helper_sync();
+      if (!s_ok) break;
+      join_states(w, slot, ht, 32 * kHelpers);
+      helper_sync();  // the states have been read
       if (more) {
         prepare(coming, slot);
         more = coming.next(a, pad);
@@ -263,29 +303,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
   } else {
     // ───────────────────────────── compute ─────────────────────────────
     const int g = lane / 4, t = lane % 4;
-    // token of matrix rows g and (8 further on) g + 8; V's are t, t + 4, t + 8, t + 12
-    const int tok_g = g / 2 + 4 * (g % 2);
-    const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-    // this lane's places in a block: of K, chunk t of row tok_g (and chunk t + 4, 64 bytes across); of V, its channels of
-    // rows t and t + 4
-    const uint32_t k_at = chunk_at<HD>(tok_g, t);
-    const uint32_t v_at = HD == 128 ? chunk_at<HD>(t, g) : chunk_at<HD>(t, g / 2) + g % 2 * 8;
-    const uint32_t v_at4 = HD == 128 ? chunk_at<HD>(t + 4, g) : chunk_at<HD>(t + 4, g / 2) + g % 2 * 8;
-    constexpr int ROWS = 512 / HD;  // rows of a warp's copy
-    const uint32_t copy_at = chunk_at<HD>(lane / (HD / 16), lane % (HD / 16));
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * C::STAGE);
+    float2* const scales = reinterpret_cast<float2*>(smem + C::SCALES) + warp * (kStages * NT);
+    // this lane's places in a block: of K, chunk t of row g's token (and chunk t + 4, 64 bytes across); of V, its channels
+    // of the tokens of rows 2 t and 2 t + 1; rows 8 further on are tokens 8 further on
+    const uint32_t k_at = chunk_at<HD>(token_of<HD>(g), t);
+    const uint32_t v_at0 = HD == 128 ? chunk_at<HD>(token_of<HD>(2 * t), g) : chunk_at<HD>(token_of<HD>(2 * t), g / 2) + g % 2 * 8;
+    const uint32_t v_at1 =
+        HD == 128 ? chunk_at<HD>(token_of<HD>(2 * t + 1), g) : chunk_at<HD>(token_of<HD>(2 * t + 1), g / 2) + g % 2 * 8;
+    // at head width 64 the line's bit 2 changes with the half of the block: the chunk's moves too
+    constexpr uint32_t kFar = HD == 128 ? 0u : 64u;
     if (lane == 0) s_ahead[warp] = w0;
     __syncwarp();
 
-    // The copies run STAGES - 1 units ahead of the arithmetic, across the segments; a unit's page ids are read one step
-    // before its copies start, a block's by every NT-th lane.
+    // The copies run kStages - 1 units ahead of the arithmetic, across the segments; a unit's page ids are read one step
+    // before its copies start.
     constexpr int kDone = -(1 << 30);  // the share holds no more units for this warp
     const int sub = lane % NT;
-    int f_end, f_at, f_wrap, f_page;  // f_at: block within the page of all heads, f_wrap: where this head's part ends
-    int f_block, f_blocks;            // of the row: this lane's, all of them
+    int f_end, f_at, f_wrap;  // f_at: block within the page of all heads, f_wrap: where this head's part ends
+    int f_block, f_blocks;    // of the row: this lane's, all of them
     const int* f_bt;
     const int step_pi = NT * kWarps / a.bpp, step_off = NT * kWarps % a.bpp;
-    const uint8_t* kp = a.c.k + lane * 16;
-    const uint8_t* vp = a.c.v + lane * 16;
     int f_unit = w0.first_of(warp);
     auto aim = [&](const W& w) {
       f_end = w.end();
@@ -296,7 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
       f_at += f_block % a.bpp;
       f_bt = a.bt + w.b * a.bt_stride + f_block / a.bpp;
     };
-    auto settle = [&]() {  // on this warp's next unit, if its share has one
+    struct Look {
+      int page, at;  // of this lane's block of a unit
+    };
+    auto look = [&]() {  // at this warp's next unit, if its share has one
       if (f_unit >= f_end) {
         W w = s_ahead[warp];
         do {
@@ -312,30 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
         if (lane == 0) s_ahead[warp] = w;
         __syncwarp();
       }
-      f_page = -1;
-      if (f_unit >= 0 && (NT == 1 || f_block < f_blocks)) f_page = *f_bt;
-    };
-    uint32_t valid = 0;  // bits i NT ..: the blocks of the unit i steps ahead have a page
-    auto fetch = [&](uint32_t stage, int steps) {
-      const bool there = (uint32_t)f_page < (uint32_t)a.c.n_pages;
-      const uint32_t n = there ? (uint32_t)f_page * (uint32_t)a.page_blocks + (uint32_t)f_at : 0u;  // block of the cache
-      const uint32_t bits = __ballot_sync(0xffffffffu, there) & ((1u << NT) - 1u);
-      valid |= bits << (NT * steps);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        const uint64_t at = (uint64_t)(NT == 1 ? n : __shfl_sync(0xffffffffu, n, x)) * C::BLOCK;
-        const bool ok = bits >> x & 1u;
-        const uint32_t dst = stage + x * C::BLOCK;
-#pragma unroll
-        for (int i = 0; i < C::BLOCK / 512; ++i) {
-          // the chunk's place depends on the row's bit 2 too: odd copies at head width 128
-          const uint32_t to = dst + 512 * i + (HD == 128 && i % 2 ? copy_at ^ 64u : copy_at);
-          copy16(to + C::K, kp + at + 512 * i, ok);
-          copy16(to + C::V, vp + at + 512 * i, ok);
-        }
-      }
-      if (lane < NT) copy8(stage + C::S + 8 * lane, a.c.scale + 2 * (uint64_t)n, there);
-      copies_commit();
+      Look x{-1, f_at};
+      if (f_unit >= 0 && (NT == 1 || f_block < f_blocks)) x.page = *f_bt;
       f_unit += kWarps;
       f_block += NT * kWarps;
       f_bt += step_pi;
@@ -344,14 +363,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
         f_at -= a.bpp;
         ++f_bt;
       }
-      settle();
+      return x;
     };
-    static_assert(ROWS == (HD == 128 ? 4 : 8), "a copy holds rows of one residue to ROWS");
+    uint32_t valid = 0;  // bits i NT ..: the blocks of the unit i steps ahead have a page
+    int f_stage = 0;
+    // line lane / 8 of every four, chunk lane % 8; the lines' bit 2 is the copy's lowest
+    const uint32_t copy_at = lane / 8 * 128 + 16 * (lane % 8 ^ lane / 8);
+    const uint8_t* const kp = a.c.k + lane * 16;
+    const uint8_t* const vp = a.c.v + lane * 16;
+    auto fetch = [&](const Look& x, int steps) {
+      const bool there = (uint32_t)x.page < (uint32_t)a.c.n_pages;
+      const uint32_t n = there ? (uint32_t)x.page * (uint32_t)a.page_blocks + (uint32_t)x.at : 0u;  // block of the cache
+      const uint32_t bits = __ballot_sync(0xffffffffu, there) & ((1u << NT) - 1u);
+      valid |= bits << (NT * steps);
+      const uint32_t stage = ring + f_stage * C::STAGE;
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        const uint64_t at = (uint64_t)(NT == 1 ? n : __shfl_sync(0xffffffffu, n, b)) * C::BLOCK;
+        const bool ok = bits >> b & 1u;
+#pragma unroll
+        for (int i = 0; i < C::BLOCK / 512; ++i) {
+          const uint32_t to = stage + b * C::BLOCK + 512 * i + (i % 2 ? copy_at ^ 64u : copy_at);
+          copy16(to + C::K, kp + at + 512 * i, ok);
+          copy16(to + C::V, vp + at + 512 * i, ok);
+        }
+      }
+      if (lane < NT) copy8(smem_u32(scales + f_stage * NT + lane), a.c.scale + 2 * (uint64_t)n, there);
+      copies_commit();
+      f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+    };
     aim(w0);
-    settle();
-    for (int i = 0; i < C::STAGES - 1; ++i) fetch(ring + i * C::STAGE, i);
-    uint32_t stage = ring, ahead = ring + (C::STAGES - 1) * C::STAGE;
-    int slot = 0;
+    Look seen;
+    {
+      Look x[kStages - 1];
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) x[i] = look();
+      seen = look();
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) fetch(x[i], i);
+    }
+    int stage = 0;
     uint32_t phase = 0;
 
     while (true) {
@@ -371,19 +422,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
       // o and l are relative to the reference m: p 2^-m, so that x fits fp16 well
       float o[2 * VW][4], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
       float limit = -1.f;  // below 0: no reference yet
+      float off[4] = {0.f, 0.f, 0.f, 0.f};  // -128 times the weights of the last units, for heads 2 t and 2 t + 1
+      int held = 0;
 #pragma unroll
       for (int i = 0; i < 2 * VW; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       for (; unit < u_end; unit += kWarps) {
-        copies_wait<C::STAGES - 2>();
-        __syncwarp();  // and every lane has read the stage that is filled again below
-        const uint32_t here = stage;
+        copies_wait<kStages - 2>();
+        __syncwarp();  // the copies are there for all, and every lane has read the stage that is filled again below
+        const uint32_t here = ring + stage * C::STAGE;
+        const float2* sc_at = scales + stage * NT;
         // tokens of the unit to be counted; the rest may be anything
         const int count = n_tok - unit * C::UTOK;
         const uint32_t pieces = valid & ((1u << NT) - 1u);
         valid >>= NT;
-        fetch(ahead, C::STAGES - 2);
-        ahead = stage;
-        stage = stage + C::STAGE == ring + C::WARP ? ring : stage + C::STAGE;
+        if (++stage == kStages) stage = 0;
         // everything the unit needs from shared memory is asked for at once
         uint32_t kw[NT][2][KW], qf[KW / 2][4], vw[NT][4][VW];
         float2 sc[NT];
@@ -391,22 +443,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            load_words<4>(kw[n][i], here + C::K + n * C::BLOCK + i * (C::BLOCK / 2) + k_at);
-            if constexpr (KW == 8) load_words<4>(kw[n][i] + 4, here + C::K + n * C::BLOCK + i * (C::BLOCK / 2) + (k_at ^ 64u));
+            const uint32_t at = here + C::K + n * C::BLOCK + i * (C::BLOCK / 2) + (i ? k_at ^ kFar : k_at);
+            load_words<4>(kw[n][i], at);
+            if constexpr (KW == 8) load_words<4>(kw[n][i] + 4, at ^ 64u);
           }
 #pragma unroll
         for (int j = 0; j < KW / 2; ++j) load_words<4>(qf[j], frag_at + j * 512);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) load_words<2>(reinterpret_cast<uint32_t*>(&sc[n]), here + C::S + 8 * n);
+        for (int n = 0; n < NT; ++n) sc[n] = sc_at[n];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            load_words<VW>(vw[n][i], here + C::V + n * C::BLOCK + i / 2 * (C::BLOCK / 2) + (i % 2 ? v_at4 : v_at));
+            load_words<VW>(vw[n][i], here + C::V + n * C::BLOCK + i / 2 * (C::BLOCK / 2) +
+                                         ((i % 2 ? v_at1 : v_at0) ^ (i / 2 ? kFar : 0u)));
+        fetch(seen, kStages - 2);
+        seen = look();
         // scores: block n, row g + 8 i, head 2 t + r
         float s[NT][2][2];
         {
-          float acc[NT][2][4];  // two chains each
+          constexpr int CHAINS = KW / NT >= 4 ? 4 : 2;  // sums that do not wait for one another
+          float acc[NT][CHAINS][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n) acc[n][0][0] = acc[n][0][2] = bias[0], acc[n][0][1] = acc[n][0][3] = bias[1];
 #pragma unroll
@@ -416,19 +473,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
               const uint32_t w0 = kw[n][0][j], w1 = kw[n][1][j];
               const uint32_t a0 = w0 & 0x00FF00FFu, a1 = w1 & 0x00FF00FFu;
               const uint32_t a2 = __byte_perm(w0, 0u, 0x4341), a3 = __byte_perm(w1, 0u, 0x4341);
-              if (j == 1)
-                mma_f16_first(acc[n][1], a0, a1, a2, a3, qf[j / 2][j % 2 * 2], qf[j / 2][j % 2 * 2 + 1]);
+              if (j > 0 && j < CHAINS)
+                mma_f16_first(acc[n][j], a0, a1, a2, a3, qf[j / 2][j % 2 * 2], qf[j / 2][j % 2 * 2 + 1]);
               else
-                mma_f16(acc[n][j % 2], a0, a1, a2, a3, qf[j / 2][j % 2 * 2], qf[j / 2][j % 2 * 2 + 1]);
+                mma_f16(acc[n][j % CHAINS], a0, a1, a2, a3, qf[j / 2][j % 2 * 2], qf[j / 2][j % 2 * 2 + 1]);
             }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float a1 = sc[n].x * 4096.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int r = 0; r < 2; ++r)
-                s[n][i][r] = fmaf((acc[n][0][2 * i + r] + acc[n][1][2 * i + r]) * a1, cs[r], -m[r]);
+              for (int r = 0; r < 2; ++r) {
+                float x = acc[n][0][2 * i + r] + acc[n][1][2 * i + r];
+                if constexpr (CHAINS == 4) x += acc[n][2][2 * i + r] + acc[n][3][2 * i + r];
+                s[n][i][r] = fmaf(x * (sc[n].x * 4096.f), cs[r], -m[r]);
+              }
           }
         }
         if (count < C::UTOK || pieces != (1u << NT) - 1u) {
@@ -437,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
             if (n * kTok >= count || !(pieces >> n & 1u)) sc[n].y = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (n * kTok + tok_g + 8 * i >= count || !(pieces >> n & 1u)) s[n][i][0] = s[n][i][1] = -INFINITY;
+              if (n * kTok + token_of<HD>(g) + 8 * i >= count || !(pieces >> n & 1u)) s[n][i][0] = s[n][i][1] = -INFINITY;
           }
         }
         float p[NT][2][2], top_x = 0.f;
@@ -481,6 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
           for (int q = 0; q < 2 * VW; ++q)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[q][x] *= keep[x & 1];
+          off[0] *= keep[0];
+          off[1] *= keep[1];
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -489,8 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
           const uint32_t b0 = transpose8x8(pack_half2(p[n][0][0] * sc[n].y, p[n][0][1] * sc[n].y));
           const uint32_t b1 = transpose8x8(pack_half2(p[n][1][0] * sc[n].y, p[n][1][1] * sc[n].y));
           constexpr uint32_t kBias = 0x80808080u;  // -128 2^-24, twice
-#pragma unroll
-          for (int j = 0; j < 2 * VW; ++j) mma_f16(o[j], kBias, kBias, kBias, kBias, b0, b1);
+          mma_f16(off, kBias, kBias, kBias, kBias, b0, b1);
 #pragma unroll
           for (int j = 0; j < VW; ++j)
 #pragma unroll
@@ -501,27 +561,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
                       __byte_perm(y, 0u, 0x4341), b0, b1);
             }
         }
+        if (++held == kHold) {
+          settle_off(o, off);
+          held = 0;
+        }
       }
+      settle_off(o, off);
 
-      // the warp's state: o in units of V, relative to m
+      // the warp's state: o in units of 2^-24 V, relative to m
       float* state = reinterpret_cast<float*>(smem + C::STATES + (slot * kWarps + warp) * C::STATE);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         l[r] = sum_over_rows(l[r]);
         float4* d = reinterpret_cast<float4*>(state + (2 * t + r) * C::LD + HD / 8 * g);
 #pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          constexpr float f = 16777216.f;
-          d[j] = make_float4(o[2 * j][r] * f, o[2 * j][2 + r] * f, o[2 * j + 1][r] * f, o[2 * j + 1][2 + r] * f);
-        }
+        for (int j = 0; j < VW; ++j) d[j] = make_float4(o[2 * j][r], o[2 * j][2 + r], o[2 * j + 1][r], o[2 * j + 1][2 + r]);
         if (g == 0) {
-          sm[slot][warp][2 * t + r] = limit < 0.f ? -INFINITY : m[r];
-          sl[slot][warp][2 * t + r] = l[r];
+          sm[slot][2 * t + r][warp] = limit < 0.f ? -INFINITY : m[r];
+          sl[slot][2 * t + r][warp] = l[r];
         }
       }
+      if (!more) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[slot]);
-      if (!more) break;
       if (++slot == kSlots) {
         slot = 0;
         phase ^= 1;
@@ -531,8 +593,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attn_kernel(const Args a) {
   }
 
   __syncthreads();
+  if (s_abort) return;
+  const W w = s_seg[slot];
+  join_states(w, slot, tid, kThreads);
   const int pieces = s_pieces;
-  if (pieces) join_pieces<HD, kThreads>(a, plan.shares, s_piece, pieces, a.part, a.arrived, a.blocks, a.rep, a.Hq, a.out);
+  if (pieces) {
+    __syncthreads();
+    join_pieces<HD, kThreads>(a, s_piece, pieces, a.part, a.arrived, a.blocks, a.rep, a.Hq, a.out);
+  }
 }
 
 int sm_count() {

@@ -218,10 +218,11 @@ def _check(q, c, bt, lens, scale=None):
     n = max(lens)
     weights = 2.0 ** -11 + 2 * (10 * 2.0 ** -23 * terms + 2.0 ** -20)
     # The output's fp32 sums: a block's two products add 2 x 17 numbers, each cut at 2^-24 of the largest, which is at
-    # most 128 x (x = p a, the bytes' offset of 128) or the sum so far; a warp sums n / 128 blocks. And an x far below
-    # the largest one, 2^11, is off by up to 2^-25, that is 2^-36 of it, times at most 127.
+    # most the sum so far (a warp sums n / 128 blocks) or the bytes' offset, 128 x (x = p a), of the up to 16 blocks for
+    # which it is taken out together. And an x far below the largest one, 2^11, is off by up to 2^-25, that is 2^-36 of
+    # it, times at most 127.
     weights = weights + 34 * 2.0 ** -24 * (n / 128 + 1)
-    low = (34 * 128 * 2.0 ** -24 + n * 127 * 2.0 ** -36) * step
+    low = (34 * 128 * 16 * 2.0 ** -24 + n * 127 * 2.0 ** -36) * step
     off, bound = (got.double() - want).abs(), BF16 * want.abs() + weights * size + low + 1e-30
     assert bool((off <= bound).all()), f"off by {(off / bound).max().item():.3g} of the bound"
     return got
@@ -263,7 +264,7 @@ def test_every_token_counts_once(hd):
     got = paged_attention_kv8(q, KV8Cache(*c), bt, torch.tensor(lens, dtype=torch.int32, device="cuda")).double()
     want, size, _, step = _exact(q, c, bt, lens, 1.0)
     # weights are all 1: times a scale, rounded to 11 bits (one rounding for the 16 tokens of a block); sums as above
-    sums = 34 * 2.0 ** -24 * (max(lens) / 128 + 1) * size + 34 * 128 * 2.0 ** -24 * step
+    sums = 34 * 2.0 ** -24 * (max(lens) / 128 + 1) * size + 34 * 128 * 16 * 2.0 ** -24 * step
     assert bool(((got - want).abs() <= BF16 * want.abs() + 2.0 ** -11 * size + sums).all())
 
 
