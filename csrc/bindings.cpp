@@ -1062,17 +1062,17 @@ Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
 // ─── paged tables ───────────────────────────────────────────────────────────
 
 void check_i32(const Tensor& t, const Tensor& table, int64_t n, const char* what) {
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && (n < 0 || t.size(0) == n) && t.device() == table.device() &&
-                  t.is_contiguous() && t.size(0) < (1LL << 31) - 4096,
-              std::string(what) + " must be contiguous int32 of one dimension on the table's device" +
-                  (n < 0 ? "" : ", [" + std::to_string(n) + "]"));
+  const bool shape = t.scalar_type() == at::kInt && t.dim() == 1 && (n < 0 || t.size(0) == n);
+  TORCH_CHECK_VALUE(shape, std::string(what) + " must be int32 [" + (n < 0 ? "n" : std::to_string(n)) + "]");
+  const bool place = t.device() == table.device() && t.is_contiguous() && t.size(0) < (1LL << 31) - 4096;
+  TORCH_CHECK(place, std::string(what) + " must be contiguous, on the table's device");
 }
 
 void check_table(const Tensor& bt) {
   CHECK_CUDA(bt);
-  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2 && (bt.size(1) <= 1 || bt.stride(1) == 1) &&
-                  bt.size(0) < (1LL << 31) && bt.size(1) < (1LL << 31),
-              "block_table must be int32 [rows, pages] with neighbouring columns");
+  TORCH_CHECK_VALUE(bt.scalar_type() == at::kInt && bt.dim() == 2, "block_table must be int32 [rows, pages]");
+  TORCH_CHECK((bt.size(1) <= 1 || bt.stride(1) == 1) && bt.size(0) < (1LL << 31) && bt.size(1) < (1LL << 31),
+              "block_table must have neighbouring columns");
 }
 
 void assign_pages_(Tensor bt, Tensor rows, Tensor have, Tensor need, Tensor pages) {
@@ -1094,8 +1094,9 @@ std::tuple<Tensor, Tensor, Tensor> token_maps_(Tensor bt, Tensor rows, Tensor st
   check_i32(rows, bt, -1, "token_maps: rows");
   check_i32(start, bt, rows.size(0), "token_maps: start");
   check_i32(lens, bt, rows.size(0), "token_maps: lens");
-  TORCH_CHECK(total >= 0 && total < (1LL << 31) - 4096, "token_maps: total out of range: " + std::to_string(total));
-  TORCH_CHECK(page > 0 && page < (1LL << 31), "token_maps: page must be positive, got " + std::to_string(page));
+  TORCH_CHECK_VALUE(total >= 0 && page > 0, "token_maps: total must not be negative and page_size positive, got " +
+                                                std::to_string(total) + " and " + std::to_string(page));
+  TORCH_CHECK(total < (1LL << 31) - 4096 && page < (1LL << 31), "token_maps: total or page_size too large");
   Tensor positions = torch::empty({total}, rows.options()), slots = torch::empty({total}, rows.options().dtype(at::kLong));
   Tensor cu = torch::empty({rows.size(0) + 1}, rows.options());
   token_maps(ptr<int>(bt), bt.stride(0), (int)bt.size(0), (int)bt.size(1), ptr<int>(rows), ptr<int>(start),
@@ -1117,13 +1118,14 @@ RotaryShape rotary_shape(const Tensor& qkv, const Tensor& pos, const c10::option
                          const c10::optional<Tensor>& kn, const Tensor& turns, int64_t Hq, int64_t Hkv, int64_t hd,
                          bool interleaved) {
   CHECK_CUDA(qkv);
-  TORCH_CHECK(Hq > 0 && Hkv > 0 && hd > 0, "rotary: heads and head_dim must be positive");
-  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * hd,
-              "rotary: qkv must be bfloat16 [rows, " + std::to_string((Hq + 2 * Hkv) * hd) + "]");
-  TORCH_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == qkv.size(0) && pos.is_contiguous() &&
-                  pos.device() == qkv.device(),
-              "rotary: positions must be int32 [rows] on qkv's device");
-  TORCH_CHECK(qn.has_value() == kn.has_value(), "rotary: both norm weights or none");
+  TORCH_CHECK_VALUE(Hq > 0 && Hkv > 0 && hd > 0, "rotary: heads and head_dim must be positive");
+  TORCH_CHECK_VALUE(qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * hd,
+                    "rotary: qkv must be [rows, " + std::to_string((Hq + 2 * Hkv) * hd) + "]");
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16, "rotary: qkv must be bfloat16 on CUDA");
+  TORCH_CHECK_VALUE(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == qkv.size(0),
+                    "rotary: positions must be int32 [" + std::to_string(qkv.size(0)) + "]");
+  TORCH_CHECK(pos.is_contiguous() && pos.device() == qkv.device(), "rotary: positions must be contiguous, on qkv's device");
+  TORCH_CHECK_VALUE(qn.has_value() == kn.has_value(), "rotary: both norm weights or none");
   for (const c10::optional<Tensor>* w : {&qn, &kn})
     if (w->has_value())
       TORCH_CHECK((*w)->scalar_type() == at::kBFloat16 && (*w)->dim() == 1 && (*w)->size(0) == hd && (*w)->is_contiguous() &&
@@ -1166,35 +1168,97 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> rotary_fwd_(
   return {q, k, v};
 }
 
-// gqkv; gqn / gkn (fp32) get the norms' gradients added.
-Tensor rotary_bwd_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
-                   c10::optional<Tensor> kn, Tensor gq, Tensor gk, Tensor gv, c10::optional<Tensor> gqn,
-                   c10::optional<Tensor> gkn, double eps) {
+struct RotaryGrads {
+  Tensor qkv, qn, kn;
+};
+
+// The gradients; those of the norms' weights are added to wq / wk (fp32) where given, else returned in bf16.
+RotaryGrads rotary_bwd_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
+                        c10::optional<Tensor> kn, Tensor gq, Tensor gk, Tensor gv, c10::optional<Tensor> wq,
+                        c10::optional<Tensor> wk, double eps) {
   TORCH_CHECK(gq.dim() == 3 && gk.dim() == 3 && gv.sizes() == gk.sizes() && gq.size(2) == gk.size(2) &&
                   gq.size(0) == qkv.size(0) && gk.size(0) == qkv.size(0),
               "rotary: gradients must be [rows, heads, head_dim]");
   const RotaryShape s = rotary_shape(qkv, pos, qn, kn, turns, gq.size(1), gk.size(1), gq.size(2), interleaved);
   const c10::cuda::CUDAGuard guard(qkv.device());
-  for (const Tensor* g : {&gq, &gk, &gv})
-    TORCH_CHECK(g->scalar_type() == at::kBFloat16 && g->is_contiguous() && g->device() == qkv.device() &&
-                    reinterpret_cast<uintptr_t>(g->data_ptr()) % 8 == 0,
-                "rotary: gradients must be contiguous bfloat16 on qkv's device");
+  for (Tensor* g : {&gq, &gk, &gv}) {
+    TORCH_CHECK(g->scalar_type() == at::kBFloat16 && g->device() == qkv.device(),
+                "rotary: gradients must be bfloat16 on qkv's device");
+    const bool ok = g->is_contiguous() && reinterpret_cast<uintptr_t>(g->data_ptr()) % 8 == 0;
+    if (!ok) *g = g->clone(at::MemoryFormat::Contiguous);
+  }
+  RotaryGrads out;
+  RotaryWeightGrad w[2] = {};
   Tensor part;
   if (qn.has_value()) {
-    TORCH_CHECK(gqn.has_value() && gkn.has_value(), "rotary: the norms' gradients have no destination");
-    for (const c10::optional<Tensor>* g : {&gqn, &gkn})
-      TORCH_CHECK((*g)->scalar_type() == at::kFloat && (*g)->numel() == s.hd && (*g)->is_contiguous() &&
-                      (*g)->device() == qkv.device(),
-                  "rotary: the norms' gradients must be float32 [head_dim] on qkv's device");
+    const c10::optional<Tensor>* to[2] = {&wq, &wk};
+    Tensor* fresh[2] = {&out.qn, &out.kn};
+    for (int i = 0; i < 2; ++i)
+      if (to[i]->has_value()) {
+        const Tensor& t = **to[i];
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == s.hd && t.is_contiguous() && t.device() == qkv.device(),
+                    "rotary: main_grad of the norms' weights must be float32 [head_dim] on qkv's device");
+        w[i].add = ptr<float>(t);
+      } else {
+        *fresh[i] = torch::empty({s.hd}, qkv.options());
+        w[i].out = ptr<bf16>(*fresh[i]);
+      }
     part = torch::empty({rotary_part_floats(s)}, qkv.options().dtype(at::kFloat));
   }
   qkv = rotary_rows(qkv);
-  Tensor gqkv = torch::empty({qkv.size(0), qkv.size(1)}, qkv.options());
+  out.qkv = torch::empty({qkv.size(0), qkv.size(1)}, qkv.options());
   rotary_bwd(s, ptr<bf16>(qkv), qkv.stride(0), ptr<int>(pos), ptr<uint64_t>(turns), (float)factor, optr<bf16>(qn),
-             optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(gqkv), optr<float>(gqn),
-             optr<float>(gkn), part.defined() ? ptr<float>(part) : nullptr, cur_stream());
-  if (s.T) count(qn.has_value() ? 2 : 1);
-  return gqkv;
+             optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(out.qkv), w[0], w[1],
+             part.defined() ? ptr<float>(part) : nullptr, cur_stream());
+  if (s.T || qn.has_value()) count(qn.has_value() && s.T ? 2 : 1);
+  return out;
+}
+
+// The differentiable call. (The backward pass of a few small kernels is bound by the host: a node of its own in C++ takes
+// half the time of one in Python.)
+class QKVRotary : public torch::autograd::Function<QKVRotary> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& qkv, const Tensor& pos,
+                                                const Tensor& turns, double factor, bool interleaved,
+                                                const c10::optional<Tensor>& qn, const c10::optional<Tensor>& kn, int64_t Hq,
+                                                int64_t Hkv, int64_t hd, double eps, const c10::optional<Tensor>& wq,
+                                                const c10::optional<Tensor>& wk) {
+    auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
+    ctx->save_for_backward({qkv, pos, turns, qn.value_or(Tensor()), kn.value_or(Tensor())});
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["eps"] = eps;
+    if (wq.has_value()) ctx->saved_data["wq"] = *wq;
+    if (wk.has_value()) ctx->saved_data["wk"] = *wk;
+    return {q, *k, *v};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
+    auto held = [&](const char* name) {
+      auto it = ctx->saved_data.find(name);
+      return it == ctx->saved_data.end() ? c10::nullopt : c10::optional<Tensor>(it->second.toTensor());
+    };
+    const RotaryGrads out = rotary_bwd_(saved[0], saved[1], saved[2], ctx->saved_data["factor"].toDouble(),
+                                        ctx->saved_data["interleaved"].toBool(), given(saved[3]), given(saved[4]), g[0],
+                                        g[1], g[2], held("wq"), held("wk"), ctx->saved_data["eps"].toDouble());
+    const Tensor none;
+    return {out.qkv, none, none, none, none, out.qn, out.kn, none, none, none, none, none, none};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qkv_rotary_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved,
+                                               c10::optional<Tensor> qn, c10::optional<Tensor> kn, int64_t Hq, int64_t Hkv,
+                                               int64_t hd, double eps, c10::optional<Tensor> wq, c10::optional<Tensor> wk) {
+  const bool grad = at::GradMode::is_enabled() && (qkv.requires_grad() || (qn.has_value() && qn->requires_grad()) ||
+                                                   (kn.has_value() && kn->requires_grad()));
+  if (!grad) {
+    auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
+    return {q, *k, *v};
+  }
+  auto out = QKVRotary::apply(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, wq, wk);
+  return {out[0], out[1], out[2]};
 }
 
 // ─── logit controls ─────────────────────────────────────────────────────────
@@ -1918,7 +1982,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("assign_pages", &assign_pages_, "pages dealt to the rows of a block table");
   m.def("token_maps", &token_maps_, "positions, slots and offsets of packed new tokens");
   m.def("rotary_fwd", &rotary_fwd_, "rotary positions of a fused QKV projection");
-  m.def("rotary_bwd", &rotary_bwd_, "gradient of rotary_fwd");
+  m.def("qkv_rotary", &qkv_rotary_, "rotary_fwd with its gradient");
   m.def("kv4_reset", &kv4_reset, "zero the attention's arrival counters after a device error");
   m.def("load_tokens", &load_tokens_, "token state (seen bits, generated counts) of admitted requests");
   m.def("apply_logit_controls", &apply_logit_controls_, "penalties, biases and token masks on logits");

@@ -25,11 +25,16 @@ struct RotaryCache {
 void rotary_fwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, const uint64_t* turns, float factor,
                 const bf16* qn, const bf16* kn, float eps, bf16* q, bf16* k, bf16* v, RotaryCache cache,
                 cudaStream_t st);
-// gq, gk, gv [T, H, hd] to gqkv [T, (Hq + 2 Hkv) hd]; with norms, gqn and gkn [hd] fp32 get their gradients added and
-// ``part`` holds rotary_part_floats() floats.
+// Where the gradient of a norm's weights goes: added to fp32, or written in bf16.
+struct RotaryWeightGrad {
+  float* add;
+  bf16* out;
+};
+// gq, gk, gv [T, H, hd] to gqkv [T, (Hq + 2 Hkv) hd]; with norms, the weights' gradients to wq and wk, and ``part`` holds
+// rotary_part_floats() floats.
 void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, const uint64_t* turns, float factor,
                 const bf16* qn, const bf16* kn, float eps, const bf16* gq, const bf16* gk, const bf16* gv, bf16* gqkv,
-                float* gqn, float* gkn, float* part, cudaStream_t st);
+                RotaryWeightGrad wq, RotaryWeightGrad wk, float* part, cudaStream_t st);
 int64_t rotary_part_floats(RotaryShape s);
 
 }  // namespace meshy

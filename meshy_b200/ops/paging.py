@@ -16,7 +16,7 @@ import torch
 
 from . import reference as ref
 from ._ext import ext
-from .checks import check_range
+from .checks import check_range, enabled
 
 
 class TokenMaps(NamedTuple):
@@ -40,14 +40,15 @@ def assign_pages(block_table: torch.Tensor, rows: torch.Tensor, have: torch.Tens
     """Deal ``pages [P]`` out in order: row ``rows[i]`` of ``block_table [R, M]`` gets the next ``need[i] - have[i]`` (none
     below zero) at columns ``have[i], ..``. All int32; ``rows`` distinct. What falls outside the table is not written,
     pages that no row needs stay out, and columns that the pages do not reach keep what they hold."""
-    _check(block_table, {"rows": rows, "have": have, "need": need})
-    if pages.dtype != torch.int32 or pages.dim() != 1:
-        raise ValueError(f"pages must be int32 [P], got {pages.dtype} {list(pages.shape)}")
-    check_range("block-table rows", rows, 0, block_table.shape[0], skip_negative=True)
-    check_range("block-table columns", need, 0, block_table.shape[1] + 1)
+    if enabled():
+        check_range("block-table rows", rows, 0, block_table.shape[0], skip_negative=True)
+        check_range("block-table columns", need, 0, block_table.shape[1] + 1)
     if block_table.is_cuda:
         ext().assign_pages(block_table, rows, have, need, pages)
         return
+    _check(block_table, {"rows": rows, "have": have, "need": need})
+    if pages.dtype != torch.int32 or pages.dim() != 1:
+        raise ValueError(f"pages must be int32 [P], got {pages.dtype} {list(pages.shape)}")
     ref.assign_pages(block_table, rows, have, need, pages)
 
 
@@ -57,12 +58,13 @@ def token_maps(block_table: torch.Tensor, rows: torch.Tensor, start: torch.Tenso
     zero), packed row after row. ``total``: entries of the result, at least the lengths' sum unless the tokens behind are
     not wanted; entries behind the last token have position 0 and slot -1, which the cache writes skip. A token whose row
     or page lies outside the table, or whose page id is negative, has slot -1 too."""
+    if enabled():
+        check_range("block-table rows", rows, 0, block_table.shape[0], skip_negative=True)
+    if block_table.is_cuda:
+        return TokenMaps(*ext().token_maps(block_table, rows, start, lens, int(total), int(page_size)))
     _check(block_table, {"rows": rows, "start": start, "lens": lens})
     if total < 0 or page_size <= 0:
         raise ValueError(f"total must not be negative and page_size positive, got {total} and {page_size}")
-    check_range("block-table rows", rows, 0, block_table.shape[0], skip_negative=True)
-    if block_table.is_cuda:
-        return TokenMaps(*ext().token_maps(block_table, rows, start, lens, int(total), int(page_size)))
     return TokenMaps(*ref.token_maps(block_table, rows, start, lens, int(total), int(page_size)))
 
 

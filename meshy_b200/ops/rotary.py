@@ -95,6 +95,8 @@ class Rope:
     rotary_dim: int | None = None
     interleaved: bool = False
     scaling: RopeScaling | Mapping[str, Any] | None = None
+    #: what the turned channels are multiplied by
+    factor: float = field(init=False, compare=False)
     _tables: dict = field(default_factory=dict, init=False, repr=False, compare=False)
 
     def __post_init__(self):
@@ -106,7 +108,11 @@ class Rope:
         if not (math.isfinite(self.theta) and self.theta > 1.0):
             raise ValueError(f"rope: theta must be finite and above 1, got {self.theta}")
         object.__setattr__(self, "rotary_dim", rot)
-        object.__setattr__(self, "scaling", RopeScaling.of(self.scaling))
+        s = RopeScaling.of(self.scaling)
+        object.__setattr__(self, "scaling", s)
+        yarn = s is not None and s.rope_type == "yarn"
+        factor = (s.attention_factor or 0.1 * math.log(s.factor) + 1.0) if yarn else 1.0
+        object.__setattr__(self, "factor", factor)
 
     def frequencies(self) -> list[float]:
         """Radians per position of each of the ``rotary_dim / 2`` pairs."""
@@ -129,19 +135,11 @@ class Rope:
             keep = [1 - (i - lo) / max(hi - lo, 1e-3) for i in range(rot // 2)]
         return [x / s.factor + min(max(k, 0.0), 1.0) * (x - x / s.factor) for x, k in zip(f, keep)]
 
-    @property
-    def factor(self) -> float:
-        """What the turned channels are multiplied by."""
-        s = self.scaling
-        if s is None or s.rope_type != "yarn":
-            return 1.0
-        return s.attention_factor if s.attention_factor is not None else 0.1 * math.log(s.factor) + 1.0
-
     def turns(self, device) -> torch.Tensor:
         """``[rotary_dim / 2]`` int64: turns per position times 2^64, modulo 2^64. Made once per device."""
-        device = torch.device(device)
         t = self._tables.get(device)
         if t is None:
+            device = torch.device(device)
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("rope: make one call on this device before a CUDA graph capture (it uploads a table)")
             words = [round(Fraction(f) / _TWO_PI * (1 << 64)) % (1 << 64) for f in self.frequencies()]
@@ -155,31 +153,6 @@ def make_rope(head_dim: int, theta: float, rotary_dim: int | None, interleaved: 
               scaling: RopeScaling | None) -> Rope:
     """One :class:`Rope` (and one table per device) for all that ask for the same."""
     return Rope(head_dim, theta, rotary_dim, interleaved, scaling)
-
-
-class _QKVRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, positions, qn, kn, rope, n_heads, n_kv, eps):
-        turns = rope.turns(qkv.device)
-        q, k, v = ext().rotary_fwd(qkv, positions, turns, rope.factor, rope.interleaved, qn, kn, n_heads, n_kv,
-                                   rope.head_dim, eps, None, None, None, True)
-        ctx.save_for_backward(qkv, positions, qn, kn)
-        ctx.meta = (rope, turns, eps)
-        return q, k, v
-
-    @staticmethod
-    def backward(ctx, gq, gk, gv):
-        qkv, positions, qn, kn = ctx.saved_tensors
-        rope, turns, eps = ctx.meta
-        acc = [None, None]
-        if qn is not None:
-            acc = [_acc_main_grad(w) for w in (qn, kn)]
-            acc = [torch.zeros(w.shape, dtype=torch.float32, device=w.device) if a is None else a
-                   for w, a in zip((qn, kn), acc)]
-        gqkv = ext().rotary_bwd(qkv, positions, turns, rope.factor, rope.interleaved, qn, kn, gq.contiguous(),
-                                gk.contiguous(), gv.contiguous(), *acc, eps)
-        grads = [None if w is None or _acc_main_grad(w) is not None else a.to(w.dtype) for w, a in zip((qn, kn), acc)]
-        return gqkv, None, *grads, None, None, None, None
 
 
 def _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm):
@@ -197,9 +170,11 @@ def qkv_rotary(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, n_heads: 
     RMS-normed with ``q_norm`` / ``k_norm [hd]`` where given, and turned. In fp32 between reading and writing, rounded
     once. Differentiable in ``qkv`` and the norms' weights (into their ``main_grad`` where they have one); the weights'
     sums have a fixed order."""
-    _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)
     if native(qkv):
-        return _QKVRotary.apply(qkv, positions, q_norm, k_norm, rope, n_heads, n_kv, float(eps))
+        acc = (None, None) if q_norm is None else (_acc_main_grad(q_norm), _acc_main_grad(k_norm))
+        return ext().qkv_rotary(qkv, positions, rope.turns(qkv.device), rope.factor, rope.interleaved, q_norm, k_norm,
+                                n_heads, n_kv, rope.head_dim, eps, *acc)
+    _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)
     return ref.qkv_rotary(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm, eps)
 
 
@@ -207,13 +182,13 @@ def qkv_rotary_to_cache(qkv, positions, rope: Rope, n_heads: int, n_kv: int, q_n
                         slot_mapping, *, keep_kv: bool = False):
     """:func:`qkv_rotary` with K and V written into the paged caches ``[pages, Hkv, page, hd]`` at ``slot_mapping [T]``
     int64 (slots outside the cache are skipped), without gradient. Returns ``q`` and, with ``keep_kv``, ``k, v``."""
-    _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)
     check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2], skip_negative=True)
     if native(qkv):
         return ext().rotary_fwd(qkv, positions, rope.turns(qkv.device), rope.factor, rope.interleaved, q_norm, k_norm,
                                 n_heads, n_kv, rope.head_dim, float(eps), k_cache, v_cache, slot_mapping, keep_kv)
     from .decode import kv_write
 
+    _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)
     q, k, v = ref.qkv_rotary(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm, eps)
     ok = (slot_mapping >= 0) & (slot_mapping < k_cache.shape[0] * k_cache.shape[2])
     kv_write(k[ok], v[ok], k_cache, v_cache, slot_mapping[ok])
