@@ -23,12 +23,8 @@
 // 2^16 times as far.) Scales below 2^-24, the smallest there is, count as that, so that p stays below 2^39; sums, the
 // normaliser and the bases' part stay in 32 bits.
 //
-// Work split: the (row, KV head, up to 8 query heads) segments are laid end to end in units of 32 tokens (64 at head
-// width 64: the same bytes, and enough of them under way to hide the memory's latency) and every CTA, one per SM, takes
-// an equal share of the sum, whatever the lengths, a change of segments counted as some units: they are read on the
-// device, so a captured graph follows them. Within a CTA, unit i belongs to warp i mod 8. A segment that spans CTAs
-// leaves partial sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and
-// results do not depend on timing.
+// Work split (kv_split.cuh): units of 32 tokens, 64 at head width 64 (the same bytes, and enough of them under way to hide
+// the memory's latency); one CTA per SM.
 //
 // A unit lies in one page, or, where the page is not a multiple of it, in pieces of 16 or 32 tokens whose page ids
 // neighbouring lanes look up (8 rows of 131072 tokens: 68 us with pages of 16, 65 with pages of 64; units of 16 tokens
@@ -53,22 +49,28 @@
 
 #include <cuda_runtime.h>
 
-#include "../include/sm100.cuh"
+#include "../include/kv_split.cuh"
 #include "kv4.h"
 
 namespace meshy {
 
 namespace {
 
+using namespace kvsplit;
+
 constexpr int kWarps = 8;                      // that compute
 constexpr int kHelpers = 4;
 constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = 16;                       // tokens of a tile
-constexpr int kHeads = 8;                      // query heads of a segment
 constexpr int kSlots = 3;                      // segments whose fragments or states are held
-constexpr uint32_t kWholeUnits = 24;           // units of equal segments that a CTA takes whole
-constexpr int kPad = 16;                        // units that a change of segments costs
-constexpr int kJoinSteps = 3;                  // steps of a warp that a join is worth
+// Equal segments up to 24 units are taken whole (one row of 700 tokens 9.0 us; more CTAs, with a join, 9.9; 16 rows of up
+// to 1400 tokens 11.2 us where unequal ones get a step of every warp, with up to 24 units 14.9). The number of CTAs goes
+// with the root of the work (the root itself took 11.5 and 15.3 us on one row of 8192 and 32768 tokens, twice as many 11.9
+// and 15.8, four times 16.4 on the latter). A change of segments counts as 16 units (64 rows of up to 8192 tokens 29.0 us,
+// with 8 29.9, with none 35.2; 200 rows of about 800 at head width 64 44.4, 45.5, 48.9; 33 rows of up to 4000 15.5, 16.2,
+// 21.5); equal segments are cut alike if that costs fewer than 3 steps (4 rows of 16384 tokens 14.9 us instead of 17.8, 64
+// of 4096 22.6 instead of 26.1).
+constexpr Rules kRules{24, 16, 3};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 11.f;                 // log2 of the largest p a' right after the reference moved
 constexpr float kLimit = 32768.f;              // how far later ones may go
@@ -93,88 +95,15 @@ struct Cfg {
   static constexpr int PART = HD + 4;                    // floats of a head in the workspace: sums, maximum, normaliser
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {  // zeros where it is not
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t* d, uint32_t p) {
-  if constexpr (N == 4)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(p));
-  else if constexpr (N == 2)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(p));
-  else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(d[0]) : "r"(p));
-}
-
-__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// the same with a zero accumulator
-__device__ __forceinline__ void mma_f16_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                              uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
-
 __device__ __forceinline__ void helper_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kHelpers) : "memory"); }
 
-__device__ __forceinline__ float max_over_rows(float v) {  // over the lanes that share lane % 4
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float sum_over_rows(float v) {
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-struct Args {
+struct Args : Rows {
   const bf16* q;
   int64_t qs, qh;
   KV4View c;
   const int* bt;
   int64_t bt_stride;
-  int max_pages;
-  const int* seq_lens;
-  int B, Hq, rep, blocks;  // blocks: groups of kHeads query heads per KV head
+  int Hq, rep, blocks;  // blocks: groups of kHeads query heads per KV head
   int ppp, page_pieces;    // pieces of a page, of a page of all heads
   float scale;
   bf16* out;
@@ -183,67 +112,10 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ int tokens_of(const Args& a, int b) {
-  const int64_t cap = (int64_t)a.max_pages * a.c.page;
-  const int n = a.seq_lens[b];
-  return n <= 0 ? 0 : (int)min((int64_t)n, cap);
-}
-template <int UTOK>
-__device__ __forceinline__ uint32_t units_of(int n) {  // an empty row has one too, which writes its zeros
-  return max(1, (n + UTOK - 1) / UTOK);
-}
-
-// A CTA's walk over its share of the units: segment (b, h), which starts at unit ``begin`` of the sum and of whose U
-// units (the last ``pad`` of them empty) the share has [first, last); ``left`` units of the share remain from ``first``
-// on.
-template <int UTOK>
-struct Walk {
-  int b, h, n, U, first, last, left;
-  uint32_t begin;
-  __device__ __forceinline__ bool next(const Args& a, int pad) {
-    left -= last - first;
-    if (left <= 0) return false;
-    first = 0;
-    begin += U;
-    if (++h == a.c.Hkv * a.blocks) {
-      h = 0;
-      ++b;
-      n = tokens_of(a, b);
-      U = units_of<UTOK>(n) + pad;
-    }
-    last = min(U, left);
-    return true;
-  }
-  __device__ __forceinline__ bool more() const { return left > last - first; }
-  __device__ __forceinline__ int end() const { return min(last, (n + UTOK - 1) / UTOK); }  // of the units with tokens
-  __device__ __forceinline__ bool whole() const { return first == 0 && last >= (int)units_of<UTOK>(n); }
-  __device__ __forceinline__ int first_of(int warp) const { return first + ((warp - (int)begin - first) & (kWarps - 1)); }
-};
-
-// CTA c of n has units [begin(c), begin(c + 1)): total / n each, and the rest spread evenly (so that equal segments are
-// cut alike).
-struct Shares {
-  uint32_t total, n, per, more;
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + c * more / n; }
-  __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
-    uint32_t c = min(n - 1, (uint32_t)((float)unit / (float)total * (float)n));
-    while (c + 1 < n && begin(c + 1) <= unit) ++c;
-    while (begin(c) > unit) --c;
-    return c;
-  }
-};
-
-// A segment (b, h) that the CTA has a piece of: its first unit and its units; then the CTAs that share it.
-struct Piece {
-  int b, h;
-  uint32_t first, n;
-  bool last;  // this CTA arrived last
-};
-
 template <int HD, int NT, int NP>
 __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   using C = Cfg<HD, NT, NP>;
-  using W = Walk<C::UTOK>;
+  using W = Walk<C::UTOK, kWarps>;
   constexpr int G = HD / 64;
   constexpr int KW = HD / 32;  // K words a lane takes of a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -252,10 +124,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   __shared__ uint64_t ready[kSlots], done[kSlots];  // fragments are there and the states free; the states are there
   __shared__ float weight[kHeads][kWarps], total_max[kHeads], total_sum[kHeads];
   __shared__ Piece s_piece[2];
-  __shared__ uint32_t scan[kWarps + kHelpers], s_begin, s_row0;
-  __shared__ int s_row, s_pieces, s_abort, s_ok;
+  __shared__ PlanShared<kThreads> s_plan;
+  __shared__ int s_pieces, s_abort, s_ok;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const uint32_t per_row = a.c.Hkv * a.blocks;  // segments of a row
   volatile int* abort_flag = &s_abort;
 
   if (tid == 0) {
@@ -270,75 +141,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   pdl_wait();
   pdl_trigger();
 
-  // all units (row by row), this CTA's share of them and the row it starts in
-  uint32_t total = 0, mine = 0, before = 0;
-  auto sum_rows = [&](int b0) {  // the units of rows b0 + tid, of the rows before it, and of all up to this block of rows
-    mine = b0 + tid < a.B ? units_of<C::UTOK>(tokens_of(a, b0 + tid)) * per_row : 0;
-    uint32_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) scan[warp] = incl;
-    if (b0 == 0 && tid == 0) s_row0 = mine;
-    __syncthreads();
-    before = total + incl - mine;
-#pragma unroll
-    for (int w = 0; w < kWarps + kHelpers; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-  };
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) sum_rows(b0);
-  // A CTA per segment where that makes a few steps of every warp: for equal segments up to 24 units (one row of 700
-  // tokens 9.0 us; more CTAs, with a join, 9.9), one step for others, whose shares are cut and joined anyway (16 rows
-  // of up to 1400 tokens 11.2 us, with up to 24 units 14.9). Else more of them: the steps shrink with their number,
-  // the join grows with it, so the best number goes with the root of the work (the root itself took 11.5 and 15.3 us on
-  // one row of 8192 and 32768 tokens, twice as many 11.9 and 15.8, four times 16.4 on the latter). Equal segments get a
-  // whole number of CTAs each, and are then cut alike, if that costs fewer steps than a join (4 rows of 16384 tokens
-  // 14.9 us instead of 17.8, 64 of 4096 22.6 instead of 26.1).
-  const uint32_t segments = a.B * per_row;
-  const bool equal = total == s_row0 * a.B;  // or as good as that: the cut is right either way
-  uint32_t n_cta = segments;
-  if (total > segments * (equal ? kWholeUnits : kWarps))
-    n_cta = max(segments, min((total + kWarps - 1) / kWarps, (uint32_t)sqrtf((float)total * (float)segments)));
-  n_cta = min(gridDim.x, n_cta);
-  if (equal && n_cta > segments) {
-    const uint32_t even = n_cta - n_cta % segments;
-    if ((float)total / even - (float)total / n_cta <= (float)(kJoinSteps * kWarps)) n_cta = even;
-  }
-  if (blockIdx.x >= n_cta) return;
-  // Where CTAs have several segments, the change from one to the next counts as kPad empty units at a segment's end: a
-  // CTA with more segments gets fewer tokens (64 rows of up to 8192 tokens 29.0 us, with 8 units 29.9, with none 35.2;
-  // 200 rows of about 800 at head width 64 44.4, 45.5, 48.9; 33 rows of up to 4000 15.5, 16.2, 21.5). Where several
-  // CTAs share each of equal segments there is no change.
-  const int pad = equal && n_cta >= 2 * segments ? 0 : kPad;
-  const uint32_t all = total + pad * segments;
-  const Shares shares{all, n_cta, all / n_cta, all % n_cta};
-  const uint32_t at = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
-  if (a.B > kThreads) total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    if (a.B > kThreads) sum_rows(b0);
-    const uint32_t row = before + pad * per_row * (b0 + tid);
-    if (b0 + tid < a.B && at - row < mine + pad * per_row) {
-      s_row = b0 + tid;
-      s_begin = row;
-    }
-    if (total + pad * per_row * min(b0 + kThreads, a.B) > at) break;
-  }
-  __syncthreads();
-  W w0;
-  w0.b = s_row;
-  w0.n = tokens_of(a, w0.b);
-  w0.U = units_of<C::UTOK>(w0.n) + pad;
-  w0.h = (at - s_begin) / w0.U;
-  w0.begin = s_begin + w0.h * w0.U;
-  w0.first = at - w0.begin;
-  w0.left = end - at;
-  w0.last = min(w0.U, w0.first + w0.left);
-  if (w0.first >= w0.U - pad && !w0.next(a, pad)) return;  // nothing of that segment is left
+  const auto plan = make_plan<C::UTOK, kWarps, kThreads>(a, s_plan, kRules);
+  if (!plan.work) return;
+  const W w0 = plan.w;
+  const int pad = plan.pad;
   const float sl2 = a.scale * kLog2e;
 
   if (warp >= kWarps) {
@@ -468,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
         }
       }
       if (!whole) {  // at most the first and the last segment of the share
-        if (ht == 0) s_piece[pieces] = {w.b, w.h, w.begin, (uint32_t)(w.U - pad), false};
+        if (ht == 0) s_piece[pieces] = piece_of(w, pad, plan.shares);
         ++pieces;
       }
       if (!w.more()) break;
@@ -805,67 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     copies_wait<0>();
   }
 
-  // The last CTA to arrive at a segment joins its pieces; arrivals wait until the share is done, so that nothing else
-  // waits for their round trip.
-  __syncthreads();
+  __syncthreads();  // (arrivals wait until the share is done, so that nothing else waits for their round trip)
   const int pieces = s_pieces;
-  if (pieces == 0) return;
-  if (tid < pieces) {
-    Piece& x = s_piece[tid];
-    const uint32_t c0 = shares.owner(x.first), np = shares.owner(x.first + x.n - 1) - c0 + 1;
-    x.first = c0;
-    x.n = np;
-    unsigned* ctr = a.arrived + (int64_t)x.b * per_row + x.h;
-    unsigned old;
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(ctr) : "memory");
-    x.last = old == np - 1;
-    if (x.last) *ctr = 0u;
-  }
-  __syncthreads();
-  for (int i = tid; i < pieces * kHeads * (HD / 4); i += kThreads) {
-    const Piece& x = s_piece[i / (kHeads * (HD / 4))];
-    const int h = i / (HD / 4) % kHeads, ch = 4 * (i % (HD / 4)), hk = x.h / a.blocks, h0 = (x.h % a.blocks) * kHeads;
-    if (!x.last || h0 + h >= a.rep) continue;
-    const float* p0 = a.part + ((int64_t)x.first * 2 * kHeads + h) * C::PART;
-    const int np = x.n;
-    float M = -INFINITY, L = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 16;
-    for (int c0 = 0; c0 < np; c0 += kBatch) {
-      float4 v[kBatch];
-      float2 ml[kBatch];
-      float Mn = M;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int c = c0 + k;
-        ml[k] = make_float2(-INFINITY, 0.f);
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < np) {
-          const float* pp = p0 + (2 * c + (c == 0 ? 1 : 0)) * kHeads * C::PART;
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(pp + HD));
-          v[k] = __ldcg(reinterpret_cast<const float4*>(pp + ch));
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) Mn = fmaxf(Mn, ml[k].x);
-      const float keep = M == -INFINITY ? 0.f : ex2(M - Mn);
-      L *= keep;
-      y.x *= keep, y.y *= keep, y.z *= keep, y.w *= keep;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float e = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - Mn);
-        L = fmaf(ml[k].y, e, L);
-        y.x = fmaf(v[k].x, e, y.x);
-        y.y = fmaf(v[k].y, e, y.y);
-        y.z = fmaf(v[k].z, e, y.z);
-        y.w = fmaf(v[k].w, e, y.w);
-      }
-      M = Mn;
-    }
-    const float e = L == 0.f ? 0.f : 1.f / L;
-    *reinterpret_cast<uint2*>(a.out + ((int64_t)x.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
-        make_uint2(pack_bf16x2(y.x * e, y.y * e), pack_bf16x2(y.z * e, y.w * e));
-  }
+  if (pieces) join_pieces<HD, kThreads>(a, s_piece, pieces, a.part, a.arrived, a.blocks, a.rep, a.Hq, a.out);
 }
 
 int sm_count() {
@@ -883,7 +631,7 @@ void launch(Args a, cudaStream_t st) {
   a.page_pieces = a.c.Hkv * a.ppp;
   // pieces are counted in 32 bits, in the cache and over the rows
   MESHY_CHECK(a.c.n_pages * a.page_pieces < (1LL << 32) - 1, "paged_attention_kv4: cache too large");
-  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.ppp) + kPad) < (1LL << 31),
+  MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.ppp) + kRules.pad) < (1LL << 31),
               "paged_attention_kv4: rows * heads * table width too large");
   static bool set[64] = {};
   int dev = 0;
@@ -907,8 +655,11 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
   max_pages = std::min(max_pages, (INT_MAX - 63) / c.page);  // lengths are rounded up to units in 32 bits
-  const Args a{q, qs, qh,  c,   bt,    bt_stride, max_pages, seq_lens, B, Hq, rep, (rep + kHeads - 1) / kHeads,
-               0, 0,  scale, out, part, arrived, err};
+  Args a;
+  const int blocks = (rep + kHeads - 1) / kHeads;
+  static_cast<Rows&>(a) = {seq_lens, B, max_pages, c.page, c.Hkv * blocks};
+  a.q = q, a.qs = qs, a.qh = qh, a.c = c, a.bt = bt, a.bt_stride = bt_stride, a.Hq = Hq, a.rep = rep, a.blocks = blocks;
+  a.scale = scale, a.out = out, a.part = part, a.arrived = arrived, a.err = err;
   if (c.hd == 128)
     c.page % 32 == 0 ? launch<128, 2, 1>(a, st) : launch<128, 2, 2>(a, st);
   else
