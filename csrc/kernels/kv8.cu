@@ -173,7 +173,7 @@ __device__ __forceinline__ bool begins(const WriteArgs& a, int64_t t, int64_t bl
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv8_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) kv8_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   pdl_wait();
   pdl_trigger();
@@ -238,8 +238,10 @@ void kv8_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
                int T, KV8View c, bf16* ko, bf16* vo, cudaStream_t st) {
   if (T == 0) return;
   const int items = 2 * c.Hkv, groups = (items + kWarps - 1) / kWarps;
+  // Few rows: a CTA to each, or more, for the latency; many: 16 rows to a CTA, whose warps take the heads of their one or
+  // two blocks (32768 tokens of 8 heads: 62.5 us, with 8 rows 65.9, with 32 65.3).
   const bool few = (int64_t)T * items <= 8192;
-  const int tile = few ? 1 : 32;
+  const int tile = few ? 1 : 16;
   const WriteArgs a{{k, v}, {ks, vs}, {kh, vh}, slots, T, tile, c, FastDiv(c.page), {ko, vo}};
   const dim3 grid((T + tile - 1) / tile, few ? groups : 1);
   launch_pdl(c.hd == 128 ? kv8_write_kernel<128> : kv8_write_kernel<64>, grid, dim3(kThreads), 0, st, a);

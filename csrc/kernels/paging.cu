@@ -1,9 +1,10 @@
 // Block tables and slot maps from request lengths.
 //
 // Both kernels deal a packed list (pages, tokens) out to rows: entry j belongs to the row i with
-// sum(c[:i]) <= j < sum(c[:i + 1]), c the rows' counts. Every CTA scans the counts itself, 1024 rows at a time, and
+// sum(c[:i]) <= j < sum(c[:i + 1]), c the rows' counts. Every CTA scans the counts itself, 256 rows at a time, and
 // looks its own entries up in the scanned block by bisection: a few hundred rows are read in the time of one load from
-// L2, so one launch does what a scan and a second kernel would.
+// L2, so one launch does what a scan and a second kernel would. Latency bounds both: lengths, the scan, the bisection, the
+// table's entry.
 #include <climits>
 
 #include <cuda_runtime.h>
@@ -16,24 +17,30 @@ namespace meshy {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 1024;  // scanned at a time
+constexpr int kRows = 256;  // scanned at a time (1024: 11.0 us for the tables and maps of 1.1 M tokens of 256 rows, here 8.9)
 constexpr int kPer = kRows / kThreads;
 
 struct Scan {
   int64_t ends[kRows + 1];  // ends[i]: entries of the rows before row i of the block, and of all before the block
   int64_t sums[kThreads / 32];
+  int rows[kRows], first[kRows];  // the table's row, and the page or token that the row's entries begin with
 };
 
-// Counts of rows b0 .. b0 + kRows (0 behind n) into s.ends, from ``carry`` on; returns the new carry.
-template <class Count>
-__device__ __forceinline__ int64_t scan_rows(Scan& s, int b0, int n, int64_t carry, Count count) {
+struct Row {
+  int count, row, first;
+};
+
+// Rows b0 .. b0 + kRows (no entries behind n) into s, the ends from ``carry`` on; returns the new carry.
+template <class Load>
+__device__ __forceinline__ int64_t scan_rows(Scan& s, int b0, int n, int64_t carry, Load load) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  int64_t c[kPer], mine = 0;
+  Row r[kPer];
+  int64_t mine = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int row = b0 + tid * kPer + i;
-    c[i] = row < n ? (int64_t)count(row) : 0;
-    mine += c[i];
+    r[i] = row < n ? load(row) : Row{0, 0, 0};
+    mine += r[i].count;
   }
   int64_t incl = mine;
 #pragma unroll
@@ -53,7 +60,9 @@ __device__ __forceinline__ int64_t scan_rows(Scan& s, int b0, int n, int64_t car
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     s.ends[tid * kPer + i] = at;
-    at += c[i];
+    s.rows[tid * kPer + i] = r[i].row;
+    s.first[tid * kPer + i] = r[i].first;
+    at += r[i].count;
   }
   if (tid == kThreads - 1) s.ends[kRows] = carry;
   __syncthreads();
@@ -80,11 +89,14 @@ __global__ void __launch_bounds__(kThreads)
   int64_t carry = 0;
   for (int b0 = 0; b0 < n && carry < last; b0 += kRows) {
     const int64_t begin = carry;
-    carry = scan_rows(s, b0, n, carry, [&](int r) { return max((int64_t)0, (int64_t)need[r] - max(have[r], 0)); });
+    carry = scan_rows(s, b0, n, carry, [&](int r) {
+      const int h = max(have[r], 0);
+      return Row{max(need[r], h) - h, rows[r], h};
+    });
     if (j >= begin && j < carry && j < P) {
       const int i = find(s, j);
-      const int row = rows[b0 + i];
-      const int64_t col = max(have[b0 + i], 0) + (j - s.ends[i]);
+      const int row = s.rows[i];
+      const int64_t col = s.first[i] + (j - s.ends[i]);
       if (row >= 0 && row < R && col < M) bt[row * bt_stride + col] = pages[j];
     }
   }
@@ -106,7 +118,7 @@ __global__ void __launch_bounds__(kThreads)
   int64_t carry = 0;
   for (int b0 = 0; b0 < n && (carry < last || blockIdx.x == 0); b0 += kRows) {
     const int64_t begin = carry;
-    carry = scan_rows(s, b0, n, carry, [&](int r) { return max(lens[r], 0); });
+    carry = scan_rows(s, b0, n, carry, [&](int r) { return Row{max(lens[r], 0), rows[r], start[r]}; });
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= min(kRows, n - b0); i += kThreads) cu[b0 + i] = (int)min(s.ends[i], (int64_t)INT_MAX);
     int i = -1, row = 0, col = -1, pg = -1;
@@ -118,8 +130,8 @@ __global__ void __launch_bounds__(kThreads)
       if (i < 0 || t >= end) {
         i = find(s, t);
         end = s.ends[i + 1];
-        row = rows[b0 + i];
-        off = start[b0 + i] - s.ends[i];
+        row = s.rows[i];
+        off = s.first[i] - s.ends[i];
         col = -1;
       }
       const int64_t p = off + t;
