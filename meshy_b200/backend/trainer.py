@@ -32,7 +32,7 @@ import torch
 import torch.distributed as dist
 
 from ..config import TrainerConfig, TrainerParamsConfig
-from ..models import build_model, get_model_args
+from ..models import build_model, get_model_args, with_hf_config
 from ..utils.timer import TimerStats
 from .batch import ADVANTAGE_TOKENS, Batch, build_micro_batch
 from .flat import FlatAdamW, FlatParams, lr_lambda
@@ -77,7 +77,7 @@ class PPOTrainer:
 
             self.cp = CpSharder(cp_group)
         self.loss_group = loss_group if loss_group is not None else dp_group
-        self.model_args = get_model_args(config.model_name, config.model_flavor)
+        self.model_args = with_hf_config(get_model_args(config.model_name, config.model_flavor), config.model_overrides)
         cdt = torch.bfloat16 if (self.device.type == "cuda" and config.dtype == "bfloat16") else torch.float32
         self.compute_dtype = cdt
         if model is None:

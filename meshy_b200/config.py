@@ -113,6 +113,10 @@ class TrainerConfig:
     compile_backend: str = "none"
     activation_checkpoint_mode: Literal["selective", "full", "memory_budget", "none"] = "selective"
     attn_backend: Literal["sdpa", "varlen"] = "sdpa"
+    # position settings that differ from the flavor's, under HF's config names (rope_theta, rope_scaling,
+    # partial_rotary_factor, max_position_embeddings); an inference service takes the same as its
+    # json_model_override_args
+    model_overrides: dict = field(default_factory=dict)
 
     def __post_init__(self) -> None:
         if self.attn_backend not in ("sdpa", "varlen"):

@@ -25,7 +25,7 @@ from ..backend.critic.metrics import StreamingGauges, critic_diagnostics
 from ..backend.critic.trainer import CriticTrainer
 from ..backend.plan import snake_deal
 from ..config import GlobalCheckpointConfig
-from ..models import get_model_args
+from ..models import get_model_args, with_hf_config
 from .spmd import SpmdEngine
 
 log = logging.getLogger(__name__)
@@ -47,7 +47,7 @@ class CriticSpmdEngine(SpmdEngine):
         super().setup()
         c = self.cfg
         tc = c.trainer_config
-        args = get_model_args(tc.model_name, tc.model_flavor)
+        args = with_hf_config(get_model_args(tc.model_name, tc.model_flavor), tc.model_overrides)
         groups = {"dp_group": self.compute_group if self.world_size > 1 else None}
         cp = max(1, int(getattr(tc, "cp_degree", 1)))
         if cp > 1 and self.world_size > 1:

@@ -18,7 +18,7 @@ import torch.distributed as dist
 
 from ..backend.plan import snake_deal
 from ..backend.topk_loss import teacher_topk
-from ..models import build_model, get_model_args
+from ..models import build_model, get_model_args, with_hf_config
 from .spmd import SpmdEngine
 from .trainer import TrainerEngine
 
@@ -52,7 +52,7 @@ class OPDTeacherEngine(SpmdEngine):
     def setup(self) -> None:
         super().setup()
         tc = self.cfg.trainer_config
-        args = get_model_args(tc.model_name, tc.model_flavor)
+        args = with_hf_config(get_model_args(tc.model_name, tc.model_flavor), tc.model_overrides)
         dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.model = build_model(args, device=self.device, dtype=dtype).eval()
         for p in self.model.parameters():

@@ -17,11 +17,18 @@ instance, mirroring the reference's torchtitan model specs:
 RoPE convention: every family uses the rotate-half pairing (dims ``i`` and
 ``i + head_dim/2``), which is the HF checkpoint convention, so HF weights load
 without the row permutation torchtitan's interleaved complex RoPE needs.
+Checkpoints of these families that were stretched to longer contexts, turn part
+of a head or pair neighbouring channels are described by ``rope_scaling``,
+``rope_dim`` and ``rope_interleaved`` (see :mod:`..ops.rotary`).
 """
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field, replace
+from dataclasses import dataclass, field, fields, replace
+from typing import TYPE_CHECKING, Any, Mapping
+
+if TYPE_CHECKING:
+    from ..ops.rotary import Rope, RopeScaling
 
 
 @dataclass(frozen=True)
@@ -59,6 +66,28 @@ class ModelArgs:
     #: matching up rows, so one GEMM output tile carries both halves of every
     #: SwiGLU pair and the activation runs in the GEMM epilogue.
     swiglu_block: int = 64
+    #: frequencies stretched for long contexts (a mapping with HF's ``rope_scaling`` keys is taken too)
+    rope_scaling: RopeScaling | None = None
+    #: rotated channels of a head, the first ones (``None``: all)
+    rope_dim: int | None = None
+    #: pairs of neighbouring channels instead of halves
+    rope_interleaved: bool = False
+
+    def __post_init__(self):
+        if self.rope_scaling is not None:
+            from ..ops.rotary import RopeScaling
+
+            object.__setattr__(self, "rope_scaling", RopeScaling.of(self.rope_scaling))
+        self.rope  # a head that it does not fit is refused here
+
+    @property
+    def rope(self) -> Rope | None:
+        """The rotary positions, or ``None`` for the plain ones (whole heads by halves, base ``rope_theta``)."""
+        if self.rope_scaling is None and self.rope_dim in (None, self.head_dim) and not self.rope_interleaved:
+            return None
+        from ..ops.rotary import make_rope
+
+        return make_rope(self.head_dim, self.rope_theta, self.rope_dim, self.rope_interleaved, self.rope_scaling)
 
     @property
     def q_dim(self) -> int:
@@ -175,19 +204,50 @@ _REGISTRY: dict[str, dict[str, ModelArgs]] = {
 }
 
 
-def get_model_args(model_name: str, flavor: str, **overrides) -> ModelArgs:
-    """Resolve ``(model_name, flavor)``; ``overrides`` replace fields (tests)."""
+def get_model_args(model_name: str, flavor: str, **overrides: Any) -> ModelArgs:
+    """Resolve ``(model_name, flavor)``; ``overrides`` replace fields (``ValueError`` for one that there is not)."""
     if model_name not in _REGISTRY:
         raise ValueError(f"unknown model {model_name!r}; available: {sorted(_REGISTRY)}")
     flavors = _REGISTRY[model_name]
     if flavor not in flavors:
         raise ValueError(f"unknown {model_name} flavor {flavor!r}; available: {sorted(flavors)}")
     args = flavors[flavor]
+    if unknown := sorted(set(overrides) - {f.name for f in fields(args)}):
+        raise ValueError(f"unknown model fields {unknown}")
     return replace(args, **overrides) if overrides else args
+
+
+def with_hf_config(args: ModelArgs, config: Mapping[str, Any] | None) -> ModelArgs:
+    """``args`` with the position settings of a HF config (or of the part of one that differs): ``rope_theta``,
+    ``rope_scaling`` (or ``rope_parameters``), ``partial_rotary_factor``, ``max_position_embeddings``, and
+    ``rope_interleaved``, which checkpoints of these families leave out. ``ValueError`` for any other key."""
+    c = dict(config or {})
+    fields_ = {}
+    if "rope_parameters" in c:
+        c["rope_scaling"] = c.pop("rope_parameters")
+    if c.get("rope_scaling") is not None:
+        scaling = dict(c["rope_scaling"])
+        for key in ("rope_theta", "partial_rotary_factor"):  # newer configs keep them there
+            if key in scaling:
+                c[key] = scaling.pop(key)
+        c["rope_scaling"] = scaling
+    if "rope_scaling" in c:
+        fields_["rope_scaling"] = c.pop("rope_scaling")
+    if "rope_theta" in c:
+        fields_["rope_theta"] = float(c.pop("rope_theta"))
+    if "partial_rotary_factor" in c:
+        fields_["rope_dim"] = int(args.head_dim * float(c.pop("partial_rotary_factor")))
+    if "rope_interleaved" in c:
+        fields_["rope_interleaved"] = bool(c.pop("rope_interleaved"))
+    if "max_position_embeddings" in c:
+        fields_["max_seq_len"] = int(c.pop("max_position_embeddings"))
+    if c:
+        raise ValueError(f"model overrides: unknown keys {sorted(c)}")
+    return replace(args, **fields_) if fields_ else args
 
 
 def list_models() -> dict[str, list[str]]:
     return {k: sorted(v) for k, v in _REGISTRY.items()}
 
 
-__all__ = ["ModelArgs", "MoEArgs", "get_model_args", "list_models"]
+__all__ = ["ModelArgs", "MoEArgs", "get_model_args", "list_models", "with_hf_config"]

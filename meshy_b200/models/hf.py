@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import json
 import os
+from dataclasses import asdict
 
 import torch
 
@@ -103,6 +104,12 @@ def hf_config(args: ModelArgs) -> dict:
         "max_position_embeddings": args.max_seq_len, "torch_dtype": "bfloat16",
         "meshy_b200": {"model_name": args.name, "flavor": args.flavor},
     }
+    if args.rope_scaling is not None:
+        cfg["rope_scaling"] = {k: v for k, v in asdict(args.rope_scaling).items() if v is not None}
+    if args.rope_dim not in (None, args.head_dim):
+        cfg["partial_rotary_factor"] = args.rope_dim / args.head_dim
+    if args.rope_interleaved:
+        cfg["rope_interleaved"] = True
     if args.moe is not None:
         cfg.update({"num_experts": args.moe.n_experts, "num_experts_per_tok": args.moe.top_k,
                     "moe_intermediate_size": args.moe.expert_ffn_dim, "norm_topk_prob": args.moe.route_norm})

@@ -11,7 +11,7 @@ state move between the two layouts.
 
 Llama-family models (``llama3``, ``minicpm5``): torchtitan applies RoPE to interleaved (even, odd) pairs,
 HF and this package to the two halves of each head, so ``wq`` / ``wk`` rows are permuted on the way
-(the same permutation the reference's MiniCPM5 adapter applies).
+(the same permutation the reference's MiniCPM5 adapter applies), unless the model pairs neighbours itself.
 """
 
 from __future__ import annotations
@@ -40,7 +40,7 @@ def _from_interleaved(w: torch.Tensor, n_heads: int) -> torch.Tensor:
 def _split_qkv(args: ModelArgs, t: torch.Tensor):
     q, kv = args.q_dim, args.kv_dim
     wq, wk, wv = t[:q], t[q:q + kv], t[q + kv:]
-    if args.name in _LLAMA_ROPE:
+    if args.name in _LLAMA_ROPE and not args.rope_interleaved:
         wq, wk = _to_interleaved(wq, args.n_heads), _to_interleaved(wk, args.n_kv_heads)
     return wq, wk, wv
 
@@ -85,7 +85,7 @@ def join_pieces(args: ModelArgs, name: str, pieces: list[torch.Tensor]) -> torch
     rest = name.split(".", 2)[2] if name.startswith("layers.") else name
     if rest in ("wqkv", "bqkv"):
         q, k, v = pieces
-        if args.name in _LLAMA_ROPE:
+        if args.name in _LLAMA_ROPE and not args.rope_interleaved:
             q, k = _from_interleaved(q, args.n_heads), _from_interleaved(k, args.n_kv_heads)
         return torch.cat([q, k, v], 0)
     if rest == "w13":

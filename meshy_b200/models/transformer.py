@@ -73,7 +73,7 @@ class Block(nn.Module):
         h = Fx.rmsnorm(x, self.attn_norm, a.norm_eps)
         qkv = Fx.linear(h, self.wqkv, self.bqkv)
         q, k, v = Fx.qkv_rope(qkv, positions, self.q_norm, self.k_norm, a.n_heads, a.n_kv_heads,
-                              a.head_dim, a.rope_theta, a.norm_eps)
+                              a.head_dim, a.rope_theta, a.norm_eps, rope=a.rope)
         o = Fx.flash_attn_varlen(q, k, v, cu_seqlens, max_seqlen)
         x = Fx.linear(o.reshape(T, a.q_dim), self.wo, residual=x)
         h = Fx.rmsnorm(x, self.mlp_norm, a.norm_eps)
@@ -91,7 +91,7 @@ class Block(nn.Module):
         h = copy_to_tp(Fx.rmsnorm(x, self.attn_norm, a.norm_eps), g)
         qkv = Fx.linear(h, self.wqkv, self.bqkv)
         q, k, v = Fx.qkv_rope(qkv, positions, self.q_norm, self.k_norm, a.n_heads, a.n_kv_heads,
-                              a.head_dim, a.rope_theta, a.norm_eps)
+                              a.head_dim, a.rope_theta, a.norm_eps, rope=a.rope)
         o = Fx.flash_attn_varlen(q, k, v, cu_seqlens, max_seqlen)
         x = x + reduce_from_tp(Fx.linear(o.reshape(T, a.n_heads * a.head_dim), self.wo), g)
         h = copy_to_tp(Fx.rmsnorm(x, self.mlp_norm, a.norm_eps), g)

@@ -252,7 +252,12 @@ class _QKVRope(torch.autograd.Function):
         return gqkv, None, gqn, gkn, None, None, None, None, None
 
 
-def qkv_rope(qkv, positions, q_norm, k_norm, n_heads, n_kv, hd, theta, eps):
+def qkv_rope(qkv, positions, q_norm, k_norm, n_heads, n_kv, hd, theta, eps, rope=None):
+    """``rope``: a :class:`.rotary.Rope`, for positions other than whole heads in the half layout at base ``theta``."""
+    if rope is not None:
+        from .rotary import qkv_rotary
+
+        return qkv_rotary(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm, eps)
     if native(qkv):
         return _QKVRope.apply(qkv, positions, q_norm, k_norm, n_heads, n_kv, hd, theta, eps)
     T = qkv.shape[0]

@@ -139,7 +139,8 @@ class Rope:
         """``[rotary_dim / 2]`` int64: turns per position times 2^64, modulo 2^64. Made once per device."""
         t = self._tables.get(device)
         if t is None:
-            device = torch.device(device)
+            if not isinstance(device, torch.device):
+                return self.turns(torch.device(device))
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("rope: make one call on this device before a CUDA graph capture (it uploads a table)")
             words = [round(Fraction(f) / _TWO_PI * (1 << 64)) % (1 << 64) for f in self.frequencies()]

@@ -20,11 +20,13 @@ Execution model:
 
 * weights live in one flat bf16 buffer with the trainer's layout;
 * the KV cache is ``[layers, 2, pages, kv_heads, page, head_dim]``; a host
-  block manager (:mod:`.kv_cache`) hands out pages. With ``kv_dtype="int4"``
-  it is a 4-bit cache per layer (:mod:`..ops.kv4`) that holds 3.55 times the
-  tokens in the same memory; prefill then attends to the values the cache
-  stands for, as decode does;
+  block manager (:mod:`.kv_cache`) hands out pages. With ``kv_dtype="int4"`` or
+  ``"int8"`` it is a quantised cache per layer (:mod:`..ops.kv4`, :mod:`..ops.kv8`)
+  that holds 3.55 or 1.99 times the tokens in the same memory; prefill then
+  attends to the values the cache stands for, as decode does;
 * prefill runs new prompts as one packed varlen forward and writes their KV;
+  block tables and the tokens' positions and slots are made on the device from
+  the prompts' lengths and the pages handed out (:mod:`..ops.paging`);
 * a decode step (embedding → layers → fused LM-head sampler → row advance) is
   captured once per batch-size bucket in a CUDA graph and replayed; rows that
   finish are compacted away every ``sync_every`` steps, the only host↔device
@@ -51,13 +53,50 @@ from ..models.transformer import DecoderLM
 from ..ops import decode as D
 from ..ops import functional as Fx
 from ..ops import kv4 as K4
+from ..ops import kv8 as K8
 from ..ops.controls import LogitControls, check_controls, load_tokens
+from ..ops.paging import assign_pages, token_maps
 from .kv_cache import BlockManager
 
 #: entries of a request's ``logit_bias``
 MAX_LOGIT_BIAS = 300
 
 _BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 128, 160, 192, 224, 256, 320, 384, 448, 512)
+
+
+class _KV4:
+    """The 4-bit cache as the engine uses it."""
+
+    name = "4-bit KV cache"
+    check = staticmethod(K4.check_geometry)
+    from_bytes = staticmethod(K4.kv4_from_bytes)
+    attention = staticmethod(K4.paged_attention_kv4)
+
+    @staticmethod
+    def page_bytes(n_kv: int, page: int, hd: int) -> int:
+        return n_kv * page * K4.row_bytes(hd)
+
+    @staticmethod
+    def write(k, v, cache, slots, keep: bool = False):
+        K4.kv4_write(k, v, cache, slots)
+        return K4.kv4_read(cache, slots, k.dtype) if keep else None
+
+
+class _KV8:
+    """The 8-bit cache as the engine uses it."""
+
+    name = "8-bit KV cache"
+    check = staticmethod(K8.check_geometry)
+    from_bytes = staticmethod(K8.kv8_from_bytes)
+    attention = staticmethod(K8.paged_attention_kv8)
+
+    @staticmethod
+    def page_bytes(n_kv: int, page: int, hd: int) -> int:
+        return n_kv * page // K8.BLOCK * K8.block_bytes(hd)
+
+    @staticmethod
+    def write(k, v, cache, slots, keep: bool = False):
+        return K8.kv8_write(k, v, cache, slots, keep=keep)
 
 
 @dataclass
@@ -123,12 +162,12 @@ class RolloutEngine:
     ):
         from ..backend.flat import Slot, _align, flatten_module
 
-        if kv_dtype not in ("auto", "int4"):
-            raise ValueError(f"kv_dtype must be 'auto' (the model's dtype) or 'int4', got {kv_dtype!r}")
+        if kv_dtype not in ("auto", "int4", "int8"):
+            raise ValueError(f"kv_dtype must be 'auto' (the model's dtype), 'int4' or 'int8', got {kv_dtype!r}")
         self.args = args
-        self.kv4 = kv_dtype == "int4"
-        if self.kv4:
-            K4.check_geometry(args.n_kv_heads, page_size, args.head_dim)
+        self.kvq = {"auto": None, "int4": _KV4, "int8": _KV8}[kv_dtype]  # a quantised cache
+        if self.kvq:
+            self.kvq.check(args.n_kv_heads, page_size, args.head_dim)
         self.device = torch.device(device)
         self.cuda = self.device.type == "cuda"
         self.dtype = torch.bfloat16 if self.cuda else torch.float32
@@ -206,8 +245,8 @@ class RolloutEngine:
         self._init_state()
         self._mega = None
         self._mega_rows = 0
-        self.mega_reason = ("not on CUDA" if not self.cuda else "4-bit KV cache" if self.kv4 else "tensor parallelism")
-        if self.cuda and self.tp_group is None and not self.kv4:
+        self.mega_reason = ("not on CUDA" if not self.cuda else self.kvq.name if self.kvq else "tensor parallelism")
+        if self.cuda and self.tp_group is None and not self.kvq:
             from .mega import MAX_ROWS, MegaDecoder
 
             self.mega_reason = MegaDecoder.reason(self.model, self.page_size)
@@ -218,15 +257,18 @@ class RolloutEngine:
     # ------------------------------------------------------------------ memory
     def _kv_bytes_per_token(self) -> int:
         a = self.local_args
-        return a.n_layers * a.n_kv_heads * K4.row_bytes(a.head_dim) if self.kv4 else a.kv_bytes_per_token(2)
+        if self.kvq:
+            return math.ceil(a.n_layers * self.kvq.page_bytes(a.n_kv_heads, self.page_size, a.head_dim) / self.page_size)
+        return a.kv_bytes_per_token(2)
 
-    def _alloc_kv4(self):
-        """One region of bytes, the layers' caches one after the other in it."""
+    def _alloc_kvq(self):
+        """One region of bytes, the layers' caches one after the other in it, on 16-byte boundaries."""
         a = self.local_args
-        per_layer = self.n_pages * a.n_kv_heads * self.page_size * K4.row_bytes(a.head_dim)
+        per_layer = self.n_pages * self.kvq.page_bytes(a.n_kv_heads, self.page_size, a.head_dim)
+        per_layer = (per_layer + 15) // 16 * 16
         raw = self._kv_region([a.n_layers * per_layer], torch.uint8)
-        self.kv = [K4.kv4_from_bytes(raw[i * per_layer:(i + 1) * per_layer], self.n_pages, a.n_kv_heads, self.page_size,
-                                     a.head_dim) for i in range(a.n_layers)]
+        self.kv = [self.kvq.from_bytes(raw[i * per_layer:(i + 1) * per_layer], self.n_pages, a.n_kv_heads, self.page_size,
+                                       a.head_dim) for i in range(a.n_layers)]
 
     def _kv_region(self, shape, dtype) -> torch.Tensor:
         """Zeroed KV memory: a virtual-memory region on CUDA (the one there is, mapped again)."""
@@ -243,8 +285,8 @@ class RolloutEngine:
         return reg.view(0, list(shape), dtype).zero_()
 
     def _alloc_kv(self):
-        if self.kv4:
-            return self._alloc_kv4()
+        if self.kvq:
+            return self._alloc_kvq()
         a = self.local_args  # this rank's KV heads
         self.kv = self._kv_region([a.n_layers, 2, self.n_pages, a.n_kv_heads, self.page_size, a.head_dim], self.dtype)
 
@@ -510,7 +552,8 @@ class RolloutEngine:
         """Grow page lists so every row can decode ``lookahead`` more tokens."""
         st = self.st
         seq = st["seq_lens"][: len(self.running)].tolist()
-        bt_updates = []
+        grow = []  # rows, their pages so far and from now on; the new pages
+        pages = []
         for i in rows:
             req = self.running[i]
             need_tokens = min(seq[i] + lookahead, len(req.prompt) + req.max_new_tokens)
@@ -519,11 +562,21 @@ class RolloutEngine:
                 new = self.blocks.allocate(need - len(req.pages))
                 if new is None:
                     raise RuntimeError("KV cache exhausted; lower max_running or raise max_total_tokens")
-                start = len(req.pages)
+                grow.append((i, len(req.pages), need))
                 req.pages.extend(new)
-                bt_updates.append((i, start, new))
-        for i, start, new in bt_updates:
-            st["block_table"][i, start:start + len(new)] = torch.tensor(new, dtype=torch.int32, device=self.device)
+                pages.extend(new)
+        if grow:
+            assign_pages(st["block_table"], *self._upload(*zip(*grow), pages))
+
+    def _upload(self, *lists: Sequence[int]) -> list[torch.Tensor]:
+        """int32 vectors on the device, in one copy (each on a 16-byte boundary)."""
+        padded = [list(x) + [0] * (-len(x) % 4) for x in lists]
+        flat = torch.tensor([v for x in padded for v in x], dtype=torch.int32).to(self.device, non_blocking=True)
+        out, at = [], 0
+        for x, p in zip(lists, padded):
+            out.append(flat[at:at + len(x)])
+            at += len(p)
+        return out
 
     # ------------------------------------------------------------------ prefill
     @torch.no_grad()
@@ -532,27 +585,28 @@ class RolloutEngine:
         lens = [len(r.prompt) for r in batch]
         T = sum(lens)
         toks = torch.tensor([t for r in batch for t in r.prompt], dtype=torch.int64)
-        pos = torch.cat([torch.arange(L, dtype=torch.int32) for L in lens])
-        slots = torch.cat([
-            torch.tensor(r.pages, dtype=torch.int64).repeat_interleave(P)[:L] * P + torch.arange(L) % P
-            for r, L in zip(batch, lens)])
-        cu = torch.tensor([0] + list(itertools.accumulate(lens)), dtype=torch.int32)
-        toks, pos, slots, cu = (t.to(dev, non_blocking=True) for t in (toks, pos, slots, cu))
+        toks = toks.to(dev, non_blocking=True)
+        st, base, n = self.st, len(self.running), len(batch)
+        row_ids, have, need, starts, ones, plen, pages = self._upload(
+            range(base, base + n), [0] * n, [len(r.pages) for r in batch], [0] * n, [1] * n, lens,
+            [pg for r in batch for pg in r.pages])
+        st["block_table"][base:base + n] = 0
+        assign_pages(st["block_table"], row_ids, have, need, pages)
+        pos, slots, cu = token_maps(st["block_table"], row_ids, starts, plen, T, P)
         m = self.model
         la = self.local_args
         x = Fx.embedding(toks, m.embed)
         for li, layer in enumerate(m.layers):
             h = Fx.rmsnorm(x, layer.attn_norm, a.norm_eps)
             qkv = Fx.linear(h, layer.wqkv, layer.bqkv)
-            if self.kv4:
+            if self.kvq:
                 q, k, v = Fx.qkv_rope(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads, a.head_dim,
-                                      a.rope_theta, a.norm_eps)
-                K4.kv4_write(k, v, self.kv[li], slots)
-                k, v = K4.kv4_read(self.kv[li], slots, self.dtype)
+                                      a.rope_theta, a.norm_eps, rope=a.rope)
+                k, v = self.kvq.write(k, v, self.kv[li], slots, keep=True)
             else:
                 q, k, v = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
                                               a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1],
-                                              slots, keep_kv=True)
+                                              slots, keep_kv=True, rope=a.rope)
             o = Fx.flash_attn_varlen(q, k, v, cu, max(lens))
             x = self._row_parallel(o.reshape(T, la.q_dim), layer.wo, x)
             h = Fx.rmsnorm(x, layer.mlp_norm, a.norm_eps)
@@ -563,19 +617,15 @@ class RolloutEngine:
         tok, lp = self._sample_rows(hl, batch)
         self.stats["prefill_tokens"] += T
         # append rows
-        st = self.st
-        base = len(self.running)
-        n = len(batch)
         rows = slice(base, base + n)
         max_new = torch.tensor([r.max_new_tokens for r in batch], dtype=torch.int32)
         req_slots = torch.tensor([r.out_slot for r in batch], dtype=torch.int32)
-        plen = torch.tensor(lens, dtype=torch.int32)
         st["req"][rows] = req_slots.to(dev)
         st["max_new"][rows] = max_new.to(dev)
         st["gen"][rows] = 1
         st["tok_in"][rows] = tok
-        st["pos"][rows] = plen.to(dev)
-        st["seq_lens"][rows] = (plen + 1).to(dev)
+        st["pos"][rows] = plen
+        st["seq_lens"][rows] = plen + 1
         rs = req_slots.to(dev).long()
         st["out_tok"][rs, 0] = tok
         st["out_lp"][rs, 0] = lp
@@ -585,12 +635,7 @@ class RolloutEngine:
             hit = torch.isin(tok.cpu(), torch.tensor(self.eos)) & ~ignore
             done = done | hit
         st["done"][rows] = done.to(torch.int32).to(dev)
-        bt = torch.zeros(n, self.max_pages_per_seq, dtype=torch.int32)
-        for j, r in enumerate(batch):
-            bt[j, : len(r.pages)] = torch.tensor(r.pages, dtype=torch.int32)
-        st["block_table"][rows] = bt.to(dev)
-        pg = torch.tensor([r.pages[L // P] for r, L in zip(batch, lens)], dtype=torch.int64)
-        st["slot"][rows] = (pg * P + plen.long() % P).to(dev)
+        st["slot"][rows] = token_maps(st["block_table"], row_ids, plen, ones, n, P).slots
         self.running.extend(batch)
 
     def _mlp(self, layer, h, x):
@@ -700,7 +745,7 @@ class RolloutEngine:
         L = len(m.layers)
         for li, layer in enumerate(m.layers):
             q = None
-            if prep is not None and fuse_rope and not self.kv4:
+            if prep is not None and fuse_rope and not self.kvq and a.rope is None:
                 q = D.qkv_rope_fused(xg[:b], layer.wqkv, layer.bqkv, pos, layer.q_norm, layer.k_norm, a.n_heads,
                                      a.n_kv_heads, a.rope_theta, a.norm_eps, self.kv[li, 0], self.kv[li, 1],
                                      st["slot"][:b], part=prep, d=a.dim)
@@ -710,16 +755,16 @@ class RolloutEngine:
                     qkv = D.linear_norm_scaled(xg[:b], layer.wqkv, layer.bqkv, prep, a.dim, a.norm_eps)
                 if qkv is None:
                     qkv = Fx.rmsnorm_linear(x, layer.attn_norm, a.norm_eps, layer.wqkv, layer.bqkv)
-                if self.kv4:
+                if self.kvq:
                     q, k, v = Fx.qkv_rope(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads, a.head_dim,
-                                          a.rope_theta, a.norm_eps)
-                    K4.kv4_write(k, v, self.kv[li], st["slot"][:b])
+                                          a.rope_theta, a.norm_eps, rope=a.rope)
+                    self.kvq.write(k, v, self.kv[li], st["slot"][:b])
                 else:
                     q, _, _ = D.qkv_rope_to_cache(qkv, pos, layer.q_norm, layer.k_norm, la.n_heads, la.n_kv_heads,
                                                   a.head_dim, a.rope_theta, a.norm_eps, self.kv[li, 0],
-                                                  self.kv[li, 1], st["slot"][:b])
-            if self.kv4:
-                o = K4.paged_attention_kv4(q, self.kv[li], st["block_table"][:b], st["seq_lens"][:b])
+                                                  self.kv[li, 1], st["slot"][:b], rope=a.rope)
+            if self.kvq:
+                o = self.kvq.attention(q, self.kv[li], st["block_table"][:b], st["seq_lens"][:b])
             else:
                 o = D.paged_attention(q, self.kv[li, 0], self.kv[li, 1], st["block_table"][:b], st["seq_lens"][:b],
                                       decode_step=True)
@@ -828,7 +873,7 @@ class RolloutEngine:
         n = len(self.running)
         if n == 0:
             return
-        if self._mega is not None or (self.kv4 and self.cuda):
+        if self._mega is not None or (self.kvq and self.cuda):
             # kernels with waits of their own report one that timed out through the device error word (this is
             # a host sync, like the finish-flag read below)
             from ..ops._ext import ext
@@ -838,8 +883,9 @@ class RolloutEngine:
                 ext().clear_device_error()
                 if self._mega is not None:
                     self._mega.reset()
-                if self.kv4:
+                if self.kvq:
                     ext().kv4_reset()
+                    ext().kv8_reset()
                 raise RuntimeError(f"decode kernel reported device error {err} (a bounded wait timed out)")
         done = self.st["done"][:n].tolist()
         rows = [i for i, d in enumerate(done) if d]

@@ -57,6 +57,8 @@ class MegaDecoder:
             return "MoE layers"
         if a.head_dim != 128 or page_size != 64:
             return "head_dim 128 and 64-token pages only"
+        if a.rope is not None:
+            return "rotary positions other than the plain ones"
         if a.n_heads % a.n_kv_heads or a.n_heads // a.n_kv_heads > 16 or a.n_kv_heads > 8:
             return "GQA group > 16 or more than 8 KV heads"
         if a.swiglu_block != 64 or a.dim % 128 or a.ffn_dim % 64:

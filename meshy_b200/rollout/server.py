@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import argparse
 import asyncio
+import json
 import logging
 import threading
 import time
@@ -239,6 +240,13 @@ def serve(engine, host: str, port: int, model_name: str = "") -> None:
     web.run_app(build_app(runner, model_name), host=host, port=port, print=None, access_log=None)
 
 
+def _json_object(text: str) -> dict:
+    value = json.loads(text)
+    if not isinstance(value, dict):
+        raise argparse.ArgumentTypeError("a JSON object is expected")
+    return value
+
+
 def main(argv=None):
     p = argparse.ArgumentParser(description="meshy_b200 rollout engine server")
     p.add_argument("--model", required=True, help="model_name:flavor of the registry")
@@ -250,8 +258,11 @@ def main(argv=None):
     p.add_argument("--max-total-tokens", type=int, default=None)
     p.add_argument("--max-seq-len", type=int, default=None)
     p.add_argument("--mem-fraction", type=float, default=0.5)
-    p.add_argument("--kv-cache-dtype", choices=["auto", "int4"], default="auto",
-                   help="KV cache in the model's dtype, or in 4 bits (3.55 times the tokens)")
+    p.add_argument("--kv-cache-dtype", choices=["auto", "int4", "int8"], default="auto",
+                   help="KV cache in the model's dtype, or in 4 or 8 bits (3.55 or 1.99 times the tokens)")
+    p.add_argument("--json-model-override-args", type=_json_object, default=None,
+                   help="position settings that differ from the flavor's, a JSON object with HF's config names "
+                        "(rope_theta, rope_scaling, partial_rotary_factor, max_position_embeddings)")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--eos", type=int, nargs="*", default=[])
     p.add_argument("--tp-size", type=int, default=1, help="tensor-parallel degree of this replica")
@@ -278,11 +289,12 @@ def main(argv=None):
 
 
 def _build_engine(a, device=None, tp_group=None):
-    from ..models import get_model_args
+    from ..models import get_model_args, with_hf_config
     from .engine import RolloutEngine
 
     name, flavor = a.model.split(":")
-    return RolloutEngine(get_model_args(name, flavor), device=device or a.device, max_running=a.max_running,
+    args = with_hf_config(get_model_args(name, flavor), a.json_model_override_args)
+    return RolloutEngine(args, device=device or a.device, max_running=a.max_running,
                          max_total_tokens=a.max_total_tokens, max_seq_len=a.max_seq_len,
                          mem_fraction=a.mem_fraction, seed=a.seed, eos_token_ids=a.eos, tp_group=tp_group,
                          ep=a.ep_size > 1, kv_dtype=a.kv_cache_dtype)

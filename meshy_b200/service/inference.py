@@ -18,6 +18,7 @@ ignitor), with the recipe's ``server_args`` translated to server flags
 
 from __future__ import annotations
 
+import json
 import logging
 import os
 import signal
@@ -43,6 +44,7 @@ _ARG_MAP = {
     "mem_fraction_static": "--mem-fraction",
     "mem_fraction": "--mem-fraction",
     "kv_cache_dtype": "--kv-cache-dtype",
+    "json_model_override_args": "--json-model-override-args",
     "random_seed": "--seed",
     "tp_size": "--tp-size",
     "ep_size": "--ep-size",
@@ -61,7 +63,7 @@ def server_args_to_cli(server_args: dict[str, Any]) -> list[str]:
         flag = _ARG_MAP.get(k)
         if flag is None:
             raise ValueError(f"unsupported inference server_args key {k!r}")
-        out += [flag, str(v)]
+        out += [flag, json.dumps(v) if isinstance(v, dict) else str(v)]
     return out
 
 

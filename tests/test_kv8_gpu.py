@@ -363,6 +363,198 @@ def test_many_calls_on_streams_at_once():
     assert all(torch.equal(g, want[i % 4]) for i, g in enumerate(got))
 
 
+@pytest.mark.parametrize("qscale", [0.0, 1e-30, 1e-6, 200.0, 1e30])
+def test_query_scales(qscale):
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [900, 64]
+    c, bt = _filled(lens, 2, 128, 64, seed=6, spread=1.0 / max(qscale, 1.0))
+    q = (_q(2, 12, 128).float() * qscale).bfloat16()
+    for scale in (None, 0.25 / max(1.0, qscale) * 1.7):
+        if qscale < 1e20 or scale:
+            _check(q, c, bt, lens, scale)
+    q[1, 3] = 0.0  # a head of zeros beside others: the mean of V
+    _check(q, c, bt, lens, 0.25 / max(1.0, qscale))
+    # a NaN in one head stays there
+    q[0, 2, 7] = math.nan
+    out = paged_attention_kv8(q, c, bt, torch.tensor(lens, dtype=torch.int32, device="cuda"), 0.25 / max(1.0, qscale))
+    assert bool(out[0, 2].isnan().all()) and int(out.isnan().any(-1).sum()) == 1
+
+
+@pytest.mark.parametrize("peak", [0, 40000, 65535])
+def test_a_long_tail_keeps_its_mass(peak):
+    """One key ahead of 65535 others by a factor 2^22: their common weight, 2^-6, has to arrive. (In the peak's block the
+    others' values are quantised beside zeros: the same scale.)"""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_write
+
+    L, hd = 65536, 128
+    k = torch.zeros(L, 1, hd, device="cuda")
+    k[peak, 0, 0] = 16.0
+    v = torch.full((L, 1, hd), 10.0, device="cuda")
+    v += (torch.arange(hd, device="cuda") % 2) * 2
+    v[peak] = 0
+    c = kv8_empty(L // 64, 1, 64, hd, "cuda")
+    kv8_write(k.bfloat16(), v.bfloat16(), c, torch.arange(L, device="cuda"))
+    q = torch.zeros(1, 2, hd, device="cuda").bfloat16()
+    q[..., 0] = 1.0
+    _check(q, c, torch.arange(L // 64, dtype=torch.int32, device="cuda")[None], [L], 22 * math.log(2) / 16)
+
+
+@pytest.mark.parametrize("L", [700, 20000])
+@pytest.mark.parametrize("every", [0, 256, 32])
+def test_small_values_beside_blocks_of_large_ones(L, every):
+    """Values that carry the result beside blocks of next to no weight whose values are ten thousand times as large, and
+    below peaks that have no values at all."""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_write
+
+    hd = 128
+    g = torch.Generator(device="cuda").manual_seed(12)
+    t = torch.arange(L, device="cuda")
+    k = torch.zeros(L, 1, hd, device="cuda")
+    v = 10 + 4 * torch.rand(L, 1, hd, generator=g, device="cuda")
+    k[t % 256 == 21, 0, 0] = 16.0                # a factor 2^22 ahead of the others
+    v[t % 256 == 21] = 0
+    if every:
+        far = t // 16 * 16 % every == 0
+        k[far, 0, 0] = -64.0                     # 2^-88 of the others
+        v[far] = 65504.0 * (torch.arange(hd, device="cuda") % 2 * 2 - 1)
+    q = torch.zeros(1, 2, hd, device="cuda").bfloat16()
+    q[..., 0] = 1.0
+    bt = torch.arange(-(-L // 64), dtype=torch.int32, device="cuda")[None]
+    c = kv8_empty(bt.shape[1], 1, 64, hd, "cuda")
+    kv8_write(k.bfloat16(), v.bfloat16(), c, t)
+    _check(q, c, bt, [L], 22 * math.log(2) / 16)
+
+
+def test_rising_scores():
+    """Every block's maximum above the last: the reference moves at every step, late keys carry the weight."""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_write
+
+    L, hd = 5000, 128
+    k = torch.zeros(L, 2, hd, device="cuda")
+    k[:, :, 0] = torch.arange(L, device="cuda")[:, None] * (60.0 / L)
+    v = torch.randn(L, 2, hd, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    c = kv8_empty(-(-L // 16), 2, 16, hd, "cuda")
+    kv8_write(k.bfloat16(), v.bfloat16(), c, torch.arange(L, device="cuda"))
+    bt = torch.arange(-(-L // 16), dtype=torch.int32, device="cuda")[None]
+    for sign in (1.0, -1.0):
+        q = torch.zeros(1, 4, hd, device="cuda").bfloat16()
+        q[..., 0] = sign * 8
+        _check(q, c, bt, [L])
+
+
+def test_nan_key_reaches_its_row_only():
+    from meshy_b200.ops.kv8 import kv8_write, paged_attention_kv8
+
+    lens = [300, 300]
+    c, bt = _filled(lens, 2, 128, 64)
+    slot = int(bt[0, 2]) * 64 + 7
+    bad = torch.full((1, 2, 128), math.nan, device="cuda").bfloat16()
+    kv8_write(bad, torch.zeros_like(bad), c, torch.tensor([slot], device="cuda"))
+    q = _q(2, 12, 128)
+    out = paged_attention_kv8(q, c, bt, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert bool(out[0].isnan().all())
+    assert torch.equal(out[1:], _check(q[1:], c, bt[1:], lens[1:]))
+
+
+def test_length_at_the_end_of_32_bits():
+    """A table that spans 2^31 tokens and a length of 2^31 - 1: rounding it up to whole units must not wrap."""
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    c, bt = _filled([200], 1, 128, 64)
+    wide = torch.full((1, (1 << 25) + 1), -1, dtype=torch.int32, device="cuda")
+    wide[:, :2] = bt[:, :2]
+    q = _q(1, 2, 128)
+    out = paged_attention_kv8(q, c, wide, torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"))
+    want, size, terms, step = _exact(q, c, bt, [128], 1 / math.sqrt(128))
+    bound = BF16 * want.abs() + (2.0 ** -11 + 2 * (10 * 2.0 ** -23 * terms + 2.0 ** -20)) * size + 34 * 128 * 16 * 2.0 ** -24 * step
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
+def test_offsets_beyond_32_bits():
+    from meshy_b200.ops.kv8 import KV8Cache, kv8_read, kv8_write
+
+    page, H, hd = 64, 2, 128
+    P = (1 << 32) // (H * page * hd) + 64  # more than 2^32 bytes of K
+    c = KV8Cache(torch.empty(P, H, page, hd, dtype=torch.uint8, device="cuda"),
+                 torch.empty(P, H, page, hd, dtype=torch.uint8, device="cuda"),
+                 torch.empty(P, H, page // 16, 2, device="cuda"))
+    pages = torch.tensor([P - 1, 0, P - 40], device="cuda")
+    t = torch.arange(150, device="cuda")
+    slots = pages[t // page] * page + t % page
+    x = _rows(150, H, hd, 9).cuda()
+    ko, vo = kv8_write(x, -x, c, slots, keep=True)
+    k, v = kv8_read(c, slots)
+    assert torch.equal(k, ko) and torch.equal(v, vo) and torch.equal(k, -v) and float((k - x).abs().max()) < 0.1
+    _check(_q(1, 12, hd), c, pages.int()[None], [150])
+
+
+def test_workspace_grows_with_the_segments():
+    """More segments than the first counters hold (16384), on a stream that has used the smaller ones, and in a capture."""
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = torch.randint(0, 40, (2100,), generator=torch.Generator().manual_seed(4)).tolist()
+    small_lens = [40, 3000]
+    c, bt = _filled(lens[:64], 8, 64, 16)
+    bt = bt.repeat(33, 1)[:2100]
+    sl = torch.tensor((lens[:64] * 33)[:2100], dtype=torch.int32, device="cuda")
+    sc, sbt = _filled(small_lens, 8, 64, 16)
+    ssl = torch.tensor(small_lens, dtype=torch.int32, device="cuda")
+    q, sq = _q(2100, 8, 64), _q(2, 8, 64)
+
+    def step():
+        return [paged_attention_kv8(sq, sc, sbt, ssl), paged_attention_kv8(q, c, bt, sl), paged_attention_kv8(q, c, bt, sl),
+                paged_attention_kv8(sq, sc, sbt, ssl)]
+
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        a = step()
+    s.synchronize()
+    assert torch.equal(a[0], a[3]) and torch.equal(a[1], a[2])
+    _check(sq, sc, sbt, small_lens)
+    want, size, terms, step_ = _exact(q[:64], c, bt[:64], lens[:64], 1 / 8)
+    bound = BF16 * want.abs() + (2.0 ** -11 + 2 * (10 * 2.0 ** -23 * terms + 2.0 ** -20)) * size + 34 * 128 * 16 * 2.0 ** -24 * step_
+    assert bool(((a[1][:64].double() - want).abs() <= bound).all())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b = step()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_graphs_come_and_go():
+    """Graphs that are made, replayed and dropped hand their workspaces on; a capture that fails hands its back too."""
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [3000, 5, 700]
+    c, bt = _filled(lens, 2, 128, 64)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = _q(3, 12, 128)
+    want = paged_attention_kv8(q, c, bt, sl)
+    free = []
+    for i in range(12):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = paged_attention_kv8(q, c, bt, sl)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del g, out
+        if i == 3:
+            with pytest.raises(RuntimeError):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    paged_attention_kv8(q, c, bt, sl)
+                    paged_attention_kv8(q[:, :5], c, bt, sl)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        free.append(torch.cuda.mem_get_info()[0])
+    assert min(free[6:]) >= free[5] - (4 << 20)  # 1.3 MB each: those of the dropped graphs were taken again
+    assert torch.equal(paged_attention_kv8(q, c, bt, sl), want)
+
+
 def test_a_step_together():
     """Rotary, maps, write and attention as a decode step chains them, against the functions of the CPU."""
     from meshy_b200.ops import kv8, paging, rotary
