@@ -38,11 +38,24 @@ __device__ __forceinline__ int64_t row_of(const KV8View& c, FastDiv page, int64_
   return p * c.Hkv * c.page + (slot - p * c.page);
 }
 
-// Steps per unit of a block whose largest magnitude is m.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / r, correctly rounded for numbers of eight significant bits: the hardware's approximation and one Newton step.
+__device__ __forceinline__ float reciprocal(float r) {
+  const float y = rcp_approx(r);
+  return fmaf(fmaf(-r, y, 1.f), y, y);
+}
+
+// Steps per unit of a block whose largest magnitude is m, a bf16 number: eight significant bits, towards zero. No quotient
+// of 127 by such a number lies within 2^-16 below one of eight bits, so an approximation moved up by 2^-20 is cut to the
+// same one.
 __device__ __forceinline__ float steps(float m) {
   if (m != m) return m;
-  const float q = __fdiv_rn(127.f, fminf(fmaxf(m, kLeast), kMost));
-  return __uint_as_float(__float_as_uint(q) & 0xFFFF0000u);  // eight significant bits, towards zero
+  const float q = 127.f * rcp_approx(fminf(fmaxf(m, kLeast), kMost)) * 1.00000095367431640625f;
+  return __uint_as_float(__float_as_uint(q) & 0xFFFF0000u);
 }
 
 // rint(x r) + 128 in the low byte: 1.5 2^23 leaves no bits behind the point.
@@ -52,14 +65,23 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// n of byte i of a word: u as 2^23 + u, less 2^23 + 128.
+__device__ __forceinline__ float number(uint32_t w, int i) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 | i)) - (8388608.f + 128.f);
+}
+
+// Correctly rounded x / y from y's correctly rounded reciprocal: one Newton step on the quotient with the exact
+// remainder (Markstein, 1990).
+__device__ __forceinline__ float quotient(float x, float y, float rcp) {
+  const float q = x * rcp;
+  return fmaf(fmaf(-q, y, x), rcp, q);
+}
+
 // Eight bytes to bf16 values.
 __device__ __forceinline__ uint4 restore(uint2 w, float a) {
   float x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = __byte_perm(i < 4 ? w.x : w.y, 0x4B000000u, 0x7440 | (i % 4));  // 2^23 + u
-    x[i] = (__uint_as_float(u) - (8388608.f + 128.f)) * a;
-  }
+  for (int i = 0; i < 8; ++i) x[i] = number(i < 4 ? w.x : w.y, i % 4) * a;
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
@@ -67,18 +89,25 @@ struct WriteArgs {
   const bf16* x[2];  // K and V
   int64_t xs[2], xh[2];
   const int64_t* slots;
-  int T, tile;       // rows of the call; rows that a CTA looks at
+  int T;  // rows of the call
   KV8View c;
   FastDiv page;
   bf16* out[2];
 };
 
-// Rows t0 .. t0 + m of the call, all of one block: head h of K (kv = 0) or V.
+// This lane's channels of row t of the call (the first lanes' of a warp), head h of K (kv = 0) or V.
 template <int HD>
-__device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int h, int kv, int lane, int64_t slot) {
+__device__ __forceinline__ const bf16* row_at(const WriteArgs& a, int64_t t, int h, int kv, int lane) {
+  return (kv ? a.x[1] + t * a.xs[1] + h * a.xh[1] : a.x[0] + t * a.xs[0] + h * a.xh[0]) + lane % (HD / 8) * 8;
+}
+
+// Rows t0 .. t0 + m of the call, all of one block: head h of K (kv = 0) or V. ``row0``: the first of them, if HAVE.
+template <int HD, bool HAVE>
+__device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int h, int kv, int lane, int64_t slot,
+                                          const uint4& row0) {
   constexpr int L = HD / 8, N = B * L / 32, STEP = 32 / L;  // lanes of a row, rows of a lane, rows side by side
   const int ch = lane % L * 8, r0 = lane / L;
-  const bf16* x = (kv ? a.x[1] + t0 * a.xs[1] + h * a.xh[1] : a.x[0] + t0 * a.xs[0] + h * a.xh[0]) + ch;
+  const bf16* x = row_at<HD>(a, t0, h, kv, lane);
   const int64_t xs = kv ? a.xs[1] : a.xs[0];
   const int64_t row = __shfl_sync(0xffffffffu, row_of(a.c, a.page, slot), 0);  // lane i has row i's slot
   bf16* out = kv ? a.out[1] : a.out[0];
@@ -93,13 +122,22 @@ __device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int
   uint8_t* data = (kv ? a.c.v : a.c.k) + first * HD + ch;
   float* scale = a.c.scale + first / B * 2 + kv;
   const float old = *scale;
+  const uint32_t held = __reduce_or_sync(0xffffffffu, lane < m ? 1u << place : 0u);
+  const bool anew = held & 1u;
+  uint2 was[N];  // the block's rows as they are: a token in three makes its block's scale larger
+  if (HAVE && !anew) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) was[j] = *reinterpret_cast<const uint2*>(data + (r0 + j * STEP) * HD);
+  }
   uint4 u[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     u[j] = make_uint4(0, 0, 0, 0);
-    if (r0 + j * STEP < m) u[j] = *reinterpret_cast<const uint4*>(x + (r0 + j * STEP) * xs);
+    if (HAVE && j == 0 && r0 == 0)
+      u[j] = row0;
+    else if (r0 + j * STEP < m)
+      u[j] = *reinterpret_cast<const uint4*>(x + (r0 + j * STEP) * xs);
   }
-  const uint32_t held = __reduce_or_sync(0xffffffffu, lane < m ? 1u << place : 0u);
   // the largest magnitude, in bf16, where it is exact; a NaN stays one
   __nv_bfloat162 top = as_bf162(0u);
 #pragma unroll
@@ -112,28 +150,31 @@ __device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int
   const float t0f = __low2float(top), t1f = __high2float(top);
   const float most = t0f != t0f ? t0f : t1f != t1f ? t1f : fmaxf(t0f, t1f);
   float r = steps(most);
-  if (!(held & 1u)) {
-    const float r_old = old > 0.f || old != old ? __bfloat162float(__float2bfloat16_rn(__fdiv_rn(1.f, old))) : INFINITY;
+  if (!anew) {
+    const float r_old = old > 0.f || old != old ? __bfloat162float(__float2bfloat16_rn(rcp_approx(old))) : INFINITY;
     if (r_old != r_old) r = r_old;
     if (r < r_old) {  // requantise the block's other rows
-#pragma unroll 1
-      for (int p = r0; p < B; p += STEP) {
-        if (held >> p & 1u) continue;
-        uint2 w = *reinterpret_cast<const uint2*>(data + p * HD);
+      if (!HAVE) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) was[j] = *reinterpret_cast<const uint2*>(data + (r0 + j * STEP) * HD);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (held >> (r0 + j * STEP) & 1u) continue;
         uint32_t y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float n = (float)(int)((i < 4 ? w.x : w.y) >> (8 * (i % 4)) & 255u) - 128.f;
-          y[i] = level(__fdiv_rn(n * r, r_old), 1.f);
+          const float n = number(i < 4 ? was[j].x : was[j].y, i % 4);
+          y[i] = level(old > 0.f ? quotient(n * r, r_old, old) : 0.f, 1.f);
         }
-        *reinterpret_cast<uint2*>(data + p * HD) =
+        *reinterpret_cast<uint2*>(data + (r0 + j * STEP) * HD) =
             make_uint2(low_bytes(y[0], y[1], y[2], y[3]), low_bytes(y[4], y[5], y[6], y[7]));
       }
     } else if (r >= r_old) {
       r = r_old;
     }
   }
-  const float back = __fdiv_rn(1.f, r);
+  const float back = reciprocal(r);
   if (lane == 0) *scale = back;
   const bool far = !(most <= kMost) || r != r;
   if (far && r != r) r = 0.f;  // nothing of a block with a NaN is kept: 128 throughout
@@ -159,40 +200,44 @@ __device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int
   }
 }
 
-// Block of row t's slot; rows outside the call and slots outside the cache: below zero.
-__device__ __forceinline__ int64_t block_of(const WriteArgs& a, int64_t t) {
-  if (t < 0 || t >= a.T) return -2;
-  const int64_t s = a.slots[t];
-  return s < 0 || s >= a.c.n_pages * a.c.page ? -1 : s / B;
-}
-
-// A row begins a run unless the row before it has its block; so does one whose block the row 16 before it has too (a
-// slot given more than once, as idle rows give the trash page's: no run is longer than a block).
-__device__ __forceinline__ bool begins(const WriteArgs& a, int64_t t, int64_t block) {
-  return block < 0 || block != block_of(a, t - 1) || block == block_of(a, t - B);
-}
-
-template <int HD>
-__global__ void __launch_bounds__(kThreads, 4) kv8_write_kernel(const WriteArgs a) {
+// A run begins at a row unless the row before it has its block, and at a row whose block the row 16 before it has too (a
+// slot given more than once, as idle rows give the trash page's: no run is longer than a block). A slot outside the cache
+// is a run of its own.
+//
+// A CTA writes the runs that begin among its TILE rows, 16 at most. With one row, the call's few, latency is what counts: its
+// channels are asked for before the slots are known, and the block's other rows before they are known to be needed.
+template <int HD, int TILE>
+__global__ void __launch_bounds__(kThreads, TILE == 1 ? 2 : 4) kv8_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   pdl_wait();
   pdl_trigger();
-  const int t0 = blockIdx.x * a.tile;
-  // the runs that begin among this CTA's rows
-  const int64_t mine = lane < a.tile ? block_of(a, t0 + lane) : -2;
-  uint32_t starts = __ballot_sync(0xffffffffu, mine > -2 && begins(a, t0 + lane, mine));
-  const int items = 2 * a.c.Hkv;
-  // warp w of the grid's row takes every so manieth (head, K or V), run by run
-  const int step = gridDim.y * kWarps;
-  int item = blockIdx.y * kWarps + warp;
+  const int64_t t0 = (int64_t)blockIdx.x * TILE, n = a.c.n_pages * a.c.page;
+  const int items = 2 * a.c.Hkv, step = gridDim.y * kWarps;
+  int item = blockIdx.y * kWarps + warp;  // warps take the (head, K or V) of all runs in turn
+  uint4 row0 = make_uint4(0, 0, 0, 0);
+  if (TILE == 1 && item < items && lane < HD / 8) row0 = *reinterpret_cast<const uint4*>(row_at<HD>(a, t0, item / 2, item % 2, lane));
+  // slots of rows t0 - 16 + lane and t0 + 16 + lane, and their blocks (outside the cache -1, outside the call -2)
+  const int64_t ta = t0 - B + lane, tb = t0 + B + lane;
+  const int64_t sa = ta >= 0 && ta < a.T ? a.slots[ta] : -1, sb = tb < a.T ? a.slots[tb] : -1;
+  auto block_of = [&](int64_t t, int64_t s) { return t < 0 || t >= a.T ? -2 : s < 0 || s >= n ? -1 : s / B; };
+  const int64_t ba = block_of(ta, sa), bb = block_of(tb, sb);
+  const int64_t last = __shfl_sync(0xffffffffu, ba, 31), low = __shfl_sync(0xffffffffu, ba, lane % 16 + 16);
+  int64_t pa = __shfl_up_sync(0xffffffffu, ba, 1), pb = __shfl_up_sync(0xffffffffu, bb, 1);
+  if (lane == 0) pb = last;
+  const int64_t first = __shfl_sync(0xffffffffu, ba, lane % 16);  // 16 rows before lane's in the upper half
+  const uint32_t begin_a = __ballot_sync(0xffffffffu, ba < 0 || ba != pa || ba == first) >> 16;
+  const uint32_t begin_b = __ballot_sync(0xffffffffu, bb < 0 || bb != pb || bb == low) & 0x7FFFu;
+  const uint32_t begins = begin_a | begin_b << 16;  // bit r: row t0 + r
+  uint32_t starts = begins & (__ballot_sync(0xffffffffu, ba != -2) >> 16) & ((1u << TILE) - 1u);
   while (starts) {
-    const int t = t0 + __ffs(starts) - 1;
+    const int i = __ffs(starts) - 1;
     starts &= starts - 1;
-    const int64_t block = block_of(a, t), here = lane < B ? block_of(a, t + lane) : -2;
-    const bool in = here == block && (lane == 0 || !begins(a, t + lane, here));
-    const int m = __ffs(~__ballot_sync(0xffffffffu, in)) - 1;
-    const int64_t slot = lane < m ? a.slots[t + lane] : -1;
-    for (; item < items; item += step) write_run<HD>(a, t, m, item / 2, item % 2, lane, slot);
+    const uint32_t later = begins >> i >> 1;
+    const int m = later ? __ffs(later) : B, at = B + i + lane;  // of the 48 slots at hand
+    const int64_t x = __shfl_sync(0xffffffffu, sa, at % 32), y = __shfl_sync(0xffffffffu, sb, at % 32);
+    const int64_t slot = lane < m ? (at < 32 ? x : y) : -1;
+    for (; item < items; item += step)
+      write_run<HD, TILE == 1>(a, (int)t0 + i, m, item / 2, item % 2, lane, slot, row0);
     item -= items;
   }
 }
@@ -241,10 +286,11 @@ void kv8_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
   // Few rows: a CTA to each, or more, for the latency; many: 16 rows to a CTA, whose warps take the heads of their one or
   // two blocks (32768 tokens of 8 heads: 62.5 us, with 8 rows 65.9, with 32 65.3).
   const bool few = (int64_t)T * items <= 8192;
-  const int tile = few ? 1 : 16;
-  const WriteArgs a{{k, v}, {ks, vs}, {kh, vh}, slots, T, tile, c, FastDiv(c.page), {ko, vo}};
-  const dim3 grid((T + tile - 1) / tile, few ? groups : 1);
-  launch_pdl(c.hd == 128 ? kv8_write_kernel<128> : kv8_write_kernel<64>, grid, dim3(kThreads), 0, st, a);
+  const WriteArgs a{{k, v}, {ks, vs}, {kh, vh}, slots, T, c, FastDiv(c.page), {ko, vo}};
+  const dim3 grid = few ? dim3(T, groups) : dim3((T + B - 1) / B);
+  auto* kernel = c.hd == 128 ? (few ? kv8_write_kernel<128, 1> : kv8_write_kernel<128, B>)
+                             : (few ? kv8_write_kernel<64, 1> : kv8_write_kernel<64, B>);
+  launch_pdl(kernel, grid, dim3(kThreads), 0, st, a);
 }
 
 void kv8_read(KV8View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st) {

@@ -121,6 +121,29 @@ def test_values_far_and_not_finite():
     _same(cpu, gpu)
 
 
+def test_scales_of_every_magnitude():
+    """All 128 mantissas of a bf16 maximum over the exponents: scales equal to the last bit, in fresh and in kept blocks."""
+    tops = torch.arange(0x0080, 0x7F80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    n = len(tops)
+    cpu, gpu = _pair(n, 1, 16, 64)
+    x = torch.zeros(n, 1, 64).bfloat16()
+    x[:, 0, 5], x[:, 0, 6], x[:, 0, 7] = tops, -tops / 2, tops / 3
+    slots = torch.arange(n) * 16
+    from meshy_b200.ops import reference as ref
+
+    # (the definition over all blocks at once; the block-by-block one takes minutes here)
+    r = ref.kv8_steps(tops.float())
+    from meshy_b200.ops.kv8 import kv8_write
+
+    kv8_write(x.cuda(), x.cuda(), gpu, slots.cuda())
+    assert torch.equal(gpu.scale[:, 0, 0, 0].cpu(), 1.0 / r)
+    level = (x[:, 0].float().clamp(-2.0 ** 126, 2.0 ** 126) * r[:, None]).round() + 128
+    assert torch.equal(gpu.k[:, 0, 0].cpu(), level.to(torch.uint8))
+    # a smaller token keeps r, which is found again from the scale
+    kv8_write(x.cuda() * 0, x.cuda() * 0, gpu, slots.cuda() + 1)
+    assert torch.equal(gpu.scale[:, 0, 0, 1].cpu(), 1.0 / r) and torch.equal(gpu.k[:, 0, 0].cpu(), level.to(torch.uint8))
+
+
 def test_repeated_slots_stay_inside():
     """Idle rows all name one slot: it holds one of them, nothing else is touched."""
     from meshy_b200.ops.kv8 import kv8_empty, kv8_read, kv8_write
