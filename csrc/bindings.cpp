@@ -1234,6 +1234,7 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rotary: the gradient is not differentiable (create_graph)");
     const auto saved = ctx->get_saved_variables();
     auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
     auto held = [&](const char* name) {

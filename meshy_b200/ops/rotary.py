@@ -136,17 +136,28 @@ class Rope:
         return [x / s.factor + min(max(k, 0.0), 1.0) * (x - x / s.factor) for x, k in zip(f, keep)]
 
     def turns(self, device) -> torch.Tensor:
-        """``[rotary_dim / 2]`` int64: turns per position times 2^64, modulo 2^64. Made once per device."""
+        """``[rotary_dim / 2]`` int64: turns per position times 2^64, modulo 2^64. Made once per device for all ropes that
+        are equal."""
         t = self._tables.get(device)
         if t is None:
             if not isinstance(device, torch.device):
                 return self.turns(torch.device(device))
-            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("rope: make one call on this device before a CUDA graph capture (it uploads a table)")
-            words = [round(Fraction(f) / _TWO_PI * (1 << 64)) % (1 << 64) for f in self.frequencies()]
-            t = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64, device=device)
-            self._tables[device] = t
+            t = self._tables[device] = _turn_table(self, device)
         return t
+
+
+@lru_cache(maxsize=256)
+def _turn_table(rope: Rope, device: torch.device) -> torch.Tensor:
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("rope: make one call on this device before a CUDA graph capture (it uploads a table)")
+    words = []
+    for f in rope.frequencies():
+        n, d = f.as_integer_ratio()
+        n, d = (n << 64) * _TWO_PI.denominator, d * _TWO_PI.numerator
+        w = (2 * n + d) // (2 * d) % (1 << 64)
+        words.append(w - (1 << 64) if w >> 63 else w)
+    with torch.inference_mode(False):  # (a backward pass may save it)
+        return torch.tensor(words, dtype=torch.int64, device=device)
 
 
 @lru_cache(maxsize=256)
@@ -172,7 +183,9 @@ def qkv_rotary(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, n_heads: 
     once. Differentiable in ``qkv`` and the norms' weights (into their ``main_grad`` where they have one); the weights'
     sums have a fixed order."""
     if native(qkv):
-        acc = (None, None) if q_norm is None else (_acc_main_grad(q_norm), _acc_main_grad(k_norm))
+        acc = (None, None)
+        if q_norm is not None and k_norm is not None:
+            acc = [_acc_main_grad(w) if w.requires_grad else None for w in (q_norm, k_norm)]
         return ext().qkv_rotary(qkv, positions, rope.turns(qkv.device), rope.factor, rope.interleaved, q_norm, k_norm,
                                 n_heads, n_kv, rope.head_dim, eps, *acc)
     _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)

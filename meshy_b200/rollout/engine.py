@@ -587,9 +587,10 @@ class RolloutEngine:
         toks = torch.tensor([t for r in batch for t in r.prompt], dtype=torch.int64)
         toks = toks.to(dev, non_blocking=True)
         st, base, n = self.st, len(self.running), len(batch)
+        held = [r.pages[:self.max_pages_per_seq] for r in batch]  # (a page more may be reserved than a row can use)
         row_ids, have, need, starts, ones, plen, pages = self._upload(
-            range(base, base + n), [0] * n, [len(r.pages) for r in batch], [0] * n, [1] * n, lens,
-            [pg for r in batch for pg in r.pages])
+            range(base, base + n), [0] * n, [len(h) for h in held], [0] * n, [1] * n, lens,
+            [pg for h in held for pg in h])
         st["block_table"][base:base + n] = 0
         assign_pages(st["block_table"], row_ids, have, need, pages)
         pos, slots, cu = token_maps(st["block_table"], row_ids, starts, plen, T, P)

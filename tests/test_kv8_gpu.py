@@ -396,6 +396,8 @@ def test_query_scales(qscale):
     for scale in (None, 0.25 / max(1.0, qscale) * 1.7):
         if qscale < 1e20 or scale:
             _check(q, c, bt, lens, scale)
+    if qscale < 1e20:
+        _check(q, c, bt, lens, -0.3 / max(1.0, qscale))
     q[1, 3] = 0.0  # a head of zeros beside others: the mean of V
     _check(q, c, bt, lens, 0.25 / max(1.0, qscale))
     # a NaN in one head stays there

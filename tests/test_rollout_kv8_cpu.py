@@ -83,6 +83,19 @@ def test_scaled_positions_in_engine_and_model_agree(overrides, kv_dtype):
     assert not torch.allclose(got, other[torch.arange(34, n - 1), ids[35:]], atol=3e-2)
 
 
+def test_a_row_that_reserves_more_pages_than_its_table_has():
+    """A prompt and its tokens that end with the longest sequence reserve a page for one token more."""
+    from meshy_b200.ops import checks
+
+    e = _engine(kv_dtype="int8")
+    checks.set_enabled(True)
+    try:
+        g = e.generate([list(range(100, 100 + 250)), [1, 2]], 6, temperature=0.0)
+    finally:
+        checks.set_enabled(False)
+    assert [len(x.output_ids) for x in g] == [6, 6] and e.blocks.num_free == e.n_pages - 1
+
+
 def test_int8_with_controls_and_interruption():
     e = _engine(kv_dtype="int8")
     out = _greedy(e, PROMPTS, 9, allowed_tokens=[7, 8, 2000], repetition_penalty=1.3)

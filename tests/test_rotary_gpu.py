@@ -198,6 +198,47 @@ def test_main_grad_and_repeatable_sums():
         _near(plain[i], sums[0][i].double() - 2.0, 2.0 ** -23 * (2 + sums[0][i].double().abs()))
 
 
+def test_frozen_norms_and_second_derivatives():
+    from meshy_b200.ops.rotary import qkv_rotary
+
+    rope = _rope(64)
+    qkv, pos, qn, kn = _inputs(5, 2, 1, 64, True)
+    qn.main_grad = torch.zeros(64, device="cuda")  # frozen: nothing is added
+    kn.requires_grad_()
+    kn.main_grad = torch.zeros(64, device="cuda")
+    x = qkv.detach().requires_grad_()
+    out = qkv_rotary(x, pos, rope, 2, 1, qn, kn)
+    torch.autograd.backward(out, [torch.ones_like(o) for o in out])
+    assert float(qn.main_grad.abs().sum()) == 0.0 and float(kn.main_grad.abs().sum()) > 0.0 and x.grad is not None
+    out = qkv_rotary(x, pos, rope, 2, 1)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(out[0].float().pow(2).sum(), x, create_graph=True)
+    with torch.inference_mode():
+        a = qkv_rotary(qkv, pos, _rope(64, 32, False, LINEAR, 7e4), 2, 1)
+    b = qkv_rotary(x, pos, _rope(64, 32, False, LINEAR, 7e4), 2, 1)
+    assert torch.equal(a[0], b[0])
+    torch.autograd.grad(b[0].float().sum(), x)
+
+
+def test_activation_checkpoint_and_retained_graph():
+    from torch.utils.checkpoint import checkpoint
+
+    from meshy_b200.ops.rotary import qkv_rotary
+
+    rope = _rope(64, 32, True, YARN)
+    qkv, pos, qn, kn = _inputs(70, 4, 2, 64, True)
+    leaves = [x.requires_grad_() for x in (qkv, qn, kn)]
+    g = [torch.randn(70, n, 64, device="cuda").bfloat16() for n in (4, 2, 2)]
+    want = torch.autograd.grad(qkv_rotary(qkv, pos, rope, 4, 2, qn, kn), leaves, g)
+    out = checkpoint(lambda x, a, b: qkv_rotary(x * 1.0, pos, rope, 4, 2, a, b), *leaves, use_reentrant=False)
+    got = torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    out = qkv_rotary(qkv, pos, rope, 4, 2, qn, kn)
+    for _ in range(2):
+        got = torch.autograd.grad(out, leaves, g, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_cache_destination():
     from meshy_b200.ops.rotary import qkv_rotary, qkv_rotary_to_cache
 
