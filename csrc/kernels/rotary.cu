@@ -46,6 +46,7 @@ struct Args {
   int nh, splits;             // heads of a group, groups of a token
   FastDiv tokens;             // T
   FastDiv q_items, k_items;   // items of a token in the gradient with norms
+  FastDiv v_row;              // 8 bytes each: V's channels of a token
   float inv_hd;
 };
 
@@ -166,13 +167,12 @@ __device__ __forceinline__ void sine_cosine(uint32_t turn, float& sine, float& c
   cosine = __uint_as_float(__float_as_uint(swap ? s : c) ^ (quarter + 1u & 2u) << 30);
 }
 
-// cos and sin of a lane's pairs at a token's position, times the factor (1 and 0 behind the rotated part).
+// cos and sin of a lane's pairs at position p, times the factor (1 and 0 behind the rotated part).
 struct Angles {
   float c[C / 2], s[C / 2];
 };
-__device__ __forceinline__ Angles angles(const Args& a, const Place& w, int lane, int t) {
+__device__ __forceinline__ Angles angles(const Args& a, const Place& w, int lane, int64_t p) {
   Angles g;
-  const int64_t p = a.pos[t];
 #pragma unroll
   for (int i = 0; i < C / 2; ++i) {
     g.c[i] = 1.f, g.s[i] = 0.f;
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, NORM ? 3 : 4) rotary_fwd_kernel(cons
   const Place w = on ? place_of(s, lane) : Place{0, 0, false};
   const bf16* src = a.qkv + t * a.qs;
   Angles g;
-  if (it.h0 < HQK) g = angles(a, w, lane, t);
+  if (it.h0 < HQK) g = angles(a, w, lane, a.pos[t]);
   const Turn plain = turn_of(g, false);
   int64_t row = -1;  // of the cache, head 0
   if (a.cache.k && it.h1 > s.Hq) {
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_bwd_kernel(const Args a) {
   const int t = it.t, HQK = s.Hq + s.Hkv;
   const Place w = place_of(s, lane);
   Angles g;
-  if (it.h0 < HQK) g = angles(a, w, lane, t);
+  if (it.h0 < HQK) g = angles(a, w, lane, a.pos[t]);
   const Turn back = turn_of(g, true);
   bf16* dst = a.gqkv + (int64_t)t * (HQK + s.Hkv) * s.hd;
   auto heads = [&](int at, int n, const bf16* grad, bool turned) {
@@ -386,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_bwd_kernel(const Args a) {
 // number of warps, whose groups take neighbouring ones. A lane keeps its channels' part of the weights' gradients, the
 // CTA's groups add theirs up in order and a second kernel adds the CTAs'. So every sum has one order.
 constexpr int kNormCtas = 148 * 2;
+constexpr int kCopies = 8;
 
 template <int L, bool INTER>
 __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args a) {
@@ -429,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args
       return r;
     };
     Load next = load();
+    int p = a.pos[t];
     Turn back;
     int held = -1;  // the token whose angles are at hand
     for (int turns = (int)(end - begin + SIDE - 1) / SIDE; turns > 0; --turns) {
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args
         z[x] = unpack<INTER>(next.g[x]);
       }
       if (__any_sync(0xffffffffu, t != held)) {
-        back = turn_of(angles(a, w, lane, t), true);
+        back = turn_of(angles(a, w, lane, p), true);
         held = t;
       }
       const int m = on && left > 0 ? N - h0 : 0;
@@ -458,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args
         gfrom += (N - wrap) * s.hd;
       }
       next = load();
+      p = a.pos[t];
 #pragma unroll
       for (int x = 0; x < kNormBatch; ++x) {
         if (w.turned) z[x] = back(z[x]);
@@ -505,33 +508,44 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args
     }
     __syncthreads();
   }
-  // V's gradient is the output's
-  const int row = s.Hkv * s.hd / 4;
-  for (int64_t t = blockIdx.x; t < s.T; t += gridDim.x) {
-    const uint2* from = reinterpret_cast<const uint2*>(a.gv + t * s.Hkv * s.hd);
-    uint2* to = reinterpret_cast<uint2*>(a.gqkv + (t * H + s.Hq + s.Hkv) * s.hd);
-    for (int c = threadIdx.x; c < row; c += kThreads) to[c] = __ldg(from + c);
+  // V's gradient is the output's: CTAs take neighbouring tokens, a thread has kCopies loads under way
+  const int64_t t0 = (int64_t)blockIdx.x * s.T / gridDim.x, t1 = (int64_t)(blockIdx.x + 1) * s.T / gridDim.x;
+  const uint32_t row = a.v_row.d, n = (uint32_t)(t1 - t0) * row;
+  const uint2* vfrom = reinterpret_cast<const uint2*>(a.gv) + t0 * row;
+  uint2* vto = reinterpret_cast<uint2*>(a.gqkv + (t0 * H + s.Hq + s.Hkv) * s.hd);
+  for (uint32_t c = threadIdx.x; c < n; c += kCopies * kThreads) {
+    uint2 u[kCopies];
+#pragma unroll
+    for (int x = 0; x < kCopies; ++x)
+      if (c + x * kThreads < n) u[x] = __ldg(vfrom + c + x * kThreads);
+#pragma unroll
+    for (int x = 0; x < kCopies; ++x) {
+      const uint32_t e = c + x * kThreads, t = a.v_row.div(e);
+      if (e < n) vto[(int64_t)t * (H * s.hd / 4) + (e - t * row)] = u[x];
+    }
   }
 }
 
-// part [n][2][hd] summed over n: 32 columns to a CTA, every eighth row to a warp.
-__global__ void __launch_bounds__(kThreads)
+// part [n][2][hd] summed over n: 32 columns to a CTA, every kJoinWarps-th row to a warp.
+constexpr int kJoinWarps = 32;
+
+__global__ void __launch_bounds__(32 * kJoinWarps)
     rotary_norm_join_kernel(const float* __restrict__ part, int n, int hd, RotaryWeightGrad wq, RotaryWeightGrad wk) {
-  __shared__ float sums[kThreads / 32][32];
+  __shared__ float sums[kJoinWarps][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
   pdl_wait();
   pdl_trigger();
   float x = 0.f;
   if (c < 2 * hd) {
-#pragma unroll 8
-    for (int i = warp; i < n; i += kThreads / 32) x += part[(int64_t)i * 2 * hd + c];
+#pragma unroll 10
+    for (int i = warp; i < n; i += kJoinWarps) x += part[(int64_t)i * 2 * hd + c];
   }
   sums[warp][lane] = x;
   __syncthreads();
   if (warp || c >= 2 * hd) return;
   x = 0.f;
 #pragma unroll
-  for (int j = 0; j < kThreads / 32; ++j) x += sums[j][lane];
+  for (int j = 0; j < kJoinWarps; ++j) x += sums[j][lane];
   const RotaryWeightGrad& g = c < hd ? wq : wk;
   const int at = c < hd ? c : c - hd;
   if (g.add)
@@ -576,7 +590,7 @@ void rotary_fwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, cons
   if (s.T == 0) return;
   const int lanes = lanes_of(s.hd), nh = heads_of(s, lanes), splits = (s.Hq + 2 * s.Hkv + nh - 1) / nh;
   Args a{s, qkv, qs, pos, turns, factor, qn, kn, eps, q, k, v, cache, nullptr, nullptr, nullptr, nullptr, nullptr, nh,
-         splits, FastDiv(s.T), FastDiv(1), FastDiv(1), 1.f / s.hd};
+         splits, FastDiv(s.T), FastDiv(1), FastDiv(1), FastDiv(1), 1.f / s.hd};
   with_lanes(s, [&](auto l, auto inter) {
     auto* kernel = qn ? rotary_fwd_kernel<l.value, true, inter.value> : rotary_fwd_kernel<l.value, false, inter.value>;
     launch_pdl(kernel, dim3(blocks_of(s, splits, lanes)), dim3(kThreads), 0, st, a);
@@ -592,7 +606,7 @@ void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, cons
   const int lanes = lanes_of(s.hd), nh = heads_of(s, lanes), splits = (s.Hq + 2 * s.Hkv + nh - 1) / nh;
   Args a{s, qkv, qs, pos, turns, factor, qn, kn, eps, nullptr, nullptr, nullptr, RotaryCache{}, gq, gk, gv, gqkv, part,
          nh, splits, FastDiv(std::max(1, s.T)), FastDiv((s.Hq + kNormBatch - 1) / kNormBatch),
-         FastDiv((s.Hkv + kNormBatch - 1) / kNormBatch), 1.f / s.hd};
+         FastDiv((s.Hkv + kNormBatch - 1) / kNormBatch), FastDiv(s.Hkv * s.hd / 4), 1.f / s.hd};
   if (!qn) {
     if (s.T == 0) return;
     with_lanes(s, [&](auto l, auto inter) {
@@ -608,7 +622,7 @@ void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, cons
     with_lanes(s, [&](auto l, auto inter) {
       launch_pdl(rotary_norm_bwd_kernel<l.value, inter.value>, dim3(ctas), dim3(kThreads), 0, st, a);
     });
-  launch_pdl(rotary_norm_join_kernel, dim3((2 * s.hd + 31) / 32), dim3(kThreads), 0, st, (const float*)part, ctas, s.hd,
+  launch_pdl(rotary_norm_join_kernel, dim3((2 * s.hd + 31) / 32), dim3(32 * kJoinWarps), 0, st, (const float*)part, ctas, s.hd,
              wq, wk);
 }
 
