@@ -1114,27 +1114,31 @@ Tensor rotary_rows(const Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-RotaryShape rotary_shape(const Tensor& qkv, const Tensor& pos, const c10::optional<Tensor>& qn,
-                         const c10::optional<Tensor>& kn, const Tensor& turns, int64_t Hq, int64_t Hkv, int64_t hd,
-                         bool interleaved) {
+void check_rotary_qkv(const Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t hd) {
   CHECK_CUDA(qkv);
   TORCH_CHECK_VALUE(Hq > 0 && Hkv > 0 && hd > 0, "rotary: heads and head_dim must be positive");
   TORCH_CHECK_VALUE(qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * hd,
                     "rotary: qkv must be [rows, " + std::to_string((Hq + 2 * Hkv) * hd) + "]");
   TORCH_CHECK(qkv.scalar_type() == at::kBFloat16, "rotary: qkv must be bfloat16 on CUDA");
-  TORCH_CHECK_VALUE(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == qkv.size(0),
-                    "rotary: positions must be int32 [" + std::to_string(qkv.size(0)) + "]");
-  TORCH_CHECK(pos.is_contiguous() && pos.device() == qkv.device(), "rotary: positions must be contiguous, on qkv's device");
+}
+
+// of rows on a device
+RotaryShape rotary_shape(int64_t rows, at::Device device, const Tensor& pos, const c10::optional<Tensor>& qn,
+                         const c10::optional<Tensor>& kn, const Tensor& turns, int64_t Hq, int64_t Hkv, int64_t hd,
+                         bool interleaved) {
+  TORCH_CHECK_VALUE(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == rows,
+                    "rotary: positions must be int32 [" + std::to_string(rows) + "]");
+  TORCH_CHECK(pos.is_contiguous() && pos.device() == device, "rotary: positions must be contiguous, on qkv's device");
   TORCH_CHECK_VALUE(qn.has_value() == kn.has_value(), "rotary: both norm weights or none");
   for (const c10::optional<Tensor>* w : {&qn, &kn})
     if (w->has_value())
       TORCH_CHECK((*w)->scalar_type() == at::kBFloat16 && (*w)->dim() == 1 && (*w)->size(0) == hd && (*w)->is_contiguous() &&
-                      (*w)->device() == qkv.device() && reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 8 == 0,
+                      (*w)->device() == device && reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 8 == 0,
                   "rotary: norm weights must be bfloat16 [" + std::to_string(hd) + "] on qkv's device, on 8-byte boundaries");
-  TORCH_CHECK(turns.scalar_type() == at::kLong && turns.dim() == 1 && turns.is_contiguous() && turns.device() == qkv.device(),
+  TORCH_CHECK(turns.scalar_type() == at::kLong && turns.dim() == 1 && turns.is_contiguous() && turns.device() == device,
               "rotary: the table must be int64 on qkv's device");
-  TORCH_CHECK(qkv.size(0) < (1LL << 31), "rotary: too many rows for one call");
-  return {(int)qkv.size(0), (int)Hq, (int)Hkv, (int)hd, (int)(2 * turns.size(0)), interleaved};
+  TORCH_CHECK(rows < (1LL << 31), "rotary: too many rows for one call");
+  return {(int)rows, (int)Hq, (int)Hkv, (int)hd, (int)(2 * turns.size(0)), interleaved};
 }
 
 // q [T, Hq, hd], k and v [T, Hkv, hd]; with caches [pages, Hkv, page, hd], k and v go there too (and are returned if
@@ -1143,7 +1147,8 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> rotary_fwd_(
     Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
     c10::optional<Tensor> kn, int64_t Hq, int64_t Hkv, int64_t hd, double eps, c10::optional<Tensor> kc,
     c10::optional<Tensor> vc, c10::optional<Tensor> slots, bool keep) {
-  const RotaryShape s = rotary_shape(qkv, pos, qn, kn, turns, Hq, Hkv, hd, interleaved);
+  check_rotary_qkv(qkv, Hq, Hkv, hd);
+  const RotaryShape s = rotary_shape(qkv.size(0), qkv.device(), pos, qn, kn, turns, Hq, Hkv, hd, interleaved);
   const c10::cuda::CUDAGuard guard(qkv.device());
   qkv = rotary_rows(qkv);
   RotaryCache cache{};
@@ -1172,17 +1177,25 @@ struct RotaryGrads {
   Tensor qkv, qn, kn;
 };
 
-// The gradients; those of the norms' weights are added to wq / wk (fp32) where given, else returned in bf16.
-RotaryGrads rotary_bwd_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved, c10::optional<Tensor> qn,
-                        c10::optional<Tensor> kn, Tensor gq, Tensor gk, Tensor gv, c10::optional<Tensor> wq,
-                        c10::optional<Tensor> wk, double eps) {
+// The gradients; those of the norms' weights are added to wq / wk (fp32) where given, else returned in bf16. The projection
+// is read for the norms alone.
+RotaryGrads rotary_bwd_(c10::optional<Tensor> qkv, Tensor pos, Tensor turns, double factor, bool interleaved,
+                        c10::optional<Tensor> qn, c10::optional<Tensor> kn, Tensor gq, Tensor gk, Tensor gv,
+                        c10::optional<Tensor> wq, c10::optional<Tensor> wk, double eps) {
   TORCH_CHECK(gq.dim() == 3 && gk.dim() == 3 && gv.sizes() == gk.sizes() && gq.size(2) == gk.size(2) &&
-                  gq.size(0) == qkv.size(0) && gk.size(0) == qkv.size(0),
+                  gq.size(0) == gk.size(0),
               "rotary: gradients must be [rows, heads, head_dim]");
-  const RotaryShape s = rotary_shape(qkv, pos, qn, kn, turns, gq.size(1), gk.size(1), gq.size(2), interleaved);
-  const c10::cuda::CUDAGuard guard(qkv.device());
+  const int64_t T = gq.size(0), Hq = gq.size(1), Hkv = gk.size(1), hd = gq.size(2);
+  CHECK_CUDA(gq);
+  TORCH_CHECK(qkv.has_value() || !qn.has_value(), "rotary: the gradient with norms needs the projection");
+  if (qkv.has_value()) {
+    check_rotary_qkv(*qkv, Hq, Hkv, hd);
+    TORCH_CHECK(qkv->size(0) == T && qkv->device() == gq.device(), "rotary: the projection and its gradients do not match");
+  }
+  const RotaryShape s = rotary_shape(T, gq.device(), pos, qn, kn, turns, Hq, Hkv, hd, interleaved);
+  const c10::cuda::CUDAGuard guard(gq.device());
   for (Tensor* g : {&gq, &gk, &gv}) {
-    TORCH_CHECK(g->scalar_type() == at::kBFloat16 && g->device() == qkv.device(),
+    TORCH_CHECK(g->scalar_type() == at::kBFloat16 && g->device() == gq.device(),
                 "rotary: gradients must be bfloat16 on qkv's device");
     const bool ok = g->is_contiguous() && reinterpret_cast<uintptr_t>(g->data_ptr()) % 8 == 0;
     if (!ok) *g = g->clone(at::MemoryFormat::Contiguous);
@@ -1196,20 +1209,20 @@ RotaryGrads rotary_bwd_(Tensor qkv, Tensor pos, Tensor turns, double factor, boo
     for (int i = 0; i < 2; ++i)
       if (to[i]->has_value()) {
         const Tensor& t = **to[i];
-        TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == s.hd && t.is_contiguous() && t.device() == qkv.device(),
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == s.hd && t.is_contiguous() && t.device() == gq.device(),
                     "rotary: main_grad of the norms' weights must be float32 [head_dim] on qkv's device");
         w[i].add = ptr<float>(t);
       } else {
-        *fresh[i] = torch::empty({s.hd}, qkv.options());
+        *fresh[i] = torch::empty({s.hd}, gq.options());
         w[i].out = ptr<bf16>(*fresh[i]);
       }
-    part = torch::empty({rotary_part_floats(s)}, qkv.options().dtype(at::kFloat));
+    part = torch::empty({rotary_part_floats(s)}, gq.options().dtype(at::kFloat));
   }
-  qkv = rotary_rows(qkv);
-  out.qkv = torch::empty({qkv.size(0), qkv.size(1)}, qkv.options());
-  rotary_bwd(s, ptr<bf16>(qkv), qkv.stride(0), ptr<int>(pos), ptr<uint64_t>(turns), (float)factor, optr<bf16>(qn),
-             optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(out.qkv), w[0], w[1],
-             part.defined() ? ptr<float>(part) : nullptr, cur_stream());
+  if (qkv.has_value()) qkv = rotary_rows(*qkv);
+  out.qkv = torch::empty({T, (Hq + 2 * Hkv) * hd}, gq.options());
+  rotary_bwd(s, optr<bf16>(qkv), qkv.has_value() ? qkv->stride(0) : 0, ptr<int>(pos), ptr<uint64_t>(turns), (float)factor,
+             optr<bf16>(qn), optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(out.qkv),
+             w[0], w[1], part.defined() ? ptr<float>(part) : nullptr, cur_stream());
   if (s.T || qn.has_value()) count(qn.has_value() && s.T ? 2 : 1);
   return out;
 }
@@ -1224,7 +1237,7 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
                                                 int64_t Hkv, int64_t hd, double eps, const c10::optional<Tensor>& wq,
                                                 const c10::optional<Tensor>& wk) {
     auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
-    ctx->save_for_backward({qkv, pos, turns, qn.value_or(Tensor()), kn.value_or(Tensor())});
+    ctx->save_for_backward({qn.has_value() ? qkv : Tensor(), pos, turns, qn.value_or(Tensor()), kn.value_or(Tensor())});
     ctx->saved_data["factor"] = factor;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
@@ -1241,7 +1254,7 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
       auto it = ctx->saved_data.find(name);
       return it == ctx->saved_data.end() ? c10::nullopt : c10::optional<Tensor>(it->second.toTensor());
     };
-    const RotaryGrads out = rotary_bwd_(saved[0], saved[1], saved[2], ctx->saved_data["factor"].toDouble(),
+    const RotaryGrads out = rotary_bwd_(given(saved[0]), saved[1], saved[2], ctx->saved_data["factor"].toDouble(),
                                         ctx->saved_data["interleaved"].toBool(), given(saved[3]), given(saved[4]), g[0],
                                         g[1], g[2], held("wq"), held("wk"), ctx->saved_data["eps"].toDouble());
     const Tensor none;

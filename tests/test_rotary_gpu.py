@@ -239,6 +239,27 @@ def test_activation_checkpoint_and_retained_graph():
         assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_projection_is_kept_for_the_norms_alone():
+    """Without norms the gradient does not read the projection: it is not held, and may be written to in between."""
+    from meshy_b200.ops.rotary import qkv_rotary
+
+    rope = _rope(64)
+    for norm in (False, True):
+        qkv, pos, qn, kn = _inputs(100, 4, 2, 64, norm)
+        leaf = qkv.clone().requires_grad_()
+        x = leaf * 1
+        out = qkv_rotary(x, pos, rope, 4, 2, qn, kn)
+        grads = [torch.randn_like(o) for o in out]
+        want = torch.autograd.grad(out, leaf, grads, retain_graph=True)[0]
+        with torch.no_grad():
+            x.zero_()
+        if norm:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(out, leaf, grads)
+        else:
+            assert torch.equal(torch.autograd.grad(out, leaf, grads)[0], want)
+
+
 def test_cache_destination():
     from meshy_b200.ops.rotary import qkv_rotary, qkv_rotary_to_cache
 
