@@ -283,11 +283,16 @@ void kv8_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
                int T, KV8View c, bf16* ko, bf16* vo, cudaStream_t st) {
   if (T == 0) return;
   const int items = 2 * c.Hkv, groups = (items + kWarps - 1) / kWarps;
-  // Few rows: a CTA to each, or more, for the latency; many: 16 rows to a CTA, whose warps take the heads of their one or
-  // two blocks (32768 tokens of 8 heads: 62.5 us, with 8 rows 65.9, with 32 65.3).
-  const bool few = (int64_t)T * items <= 8192;
+  // Few rows: a CTA to each, or more, for the latency. More: 16 rows to a CTA (32768 tokens of 8 heads 62.5 us, with 8 rows
+  // 65.9, with 32 65.3), whose warps take the heads of its runs in turn, and as many CTAs to those as make kCtas of
+  // them. (us, first a prompt, then a row to a block, as in decoding; 8 heads: 256 rows 4.2, 5.2, by the other rule 3.5,
+  // 7.6; 512 rows 4.3, 10.7, by the other 5.6, 10.2, with one CTA to the runs 5.2, 48; 2 heads: 512 rows 3.4, 4.6, by the
+  // other 3.1, 6.0; 1024 rows 3.4, 7.6, by the other 4.7, 8.4, with one CTA to the runs 2.9, 15.)
+  constexpr int kCtas = 296;
+  const bool few = (int64_t)T * groups <= 512;
   const WriteArgs a{{k, v}, {ks, vs}, {kh, vh}, slots, T, c, FastDiv(c.page), {ko, vo}};
-  const dim3 grid = few ? dim3(T, groups) : dim3((T + B - 1) / B);
+  const int tiles = (T + B - 1) / B;
+  const dim3 grid = few ? dim3(T, groups) : dim3(tiles, std::max(1, std::min(kCtas / tiles, B * items / kWarps)));
   auto* kernel = c.hd == 128 ? (few ? kv8_write_kernel<128, 1> : kv8_write_kernel<128, B>)
                              : (few ? kv8_write_kernel<64, 1> : kv8_write_kernel<64, B>);
   launch_pdl(kernel, grid, dim3(kThreads), 0, st, a);
@@ -301,7 +306,9 @@ void kv8_read(KV8View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStre
     launch_pdl(kernel, dim3((unsigned)((items + per - 1) / per)), dim3(kThreads), 0, st, c, slots, (uint32_t)items, k, v,
                FastDiv((uint32_t)splits), FastDiv(c.page));
   };
-  const bool many = (int64_t)T * c.Hkv >= 1 << 16;
+  // four heads to a lane where there is work for all (8 heads: 512 tokens 2.0 us, one to a lane 1.8; 1024 2.1, 2.6; 16384
+  // 14.4, 18.6)
+  const bool many = (int64_t)T * c.Hkv >= 8192;
   if (c.hd == 128)
     many ? go(kv8_read_kernel<128, 4>, 4) : go(kv8_read_kernel<128, 1>, 1);
   else

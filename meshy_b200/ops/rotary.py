@@ -146,7 +146,7 @@ class Rope:
         return t
 
 
-@lru_cache(maxsize=256)
+@lru_cache(maxsize=None)  # kept for good: captured graphs read them, and one is half a kilobyte
 def _turn_table(rope: Rope, device: torch.device) -> torch.Tensor:
     if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("rope: make one call on this device before a CUDA graph capture (it uploads a table)")

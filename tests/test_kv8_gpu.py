@@ -96,6 +96,31 @@ def test_runs_in_any_order_and_slots_outside():
     assert int(gpu.k[0].sum()) == 0 and int(gpu.k[4].sum()) == 0
 
 
+@pytest.mark.parametrize("H, hd", [(1, 64), (2, 128), (8, 128), (11, 64), (70, 64)])
+@pytest.mark.parametrize("T", [250, 600, 1500])
+def test_many_rows_in_runs_of_any_length(T, H, hd):
+    """A row to a block, whole blocks and anything between, in one call: twice, so that the second appends to blocks."""
+    rng = random.Random(T + H)
+    page, pages = 32, T // 2 + 2
+    cpu, gpu = _pair(pages, H, page, hd)
+    blocks = [b for b in range(2, 2 * pages)]
+    rng.shuffle(blocks)
+    most = rng.choice([1, 3, 16])
+    runs, slots = [], []
+    while len(slots) < T:
+        first, n = rng.choice([0, 0, 5]), min(rng.randint(1, most), 8, T - len(slots))
+        runs.append((blocks.pop(), first + n))
+        slots += [runs[-1][0] * 16 + p for p in range(first, first + n)]
+    _write(cpu, gpu, _rows(T, H, hd), _rows(T, H, hd, 1), torch.tensor(slots))
+    _same(cpu, gpu)
+    slots = [b * 16 + p for b, p in runs]  # the next token of each
+    n = len(slots)
+    spread = 2.0 ** torch.tensor([float(rng.randint(-2, 2)) for _ in slots])[:, None, None]
+    k, v = ((_rows(n, H, hd, 2 + i).float() * spread).bfloat16() for i in range(2))
+    _write(cpu, gpu, k, v, torch.tensor(slots), keep=False)
+    _same(cpu, gpu)
+
+
 def test_values_far_and_not_finite():
     H, page, hd = 2, 16, 128
     cpu, gpu = _pair(12, H, page, hd)
