@@ -12,6 +12,7 @@ HF rotate-half convention natively).
 from __future__ import annotations
 
 import json
+import math
 import os
 from dataclasses import asdict
 
@@ -107,7 +108,8 @@ def hf_config(args: ModelArgs) -> dict:
     if args.rope_scaling is not None:
         cfg["rope_scaling"] = {k: v for k, v in asdict(args.rope_scaling).items() if v is not None}
     if args.rope_dim not in (None, args.head_dim):
-        cfg["partial_rotary_factor"] = args.rope_dim / args.head_dim
+        f = args.rope_dim / args.head_dim  # readers cut the product off
+        cfg["partial_rotary_factor"] = f if int(args.head_dim * f) == args.rope_dim else math.nextafter(f, 1.0)
     if args.rope_interleaved:
         cfg["rope_interleaved"] = True
     if args.moe is not None:

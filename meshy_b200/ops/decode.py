@@ -56,8 +56,8 @@ def kv_write(k, v, k_cache, v_cache, slot_mapping):
 
 def qkv_rope_to_cache(qkv, positions, q_norm, k_norm, n_heads, n_kv, hd, theta, eps, k_cache, v_cache,
                       slot_mapping, *, keep_kv: bool = False, rope=None):
-    """QK-norm + RoPE (``rope``: a :class:`.rotary.Rope`, else base ``theta``) of a fused ``qkv [T, (Hq + 2 Hkv) hd]`` row block with K and V written straight
-    into the paged cache at ``slot_mapping`` (one kernel instead of rope + scatter).
+    """QK-norm + RoPE (``rope``: a :class:`.rotary.Rope`, else base ``theta``) of a fused ``qkv [T, (Hq + 2 Hkv) hd]`` row
+    block with K and V written straight into the paged cache at ``slot_mapping`` (one kernel instead of rope + scatter).
 
     Returns ``q [T, Hq, hd]`` and, with ``keep_kv`` (prefill needs them for attention), ``k, v``.
     """

@@ -134,6 +134,18 @@ def test_model_configuration():
         get_model_args("llama3", "debugmodel", rope_scalling=LLAMA3)
 
 
+def test_exported_part_of_a_head_is_read_back():
+    """The factor times the head's width is cut off to a whole number, by this reader and others."""
+    a = get_model_args("llama3", "debugmodel")
+    for hd in range(8, 257, 8):
+        for rot in range(8, hd, 8):
+            args = dataclasses.replace(a, head_dim=hd, rope_dim=rot)
+            cfg = hf_config(args)
+            back = with_hf_config(dataclasses.replace(args, rope_dim=None),
+                                  {"partial_rotary_factor": json.loads(json.dumps(cfg["partial_rotary_factor"]))})
+            assert back.rope_dim == rot, (hd, rot)
+
+
 @pytest.mark.parametrize("scaling", [LLAMA3, YARN, LINEAR], ids=lambda s: s.get("rope_type", "linear"))
 def test_logits_match_hf_llama_with_scaling(scaling):
     from transformers import LlamaConfig, LlamaForCausalLM
