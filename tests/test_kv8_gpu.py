@@ -539,6 +539,24 @@ def test_offsets_beyond_32_bits():
     _check(_q(1, 12, hd), c, pages.int()[None], [150])
 
 
+def test_rows_beyond_32_bits():
+    """More than 2^31 channels in one call: its last rows hold what a call on them alone gives."""
+    from meshy_b200.ops.kv8 import kv8_empty, kv8_read, kv8_write
+
+    H, hd, page, T = 16, 128, 64, (1 << 20) + 640
+    base = _rows(997, H, hd, 3).cuda()
+    x = base[torch.arange(T, device="cuda") % 997]
+    c = kv8_empty(T // page, H, page, hd, "cuda")
+    slots = torch.arange(T, device="cuda")
+    ko, vo = kv8_write(x, x, c, slots, keep=True)
+    k, v = kv8_read(c, slots)
+    tail = kv8_empty(16, H, page, hd, "cuda")
+    want, _ = kv8_write(x[-1024:], x[-1024:], tail, torch.arange(1024, device="cuda"), keep=True)
+    for got in (ko, vo, k, v):
+        assert torch.equal(got[-1024:], want)
+    assert torch.equal(ko, k) and torch.equal(vo, v) and torch.equal(c.k[-16:], tail.k) and torch.equal(c.scale[-16:], tail.scale)
+
+
 def test_workspace_grows_with_the_segments():
     """More segments than the first counters hold (16384), on a stream that has used the smaller ones, and in a capture."""
     from meshy_b200.ops.kv8 import paged_attention_kv8

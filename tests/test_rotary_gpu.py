@@ -320,6 +320,25 @@ def test_capture_and_streams():
     assert not torch.equal(again[0], want[0])
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_rows_beyond_32_bits(norm):
+    """More than 2^31 channels in one call: its last rows hold what a call on them alone gives."""
+    from meshy_b200.ops.rotary import qkv_rotary
+
+    T, Hq, Hkv, hd, n = (1 << 20) + 640, 4, 2, 256, 1000
+    rope = _rope(hd, 64, norm, YARN)
+    qkv, pos, qn, kn = _inputs(n, Hq, Hkv, hd, norm)
+    at = torch.arange(T, device="cuda") % n
+    x, p = qkv[at].requires_grad_(), pos[at]
+    out = qkv_rotary(x, p, rope, Hq, Hkv, qn, kn)
+    grads = [g.contiguous() for g in (o.detach().flip(-1) for o in out)]
+    dx = torch.autograd.grad(out, x, grads)[0]
+    few = x.detach()[-n:].clone().requires_grad_()
+    want = qkv_rotary(few, p[-n:], rope, Hq, Hkv, qn, kn)
+    dw = torch.autograd.grad(want, few, [g[-n:] for g in grads])[0]
+    assert all(torch.equal(a[-n:], b) for a, b in zip(out, want)) and torch.equal(dx[-n:], dw)
+
+
 def test_refusals():
     from meshy_b200.ops._ext import ext
     from meshy_b200.ops.rotary import qkv_rotary, qkv_rotary_to_cache
