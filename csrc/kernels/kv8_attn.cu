@@ -56,11 +56,11 @@ constexpr int kThreads = 32 * (kWarps + kHelpers);
 constexpr int kTok = kKV8Block;
 constexpr int kStages = 3;
 constexpr int kSlots = 2;  // segments whose fragments or states are held
-// (us; as in kv_split.cuh) Equal segments up to 24 units are taken whole (one row of 700 tokens 7.4, up to 64 units 7.6, up
-// to 8 units 7.4); a change of segments counts as 24 units (64 rows of up to 8192 tokens 28.4, 8 units 31.9, 48 units 28.7,
-// none 33.7; 64 rows of up to 600 and 8 KV heads 17.5, 21.9, 18.1, 39.5); a join is worth 6 steps (64 rows of 4096 26.8, 2
-// steps 30.1, 16 steps 26.8; 8 rows of 131072 88, 2 steps 89.7).
-constexpr Rules kRules{24, 24, 6};
+// (us; as in kv_split.cuh) Equal segments up to 32 units are taken whole (a row of 512 tokens with cold caches 8.4, cut 9.1;
+// of 700 whole 9.5, cut 9.3); a change of segments counts as 24 units (64 rows of up to 8192 tokens 28.4, 8 units 31.9, 48
+// units 28.7, none 33.7; 64 rows of up to 600 and 8 KV heads 17.5, 21.9, 18.1, 39.5); a join is worth 6 steps (64 rows of
+// 4096 26.8, 2 steps 30.1, 16 steps 26.8; 8 rows of 131072 88, 2 steps 89.7).
+constexpr Rules kRules{32, 24, 6};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 11.f;           // log2 of the largest p a' right after the reference moved
 constexpr float kLimit = 32768.f;        // how far later ones may go
