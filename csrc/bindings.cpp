@@ -929,7 +929,6 @@ class KV8Workspaces {
   }
 
   KV8Workspace take(int dev, cudaStream_t st, int64_t segments) {
-    std::unique_lock<std::mutex> g(mu_);
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long capture = 0;
     cudaGraph_t graph = nullptr;
@@ -937,9 +936,18 @@ class KV8Workspaces {
     TORCH_CHECK(status != cudaStreamCaptureStatusInvalidated, "paged_attention_kv8: the stream's capture was invalidated");
     const bool capturing = status == cudaStreamCaptureStatusActive;
     const Key key{dev, st, capturing, capture};
-    auto it = held_.find(key);
-    if (it != held_.end() && it->second->segments >= segments) return *it->second;
-    KV8Workspace* w = pooled(dev, segments);
+    KV8Workspace* w = nullptr;
+    {
+      std::lock_guard<std::mutex> g(mu_);
+      auto it = held_.find(key);
+      if (it != held_.end() && it->second->segments >= segments) return *it->second;
+      for (size_t i = 0; !w && i < free_.size(); ++i)
+        if (free_[i]->dev == dev && free_[i]->segments >= segments) {
+          w = free_[i];
+          free_.erase(free_.begin() + i);
+        }
+    }
+    if (!w) w = make(dev, segments);
     if (capturing) {
       // (a smaller one of this capture stays with the graph, whose earlier launches use it)
       Lease* lease = new Lease{key, w};
@@ -947,7 +955,6 @@ class KV8Workspaces {
       cudaError_t e = cudaUserObjectCreate(&object, lease, &KV8Workspaces::give_back, 1, cudaUserObjectNoDestructorSync);
       if (e == cudaSuccess) e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
       if (e != cudaSuccess) {
-        g.unlock();
         if (object)
           cudaUserObjectRelease(object, 1);  // gives it back
         else
@@ -955,13 +962,18 @@ class KV8Workspaces {
         MESHY_CUDA_CHECK(e);
       }
     }
+    std::lock_guard<std::mutex> g(mu_);
     held_[key] = w;  // a stream's smaller one is kept unused: launches under way may be using it
     return *w;
   }
 
   void reset() {
-    std::lock_guard<std::mutex> g(mu_);
-    for (KV8Workspace& w : all_) {
+    std::vector<KV8Workspace> all;
+    {
+      std::lock_guard<std::mutex> g(mu_);
+      all.assign(all_.begin(), all_.end());
+    }
+    for (const KV8Workspace& w : all) {
       const c10::cuda::CUDAGuard guard((c10::DeviceIndex)w.dev);
       MESHY_CUDA_CHECK(cudaMemsetAsync(w.arrived, 0, w.segments * sizeof(unsigned), cur_stream()));
     }
@@ -982,7 +994,7 @@ class KV8Workspaces {
     KV8Workspace* w;
   };
 
-  static void CUDART_CB give_back(void* p) {  // calls no CUDA function, as its caller demands
+  static void CUDART_CB give_back(void* p) noexcept {  // calls no CUDA function, as its caller demands
     Lease* lease = static_cast<Lease*>(p);
     KV8Workspaces& s = get();
     std::lock_guard<std::mutex> g(s.mu_);
@@ -992,13 +1004,7 @@ class KV8Workspaces {
     delete lease;
   }
 
-  KV8Workspace* pooled(int dev, int64_t segments) {
-    for (size_t i = 0; i < free_.size(); ++i)
-      if (free_[i]->dev == dev && free_[i]->segments >= segments) {
-        KV8Workspace* w = free_[i];
-        free_.erase(free_.begin() + i);
-        return w;
-      }
+  KV8Workspace* make(int dev, int64_t segments) {
     // memory that no capture sees: neither the allocation nor the clearing is part of the graph
     struct Mode {
       cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
@@ -1020,11 +1026,13 @@ class KV8Workspaces {
       cudaFree(mem);
       MESHY_CUDA_CHECK(e);
     }
+    std::lock_guard<std::mutex> g(mu_);
+    free_.reserve(all_.size() + 1);  // give_back must not allocate: its caller is C code
     all_.push_back({dev, n, static_cast<float*>(mem), arrived});
     return &all_.back();
   }
 
-  std::mutex mu_;
+  std::mutex mu_;  // never held over a CUDA call, one of which may be waiting for give_back
   std::list<KV8Workspace> all_;
   std::vector<KV8Workspace*> free_;
   std::map<Key, KV8Workspace*> held_;

@@ -411,6 +411,46 @@ def test_many_calls_on_streams_at_once():
     assert all(torch.equal(g, want[i % 4]) for i, g in enumerate(got))
 
 
+def test_calls_from_several_threads():
+    """Each on a stream of its own, calls and captured graphs that come and go."""
+    import threading
+
+    from meshy_b200.ops.kv8 import paged_attention_kv8
+
+    lens = [900, 30, 2000]
+    c, bt = _filled(lens, 2, 64, 32)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = [_q(3, 12, 64, s) for s in range(4)]
+    want = [paged_attention_kv8(q, c, bt, sl) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for turn in range(6):
+                    got = paged_attention_kv8(qs[i], c, bt, sl)
+                    graph = torch.cuda.CUDAGraph()
+                    graph.capture_begin(capture_error_mode="thread_local")
+                    held = paged_attention_kv8(qs[i], c, bt, sl)
+                    graph.capture_end()
+                    graph.replay()
+                    s.synchronize()
+                    if not (torch.equal(got, want[i]) and torch.equal(held, want[i])):
+                        wrong.append((i, turn))
+                    del graph, held
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not any(t.is_alive() for t in threads) and not wrong, wrong
+
+
 @pytest.mark.parametrize("qscale", [0.0, 1e-30, 1e-6, 200.0, 1e30])
 def test_query_scales(qscale):
     from meshy_b200.ops.kv8 import paged_attention_kv8
