@@ -433,7 +433,8 @@ class RolloutEngine:
                allowed_tokens: Sequence[int] | None = None, n_generated: int = 0) -> Any:
         """Queue a request. The penalties, ``logit_bias`` and ``allowed_tokens`` act on the logits before temperature
         and filters (:mod:`..ops.controls`); ``n_generated``: so many tokens at the prompt's end are output of an
-        earlier, aborted call (the frequency and presence penalties count them)."""
+        earlier, aborted call (the frequency and presence penalties count them). ``ValueError`` for a prompt that the
+        block table does not hold (``max_seq_len`` rounded up to whole pages); one that fills it gets one token."""
         # (copies: the request is looked at again when it is admitted)
         controls = {k: float(v) for k, v, off in (("repetition_penalty", repetition_penalty, 1.0),
                                                   ("frequency_penalty", frequency_penalty, 0.0),
@@ -445,6 +446,9 @@ class RolloutEngine:
         check_controls(self.args.vocab_size, MAX_LOGIT_BIAS, **controls)
         if not 0 <= n_generated <= len(prompt):
             raise ValueError(f"n_generated must be between 0 and the prompt's length, got {n_generated}")
+        fits = self.max_pages_per_seq * self.page_size
+        if len(prompt) > fits:
+            raise ValueError(f"a prompt of {len(prompt)} tokens is longer than the {fits} of a sequence")
         rid = next(self._rid) if rid is None else rid
         if len(prompt) + max_new_tokens > self.max_seq_len:
             max_new_tokens = max(1, self.max_seq_len - len(prompt))
@@ -626,7 +630,8 @@ class RolloutEngine:
         st["gen"][rows] = 1
         st["tok_in"][rows] = tok
         st["pos"][rows] = plen
-        st["seq_lens"][rows] = plen + 1
+        # (a prompt that fills its table is done, and idles like a parked row: no key behind the table, the trash page's slot)
+        st["seq_lens"][rows] = (plen + 1).clamp(max=self.max_pages_per_seq * P)
         rs = req_slots.to(dev).long()
         st["out_tok"][rs, 0] = tok
         st["out_lp"][rs, 0] = lp
@@ -636,7 +641,7 @@ class RolloutEngine:
             hit = torch.isin(tok.cpu(), torch.tensor(self.eos)) & ~ignore
             done = done | hit
         st["done"][rows] = done.to(torch.int32).to(dev)
-        st["slot"][rows] = token_maps(st["block_table"], row_ids, plen, ones, n, P).slots
+        st["slot"][rows] = token_maps(st["block_table"], row_ids, plen, ones, n, P).slots.clamp(min=0)
         self.running.extend(batch)
 
     def _mlp(self, layer, h, x):
