@@ -745,6 +745,7 @@ __global__ void kv_write_kernel(const bf16* __restrict__ k, const bf16* __restri
   int t = (int)(idx / per), r = (int)(idx % per);
   int h = r / (HD / 8), c = (r % (HD / 8)) * 8;
   int64_t slot = slots[t];
+  if (slot < 0) return;  // no slot: not written
   int64_t pg = slot / page, off = slot % page;
   size_t dst = (((size_t)pg * Hkv + h) * page + off) * HD + c;
   size_t src = ((size_t)t * Hkv + h) * HD + c;

@@ -1015,6 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int hk = tile - Hqk;
               for (int tt = 0; tt < a.B; ++tt) {
                 const int64_t sl = slot_s[tt];
+                if (sl < 0) continue;  // no slot: not written
                 const size_t row = ((size_t)((layer * 2 + 1) * a.n_cache_pages + sl / kMegaPage) * a.Hkv + hk) *
                                        kMegaPage + (size_t)(sl % kMegaPage);
                 a.kv[row * kMegaHeadDim + f] = __float2bfloat16(sm[tt * 128 + f]);
@@ -1053,6 +1054,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else {
                   const int hk = tile - a.Hq;
                   const int64_t sl = slot_s[tt];
+                  if (sl < 0) continue;
                   const size_t row = ((size_t)((layer * 2 + 0) * a.n_cache_pages + sl / kMegaPage) * a.Hkv + hk) *
                                          kMegaPage + (size_t)(sl % kMegaPage);
                   a.kv[row * kMegaHeadDim + f] = __float2bfloat16(out);

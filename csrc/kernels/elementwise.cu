@@ -190,9 +190,10 @@ __global__ void qkv_rope_fwd_kernel(const bf16* __restrict__ qkv, const int* __r
   if (gw >= (long long)T * H) return;
   const int t = (int)(gw / H), h = (int)(gw % H);
   const int half = hd / 2;
-  // paged-cache row of this token for head hh: [n_pages, Hkv, page, hd]
+  // paged-cache row of this token for head hh: [n_pages, Hkv, page, hd]; null for a slot below zero, which is not written
   auto cache_row = [&](bf16* base, int hh) -> bf16* {
     const int64_t slot = slots[t];
+    if (slot < 0) return nullptr;
     return base + (((size_t)(slot / page) * Hkv + hh) * page + (size_t)(slot % page)) * hd;
   };
   const bf16* src = qkv + (size_t)t * H * hd + (size_t)h * hd;
@@ -214,8 +215,10 @@ __global__ void qkv_rope_fwd_kernel(const bf16* __restrict__ qkv, const int* __r
       }
       if (vc) {
         bf16* dst = cache_row(vc, h - Hq - Hkv);
-        *reinterpret_cast<uint32_t*>(dst + i0) = lo;
-        *reinterpret_cast<uint32_t*>(dst + i0 + half) = hi;
+        if (dst) {
+          *reinterpret_cast<uint32_t*>(dst + i0) = lo;
+          *reinterpret_cast<uint32_t*>(dst + i0 + half) = hi;
+        }
       }
     }
     return;
@@ -248,8 +251,10 @@ __global__ void qkv_rope_fwd_kernel(const bf16* __restrict__ qkv, const int* __r
   }
   if (!is_q && kc) {
     bf16* c = cache_row(kc, h - Hq);
-    *reinterpret_cast<uint32_t*>(c + i0) = lo;
-    *reinterpret_cast<uint32_t*>(c + i0 + half) = hi;
+    if (c) {
+      *reinterpret_cast<uint32_t*>(c + i0) = lo;
+      *reinterpret_cast<uint32_t*>(c + i0 + half) = hi;
+    }
   }
 }
 

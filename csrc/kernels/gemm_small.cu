@@ -717,6 +717,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
               const int m = 4 * g + i;
               if (m < p.M) {
                 const int64_t sl = pf ? pre_slot[i] : p.slots[m];
+                if (sl < 0) continue;  // no slot: not written
                 p.vc[(((size_t)(sl / 64) * p.hkv + hk) * 64 + (size_t)(sl % 64)) * 128 + f] = __float2bfloat16(y[i]);
               }
             }
@@ -755,6 +756,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                   p.q_out[((size_t)m * p.hq + nt) * 128 + f] = __float2bfloat16(o);
                 } else {
                   const int64_t sl = pf ? pre_slot[i] : p.slots[m];
+                  if (sl < 0) continue;
                   p.kc[(((size_t)(sl / 64) * p.hkv + (nt - p.hq)) * 64 + (size_t)(sl % 64)) * 128 + f] =
                       __float2bfloat16(o);
                 }

@@ -38,16 +38,20 @@ from .functional import native
 
 
 def kv_write(k, v, k_cache, v_cache, slot_mapping):
-    """``k/v [B, Hkv, hd]`` → cache ``[n_pages, Hkv, page, hd]`` at ``slot_mapping [B]``."""
+    """``k/v [B, Hkv, hd]`` → cache ``[n_pages, Hkv, page, hd]`` at ``slot_mapping [B]`` (a row whose slot is below zero is
+    not written, here and in the writes fused with the rotary embedding)."""
     from .checks import check_range
 
-    check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2])
+    check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2], skip_negative=True)
     if native(k):
         from ._ext import ext
 
         ext().kv_write(k, v, k_cache, v_cache, slot_mapping)
         return
     page = k_cache.shape[2]
+    if bool((slot_mapping < 0).any()):
+        ok = slot_mapping >= 0
+        k, v, slot_mapping = k[ok], v[ok], slot_mapping[ok]
     pg = (slot_mapping // page).long()
     off = (slot_mapping % page).long()
     k_cache[pg, :, off] = k.to(k_cache.dtype)
@@ -71,7 +75,7 @@ def qkv_rope_to_cache(qkv, positions, q_norm, k_norm, n_heads, n_kv, hd, theta, 
         from ._ext import ext
         from .checks import check_range
 
-        check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2])
+        check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2], skip_negative=True)
         q = torch.empty(T, n_heads, hd, dtype=qkv.dtype, device=qkv.device)
         k = torch.empty(T, n_kv, hd, dtype=qkv.dtype, device=qkv.device) if keep_kv else None
         v = torch.empty(T, n_kv, hd, dtype=qkv.dtype, device=qkv.device) if keep_kv else None
@@ -128,7 +132,7 @@ def qkv_rope_fused(x, w, bias, positions, q_norm, k_norm, n_heads, n_kv, theta, 
     from ._ext import ext
     from .checks import check_range
 
-    check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2])
+    check_range("KV-cache slots", slot_mapping, 0, k_cache.shape[0] * k_cache.shape[2], skip_negative=True)
     T = x.shape[0]
     q = torch.empty(T, n_heads, 128, dtype=x.dtype, device=x.device)
     ok = ext().gemm_qkv_rope(x, w, bias, part, (d + 127) // 128 if part is not None else 0, float(d), float(eps),
