@@ -9,7 +9,7 @@
 // A write that holds a block's first token starts the block anew. Any other takes r' = min(r, r of its own rows); where
 // that is below r, the other tokens of the block are requantised, rint(n r' / r): n r' is exact, and no quotient of it
 // by r lies so near a half that fp32's rounding could move it there. A token that is written again changes nothing. Each such
-growth adds up to half a step of the new scale to the other tokens' errors: (1 + g) / 2 steps at most after g of them.
+// growth adds up to half a step of the new scale to the other tokens' errors: (1 + g) / 2 steps at most after g of them.
 //
 // A warp owns a block's rows: runs of neighbouring rows of the call whose slots lie in one block. Magnitudes are taken
 // in [2^-100, 2^126]; a NaN gives the block the scale NaN (and its new rows the byte 128).
