@@ -20,8 +20,9 @@
 // P carries the scale of V (x = p a'), so a reference m per warp and head keeps it in fp16's range: p is taken relative
 // to m, which is set so that the largest p a' seen is 2^11, and moves again only when a later one passes 2^15. So most
 // blocks take neither the maximum's shuffles nor a rescaling. x is rounded to fp16's 11 bits, or by 2^-25 where it is
-// below 2^-14: less than 2^-35 of the largest. Scales below 2^-64 count as that for the reference, so that p stays below
-// 2^79; sums and the normaliser stay in 32 bits.
+// below 2^-14: less than 2^-35 of the largest. Scales below 2^-64 count as that for the reference. All of V's scales are
+// taken 2^-16 times, which keeps p between 2^-92 (the largest, beside values of 2^126) and 2^95 in fp32's range with the
+// weights that count; sums and the normaliser stay in 32 bits.
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory (a unit is
 // a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead,
@@ -64,7 +65,9 @@ constexpr Rules kRules{32, 24, 6};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 11.f;           // log2 of the largest p a' right after the reference moved
 constexpr float kLimit = 32768.f;        // how far later ones may go
-constexpr float kMinA = 5.4210109e-20f;  // 2^-64
+constexpr float kShrink = 1.52587890625e-5f;       // 2^-16, times V's scales
+constexpr float kMinA = 5.42101086e-20f * kShrink;  // 2^-64
+constexpr float kUnit = 16777216.f;                // 2^24: the bytes stand for 2^-24 of themselves
 
 template <int HD>
 struct Cfg {
@@ -176,14 +179,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         x.z = fmaf(v[k].z, e, x.z);
         x.w = fmaf(v[k].w, e, x.w);
       }
-      constexpr float f = 16777216.f;  // the bytes' 2^-24
+      constexpr float f = kUnit / kShrink;
+      x.x *= f, x.y *= f, x.z *= f, x.w *= f;  // (before the division: L may be as small as p)
       if (w.whole()) {
-        const float e = L == 0.f ? 0.f : __fdividef(f, L);
+        const float e = L == 0.f ? 0.f : __fdividef(1.f, L);
         *reinterpret_cast<uint2*>(a.out + ((int64_t)w.b * a.Hq + hk * a.rep + h0 + h) * HD + ch) =
             make_uint2(pack_bf16x2(x.x * e, x.y * e), pack_bf16x2(x.z * e, x.w * e));
       } else {
         float* pp = a.part + ((int64_t)(2 * blockIdx.x + (w.first == 0 ? 1 : 0)) * kHeads + h) * C::PART;
-        *reinterpret_cast<float4*>(pp + ch) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+        *reinterpret_cast<float4*>(pp + ch) = x;
         if (ch == 0) *reinterpret_cast<float2*>(pp + HD) = make_float2(M, L);
       }
     }
@@ -193,10 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ───────────────────────────── helpers ─────────────────────────────
     const int hw = warp - kWarps, ht = tid - 32 * kWarps;
     // A segment's query rows as matrix fragments, a warp per head: scaled so that the largest is in [2^14, 2^15); -128
-    // times their sum, in units of 2^-24 as the products are; the factor that takes the powers back, with the softmax
-    // scale (2^12 of it are left to the blocks' scales).
+    // times their sum, in units of 2^-24 as the products are; the factor that takes the query's power back, with the softmax
+    // scale.
     constexpr int CH = HD / 32;  // channels of a lane
-    const float sl2 = a.scale * (kLog2e * 4096.f);
+    const float sl2 = a.scale * kLog2e;
     uint32_t raw[kHeads / kHelpers][CH / 2];
     auto load_q = [&](const W& w) {
       const int h0 = (w.h % a.blocks) * kHeads;
@@ -230,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 0; k < kHeads / kHelpers; ++k) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
 #pragma unroll
       for (int k = 0; k < kHeads / kHelpers; ++k) {
-        // 2^14 over the largest's power of two; magnitudes outside [2^-100, 2^126) as they are at its ends
-        const uint32_t power = min(max(__float_as_uint(mx[k]), 27u << 23), (252u << 23)) & 0x7F800000u;
+        // 2^14 over the largest's power of two; magnitudes below 2^-100 as they are there
+        const uint32_t power = min(max(__float_as_uint(mx[k]), 27u << 23), (254u << 23)) & 0x7F800000u;
         const float up = __uint_as_float(((127u + 14u + 127u) << 23) - power);
         down[k] = __uint_as_float(power - (14u << 23));
         sum[k] = 0.f;
@@ -448,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < KW / 2; ++j) load_words<4>(qf[j], frag_at + j * 512);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n] = sc_at[n];
+        for (int n = 0; n < NT; ++n) sc[n] = sc_at[n], sc[n].y *= kShrink;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -484,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int r = 0; r < 2; ++r) {
                 float x = acc[n][0][2 * i + r] + acc[n][1][2 * i + r];
                 if constexpr (CHAINS == 4) x += acc[n][2][2 * i + r] + acc[n][3][2 * i + r];
-                s[n][i][r] = fmaf(x * (sc[n].x * 4096.f), cs[r], -m[r]);
+                // |x| < 2^5: in this order nothing is out of fp32's range unless the score is
+                s[n][i][r] = fmaf(x * sc[n].x * cs[r], kUnit, -m[r]);
               }
           }
         }
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
 
-      // the warp's state: o in units of 2^-24 V, relative to m
+      // the warp's state: o in units of 2^-40 V, relative to m
       float* state = reinterpret_cast<float*>(smem + C::STATES + (slot * kWarps + warp) * C::STATE);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
