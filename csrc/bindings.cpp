@@ -1273,6 +1273,8 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
 std::tuple<Tensor, Tensor, Tensor> qkv_rotary_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved,
                                                c10::optional<Tensor> qn, c10::optional<Tensor> kn, int64_t Hq, int64_t Hkv,
                                                int64_t hd, double eps, c10::optional<Tensor> wq, c10::optional<Tensor> wk) {
+  for (const Tensor& t : {qkv, qn.value_or(Tensor()), kn.value_or(Tensor())})
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rotary: there is no forward-mode derivative on CUDA");
   const bool grad = at::GradMode::is_enabled() && (qkv.requires_grad() || (qn.has_value() && qn->requires_grad()) ||
                                                    (kn.has_value() && kn->requires_grad()));
   if (!grad) {

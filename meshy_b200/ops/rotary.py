@@ -180,8 +180,8 @@ def qkv_rotary(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, n_heads: 
                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6):
     """``q [T, Hq, hd], k, v [T, Hkv, hd]`` of ``qkv [T, (Hq + 2 Hkv) hd]`` at ``positions [T]`` (int32): the heads split,
     RMS-normed with ``q_norm`` / ``k_norm [hd]`` where given, and turned. In fp32 between reading and writing, rounded
-    once. Differentiable in ``qkv`` and the norms' weights (into their ``main_grad`` where they have one); the weights'
-    sums have a fixed order."""
+    once. Differentiable in ``qkv`` and the norms' weights (into their ``main_grad`` where they have one), once and
+    backward only; the weights' sums have a fixed order."""
     if native(qkv):
         acc = (None, None)
         if q_norm is not None and k_norm is not None:

@@ -1,0 +1,36 @@
+"""The rotary embedding's derivative: what it refuses, weights that are used twice or whose gradient moves (GPU)."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from meshy_b200.ops.rotary import Rope, qkv_rotary
+
+pytestmark = pytest.mark.gpu
+Hq, Hkv, HD = 4, 2, 64
+ROPE = Rope(HD, 1e4)
+
+
+def _inputs(T=37, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * HD, generator=g, device="cuda").bfloat16()
+    w = [(1 + 0.2 * torch.randn(HD, generator=g, device="cuda")).bfloat16() for _ in range(2)]
+    grads = [torch.randn(T, h, HD, generator=g, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv)]
+    return qkv, torch.arange(T, dtype=torch.int32, device="cuda") * 3, w, grads
+
+
+@pytest.mark.parametrize("which", ["qkv", "q_norm", "k_norm"])
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("requires_grad", [True, False])
+def test_forward_mode_is_refused(which, grad_mode, requires_grad):
+    """A tangent must not vanish in silence, whether or not a backward pass is recorded."""
+    qkv, pos, (wq, wk), _ = _inputs()
+    args = {"qkv": qkv, "q_norm": wq, "k_norm": wk}
+    if requires_grad:
+        args["qkv"].requires_grad_()
+    with fwAD.dual_level(), torch.set_grad_enabled(grad_mode):
+        args[which] = fwAD.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+            qkv_rotary(args["qkv"], pos, ROPE, Hq, Hkv, args["q_norm"], args["k_norm"])
+        # tensors without a tangent are served inside a dual level as well
+        qkv_rotary(_inputs()[0], pos, ROPE, Hq, Hkv, wq, wk)
