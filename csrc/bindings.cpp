@@ -1242,15 +1242,12 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& qkv, const Tensor& pos,
                                                 const Tensor& turns, double factor, bool interleaved,
                                                 const c10::optional<Tensor>& qn, const c10::optional<Tensor>& kn, int64_t Hq,
-                                                int64_t Hkv, int64_t hd, double eps, const c10::optional<Tensor>& wq,
-                                                const c10::optional<Tensor>& wk) {
+                                                int64_t Hkv, int64_t hd, double eps) {
     auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
     ctx->save_for_backward({qn.has_value() ? qkv : Tensor(), pos, turns, qn.value_or(Tensor()), kn.value_or(Tensor())});
     ctx->saved_data["factor"] = factor;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
-    if (wq.has_value()) ctx->saved_data["wq"] = *wq;
-    if (wk.has_value()) ctx->saved_data["wk"] = *wk;
     return {q, *k, *v};
   }
 
@@ -1258,21 +1255,28 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "rotary: the gradient is not differentiable (create_graph)");
     const auto saved = ctx->get_saved_variables();
     auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
-    auto held = [&](const char* name) {
-      auto it = ctx->saved_data.find(name);
-      return it == ctx->saved_data.end() ? c10::nullopt : c10::optional<Tensor>(it->second.toTensor());
-    };
     const RotaryGrads out = rotary_bwd_(given(saved[0]), saved[1], saved[2], ctx->saved_data["factor"].toDouble(),
                                         ctx->saved_data["interleaved"].toBool(), given(saved[3]), given(saved[4]), g[0],
-                                        g[1], g[2], held("wq"), held("wk"), ctx->saved_data["eps"].toDouble());
+                                        g[1], g[2], main_grad(saved[3]), main_grad(saved[4]),
+                                        ctx->saved_data["eps"].toDouble());
     const Tensor none;
-    return {out.qkv, none, none, none, none, out.qn, out.kn, none, none, none, none, none, none};
+    return {out.qkv, none, none, none, none, out.qn, out.kn, none, none, none, none};
+  }
+
+ private:
+  // A weight's ``main_grad`` as it is now, if its gradient is wanted: the attribute may be given, moved or taken away between
+  // the passes.
+  static c10::optional<Tensor> main_grad(const Tensor& w) {
+    if (!w.defined() || !w.requires_grad()) return c10::nullopt;
+    const pybind11::gil_scoped_acquire gil;
+    const pybind11::object to = pybind11::getattr(pybind11::cast(w), "main_grad", pybind11::none());
+    return to.is_none() ? c10::nullopt : c10::optional<Tensor>(to.cast<Tensor>());
   }
 };
 
 std::tuple<Tensor, Tensor, Tensor> qkv_rotary_(Tensor qkv, Tensor pos, Tensor turns, double factor, bool interleaved,
                                                c10::optional<Tensor> qn, c10::optional<Tensor> kn, int64_t Hq, int64_t Hkv,
-                                               int64_t hd, double eps, c10::optional<Tensor> wq, c10::optional<Tensor> wk) {
+                                               int64_t hd, double eps) {
   for (const Tensor& t : {qkv, qn.value_or(Tensor()), kn.value_or(Tensor())})
     TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rotary: there is no forward-mode derivative on CUDA");
   const bool grad = at::GradMode::is_enabled() && (qkv.requires_grad() || (qn.has_value() && qn->requires_grad()) ||
@@ -1281,7 +1285,7 @@ std::tuple<Tensor, Tensor, Tensor> qkv_rotary_(Tensor qkv, Tensor pos, Tensor tu
     auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
     return {q, *k, *v};
   }
-  auto out = QKVRotary::apply(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, wq, wk);
+  auto out = QKVRotary::apply(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps);
   return {out[0], out[1], out[2]};
 }
 

@@ -26,7 +26,7 @@ import torch
 from . import reference as ref
 from ._ext import ext
 from .checks import check_range
-from .functional import _acc_main_grad, native
+from .functional import native
 
 #: 2 pi to 200 bits
 _TWO_PI = Fraction(2 * 314159265358979323846264338327950288419716939937510582097494459, 10 ** 62)
@@ -180,14 +180,11 @@ def qkv_rotary(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, n_heads: 
                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6):
     """``q [T, Hq, hd], k, v [T, Hkv, hd]`` of ``qkv [T, (Hq + 2 Hkv) hd]`` at ``positions [T]`` (int32): the heads split,
     RMS-normed with ``q_norm`` / ``k_norm [hd]`` where given, and turned. In fp32 between reading and writing, rounded
-    once. Differentiable in ``qkv`` and the norms' weights (into their ``main_grad`` where they have one), once and
-    backward only; the weights' sums have a fixed order."""
+    once. Differentiable in ``qkv`` and the norms' weights (into the ``main_grad`` that they have in the backward pass,
+    if any), once and backward only; the weights' sums have a fixed order."""
     if native(qkv):
-        acc = (None, None)
-        if q_norm is not None and k_norm is not None:
-            acc = [_acc_main_grad(w) if w.requires_grad else None for w in (q_norm, k_norm)]
         return ext().qkv_rotary(qkv, positions, rope.turns(qkv.device), rope.factor, rope.interleaved, q_norm, k_norm,
-                                n_heads, n_kv, rope.head_dim, eps, *acc)
+                                n_heads, n_kv, rope.head_dim, eps)
     _check(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm)
     return ref.qkv_rotary(qkv, positions, rope, n_heads, n_kv, q_norm, k_norm, eps)
 

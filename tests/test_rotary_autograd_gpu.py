@@ -34,3 +34,34 @@ def test_forward_mode_is_refused(which, grad_mode, requires_grad):
             qkv_rotary(args["qkv"], pos, ROPE, Hq, Hkv, args["q_norm"], args["k_norm"])
         # tensors without a tangent are served inside a dual level as well
         qkv_rotary(_inputs()[0], pos, ROPE, Hq, Hkv, wq, wk)
+
+
+def _plain(w, inputs, w2=None):
+    """The gradients of the norms' weights without a ``main_grad``."""
+    qkv, pos, _, grads = inputs
+    leaves = [w.clone().requires_grad_(), (w if w2 is None else w2).clone().requires_grad_()]
+    return torch.autograd.grad(qkv_rotary(qkv, pos, ROPE, Hq, Hkv, *leaves), leaves, grads)
+
+
+@pytest.mark.parametrize("when", ["given", "moved", "taken away"])
+def test_main_grad_is_looked_up_in_the_backward_pass(when):
+    """As the other operators do: a trainer may hand the buffers out, swap or drop them after the forward pass."""
+    inputs = _inputs()
+    qkv, pos, weights, grads = inputs
+    want = _plain(weights[0], inputs, weights[1])
+    w = [x.clone().requires_grad_() for x in weights]
+    early, late = ([torch.full((HD,), 3.0, device="cuda") for _ in w] for _ in range(2))
+    if when != "given":
+        for x, m in zip(w, early):
+            x.main_grad = m
+    out = qkv_rotary(qkv, pos, ROPE, Hq, Hkv, *w)
+    for x, m in zip(w, late):
+        x.main_grad = None if when == "taken away" else m
+    torch.autograd.backward(out, grads)
+    assert all(bool((m == 3.0).all()) for m in early)
+    for x, m, g in zip(w, late, want):
+        if when == "taken away":
+            assert torch.equal(x.grad, g) and bool((m == 3.0).all())
+        else:  # (the gradient in bf16 is the same sum rounded once more; adding 3 and taking it off again rounds in fp32)
+            assert x.grad is None
+            assert bool(((m - 3.0 - g.float()).abs() <= 2.0 ** -8 * g.float().abs() + 2.0 ** -23 * (m.abs() + 3)).all())
