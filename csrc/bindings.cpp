@@ -1231,7 +1231,7 @@ RotaryGrads rotary_bwd_(c10::optional<Tensor> qkv, Tensor pos, Tensor turns, dou
   rotary_bwd(s, optr<bf16>(qkv), qkv.has_value() ? qkv->stride(0) : 0, ptr<int>(pos), ptr<uint64_t>(turns), (float)factor,
              optr<bf16>(qn), optr<bf16>(kn), (float)eps, ptr<bf16>(gq), ptr<bf16>(gk), ptr<bf16>(gv), ptr<bf16>(out.qkv),
              w[0], w[1], part.defined() ? ptr<float>(part) : nullptr, cur_stream());
-  if (s.T || qn.has_value()) count(qn.has_value() && s.T ? 2 : 1);
+  if (s.T || qn.has_value()) count((s.T ? 1 : 0) + (qn.has_value() ? 1 : 0) + (rotary_shared_grad(w[0], w[1], s.hd) ? 1 : 0));
   return out;
 }
 

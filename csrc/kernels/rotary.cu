@@ -536,23 +536,24 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_norm_bwd_kernel(const Args
   }
 }
 
-// part [n][2][hd] summed over n: 32 columns to a CTA, every kJoinWarps-th row to a warp.
+// part [n][2][hd] summed over n, columns first .. end: 32 of them to a CTA, every kJoinWarps-th row to a warp.
 constexpr int kJoinWarps = 32;
 
 __global__ void __launch_bounds__(32 * kJoinWarps)
-    rotary_norm_join_kernel(const float* __restrict__ part, int n, int hd, RotaryWeightGrad wq, RotaryWeightGrad wk) {
+    rotary_norm_join_kernel(const float* __restrict__ part, int n, int hd, int first, int end, RotaryWeightGrad wq,
+                            RotaryWeightGrad wk) {
   __shared__ float sums[kJoinWarps][32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = first + blockIdx.x * 32 + lane;
   pdl_wait();
   pdl_trigger();
   float x = 0.f;
-  if (c < 2 * hd) {
+  if (c < end) {
 #pragma unroll 10
     for (int i = warp; i < n; i += kJoinWarps) x += part[(int64_t)i * 2 * hd + c];
   }
   sums[warp][lane] = x;
   __syncthreads();
-  if (warp || c >= 2 * hd) return;
+  if (warp || c >= end) return;
   x = 0.f;
 #pragma unroll
   for (int j = 0; j < kJoinWarps; ++j) x += sums[j][lane];
@@ -608,6 +609,10 @@ void rotary_fwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, cons
   });
 }
 
+bool rotary_shared_grad(RotaryWeightGrad wq, RotaryWeightGrad wk, int hd) {
+  return wq.add && wk.add && wq.add < wk.add + hd && wk.add < wq.add + hd;
+}
+
 int64_t rotary_part_floats(RotaryShape s) { return (int64_t)kNormCtas * 2 * s.hd; }
 
 void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, const uint64_t* turns, float factor,
@@ -633,8 +638,16 @@ void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, cons
     with_lanes(s, [&](auto l, auto inter) {
       launch_pdl(rotary_norm_bwd_kernel<l.value, inter.value>, dim3(ctas), dim3(kThreads), 0, st, a);
     });
-  launch_pdl(rotary_norm_join_kernel, dim3((2 * s.hd + 31) / 32), dim3(32 * kJoinWarps), 0, st, (const float*)part, ctas, s.hd,
-             wq, wk);
+  auto join = [&](int first, int end) {
+    launch_pdl(rotary_norm_join_kernel, dim3((end - first + 31) / 32), dim3(32 * kJoinWarps), 0, st, (const float*)part, ctas,
+               s.hd, first, end, wq, wk);
+  };
+  if (rotary_shared_grad(wq, wk, s.hd)) {  // one after the other
+    join(0, s.hd);
+    join(s.hd, 2 * s.hd);
+  } else {
+    join(0, 2 * s.hd);
+  }
 }
 
 }  // namespace meshy

@@ -30,6 +30,8 @@ struct RotaryWeightGrad {
   float* add;
   bf16* out;
 };
+// Both are added to the same memory (one weight for queries and keys): that takes a launch for each.
+bool rotary_shared_grad(RotaryWeightGrad wq, RotaryWeightGrad wk, int hd);
 // gq, gk, gv [T, H, hd] to gqkv [T, (Hq + 2 Hkv) hd]; with norms, the weights' gradients to wq and wk, and ``part`` holds
 // rotary_part_floats() floats.
 void rotary_bwd(RotaryShape s, const bf16* qkv, int64_t qs, const int* pos, const uint64_t* turns, float factor,

@@ -65,3 +65,45 @@ def test_main_grad_is_looked_up_in_the_backward_pass(when):
         else:  # (the gradient in bf16 is the same sum rounded once more; adding 3 and taking it off again rounds in fp32)
             assert x.grad is None
             assert bool(((m - 3.0 - g.float()).abs() <= 2.0 ** -8 * g.float().abs() + 2.0 ** -23 * (m.abs() + 3)).all())
+
+
+@pytest.mark.parametrize("T", [1, 37, 5003, 0])
+@pytest.mark.parametrize("hd", [64, 176])
+def test_one_weight_for_queries_and_keys(T, hd):
+    """Tied norms: their ``main_grad`` gets both sums, whatever the timing."""
+    rope = Rope(hd, 1e4)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * hd, generator=g, device="cuda").bfloat16()
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    w = (1 + 0.2 * torch.randn(hd, generator=g, device="cuda")).bfloat16()
+    grads = [torch.randn(T, h, hd, generator=g, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv)]
+
+    def run(*leaves):
+        torch.autograd.backward(qkv_rotary(qkv, pos, rope, Hq, Hkv, *leaves), grads)
+
+    apart = [w.clone().requires_grad_() for _ in range(2)]
+    for x in apart:
+        x.main_grad = torch.zeros(hd, device="cuda")
+    run(*apart)
+    tied = w.clone().requires_grad_()
+    tied.main_grad = torch.zeros(hd, device="cuda")
+    for _ in range(20):
+        tied.main_grad.zero_()
+        run(tied, tied)
+        assert tied.grad is None and torch.equal(tied.main_grad, apart[0].main_grad + apart[1].main_grad)
+    # two weights whose buffers are one
+    for x in apart:
+        x.main_grad = tied.main_grad
+    tied.main_grad.zero_()
+    run(*apart)
+    torch.cuda.synchronize()
+    total = tied.main_grad.clone()
+    tied.main_grad.zero_()
+    run(tied, tied)
+    assert torch.equal(total, tied.main_grad)
+    # without one, autograd adds the two up
+    free = w.clone().requires_grad_()
+    run(free, free)
+    lone = [w.clone().requires_grad_() for _ in range(2)]
+    run(*lone)
+    assert torch.equal(free.grad, lone[0].grad + lone[1].grad)
