@@ -1165,6 +1165,8 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> rotary_fwd_(
                     kc->size(3) == hd && kc->scalar_type() == at::kBFloat16 && vc->scalar_type() == at::kBFloat16 &&
                     kc->is_contiguous() && vc->is_contiguous() && kc->device() == qkv.device() && vc->device() == qkv.device(),
                 "rotary: caches must be contiguous bfloat16 [pages, Hkv, page, hd] on qkv's device");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(kc->data_ptr()) % 8 == 0 && reinterpret_cast<uintptr_t>(vc->data_ptr()) % 8 == 0,
+                "rotary: caches must start on 8-byte boundaries");
     check_slots(*slots, *kc, qkv.size(0), "rotary");
     TORCH_CHECK(kc->size(2) > 0 && kc->size(2) < (1LL << 31), "rotary: empty pages");
     cache = {ptr<bf16>(*kc), ptr<bf16>(*vc), ptr<int64_t>(*slots), kc->size(0), (int)kc->size(2)};
