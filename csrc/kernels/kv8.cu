@@ -207,8 +207,8 @@ __device__ __forceinline__ void write_run(const WriteArgs& a, int t0, int m, int
 }
 
 // A run begins at a row unless the row before it has its block, and at a row whose block the row 16 before it has too (a
-// slot given more than once, as idle rows give the trash page's: no run is longer than a block). A slot outside the cache
-// is a run of its own.
+// slot given more than once, as idle rows give the trash page's: no run is longer than a block; warps then write one block
+// at once, and what it holds is nobody's). A slot outside the cache is a run of its own.
 //
 // A CTA writes the runs that begin among its TILE rows, 16 at most. With one row, the call's few, latency is what counts:
 // its channels are asked for before the slots are known, and the block's other rows before they are known to be needed (64

@@ -21,8 +21,9 @@ struct KV8View {
 };
 
 // Quantise rows k, v [T, Hkv, hd] bf16 (element strides ks / vs between tokens, kh / vh between heads; inner stride 1,
-// 16-byte aligned rows) into the cache at slots [T] (page * page_size + offset); rows of one block stand together.
-// Slots outside the cache are skipped. ko, vo [T, Hkv, hd]: the values now held (zeros for a slot outside), or null.
+// 16-byte aligned rows) into the cache at slots [T] (page * page_size + offset); rows of one block stand together,
+// each slot once (a block for which that does not hold is left undefined). Slots outside the cache are skipped.
+// ko, vo [T, Hkv, hd]: the values now held (zeros for a slot outside), or null.
 void kv8_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs, int64_t vh, const int64_t* slots,
                int T, KV8View c, bf16* ko, bf16* vo, cudaStream_t st);
 // The bf16 values the cache stands for at ``slots``: k, v [T, Hkv, hd] contiguous (zero for a slot outside it).

@@ -91,22 +91,28 @@ def kv8_from_bytes(raw: torch.Tensor, n_pages: int, n_kv: int, page: int, hd: in
                     raw[2 * half:size].view(torch.float32).view(n_pages, n_kv, page // BLOCK, 2))
 
 
-def _check_runs(slots: torch.Tensor) -> None:
-    """Debug mode: rows of one block stand together."""
+def _check_runs(slots: torch.Tensor, page: int) -> None:
+    """Debug mode: rows of one block stand together and name each slot once (but for page 0, where idle rows write)."""
     if not enabled() or slots.numel() == 0:
         return
-    b = torch.where(slots >= 0, slots // BLOCK, -1)
-    b = b[b >= 0]
-    if b.numel() and 1 + int((b[1:] != b[:-1]).sum()) != b.unique().numel():
+    b = torch.where(slots >= page, slots // BLOCK, -1)
+    begins = b >= 0  # a run: the first row, and each whose block is not that of the row before (a skipped row has none)
+    begins[1:] &= b[1:] != b[:-1]
+    held = slots[b >= 0]
+    if int(begins.sum()) != b[b >= 0].unique().numel():
         raise IndexError("kv8_write: rows whose slots lie in one block must stand together")
+    if held.unique().numel() != held.numel():
+        raise IndexError("kv8_write: a slot is given twice")
 
 
 def kv8_write(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, slot_mapping: torch.Tensor, *, keep: bool = False):
     """``k/v [T, Hkv, hd]`` (any strides) into ``cache`` at ``slot_mapping [T]`` int64: distinct slots, those of one block on
-    neighbouring rows in any order (a slot given twice holds one of its rows). With ``keep``, the values that the cache now
-    holds for these rows, ``(k', v')`` (zeros for a slot outside it)."""
+    neighbouring rows in any order, with no other row between them, skipped ones included. What a block holds whose rows
+    stand apart, or one of whose slots is given twice, is undefined: rows' pieces and scales may be mixed, its other tokens' too
+    (only idle rows, on a page that nothing reads, may do so; other blocks are not touched). With ``keep``, the values that
+    the cache now holds for these rows, ``(k', v')`` (zeros for a slot outside it)."""
     check_range("KV-cache slots", slot_mapping, 0, cache.k.shape[0] * cache.k.shape[2], skip_negative=True)
-    _check_runs(slot_mapping)
+    _check_runs(slot_mapping, cache.k.shape[2])
     if k.is_cuda:
         return ext().kv8_write(k, v, cache.k, cache.v, cache.scale, slot_mapping, bool(keep))
     ref.kv8_write(k, v, cache, slot_mapping)
