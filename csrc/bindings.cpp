@@ -910,7 +910,8 @@ std::tuple<Tensor, Tensor> kv8_read_(Tensor kc, Tensor vc, Tensor scale, Tensor 
   return {k, v};
 }
 
-// Workspaces of the attention kernel: partial sums and arrival counters (zeroed once, left zero by every launch). Launches
+// Workspaces of the attention kernel: partial sums and arrival counters (zeroed once, left zero by every launch, one in
+// which a wait gave up included). Launches
 // that may run at the same time must not share one, so each stream has its own, and so has each stream of each capture:
 // graphs replay beside one another, whatever stream they were captured on. A graph owns its workspaces (as a user object
 // of it); they return to the pool when the graph and what was instantiated from it are gone.
@@ -965,18 +966,6 @@ class KV8Workspaces {
     std::lock_guard<std::mutex> g(mu_);
     held_[key] = w;  // a stream's smaller one is kept unused: launches under way may be using it
     return *w;
-  }
-
-  void reset() {
-    std::vector<KV8Workspace> all;
-    {
-      std::lock_guard<std::mutex> g(mu_);
-      all.assign(all_.begin(), all_.end());
-    }
-    for (const KV8Workspace& w : all) {
-      const c10::cuda::CUDAGuard guard((c10::DeviceIndex)w.dev);
-      MESHY_CUDA_CHECK(cudaMemsetAsync(w.arrived, 0, w.segments * sizeof(unsigned), cur_stream()));
-    }
   }
 
  private:
@@ -1038,10 +1027,8 @@ class KV8Workspaces {
   std::map<Key, KV8Workspace*> held_;
 };
 
-// After a device error (a wait that gave up) the counters may be left nonzero.
-void kv8_reset() { KV8Workspaces::get().reset(); }
-
-Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
+// ``wait``: cycles after which the kernel's waits give up, below zero the usual limit (a test's handle on that path).
+Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale, int64_t wait) {
   const KV8View c = kv8_view(kc, vc, scale_t);
   const c10::cuda::CUDAGuard guard(kc.device());
   q = cache_rows(q, "paged_attention_kv8: q", kc, c.hd);
@@ -1062,7 +1049,7 @@ Tensor kv8_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
                                                     kv8_attention_segments((int)B, (int)Hq, c.Hkv));
   kv8_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
                 ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ws.part, ws.arrived,
-                ptr<int>(scratch(0, 0).err), cur_stream());
+                ptr<int>(scratch(0, 0).err), wait, cur_stream());
   count();
   return out;
 }
@@ -2007,8 +1994,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache");
   m.def("kv8_write", &kv8_write_, "quantise K / V rows into the 8-bit paged cache");
   m.def("kv8_read", &kv8_read_, "the values the 8-bit paged cache holds at given slots");
-  m.def("kv8_attention", &kv8_attention_, "paged decode attention over the 8-bit cache");
-  m.def("kv8_reset", &kv8_reset, "zero the attention's arrival counters after a device error");
+  m.def("kv8_attention", &kv8_attention_, "paged decode attention over the 8-bit cache", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("cache_scale"), py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"),
+        py::arg("wait") = -1);
   m.def("assign_pages", &assign_pages_, "pages dealt to the rows of a block table");
   m.def("token_maps", &token_maps_, "positions, slots and offsets of packed new tokens");
   m.def("rotary_fwd", &rotary_fwd_, "rotary positions of a fused QKV projection");

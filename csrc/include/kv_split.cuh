@@ -275,6 +275,33 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
   return p;
 }
 
+// Counts this CTA's piece; true for the last of the segment, which leaves the counter at zero.
+__device__ __forceinline__ bool arrive(const Rows& a, const Piece& x, unsigned* arrived) {
+  unsigned* ctr = arrived + (int64_t)x.b * a.per_row + x.h;
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(ctr) : "memory");
+  const bool last = old == x.n - 1;
+  if (last) *ctr = 0u;
+  return last;
+}
+
+// Where a CTA's share began, kept for one that gives up.
+template <class W>
+struct Start {
+  W w;
+  Shares shares;
+  int pad;
+};
+// A CTA in which a wait gave up joins nothing, but one thread counts its pieces all the same: the counters are zero when the
+// launch ends, whatever became of it, and the next one's results are right.
+template <class W>
+__device__ __forceinline__ void arrive_all(const Rows& a, const Start<W>& s, unsigned* arrived) {
+  W w = s.w;
+  do {
+    if (!w.whole()) arrive(a, piece_of(w, s.pad, s.shares), arrived);
+  } while (w.next(a, s.pad));
+}
+
 // The last CTA to arrive at a segment joins its pieces. ``part``: [2 CTAs][kHeads][HD + 4] floats (sums, maximum,
 // normaliser), of which CTA c's segment that began before its share is at 2 c, another at 2 c + 1; ``arrived``: zero
 // between launches. Every thread takes part, the CTA's own pieces having been written before a barrier.
@@ -285,11 +312,7 @@ __device__ __forceinline__ void join_pieces(const Rows& a, Piece* piece, int pie
   const int tid = threadIdx.x;
   if (tid < pieces) {
     Piece& x = piece[tid];
-    unsigned* ctr = arrived + (int64_t)x.b * a.per_row + x.h;
-    unsigned old;
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(ctr) : "memory");
-    x.last = old == x.n - 1;
-    if (x.last) *ctr = 0u;
+    x.last = arrive(a, x, arrived);
   }
   __syncthreads();
   for (int i = tid; i < pieces * kHeads * (HD / 4); i += THREADS) {

@@ -53,16 +53,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t phase) {
 }
 
 // Bounded wait. Returns false if the wait timed out or another role of the
-// CTA already aborted (``*abort`` set); on a timeout it sets ``*abort`` and
-// records ``code`` in ``err`` (first error wins).
+// CTA already aborted (``*abort`` set); on a timeout (``cycles``; with 0 it does
+// not look at all) it sets ``*abort`` and records ``code`` in ``err`` (first error wins).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t phase, volatile int* abort, int* err,
-                                          int code) {
-  if (mbar_try_wait(bar, phase)) return true;
+                                          int code, long long cycles = kWaitCycles) {
+  if (cycles > 0 && mbar_try_wait(bar, phase)) return true;
   long long t0 = clock64();
   while (true) {
-    if (mbar_try_wait(bar, phase)) return true;
+    if (cycles > 0 && mbar_try_wait(bar, phase)) return true;
     if (*abort) return false;
-    if (clock64() - t0 > kWaitCycles) {
+    if (cycles <= 0 || clock64() - t0 > cycles) {
       *abort = 1;
       if (err) atomicCAS(err, 0, code);
       return false;

@@ -29,13 +29,13 @@ void kv8_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
 // The bf16 values the cache stands for at ``slots``: k, v [T, Hkv, hd] contiguous (zero for a slot outside it).
 void kv8_read(KV8View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st);
 // Decode attention of q [B, Hq, hd] (strides qs between rows, qh between heads) over each row's first seq_lens[b]
-// tokens, whose pages are bt[b, :]; a row of length 0 gives zeros. A bounded wait inside the kernel that gives up records
-// its code in ``err``. ``part`` holds kv8_part_floats() floats, ``arrived`` kv8_attention_segments() counters that are
+// tokens, whose pages are bt[b, :]; a row of length 0 gives zeros. A bounded wait inside the kernel that gives up (after
+// ``wait`` cycles; below zero: the usual limit) records its code in ``err``; the result is then undefined. ``part`` holds kv8_part_floats() floats, ``arrived`` kv8_attention_segments() counters that are
 // zero between launches; launches that may run at the same time need workspaces of their own.
 int64_t kv8_attention_segments(int B, int Hq, int Hkv);
 int64_t kv8_part_floats();
 void kv8_attention(const bf16* q, int64_t qs, int64_t qh, KV8View c, const int* bt, int64_t bt_stride, int max_pages,
                    const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived, int* err,
-                   cudaStream_t st);
+                   int64_t wait, cudaStream_t st);
 
 }  // namespace meshy

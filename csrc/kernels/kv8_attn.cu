@@ -28,7 +28,7 @@
 // a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead,
 // across the segments, and at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare
 // the query fragments of the coming segments and join the eight states of the finished ones; the states of a share's last
-// segment are joined by all twelve. Every wait is bounded; one that gives up records an error code. How the work is split
+// segment are joined by all twelve. Every wait is bounded; one that gives up records an error code, and the CTA's pieces are counted all the same. How the work is split
 // over CTAs stands in kv_split.cuh.
 //
 // Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 538 MB) 88 us, 6.1 TB/s; 128 rows of 16384 at head width 64
@@ -118,6 +118,7 @@ struct Args : Rows {
   float* part;        // [2 CTAs][kHeads][PART]
   unsigned* arrived;  // [segments], zero between launches
   int* err;
+  long long wait;  // cycles after which a wait gives up
 };
 
 template <int HD>
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t ready[kSlots], done[kSlots];  // fragments are there and the states free; the states are there
   __shared__ Piece s_piece[2];
   __shared__ PlanShared<kThreads> s_plan;
+  __shared__ Start<W> s_start;
   __shared__ int s_pieces, s_abort, s_ok;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   volatile int* abort_flag = &s_abort;
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       more = coming.next(a, pad);
       if (more) load_q(coming);  // on its way until a slot is free
     }
+    if (ht == 64) s_start = {w0, plan.shares, pad};  // (before the first wait; at the kernel's start it costs 0.3 us)
     int pieces = 0;
     uint32_t phase = 0;
     while (true) {
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++pieces;
       }
       if (!w.more()) break;
-      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue);
+      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue, a.wait);
       helper_sync();
       if (!s_ok) break;
       join_states(w, slot, ht, 32 * kHelpers);
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
 
     while (true) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&ready[slot], phase, abort_flag, a.err, kErrTimeoutMma))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&ready[slot], phase, abort_flag, a.err, kErrTimeoutMma, a.wait))) break;
       const W* seg = &s_seg[slot];
       const int n_tok = seg->n, u_end = seg->end();
       int unit = seg->first_of(warp);
@@ -594,7 +597,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   __syncthreads();
-  if (s_abort) return;
+  if (s_abort) {
+    if (tid == 0) arrive_all(a, s_start, a.arrived);
+    return;
+  }
   const W w = s_seg[slot];
   join_states(w, slot, tid, kThreads);
   const int pieces = s_pieces;
@@ -636,7 +642,7 @@ int64_t kv8_part_floats() { return (int64_t)2 * sm_count() * kHeads * Cfg<128>::
 
 void kv8_attention(const bf16* q, int64_t qs, int64_t qh, KV8View c, const int* bt, int64_t bt_stride, int max_pages,
                    const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived, int* err,
-                   cudaStream_t st) {
+                   int64_t wait, cudaStream_t st) {
   if (B == 0) return;
   max_pages = std::min(max_pages, (INT_MAX - 63) / c.page);  // lengths are rounded up to units in 32 bits
   Args a;
@@ -644,6 +650,7 @@ void kv8_attention(const bf16* q, int64_t qs, int64_t qh, KV8View c, const int* 
   static_cast<Rows&>(a) = {seq_lens, B, max_pages, c.page, c.Hkv * blocks};
   a.q = q, a.qs = qs, a.qh = qh, a.c = c, a.bt = bt, a.bt_stride = bt_stride, a.Hq = Hq, a.rep = rep, a.blocks = blocks;
   a.bpp = bpp, a.page_blocks = c.Hkv * bpp, a.scale = scale, a.out = out, a.part = part, a.arrived = arrived, a.err = err;
+  a.wait = wait < 0 ? kWaitCycles : wait;
   c.hd == 128 ? launch<128>(a, st) : launch<64>(a, st);
 }
 
