@@ -795,7 +795,7 @@ std::tuple<Tensor, Tensor> kv4_read_(Tensor kc, Tensor vc, Tensor scale, Tensor 
 }
 
 // Workspace of the attention kernel, one per (device, stream): partial sums and arrival counters (zeroed once, left
-// zero by every launch). A buffer that grew is kept: captured graphs may refer to it.
+// zero by every launch, one in which a wait gave up included). A buffer that grew is kept: captured graphs may refer to it.
 struct KV4Workspace {
   Tensor part, arrived;
 };
@@ -814,14 +814,8 @@ KV4Workspace kv4_workspace(const Tensor& cache, int64_t segments) {
   return w.back();
 }
 
-// After a device error (a wait that gave up) the counters may be left nonzero.
-void kv4_reset() {
-  std::lock_guard<std::mutex> g(g_mu);
-  for (auto& e : g_kv4_ws)
-    for (KV4Workspace& w : e.second) w.arrived.zero_();
-}
-
-Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale) {
+// ``wait``: cycles after which the kernel's waits give up, below zero the usual limit (a test's handle on that path).
+Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt, Tensor seq_lens, double scale, int64_t wait) {
   const KV4View c = kv4_view(kc, vc, scale_t);
   const c10::cuda::CUDAGuard guard(kc.device());
   q = cache_rows(q, "paged_attention_kv4: q", kc, c.hd);
@@ -841,7 +835,7 @@ Tensor kv4_attention_(Tensor q, Tensor kc, Tensor vc, Tensor scale_t, Tensor bt,
   const KV4Workspace ws = kv4_workspace(kc, kv4_attention_segments((int)B, (int)Hq, c.Hkv));
   kv4_attention(ptr<bf16>(q), q.stride(0), q.stride(1), c, ptr<int>(bt), bt.stride(0), (int)bt.size(1),
                 ptr<int>(seq_lens), (int)B, (int)Hq, (float)scale, ptr<bf16>(out), ptr<float>(ws.part),
-                ptr<unsigned>(ws.arrived), ptr<int>(scratch(0, 0).err), cur_stream());
+                ptr<unsigned>(ws.arrived), ptr<int>(scratch(0, 0).err), wait, cur_stream());
   count();
   return out;
 }
@@ -1991,7 +1985,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "decode attention split count override (0 = heuristic); for tests and benchmarks");
   m.def("kv4_write", &kv4_write_, "quantise K / V rows into the 4-bit paged cache");
   m.def("kv4_read", &kv4_read_, "the values the 4-bit paged cache holds at given slots");
-  m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache");
+  m.def("kv4_attention", &kv4_attention_, "paged decode attention over the 4-bit cache", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("cache_scale"), py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"),
+        py::arg("wait") = -1);
   m.def("kv8_write", &kv8_write_, "quantise K / V rows into the 8-bit paged cache");
   m.def("kv8_read", &kv8_read_, "the values the 8-bit paged cache holds at given slots");
   m.def("kv8_attention", &kv8_attention_, "paged decode attention over the 8-bit cache", py::arg("q"), py::arg("k"),
@@ -2001,7 +1997,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_maps", &token_maps_, "positions, slots and offsets of packed new tokens");
   m.def("rotary_fwd", &rotary_fwd_, "rotary positions of a fused QKV projection");
   m.def("qkv_rotary", &qkv_rotary_, "rotary_fwd with its gradient");
-  m.def("kv4_reset", &kv4_reset, "zero the attention's arrival counters after a device error");
   m.def("load_tokens", &load_tokens_, "token state (seen bits, generated counts) of admitted requests");
   m.def("apply_logit_controls", &apply_logit_controls_, "penalties, biases and token masks on logits");
   m.def("decode_advance", &decode_advance_);

@@ -30,7 +30,7 @@ void kv4_write(const bf16* k, int64_t ks, int64_t kh, const bf16* v, int64_t vs,
 void kv4_read(KV4View c, const int64_t* slots, int T, bf16* k, bf16* v, cudaStream_t st);
 // Decode attention of q [B, Hq, hd] (strides qs between rows, qh between heads) over each row's first
 // seq_lens[b] tokens, whose pages are bt[b, :]; a row of length 0 gives zeros. A bounded wait inside the kernel that
-// gives up records its code in ``err``. ``part`` holds kv4_part_floats(hd) floats, ``arrived``
+// gives up (after ``wait`` cycles; below zero: the usual limit) records its code in ``err``; the result is then undefined. ``part`` holds kv4_part_floats(hd) floats, ``arrived``
 // kv4_attention_segments() counters that are zero between launches; launches that may run at the same time need
 // workspaces of their own.
 int kv4_attention_ctas();
@@ -38,6 +38,6 @@ int64_t kv4_attention_segments(int B, int Hq, int Hkv);
 inline int64_t kv4_part_floats(int hd) { return (int64_t)2 * kv4_attention_ctas() * 8 * (hd + 4); }
 void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* bt, int64_t bt_stride, int max_pages,
                    const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived, int* err,
-                   cudaStream_t st);
+                   int64_t wait, cudaStream_t st);
 
 }  // namespace meshy

@@ -110,6 +110,7 @@ struct Args : Rows {
   float* part;         // [2 CTAs][kHeads][PART]
   unsigned* arrived;   // [segments], zero between launches
   int* err;
+  long long wait;      // cycles after which a wait gives up
 };
 
 template <int HD, int NT, int NP>
@@ -223,9 +224,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     int slot = 0, pieces = 0;
     uint32_t phase = 0;
     while (true) {
-      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue);
+      if (ht == 0) s_ok = mbar_wait(&done[slot], phase, abort_flag, a.err, kErrTimeoutEpilogue, a.wait);
       helper_sync();
-      if (!s_ok) break;
+      if (!s_ok) {  // (so it is if another wait gave up: every segment's states are waited for here)
+        pieces = 0;
+        if (ht == 0) arrive_all(a, Start<W>{w0, plan.shares, pad}, a.arrived);
+        break;
+      }
       const W w = s_seg[slot];
       const int hk = w.h / a.blocks, h0 = (w.h % a.blocks) * kHeads, nh = min(kHeads, a.rep - h0);
       // the warps' weights: eight neighbouring threads have a head's eight states
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
     uint32_t phase = 0;
 
     while (true) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&ready[slot], phase, abort_flag, a.err, kErrTimeoutMma))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&ready[slot], phase, abort_flag, a.err, kErrTimeoutMma, a.wait))) break;
       const W* seg = &s_seg[slot];
       const int n_tok = seg->n, u_end = seg->end();
       int unit = seg->first_of(warp);
@@ -651,7 +656,7 @@ int64_t kv4_attention_segments(int B, int Hq, int Hkv) { return (int64_t)B * Hkv
 
 void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* bt, int64_t bt_stride, int max_pages,
                    const int* seq_lens, int B, int Hq, float scale, bf16* out, float* part, unsigned* arrived, int* err,
-                   cudaStream_t st) {
+                   int64_t wait, cudaStream_t st) {
   if (B == 0) return;
   const int rep = Hq / c.Hkv;
   max_pages = std::min(max_pages, (INT_MAX - 63) / c.page);  // lengths are rounded up to units in 32 bits
@@ -660,6 +665,7 @@ void kv4_attention(const bf16* q, int64_t qs, int64_t qh, KV4View c, const int* 
   static_cast<Rows&>(a) = {seq_lens, B, max_pages, c.page, c.Hkv * blocks};
   a.q = q, a.qs = qs, a.qh = qh, a.c = c, a.bt = bt, a.bt_stride = bt_stride, a.Hq = Hq, a.rep = rep, a.blocks = blocks;
   a.scale = scale, a.out = out, a.part = part, a.arrived = arrived, a.err = err;
+  a.wait = wait < 0 ? kWaitCycles : wait;
   if (c.hd == 128)
     c.page % 32 == 0 ? launch<128, 2, 1>(a, st) : launch<128, 2, 2>(a, st);
   else

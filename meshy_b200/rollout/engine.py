@@ -889,8 +889,6 @@ class RolloutEngine:
                 ext().clear_device_error()
                 if self._mega is not None:
                     self._mega.reset()
-                if self.kvq is _KV4:
-                    ext().kv4_reset()
                 raise RuntimeError(f"decode kernel reported device error {err} (a bounded wait timed out)")
         done = self.st["done"][:n].tolist()
         rows = [i for i, d in enumerate(done) if d]
