@@ -54,6 +54,28 @@ T* optr(const c10::optional<Tensor>& t) {
   return (t.has_value() && t->defined()) ? reinterpret_cast<T*>(t->data_ptr()) : nullptr;
 }
 
+// Memory of the current device that no capture sees, of which the last ``zeros`` of ``bytes`` are zero: neither the allocation
+// nor the clearing is part of a graph, and any stream may use it at once.
+void* uncaptured_memory(size_t bytes, size_t zeros) {
+  struct Mode {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    Mode() { MESHY_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode)); }
+    ~Mode() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  } relaxed;
+  void* mem = nullptr;
+  MESHY_CUDA_CHECK(cudaMalloc(&mem, bytes));
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(mem) + (bytes - zeros), 0, zeros, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  if (e != cudaSuccess) {
+    cudaFree(mem);
+    MESHY_CUDA_CHECK(e);
+  }
+  return mem;
+}
+
 struct DeviceScratch {
   Tensor ws, counters, err;
 };
@@ -64,15 +86,15 @@ DeviceScratch& scratch(int64_t ws_elems, int64_t n_counters) {
   std::lock_guard<std::mutex> g(g_mu);
   DeviceScratch& s = per_dev[dev];
   auto opts = torch::TensorOptions().device(torch::kCUDA, dev);
-  if (!s.err.defined()) s.err = torch::zeros({1}, opts.dtype(torch::kInt32));
-  if (!s.ws.defined() || s.ws.numel() < ws_elems) {
+  if (!s.err.defined()) s.err = torch::from_blob(uncaptured_memory(sizeof(int), sizeof(int)), {1}, opts.dtype(torch::kInt32));
+  if (ws_elems > 0 && (!s.ws.defined() || s.ws.numel() < ws_elems)) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     MESHY_CUDA_CHECK(cudaStreamIsCapturing(cur_stream(), &cap));
     TORCH_CHECK(cap == cudaStreamCaptureStatusNone,
                 "split-K workspace must be sized before CUDA graph capture (run the shape once uncaptured)");
     s.ws = torch::zeros({std::max<int64_t>(ws_elems, 16 << 20)}, opts.dtype(torch::kFloat));
   }
-  if (!s.counters.defined() || s.counters.numel() < n_counters)
+  if (n_counters > 0 && (!s.counters.defined() || s.counters.numel() < n_counters))
     s.counters = torch::zeros({std::max<int64_t>(n_counters, 1 << 16)}, opts.dtype(torch::kInt32));
   return s;
 }
@@ -988,27 +1010,11 @@ class KV8Workspaces {
   }
 
   KV8Workspace* make(int dev, int64_t segments) {
-    // memory that no capture sees: neither the allocation nor the clearing is part of the graph
-    struct Mode {
-      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-      Mode() { MESHY_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode)); }
-      ~Mode() { cudaThreadExchangeStreamCaptureMode(&mode); }
-    } relaxed;
     int64_t n = 1 << 14;
     while (n < segments) n *= 2;
-    const size_t floats = kv8_part_floats() * sizeof(float);
-    void* mem = nullptr;
-    MESHY_CUDA_CHECK(cudaMalloc(&mem, floats + n * sizeof(unsigned)));
+    const size_t floats = kv8_part_floats() * sizeof(float), counters = n * sizeof(unsigned);
+    void* mem = uncaptured_memory(floats + counters, counters);
     unsigned* arrived = reinterpret_cast<unsigned*>(static_cast<char*>(mem) + floats);
-    cudaStream_t st = nullptr;
-    cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMemsetAsync(arrived, 0, n * sizeof(unsigned), st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (st) cudaStreamDestroy(st);
-    if (e != cudaSuccess) {
-      cudaFree(mem);
-      MESHY_CUDA_CHECK(e);
-    }
     std::lock_guard<std::mutex> g(mu_);
     free_.reserve(all_.size() + 1);  // give_back must not allocate: its caller is C code
     all_.push_back({dev, n, static_cast<float*>(mem), arrived});
