@@ -6,9 +6,12 @@
 // partial sums in a workspace; the last CTA to arrive joins them in CTA order. So every sum has one order, and results do
 // not depend on timing.
 #pragma once
+#include <atomic>
+
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "quotient.cuh"
 #include "sm100.cuh"
 
 namespace meshy {
@@ -138,13 +141,8 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// x / d for quotients below 2^20, r ~ 1 / d
-__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d, float r) {
+// x / d in whole numbers, for quotients below 2^20, r ~ 1 / d
+__device__ __forceinline__ uint32_t whole_quotient(uint32_t x, uint32_t d, float r) {
   uint32_t q = (uint32_t)((float)x * r);
   const int rest = (int)(x - q * d);
   if (rest < 0) --q;
@@ -157,7 +155,7 @@ __device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d, float r) {
 struct Shares {
   uint32_t total, n, per, more;
   float r;  // ~ 1 / n
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + quotient(c * more, n, r); }
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * per + whole_quotient(c * more, n, r); }
   __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
     uint32_t c = min(n - 1, (uint32_t)((float)unit * rcp_approx((float)total) * (float)n));
     while (c + 1 < n && begin(c + 1) <= unit) ++c;
@@ -240,7 +238,7 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
     n_cta = max(segments, min((total + WARPS - 1) / WARPS, (uint32_t)sqrt_approx((float)total * (float)segments)));
   n_cta = min(gridDim.x, n_cta);
   if (equal && n_cta > segments) {
-    const uint32_t even = quotient(n_cta, segments, rcp_approx((float)segments)) * segments;
+    const uint32_t even = whole_quotient(n_cta, segments, rcp_approx((float)segments)) * segments;
     if ((float)total * (rcp_approx((float)even) - rcp_approx((float)n_cta)) <= (float)(rules.join_steps * WARPS)) n_cta = even;
   }
   if (blockIdx.x >= n_cta) return p;
@@ -266,7 +264,7 @@ __device__ __forceinline__ Plan<Walk<UTOK, WARPS>> make_plan(const Rows& a, Plan
   p.w.b = s.row;
   p.w.n = s.n;
   p.w.U = units_of<UTOK>(p.w.n) + p.pad;
-  p.w.h = quotient(at - s.begin, p.w.U, rcp_approx((float)p.w.U));
+  p.w.h = whole_quotient(at - s.begin, p.w.U, rcp_approx((float)p.w.U));
   p.w.begin = s.begin + p.w.h * p.w.U;
   p.w.first = at - p.w.begin;
   p.w.left = end - at;
@@ -359,6 +357,34 @@ __device__ __forceinline__ void join_pieces(const Rows& a, Piece* piece, int pie
     *reinterpret_cast<uint2*>(out + ((int64_t)x.b * Hq + hk * rep + h0 + h) * HD + ch) =
         make_uint2(pack_bf16x2(y.x * e, y.y * e), pack_bf16x2(y.z * e, y.w * e));
   }
+}
+
+// ─── host ──────────────────────────────────────────────────────────────────
+
+constexpr int kDevices = 64;
+
+inline int sm_count() {
+  static std::atomic<int> counts[kDevices];
+  int dev = 0, n = 0;
+  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
+  if ((n = counts[dev].load(std::memory_order_relaxed)) == 0) {
+    MESHY_CUDA_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    counts[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// One CTA to every SM.
+template <auto Kernel, class Args>
+void launch_split(int threads, int smem, const Args& a, cudaStream_t st) {
+  static std::atomic<bool> set[kDevices];
+  int dev = 0;
+  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!set[dev].load(std::memory_order_relaxed)) {
+    MESHY_CUDA_CHECK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    set[dev].store(true, std::memory_order_relaxed);
+  }
+  launch_pdl(Kernel, dim3(sm_count()), dim3(threads), smem, st, a);
 }
 
 }  // namespace kvsplit

@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include "../include/fastdiv.cuh"
+#include "../include/quotient.cuh"
 #include "kv4.h"
 
 namespace meshy {
@@ -22,13 +23,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr float kHalfMax = 65504.f;
-
-// Correctly rounded x / y from y's correctly rounded reciprocal: one Newton step on the quotient with the exact
-// remainder (Markstein, 1990).
-__device__ __forceinline__ float quotient(float x, float y, float rcp) {
-  const float q = x * rcp;
-  return fmaf(fmaf(-q, y, x), rcp, q);
-}
 
 // Two fp32 numbers and their sums and products, one instruction to a pair.
 __device__ __forceinline__ uint64_t pair(float x, float y) {

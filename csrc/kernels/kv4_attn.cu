@@ -621,14 +621,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Args a) {
   if (pieces) join_pieces<HD, kThreads>(a, s_piece, pieces, a.part, a.arrived, a.blocks, a.rep, a.Hq, a.out);
 }
 
-int sm_count() {
-  static int n[64] = {};
-  int dev = 0;
-  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
-  if (!n[dev]) MESHY_CUDA_CHECK(cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev));
-  return n[dev];
-}
-
 template <int HD, int NT, int NP>
 void launch(Args a, cudaStream_t st) {
   using C = Cfg<HD, NT, NP>;
@@ -638,15 +630,7 @@ void launch(Args a, cudaStream_t st) {
   MESHY_CHECK(a.c.n_pages * a.page_pieces < (1LL << 32) - 1, "paged_attention_kv4: cache too large");
   MESHY_CHECK((int64_t)a.B * a.c.Hkv * a.blocks * (std::max<int64_t>(1, (int64_t)a.max_pages * a.ppp) + kRules.pad) < (1LL << 31),
               "paged_attention_kv4: rows * heads * table width too large");
-  static bool set[64] = {};
-  int dev = 0;
-  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
-  if (!set[dev]) {
-    MESHY_CUDA_CHECK(
-        cudaFuncSetAttribute(kv4_attn_kernel<HD, NT, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    set[dev] = true;
-  }
-  launch_pdl(kv4_attn_kernel<HD, NT, NP>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
+  launch_split<kv4_attn_kernel<HD, NT, NP>>(kThreads, C::SMEM, a, st);
 }
 
 }  // namespace

@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include "../include/fastdiv.cuh"
+#include "../include/quotient.cuh"
 #include "kv8.h"
 
 namespace meshy {
@@ -44,11 +45,6 @@ __device__ __forceinline__ int64_t row_of(const KV8View& c, FastDiv page, int64_
   return p * c.Hkv * c.page + (slot - p * c.page);
 }
 
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 1 / r, correctly rounded for numbers of eight significant bits: the hardware's approximation and one Newton step.
 __device__ __forceinline__ float reciprocal(float r) {
   const float y = rcp_approx(r);
@@ -74,13 +70,6 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 // n of byte i of a word: u as 2^23 + u, less 2^23 + 128.
 __device__ __forceinline__ float number(uint32_t w, int i) {
   return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 | i)) - (8388608.f + 128.f);
-}
-
-// Correctly rounded x / y from y's correctly rounded reciprocal: one Newton step on the quotient with the exact
-// remainder (Markstein, 1990).
-__device__ __forceinline__ float quotient(float x, float y, float rcp) {
-  const float q = x * rcp;
-  return fmaf(fmaf(-q, y, x), rcp, q);
 }
 
 // Eight bytes to bf16 values.

@@ -610,14 +610,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-int sm_count() {
-  static int n[64] = {};
-  int dev = 0;
-  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
-  if (!n[dev]) MESHY_CUDA_CHECK(cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev));
-  return n[dev];
-}
-
 template <int HD>
 void launch(const Args& a, cudaStream_t st) {
   using C = Cfg<HD>;
@@ -625,14 +617,7 @@ void launch(const Args& a, cudaStream_t st) {
   MESHY_CHECK(a.c.n_pages * (int64_t)a.page_blocks < (1LL << 32) - 1, "paged_attention_kv8: cache too large");
   MESHY_CHECK((int64_t)a.B * a.per_row * ((int64_t)a.max_pages * a.bpp + 1 + kRules.pad) < (1LL << 31),
               "paged_attention_kv8: rows * heads * table width too large");
-  static bool set[64] = {};
-  int dev = 0;
-  MESHY_CUDA_CHECK(cudaGetDevice(&dev));
-  if (!set[dev]) {
-    MESHY_CUDA_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    set[dev] = true;
-  }
-  launch_pdl(kv8_attn_kernel<HD>, dim3(sm_count()), dim3(kThreads), C::SMEM, st, a);
+  launch_split<kv8_attn_kernel<HD>>(kThreads, C::SMEM, a, st);
 }
 
 }  // namespace
