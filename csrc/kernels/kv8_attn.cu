@@ -22,18 +22,20 @@
 // blocks take neither the maximum's shuffles nor a rescaling. x is rounded to fp16's 11 bits, or by 2^-25 where it is
 // below 2^-14: less than 2^-35 of the largest. Scales below 2^-64 count as that for the reference. All of V's scales are
 // taken 2^-16 times, which keeps p between 2^-92 (the largest, beside values of 2^126) and 2^95 in fp32's range with the
-// weights that count; sums and the normaliser stay in 32 bits.
+// weights that count; sums and the normaliser stay in 32 bits. The 11 bits add up to 8e-6 to the bf16 output's error of 1.6e-3
+// (root mean square); x in two terms, 22 bits, would take that away for 88.2 us instead of 87.0 on the 8 long rows, 95.5 for
+// 92.4 at width 64 and 109.7 for 106.5 on the 256.
 //
 // Eight warps compute and never wait for one another: each keeps a ring of units of its own in shared memory (a unit is
 // a block at head width 128, two at 64: the same bytes), filled by 16-byte asynchronous copies kStages - 1 units ahead,
 // across the segments, and at a segment's end leaves its state in one of kSlots slots and goes on. Four helper warps prepare
 // the query fragments of the coming segments and join the eight states of the finished ones; the states of a share's last
-// segment are joined by all twelve. Every wait is bounded; one that gives up records an error code, and the CTA's pieces are counted all the same. How the work is split
-// over CTAs stands in kv_split.cuh.
+// segment are joined by all twelve. Every wait is bounded; one that gives up records an error code, and the CTA's pieces are
+// counted all the same. How the work is split over CTAs stands in kv_split.cuh.
 //
-// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 538 MB) 88 us, 6.1 TB/s; 128 rows of 16384 at head width 64
-// (14 / 2, 540 MB) 94 us, 5.8 TB/s; 256 rows of up to 1500 (32 / 8 heads, 639 MB) 107 us, 6.0 TB/s; 64 rows of up to 8192 (12
-// / 2, 125 MB) 28 us; one row of 700 tokens 7.4 us. Long rows are bound by memory (a copy runs at 6.5 TB/s; 42 % of the
+// Measured: 8 rows of 131072 tokens (16 / 2 heads, 128 wide, 538 MB) 87 us, 6.2 TB/s; 128 rows of 16384 at head width 64
+// (14 / 2, 540 MB) 92 us, 5.9 TB/s; 256 rows of up to 1500 (32 / 8 heads, 639 MB) 106.5 us, 6.0 TB/s; 64 rows of up to 8192 (12
+// / 2, 125 MB) 28 us; one row of 700 tokens 7.2 us. Long rows are bound by memory (a copy runs at 6.5 TB/s; 42 % of the
 // issue slots are busy), few tokens by the chain of lengths, page ids, copies, join (3.5 us for a row without tokens).
 // Copies of whole 2 KB boxes by TMA took 102 us on the first, units of two blocks at width 128 spilled and took 101. A
 // ring of four: 104.5 us on the 256 rows, but 13.9 -> 14.7 on 33 rows of up to 4000 and 13.5 -> 14.6 on one of 32768, as

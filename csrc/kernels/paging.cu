@@ -3,9 +3,10 @@
 // Both kernels deal a packed list (pages, tokens) out to rows: entry j belongs to the row i with
 // sum(c[:i]) <= j < sum(c[:i + 1]), c the rows' counts. Every CTA scans the counts itself, 256 rows at a time, and
 // looks its own entries up in the scanned block by bisection: a few hundred rows are read in the time of one load from
-// L2, so one launch does what a scan and a second kernel would. Latency bounds both: lengths, the scan, the bisection, the
-// table's entry. Measured: pages and maps of 16 rows 4.4 us, two launches; of 256 rows and 1.1 M tokens 8.8, of which the
-// 14 MB take 2.2.
+// L2, so one launch does what a scan and a second kernel would. A chain bounds the pages, and the maps of few tokens: lengths,
+// the scan, the bisection, the table's entry. Maps of many tokens are bound by instructions (58 % of the issue slots are busy:
+// a scan in every CTA, eight steps of bisection on 64-bit ends for every four tokens). Measured: pages and maps of 16 rows
+// 1.7 and 2.6 us, 4.3 together; of 256 rows and 1.1 M tokens 1.8 and 6.6, 8.8 together, of which the 14 MB take 2.2.
 #include <climits>
 
 #include <cuda_runtime.h>
