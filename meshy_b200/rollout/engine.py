@@ -465,8 +465,14 @@ class RolloutEngine:
         prompt."""
         if isinstance(max_new_tokens, int):
             max_new_tokens = [max_new_tokens] * len(prompts)
-        rids = [self.submit(p, m, temperature=temperature, top_k=top_k, top_p=top_p, ignore_eos=ignore_eos, **controls)
-                for p, m in zip(prompts, max_new_tokens)]
+        with self.lock:
+            queued = len(self.waiting)
+            try:
+                rids = [self.submit(p, m, temperature=temperature, top_k=top_k, top_p=top_p, ignore_eos=ignore_eos, **controls)
+                        for p, m in zip(prompts, max_new_tokens)]
+            except Exception:  # one is refused: none stays queued
+                del self.waiting[queued:]
+                raise
         self.run_until_idle()
         return [self.finished.pop(r) for r in rids]
 

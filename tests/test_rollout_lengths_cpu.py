@@ -73,8 +73,16 @@ def test_longer_prompts_are_refused(kv_dtype, n):
         e.submit([1] * n, 4)
     with pytest.raises(ValueError, match="longer than the 64"):
         e.generate([[1, 2], [1] * n], 4)
-    e.abort_all()  # (the first of the pair had been queued)
-    assert not e.waiting and e.blocks.num_free == e.n_pages - 1
+    with pytest.raises(ValueError, match="longer than the 64"):
+        e.generate([[1, 2], [3], [1] * n, [4]], [4, 4, 4, 4])
+    assert not e.waiting and not e.has_work()  # the prompts before it are not left in the queue
+    e.submit([9], 2, rid="other")
+    with pytest.raises(ValueError, match="longer than the 64"):
+        e.generate([[1, 2], [1] * n], 4)
+    assert [r.rid for r in e.waiting] == ["other"]
+    e.abort_all()
+    e.finished.clear()
+    assert e.blocks.num_free == e.n_pages - 1
     assert len(e.generate([[1, 2]], 4, temperature=0.0)[0].output_ids) == 4
 
 
