@@ -1234,6 +1234,9 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
                                                 int64_t Hkv, int64_t hd, double eps) {
     auto [q, k, v] = rotary_fwd_(qkv, pos, turns, factor, interleaved, qn, kn, Hq, Hkv, hd, eps, {}, {}, {}, true);
     ctx->save_for_backward({qn.has_value() ? qkv : Tensor(), pos, turns, qn.value_or(Tensor()), kn.value_or(Tensor())});
+    // the weights themselves too: what is unpacked may be another tensor (of a recomputed pass, of a saved-tensor hook)
+    if (qn.has_value()) ctx->saved_data["qn"] = *qn;
+    if (kn.has_value()) ctx->saved_data["kn"] = *kn;
     ctx->saved_data["factor"] = factor;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
@@ -1246,7 +1249,7 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
     auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
     const RotaryGrads out = rotary_bwd_(given(saved[0]), saved[1], saved[2], ctx->saved_data["factor"].toDouble(),
                                         ctx->saved_data["interleaved"].toBool(), given(saved[3]), given(saved[4]), g[0],
-                                        g[1], g[2], main_grad(saved[3]), main_grad(saved[4]),
+                                        g[1], g[2], main_grad(ctx, "qn"), main_grad(ctx, "kn"),
                                         ctx->saved_data["eps"].toDouble());
     const Tensor none;
     return {out.qkv, none, none, none, none, out.qn, out.kn, none, none, none, none};
@@ -1255,8 +1258,11 @@ class QKVRotary : public torch::autograd::Function<QKVRotary> {
  private:
   // A weight's ``main_grad`` as it is now, if its gradient is wanted: the attribute may be given, moved or taken away between
   // the passes.
-  static c10::optional<Tensor> main_grad(const Tensor& w) {
-    if (!w.defined() || !w.requires_grad()) return c10::nullopt;
+  static c10::optional<Tensor> main_grad(torch::autograd::AutogradContext* ctx, const char* name) {
+    const auto it = ctx->saved_data.find(name);
+    if (it == ctx->saved_data.end()) return c10::nullopt;
+    const Tensor w = it->second.toTensor();
+    if (!w.requires_grad()) return c10::nullopt;
     const pybind11::gil_scoped_acquire gil;
     const pybind11::object to = pybind11::getattr(pybind11::cast(w), "main_grad", pybind11::none());
     return to.is_none() ? c10::nullopt : c10::optional<Tensor>(to.cast<Tensor>());

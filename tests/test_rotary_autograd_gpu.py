@@ -107,3 +107,83 @@ def test_one_weight_for_queries_and_keys(T, hd):
     lone = [w.clone().requires_grad_() for _ in range(2)]
     run(*lone)
     assert torch.equal(free.grad, lone[0].grad + lone[1].grad)
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_and_repeated_backward_passes(reentrant):
+    """Activation checkpointing gives the plain pass's gradients; a second pass over a kept graph adds them once more."""
+    from torch.utils.checkpoint import checkpoint
+
+    qkv, pos, weights, grads = _inputs(T=300)
+
+    def run(wrap):
+        x, w = qkv.clone().requires_grad_(), [y.clone().requires_grad_() for y in weights]
+        for y in w:
+            y.main_grad = torch.zeros(HD, device="cuda")
+        f = lambda x: qkv_rotary(x, pos, ROPE, Hq, Hkv, *w)  # noqa: E731  (a module's own weights)
+        out = checkpoint(f, x, use_reentrant=reentrant) if wrap else f(x)
+        torch.autograd.backward(out, grads, retain_graph=not wrap)
+        return x, w, out
+
+    x, w, out = run(False)
+    y, v, _ = run(True)
+    assert torch.equal(x.grad, y.grad) and all(torch.equal(a.main_grad, b.main_grad) for a, b in zip(w, v))
+    assert all(a.grad is None for a in w + v)
+    once = [a.main_grad.clone() for a in w]
+    torch.autograd.backward(out, grads)
+    assert all(torch.equal(a.main_grad, 2 * b) for a, b in zip(w, once))
+
+
+def test_backward_passes_of_several_threads():
+    """The passes look the weights' buffers up under Python's lock, from autograd's thread."""
+    import threading
+
+    wrong = []
+
+    def work(i):
+        try:
+            inputs = _inputs(seed=i)
+            want = _plain(inputs[2][0], inputs, inputs[2][1])
+            for _ in range(30):
+                w = [y.clone().requires_grad_() for y in inputs[2]]
+                for y in w:
+                    y.main_grad = torch.zeros(HD, device="cuda")
+                torch.autograd.backward(qkv_rotary(inputs[0], inputs[1], ROPE, Hq, Hkv, *w), inputs[3])
+                torch.cuda.synchronize()
+                if not all(torch.equal(y.main_grad.bfloat16(), g) for y, g in zip(w, want)):
+                    wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not any(t.is_alive() for t in threads) and not wrong, wrong
+
+
+def test_a_captured_backward_pass_adds_to_main_grad():
+    qkv, pos, weights, grads = _inputs(T=64)
+    w = [y.clone().requires_grad_() for y in weights]
+    for y in w:
+        y.main_grad = torch.zeros(HD, device="cuda")
+
+    def step():
+        torch.autograd.backward(qkv_rotary(qkv, pos, ROPE, Hq, Hkv, *w), grads)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    once = [y.main_grad.clone() for y in w]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for y in w:
+        y.main_grad.zero_()
+    graph.replay(), graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y.main_grad, 2 * g) for y, g in zip(w, once))
